@@ -387,6 +387,126 @@ int moe_attention(const float *q, int64_t q_stride, int32_t rows, int32_t heads,
  * src/sample.rs:87-95).  x [rows, n]; out: device int32 [rows]. */
 int moe_argmax(const float *x, int32_t rows, int32_t n, int32_t *out, void *stream);
 
+/* ------------------------------------------ the paged 4-bit key/value cache
+ * A cache for serving: sequences take pages of positions from a pool as they
+ * grow, keys and values are held in 4 bits, attention splits long contexts
+ * over the chip or reads only the pages a query chooses.  The reference keeps
+ * one f32 cache per sequence (State, src/model.rs:93-114) and attends over all
+ * of it (src/model.rs:790-831); its Q4 block and quantiser (src/quant.rs:
+ * 304-365) are what rows are stored in here.  Everything below runs on
+ * `stream`, allocates nothing, reads lengths and positions on the device only
+ * and may be captured into a graph. */
+
+/* One layer's cache.  32 consecutive values of a head share an f16 scale
+ * d = max|v| / 7 and are stored as codes round(v / d) + 8 in 0..15, exactly as
+ * moe_quantize_rows stores a Q4_0 row.  A page is `page` positions of all kv
+ * heads, a tile 32 positions of one kv head:
+ *   [page][kv head][page / 32 tiles][tile: 18 (qd + vd) bytes]
+ * A tile holds the keys' codes (16 qd bytes), the values' codes (16 vd), the
+ * keys' scales (2 qd), the values' scales (2 vd).  Codes are words of 4 bytes:
+ * words 4c..4c+3 of 64 lanes are chunk c, 16 bytes a lane (8 in the last chunk
+ * of an odd number of blocks); block b of positions 0..15 (half 0) or 16..31
+ * (half 1) is word 2 b + half.  For j = 0..15, dims j (low four bits) and
+ * j + 16 (high) of block b at position p are in
+ *   keys    lane 16 (j / 4) + p % 16, byte j % 4 of the word
+ *   values  lane 16 (p % 16 / 4) + j, byte p % 4 of the word
+ * and its scale is number 32 b + 8 (p % 16 / 4) + 4 (p / 16) + p % 4 of its
+ * region.  `means` (or NULL): f16 [n_pages][n_kv][qd], the mean key of every
+ * full page, which moe_kv4_select scores pages by. */
+typedef struct moe_kv4 {
+    void *pool;            /* device, 16-byte aligned */
+    uint64_t pool_bytes;
+    const int32_t *table;  /* device [n_seq][max_pages]: the page holding a sequence's positions page * i ... */
+    void *means;           /* device f16 [n_pages][n_kv][qd], or NULL */
+    int32_t n_seq, max_pages, n_pages;
+    int32_t page;          /* positions of a page: 32, 64, 128 ... 4096 */
+    int32_t n_kv, qd, vd;  /* kv heads, key and value widths: multiples of 32 up to 256 */
+    int32_t _reserved;
+} moe_kv4;
+
+/* Bytes of a pool of c->n_pages pages (of c's page, n_kv, qd and vd). */
+int moe_kv4_pool_size(const moe_kv4 *c, uint64_t *bytes);
+
+/* Block tables and slot maps from request lengths.  Sequence i has length[i]
+ * positions cached and wants add[i] more; add[i] < 0 ends it.  The free pages
+ * are `count` entries of ring[n_pages] from `head` on, wrapping; state is
+ * {head, count}.  For each sequence in order:
+ *   add < 0    its pages go to the ring's end, its new length is 0
+ *   add >= 0   the pages it lacks for length + add positions are taken from
+ *              the ring's head and entered in its table row; it gets add rows
+ * and status[i] says what was refused (its length and pages stay, it gets no
+ * rows): 2 it would not fit its table row; 3 the rows up to it (those refused
+ * for this among them) are more than max_rows; 1 the pages wanted up to it
+ * (those refused for this among them) are more than were free at the start.
+ * So rows and pages go to sequences in order.  Pages given back are free from
+ * the next call on.
+ *   row_start  int32 [n_seq + 1]: sequence i's rows are row_start[i] to
+ *              row_start[i + 1] - 1
+ *   seq, pos   int32 [max_rows]: each row's sequence and position
+ *   slot       int64 [max_rows]: page * `page` + offset, where moe_kv4_store
+ *              writes it
+ * Rows behind the last sequence's get -1 in all three.  length_out and
+ * state_out may be length and state themselves.  Table entries behind a
+ * sequence's pages are left as they were.  Lengths outside 0 ... max_pages *
+ * page count as the nearest of the two; sequences of pages that are in use
+ * elsewhere are the caller's mistake and are not found.  `workspace`: device,
+ * 8-byte aligned, moe_pages_workspace_size bytes.  No counterpart in the
+ * reference, whose sequences own whole caches. */
+int moe_pages_workspace_size(int32_t n_seq, uint64_t *bytes);
+int moe_pages_advance(int32_t n_seq, const int32_t *length, const int32_t *add, int32_t *length_out, int32_t *table,
+                      int32_t max_pages, int32_t page, int32_t *ring, int32_t n_pages, const int32_t *state,
+                      int32_t *state_out, int32_t max_rows, int32_t *row_start, int32_t *seq, int32_t *pos,
+                      int64_t *slot, int32_t *status, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* Write rows into their slots (the cache write of src/model.rs:732-733 and
+ * 773-787): k [rows, n_kv * qd] and v [rows, n_kv * vd] f32, k_stride and
+ * v_stride floats apart, quantised as moe_quantize_rows(Q4_0) does, NaNs (read
+ * as 0) and infinities (their block reads as NaN) included.  slots: device
+ * int64 [rows], distinct; rows whose slot is negative or past the pool are
+ * skipped.  With c->means, a page whose last position is among the rows gets
+ * its mean key: the sum over its positions in 64 bits, divided, rounded to f32,
+ * bounded by the largest f16 and rounded to it. */
+int moe_kv4_store(const moe_kv4 *c, const float *k, int64_t k_stride, const float *v, int64_t v_stride, int32_t rows,
+                  const int64_t *slots, void *stream);
+
+/* The rows of slots as f32 (k or v may be NULL); rows whose slot is negative
+ * or past the pool are left as they were. */
+int moe_kv4_load(const moe_kv4 *c, const int64_t *slots, int32_t rows, float *k, int64_t k_stride, float *v,
+                 int64_t v_stride, void *stream);
+
+/* Causal attention over the cache (src/model.rs:790-831): as moe_attention,
+ * row r of q (heads x qd values) belonging to sequence seq[r] at position
+ * pos[r], with the sequence's positions found through its table row.  heads is
+ * a multiple of c->n_kv.  With `lists` (device int32 [rows][n_kv][n_sel]) a
+ * row's kv head reads only the positions of the pages listed there (numbers in
+ * the table row, ascending; an entry that is negative or not above the one
+ * before it is skipped).  max_pos bounds every pos[r].  A row with pos[r] < 0
+ * or seq[r] outside 0 ... n_seq - 1 is left as it was; pages outside the pool
+ * and behind max_pages hold no positions; a row that sees no position at all
+ * is 0.  What positions a row does not see hold does not matter.  `workspace`:
+ * device, 16-byte aligned, moe_kv4_attention_workspace_size bytes (its
+ * arguments as the call's; it may be 0 bytes).  Calls that share one must be
+ * ordered. */
+int moe_kv4_attention_workspace_size(const moe_kv4 *c, int32_t rows, int32_t heads, int32_t max_pos, int32_t window,
+                                     int32_t n_sel, uint64_t *bytes);
+int moe_kv4_attention(const moe_kv4 *c, const float *q, int64_t q_stride, int32_t rows, int32_t heads, float scale,
+                      const int32_t *seq, const int32_t *pos, int32_t max_pos, int32_t window, const int32_t *lists,
+                      int32_t n_sel, float *out, int64_t out_stride, void *workspace, uint64_t workspace_bytes,
+                      void *stream);
+
+/* Choose pages for moe_kv4_attention: for every row and kv head the n_sel
+ * pages among those up to the row's own (pos[r] / page) that are its first
+ * `sinks`, its last `recent` (1 or more, its own among them), and then those
+ * of the highest score, the largest over the kv head's query heads of q . mean
+ * key, in 64 bits; equal scores: the lower page first; a NaN counts as the
+ * lowest.  lists [rows][n_kv][n_sel]: ascending, -1 behind the last.  Needs
+ * c->means.  Rows with pos[r] < 0 or a sequence outside the table get -1s.
+ * `workspace`: device, 16-byte aligned, moe_kv4_select_workspace_size bytes. */
+int moe_kv4_select_workspace_size(const moe_kv4 *c, int32_t rows, int32_t max_pos, uint64_t *bytes);
+int moe_kv4_select(const moe_kv4 *c, const float *q, int64_t q_stride, int32_t rows, int32_t heads, const int32_t *seq,
+                   const int32_t *pos, int32_t max_pos, int32_t sinks, int32_t recent, int32_t n_sel, int32_t *lists,
+                   void *workspace, uint64_t workspace_bytes, void *stream);
+
 /* --------------------------------------------------- checkpoint containers */
 
 /* One tensor of a single-file checkpoint: Store's Rec (src/store.rs:25-47).

@@ -57,6 +57,12 @@ class RecC(C.Structure):
                 ("rows", C.c_uint64), ("cols", C.c_uint64), ("offset", C.c_uint64), ("bytes", C.c_uint64)]
 
 
+class Kv4C(C.Structure):
+    _fields_ = [("pool", C.c_void_p), ("pool_bytes", C.c_uint64), ("table", C.c_void_p), ("means", C.c_void_p),
+                ("n_seq", C.c_int32), ("max_pages", C.c_int32), ("n_pages", C.c_int32), ("page", C.c_int32),
+                ("n_kv", C.c_int32), ("qd", C.c_int32), ("vd", C.c_int32), ("_reserved", C.c_int32)]
+
+
 DT_Q6_REF = -2
 
 
@@ -130,6 +136,24 @@ PROTOTYPES = {
                                 C.c_float, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int32,
                                 C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),
     "moe_argmax": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
+    "moe_pages_workspace_size": (C.c_int, [C.c_int32, C.POINTER(C.c_uint64)]),
+    "moe_pages_advance": (C.c_int, [C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
+                                    C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p,
+                                    C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "moe_kv4_pool_size": (C.c_int, [C.POINTER(Kv4C), C.POINTER(C.c_uint64)]),
+    "moe_kv4_store": (C.c_int, [C.POINTER(Kv4C), C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p,
+                                C.c_void_p]),
+    "moe_kv4_load": (C.c_int, [C.POINTER(Kv4C), C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                               C.c_void_p]),
+    "moe_kv4_attention_workspace_size": (C.c_int, [C.POINTER(Kv4C), C.c_int32, C.c_int32, C.c_int32, C.c_int32,
+                                                   C.c_int32, C.POINTER(C.c_uint64)]),
+    "moe_kv4_attention": (C.c_int, [C.POINTER(Kv4C), C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_float,
+                                    C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p,
+                                    C.c_int64, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "moe_kv4_select_workspace_size": (C.c_int, [C.POINTER(Kv4C), C.c_int32, C.c_int32, C.POINTER(C.c_uint64)]),
+    "moe_kv4_select": (C.c_int, [C.POINTER(Kv4C), C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p,
+                                 C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_uint64,
+                                 C.c_void_p]),
 }
 
 STAGES = ("router", "gating", "dispatch", "expert_up", "expert_down", "combine", "encode")

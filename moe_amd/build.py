@@ -46,7 +46,7 @@ EXTRA = {"expert_stream.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 SOURCES = ["route.hip", "expert_gemv.hip", "expert_decode.hip", "expert_batch.hip", "expert_mfma.hip",
            "expert_stream.hip", "expert_skinny.hip", "combine.hip", "attention.hip",
-           "model_ops.hip", "moe_abi.hip"]
+           "pages.hip", "kv4_cache.hip", "kv4_attention.hip", "kv4_select.hip", "model_ops.hip", "moe_abi.hip"]
 HOST_SOURCES = ["host_util.cpp", "container.cpp"]
 
 

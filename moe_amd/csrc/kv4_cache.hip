@@ -1,0 +1,196 @@
+// kv4_cache.hip — writing and reading rows of the paged 4-bit cache
+// (moe_kv4_store, moe_kv4_load): layout in kv4.h, quantiser as
+// moe_quantize_rows(Q4_0) (src/quant.rs:304-365).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "gmem.h"
+#include "kv4.h"
+
+namespace moe {
+int fail(int code, const char *fmt, ...);
+
+int kv4_of(const char *what, const moe_kv4 *c, Kv4 *out) {
+    if (!c || !c->pool || !c->table) return fail(MOE_EINVAL, "%s: a cache without a pool or a table", what);
+    if (c->n_seq <= 0 || c->max_pages <= 0 || c->n_pages <= 0 || c->n_kv <= 0)
+        return fail(MOE_EINVAL, "%s: %d sequences of %d pages, pool of %d, %d kv heads", what, c->n_seq, c->max_pages,
+                    c->n_pages, c->n_kv);
+    if (c->page < 32 || c->page > 4096 || (c->page & (c->page - 1)) || (int64_t)c->max_pages * c->page > INT32_MAX)
+        return fail(MOE_EINVAL, "%s: pages of %d positions, %d a sequence (32, 64 ... 4096; fewer than 2^31 positions)",
+                    what, c->page, c->max_pages);
+    if (c->qd <= 0 || c->vd <= 0 || c->qd % 32 || c->vd % 32 || c->qd > 256 || c->vd > 256)
+        return fail(MOE_EUNSUP, "%s: key width %d, value width %d (multiples of 32 up to 256)", what, c->qd, c->vd);
+    Kv4 k{};
+    k.pool = static_cast<uint8_t *>(c->pool), k.table = c->table, k.means = static_cast<__half *>(c->means);
+    k.n_seq = c->n_seq, k.max_pages = c->max_pages, k.n_pages = c->n_pages, k.n_kv = c->n_kv, k.qd = c->qd, k.vd = c->vd;
+    k.page_shift = __builtin_ctz((unsigned)c->page);
+    k.tile_bytes = 18 * (c->qd + c->vd);
+    uint64_t need = 0;
+    if (__builtin_mul_overflow((uint64_t)k.n_pages * (uint64_t)k.tiles(), (uint64_t)k.n_kv * k.tile_bytes, &need))
+        return fail(MOE_EINVAL, "%s: the pool's size overflows", what);
+    if ((uintptr_t)c->pool % 16 || (uintptr_t)c->means % 16 || c->pool_bytes < need)
+        return fail(MOE_EINVAL, "%s: a pool of %llu bytes (16-byte aligned), %llu needed", what,
+                    (unsigned long long)c->pool_bytes, (unsigned long long)need);
+    *out = k;
+    return MOE_OK;
+}
+
+namespace {
+
+// f32 -> f16 as the quantiser rounds it (src/quant.rs:149-174): nearest even
+// for normals, half up for subnormals, too large and NaN to infinity; v >= 0.
+__device__ inline uint32_t half_bits(float f) {
+    const uint32_t x = __float_as_uint(f);
+    int e = (int)(x >> 23) - 112;
+    const uint32_t m = x & 0x7fffffu;
+    if (e >= 31) return 0x7c00u;
+    if (e <= 0) return e < -10 ? 0u : (((m | 0x800000u) >> (1 - e)) + 0x1000u) >> 13;
+    const uint32_t r = m + 0x0fffu + ((m >> 13) & 1u);
+    if (r & 0x800000u) e++;
+    return e >= 31 ? 0x7c00u : (uint32_t)e << 10 | (r & 0x7fffffu) >> 13;
+}
+
+// round() half away from zero, + 8, within 0..15; NaN 8.
+__device__ inline uint32_t code_of(float v, float inv) {
+    const float q = roundf(v * inv) + 8.0f;
+    return q != q ? 8u : (uint32_t)fminf(fmaxf(q, 0.0f), 15.0f);
+}
+
+__device__ inline bool slot_ok(const Kv4 &c, int64_t slot) {
+    return slot >= 0 && slot < ((int64_t)c.n_pages << c.page_shift);
+}
+// The tile of a slot's kv head and its position in it.
+__device__ inline uint8_t *tile_of(const Kv4 &c, int64_t slot, int kv, int &p) {
+    const int off = (int)(slot & ((1 << c.page_shift) - 1));
+    p = off & (kTile - 1);
+    return c.head((int)(slot >> c.page_shift), kv) + (size_t)(off >> 5) * c.tile_bytes;
+}
+
+// Eight lanes per 32-value block, four values each; a block of threads takes
+// 32 blocks of a row's keys and values.
+__global__ __launch_bounds__(256) void kv4_store_kernel(const Kv4 c, const float *__restrict__ k, int64_t ks,
+                                                        const float *__restrict__ v, int64_t vs,
+                                                        const int64_t *__restrict__ slots) {
+    const int row = blockIdx.x;
+    const int64_t slot = slots[row];
+    if (!slot_ok(c, slot)) return;
+    const int nk = c.qd / 32, nv = c.vd / 32, i = threadIdx.x & 7;
+    const int at = blockIdx.y * 32 + (threadIdx.x >> 3);
+    if (at >= c.n_kv * (nk + nv)) return;
+    const bool key = at < c.n_kv * nk;
+    const int blk = key ? at : at - c.n_kv * nk, nb = key ? nk : nv, kv = blk / nb, s = blk % nb;
+    const float *src = (key ? k + (size_t)row * ks : v + (size_t)row * vs) + (size_t)blk * 32 + 4 * i;
+    float x[4], top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] = src[e], top = fmaxf(top, fabsf(x[e]));  // fmaxf drops NaNs
+#pragma unroll
+    for (int o = 4; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    const float d = top / 7.0f;
+    const uint32_t h = half_bits(d);
+    const float inv = d > 0.0f ? 1.0f / __half2float(__ushort_as_half((unsigned short)h)) : 0.0f;
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) w |= code_of(x[e], inv) << (8 * e);
+    w |= (uint32_t)__shfl_down((int)w, 4, 64) << 4;  // dims j + 16 into the high nibbles (lanes 0..3)
+    int p;
+    uint8_t *tile = tile_of(c, slot, kv, p);
+    if (i == 0)
+        *(uint16_t *)(tile + (key ? c.k_scales() : c.v_scales()) + 2 * kv4_scale_at(p, s)) = (uint16_t)h;
+    if (i >= 4) return;
+    if (key) {
+        *(uint32_t *)(tile + kv4_key_byte(nk, p, s, 4 * i)) = w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) tile[c.v_codes() + kv4_value_byte(nv, p, s, 4 * i + e)] = (uint8_t)(w >> (8 * e));
+    }
+}
+
+__device__ inline float value_at(const Kv4 &c, const uint8_t *tile, bool key, int p, int d) {
+    const int nb = (key ? c.qd : c.vd) / 32, s = d >> 5, j = d & 15;
+    const uint8_t b = key ? tile[kv4_key_byte(nb, p, s, j)] : tile[c.v_codes() + kv4_value_byte(nb, p, s, j)];
+    const __half h = ((const __half *)(tile + (key ? c.k_scales() : c.v_scales())))[kv4_scale_at(p, s)];
+    return __half2float(h) * (float)((int)(d & 16 ? b >> 4 : b & 15) - 8);
+}
+
+// The mean key of pages whose last position a row of this call wrote.
+__global__ __launch_bounds__(256) void kv4_means_kernel(const Kv4 c, const int64_t *__restrict__ slots) {
+    const int64_t slot = slots[blockIdx.x];
+    const int kv = blockIdx.y, last = (1 << c.page_shift) - 1, d = threadIdx.x;
+    if (!slot_ok(c, slot) || (slot & last) != last || d >= c.qd) return;
+    const int page = (int)(slot >> c.page_shift);
+    const uint8_t *head = c.head(page, kv);
+    double sum = 0.0;
+    for (int j = 0; j <= last; j++) sum += (double)value_at(c, head + (size_t)(j >> 5) * c.tile_bytes, true, j & 31, d);
+    float m = (float)(sum / (double)(last + 1));
+    m = m > 65504.0f ? 65504.0f : m < -65504.0f ? -65504.0f : m;
+    c.means[((size_t)page * c.n_kv + kv) * c.qd + d] = __float2half_rn(m);
+}
+
+__global__ __launch_bounds__(256) void kv4_load_kernel(const Kv4 c, const int64_t *__restrict__ slots,
+                                                       float *__restrict__ k, int64_t ks, float *__restrict__ v,
+                                                       int64_t vs) {
+    const int64_t slot = slots[blockIdx.x];
+    if (!slot_ok(c, slot)) return;
+    int p;
+    if (k)
+        for (int i = threadIdx.x; i < c.n_kv * c.qd; i += 256)
+            k[(size_t)blockIdx.x * ks + i] = value_at(c, tile_of(c, slot, i / c.qd, p), true, (int)slot & 31, i % c.qd);
+    if (v)
+        for (int i = threadIdx.x; i < c.n_kv * c.vd; i += 256)
+            v[(size_t)blockIdx.x * vs + i] = value_at(c, tile_of(c, slot, i / c.vd, p), false, (int)slot & 31, i % c.vd);
+}
+
+int rc_of(const char *what) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? MOE_OK : fail(MOE_EHIP, "%s: %s", what, hipGetErrorString(e));
+}
+
+}  // namespace
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+int moe_kv4_pool_size(const moe_kv4 *c, uint64_t *bytes) {
+    Kv4 k;
+    if (!c || !bytes) return fail(MOE_EINVAL, "moe_kv4_pool_size: bad argument");
+    moe_kv4 any = *c;  // the sizes alone count
+    any.pool = reinterpret_cast<void *>(16), any.pool_bytes = UINT64_MAX, any.means = nullptr;
+    any.table = reinterpret_cast<const int32_t *>(16);
+    any.n_seq = any.max_pages = 1;
+    const int rc = kv4_of("moe_kv4_pool_size", &any, &k);
+    if (rc) return rc;
+    *bytes = (uint64_t)k.n_pages * (uint64_t)k.tiles() * (uint64_t)k.n_kv * (uint64_t)k.tile_bytes;
+    return MOE_OK;
+}
+
+int moe_kv4_store(const moe_kv4 *c, const float *k, int64_t k_stride, const float *v, int64_t v_stride, int32_t rows,
+                  const int64_t *slots, void *stream) {
+    Kv4 a;
+    if (const int rc = kv4_of("moe_kv4_store", c, &a)) return rc;
+    if (rows < 0 || (rows > 0 && (!k || !v || !slots)))
+        return fail(MOE_EINVAL, "moe_kv4_store: bad argument (%d rows)", rows);
+    if (rows == 0) return MOE_OK;
+    hipStream_t s = (hipStream_t)stream;
+    const int blocks = a.n_kv * (a.qd + a.vd) / 32;
+    hipLaunchKernelGGL(kv4_store_kernel, dim3(rows, (blocks + 31) / 32), dim3(256), 0, s, a, k, k_stride, v, v_stride,
+                       slots);
+    if (a.means) hipLaunchKernelGGL(kv4_means_kernel, dim3(rows, a.n_kv), dim3(256), 0, s, a, slots);
+    return rc_of("cache write kernel");
+}
+
+int moe_kv4_load(const moe_kv4 *c, const int64_t *slots, int32_t rows, float *k, int64_t k_stride, float *v,
+                 int64_t v_stride, void *stream) {
+    Kv4 a;
+    if (const int rc = kv4_of("moe_kv4_load", c, &a)) return rc;
+    if (rows < 0 || (rows > 0 && !slots)) return fail(MOE_EINVAL, "moe_kv4_load: bad argument (%d rows)", rows);
+    if (rows == 0 || (!k && !v)) return MOE_OK;
+    hipLaunchKernelGGL(kv4_load_kernel, dim3(rows), dim3(256), 0, (hipStream_t)stream, a, slots, k, k_stride, v,
+                       v_stride);
+    return rc_of("cache read kernel");
+}
+
+}  // extern "C"

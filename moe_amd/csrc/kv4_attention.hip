@@ -1,9 +1,26 @@
 // kv4_attention.hip — causal attention over the paged 4-bit cache
-// (moe_kv4_attention).
+// (moe_kv4_attention), layout in kv4.h.
 //
-// One wavefront per (row, query head): a tile's 32 positions at a time, two
-// lanes a position for the scores (half of the dims each), a running maximum
-// and sum, then each lane its value columns.  All in f32.
+// Rows find their sequence and position on the device, so one kernel serves
+// decode steps, prompts and chunks.  A block takes a group of consecutive rows
+// and one kv head, splits the group into runs of one sequence and makes each
+// run's (row, query head) pairs the 16 or 32 columns of its products on the
+// f16 matrix cores; its waves (and, where there are few rows, several blocks)
+// split the run's tiles of 32 positions and merge at the end.
+//
+// A code minus 8 is exact in f16, and a block of 32 dims is one step of the
+// 16x16x32 instruction, so nothing is dequantised: per block of a key
+//   S^T += d_k (C Q_hi^T + C Q_lo^T)
+// with q scale log2(e) 2^k in two f16 pieces (22 bits of the row's largest
+// value) and the block's scale applied to the f32 sum.  The result's layout
+// (lane = column, positions 4g.. of both halves) is the B operand of the
+// second product, whose sum runs over positions with a scale each:
+//   O^T += C (P d_v)_hi + C (P d_v)_lo
+// The weights P = 2^(s - ref) are kept so large that two f16 pieces hold
+// their products with the scales to 2^-30 of the largest: ref = m + E - 9 with
+// m a running maximum (it moves when a score exceeds it by 6) and 2^E above
+// every value scale seen, so P d_v stays below 2^15 and mostly above 2^-10.
+// Sums are f32; the two pieces' rounding is 2^-22, as f32 dot products' own.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -17,80 +34,507 @@ int fail(int code, const char *fmt, ...);
 
 namespace {
 
-__global__ __launch_bounds__(64) void kv4_attention_kernel(const Kv4 c, const float *__restrict__ q, int64_t qs, int heads,
-                                                           float scale, const int32_t *__restrict__ seq,
-                                                           const int32_t *__restrict__ pos, int window,
-                                                           const int32_t *__restrict__ lists, int n_sel,
-                                                           float *__restrict__ out, int64_t os) {
-    __shared__ float sq[256], sp[32];
-    const int r = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, rep = heads / c.n_kv, kv = h / rep;
-    const int sid = seq[r], top = pos[r];
-    if (top < 0 || sid < 0 || sid >= c.n_seq) return;
-    const int lo = window > 0 ? max(0, top + 1 - window) : 0;
-    for (int i = lane; i < c.qd; i += 64) sq[i] = q[(size_t)r * qs + (size_t)h * c.qd + i];
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const int first = lists ? 0 : lo >> c.page_shift, n = lists ? n_sel : (top >> c.page_shift) + 1;
-    int before = -1;
-    for (int i = first; i < n; i++) {
-        int page = i;
-        if (lists) {
-            page = lists[((size_t)r * c.n_kv + kv) * n_sel + i];
-            const bool skip = page <= before;
-            before = page;
-            if (skip) continue;
-        }
-        if (page >= c.max_pages) continue;
-        const int id = c.table[(size_t)sid * c.max_pages + page];
-        if ((unsigned)id >= (unsigned)c.n_pages) continue;
-        for (int t = 0; t < c.tiles(); t++) {
-            const int base = (page << c.page_shift) + t * kTile;
-            if (base > top || base + kTile <= lo) continue;
-            const uint8_t *tile = c.head(id, kv) + (size_t)t * c.tile_bytes;
-            const int p = lane & 31, half = lane >> 5, at = base + p;
-            float s = 0.0f;
-            for (int b = 0; b < c.qd / 32; b++) {
-                float sum = 0.0f;
-                for (int j = 0; j < 16; j++) {
-                    const uint8_t byte = tile[kv4_key_byte(c.qd / 32, p, b, j)];
-                    sum = fmaf((float)((int)(half ? byte >> 4 : byte & 15) - 8), sq[32 * b + 16 * half + j], sum);
-                }
-                s = fmaf(__half2float(((const __half *)(tile + c.k_scales()))[kv4_scale_at(p, b)]), sum, s);
-            }
-            s = (s + __shfl_xor(s, 32, 64)) * scale;
-            const bool seen = at >= lo && at <= top;
-            if (!seen) s = -INFINITY;
-            float x = s;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+
+struct Args {
+    Kv4 c;
+    const float *q;
+    const int32_t *seq, *pos, *lists;
+    float *out, *part, *part_ml;  // part [row][head][ps][vd], part_ml [row][head][ps][2]
+    int64_t q_stride, out_stride;
+    int rows, heads, rep, window, n_sel;
+    float scale;
+    int tt, groups;  // rows of a group, groups
+    int rc, chunks;  // query heads of a block, blocks that share a kv head's
+    int split;       // blocks that share a group's runs
+    int ps;          // blocks that share a run's tiles
+};
+
+__device__ inline half2v as_h2(uint32_t v) { return __builtin_bit_cast(half2v, v); }
+
+// Eight codes minus 8 as f16 from one word: low nibbles of its bytes 0, 2, 1,
+// 3, then high ones.  A nibble becomes the low mantissa bits of 1024 (or, four
+// bits up, of 64); the subtraction is exact.
+__device__ inline half8 codes_lo_hi(uint32_t w) {
+    const uint32_t x = w >> 8;
+    const half2v a = as_h2((w & 0x000f000fu) | 0x64006400u), b = as_h2((x & 0x000f000fu) | 0x64006400u);
+    const half2v c = as_h2((w & 0x00f000f0u) | 0x54005400u), d = as_h2((x & 0x00f000f0u) | 0x54005400u);
+    const half2v k = {(_Float16)1032.0f, (_Float16)1032.0f}, m = {(_Float16)72.0f, (_Float16)72.0f};
+    const half2v r0 = a - k, r1 = b - k, r2 = c - m, r3 = d - m;
+    return half8{r0[0], r0[1], r1[0], r1[1], r2[0], r2[1], r3[0], r3[1]};
+}
+// The low (high) nibbles of two words' bytes 0, 2, 1, 3.
+template <bool HIGH>
+__device__ inline half8 codes_of(uint32_t w0, uint32_t w1) {
+    const uint32_t mask = HIGH ? 0x00f000f0u : 0x000f000fu, one = HIGH ? 0x54005400u : 0x64006400u;
+    const _Float16 off = HIGH ? 72.0f : 1032.0f;
+    const half2v k = {off, off};
+    const half2v r0 = as_h2((w0 & mask) | one) - k, r1 = as_h2((w0 >> 8 & mask) | one) - k;
+    const half2v r2 = as_h2((w1 & mask) | one) - k, r3 = as_h2((w1 >> 8 & mask) | one) - k;
+    return half8{r0[0], r0[1], r1[0], r1[1], r2[0], r2[1], r3[0], r3[1]};
+}
+
+// A tile's words of a lane.
+template <int QC, int VC>
+struct Tile {
+    static constexpr int NS = (QC + VC + 3) / 4;
+    uint32_t k[2 * QC], v[2 * VC], s[NS];
+    int base;  // position of its first row
+    int ok;    // whether there is such a tile
+};
+
+template <int NB, bool EX>
+__device__ inline void load_words(uint32_t (&w)[2 * NB], const uint8_t *p, int nb, int lane) {
 #pragma unroll
-            for (int w = 16; w >= 1; w >>= 1) x = fmaxf(x, __shfl_xor(x, w, 64));
-            const float mn = fmaxf(m, x), f = mn == -INFINITY ? 1.0f : expf(m - mn);
-            const float e = seen ? expf(s - (mn == -INFINITY ? 0.0f : mn)) : 0.0f;
-            m = mn;
-            float sum = e;
+    for (int c = 0; c < (NB + 1) / 2; c++) {
+        if (EX ? 2 * c + 2 <= NB : 2 * c + 2 <= nb) {
+            const u32x4 x = gload((const u32x4 *)(p + 1024 * c + 16 * lane));
 #pragma unroll
-            for (int w = 16; w >= 1; w >>= 1) sum += __shfl_xor(sum, w, 64);
-            l = l * f + sum;
-            if (half == 0) sp[p] = e;
-            __syncthreads();
-            for (int k = 0; k < 4; k++) {
-                const int d = lane + 64 * k;
-                if (d >= c.vd) continue;
-                float acc = 0.0f;  // a tile's sum first: fewer roundings of the long sum
-                for (int j = 0; j < 32; j++) {
-                    if (base + j < lo || base + j > top) continue;
-                    const uint8_t byte = tile[c.v_codes() + kv4_value_byte(c.vd / 32, j, d >> 5, d & 15)];
-                    const float dv = __half2float(((const __half *)(tile + c.v_scales()))[kv4_scale_at(j, d >> 5)]);
-                    acc = fmaf(sp[j], dv * (float)((int)(d & 16 ? byte >> 4 : byte & 15) - 8), acc);
-                }
-                o[k] = fmaf(o[k], f, acc);
-            }
-            __syncthreads();
+            for (int i = 0; i < 4; i++)
+                if (4 * c + i < 2 * NB) w[4 * c + i] = x[i];
+        } else if (EX || 2 * c < nb) {
+            const u32x2 x = gload((const u32x2 *)(p + 1024 * c + 8 * lane));
+            w[4 * c] = x[0], w[4 * c + 1] = x[1];
         }
     }
-    for (int k = 0; k < 4; k++) {
-        const int d = lane + 64 * k;
-        if (d < c.vd) out[(size_t)r * os + (size_t)h * c.vd + d] = l == 0.0f ? 0.0f : o[k] / l;
+}
+
+// QC, VC: blocks of a key and a value (EX) or the most there may be.  C:
+// 16-column tiles.  W: waves.
+template <int QC, int VC, bool EX, int C, int W>
+__global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) {
+    typedef Tile<QC, VC> T;
+    constexpr int kQ = C * QC * 2 * 64;  // Q operands: [column tile][block][hi, lo][lane] of 16 bytes
+    constexpr int kMerge = W / 2 * C * VC * 2 * 64;
+    __shared__ u32x4 sm[kQ > kMerge ? kQ : kMerge];
+    __shared__ uint32_t ssc[W][T::NS * 64];
+    __shared__ float sm_r[W][C * 16], sm_l[W][C * 16], sm_k[C * 16];
+    const Kv4 &kc = a.c;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+    const int nq = EX ? QC : kc.qd / 32, nv = EX ? VC : kc.vd / 32;
+    // Kv heads next to each other go to the XCDs in turn, so that one head's
+    // blocks find its tiles in their L2.  Later rows of a prompt see more
+    // positions: the last groups go first.  A group's blocks that find no run
+    // of their own leave at once, so the first ones come together.
+    int id = blockIdx.x;
+    const int kv = id % kc.n_kv;
+    id /= kc.n_kv;
+    const int chunk = id % a.chunks;
+    id /= a.chunks;
+    const int part = id % a.ps;
+    id /= a.ps;
+    const int sub = id / a.groups;
+    const int r0 = (a.groups - 1 - id % a.groups) * a.tt;
+    const int nr = min(a.tt, a.rows - r0);
+    const int h0 = kv * a.rep + chunk * a.rc, hn = min(a.rc, a.rep - chunk * a.rc);
+    const int my_seq = gload(a.seq + r0 + min(lane, nr - 1)), my_pos = gload(a.pos + r0 + min(lane, nr - 1));
+    const bool valid = lane < nr && my_pos >= 0 && (unsigned)my_seq < (unsigned)kc.n_seq;
+    const int before = __shfl_up(my_seq, 1, 64);
+    const bool before_ok = __shfl_up((int)valid, 1, 64);
+    // Lanes that begin a run or are none; the runs' first lanes.
+    const unsigned long long cuts = __ballot(!valid || lane == 0 || my_seq != before || !before_ok);
+    unsigned long long starts = cuts & __ballot(valid);
+    const int tshift = kc.page_shift - 5;
+
+    for (int run = 0; starts; run++) {
+        const int first = __builtin_ctzll(starts);
+        starts &= starts - 1;
+        if (run % a.split != sub) continue;
+        const unsigned long long after = first < 63 ? cuts >> (first + 1) : 0;
+        const int end = min(nr, after ? first + 1 + __builtin_ctzll(after) : 64);
+        const int ncol = (end - first) * hn;
+        const bool mine = lane >= first && lane < end;
+        int hi = mine ? my_pos : -1;
+        int lo = mine ? (a.window > 0 ? max(0, my_pos + 1 - a.window) : 0) : 0x7fffffff;
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) {
+            hi = max(hi, __shfl_xor(hi, o, 64));
+            lo = min(lo, __shfl_xor(lo, o, 64));
+        }
+        hi = __builtin_amdgcn_readfirstlane(hi);
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        const int sq = __builtin_amdgcn_readfirstlane(__shfl(my_seq, first, 64));
+        int cp[C], cl[C];
+        bool cv[C];
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const int cc = c * 16 + col;
+            cv[c] = cc < ncol;
+            const int p = __shfl(my_pos, first + (cv[c] ? cc / hn : 0), 64);
+            cp[c] = p;
+            cl[c] = a.window > 0 ? max(0, p + 1 - a.window) : 0;
+        }
+
+        // Q: a column's values times scale log2(e), by a power of two that
+        // brings its largest into [2^14, 2^15), in two f16 pieces.  16 threads a
+        // column, twice over its values.
+        __syncthreads();  // the previous run's reads of sm
+        for (int cc = threadIdx.x >> 4; cc < C * 16; cc += W * 4) {
+            const float *row = a.q + (size_t)(r0 + first + min(cc, ncol - 1) / hn) * a.q_stride +
+                               (size_t)(h0 + min(cc, ncol - 1) % hn) * kc.qd;
+            const float f = cc < ncol ? a.scale * 1.44269504f : 0.0f;
+            const int i = threadIdx.x & 15;
+            float top = 0.0f;
+            for (int d = i; d < kc.qd; d += 16) top = fmaxf(top, fabsf(gload(row + d) * f));
+#pragma unroll
+            for (int o = 8; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+            // 2^(14 - exponent of top), within what both it and its inverse can be.
+            const int k = min(max(127 + 14 - ((int)(__float_as_uint(top) >> 23) - 127), 1), 253);
+            const float up = __uint_as_float((uint32_t)k << 23);
+            if (i == 0) sm_k[cc] = __uint_as_float((uint32_t)(254 - k) << 23);
+            _Float16 *dst = (_Float16 *)sm;
+            for (int d = i; d < kc.qd; d += 16) {
+                const float v = gload(row + d) * f * up;
+                const _Float16 hv = (_Float16)v;
+                // Dim 32 s + 16 h + 4 g + e is element 4 h + {0, 2, 1, 3}[e] of lane (g, column).
+                const int s = d >> 5, e = d & 3, gg = (d >> 2) & 3, el = (d >> 4 & 1) * 4 + (e >> 1) + (e & 1) * 2;
+                const int at = (((cc >> 4) * QC + s) * 2 * 64 + gg * 16 + (cc & 15)) * 8 + el;
+                dst[at] = hv;
+                dst[at + 64 * 8] = (_Float16)(v - (float)hv);
+            }
+        }
+        __syncthreads();
+        float ck[C];
+#pragma unroll
+        for (int c = 0; c < C; c++) ck[c] = sm_k[c * 16 + col];
+        half8 qr[C == 1 ? QC * 2 : 1];
+        if (C == 1) {
+#pragma unroll
+            for (int i = 0; i < QC * 2; i++)
+                if (EX || i < 2 * nq) qr[i] = __builtin_bit_cast(half8, sm[i * 64 + lane]);
+        }
+
+        // This wave's tiles: v0 .. v1 - 1 of the run's (of the lists' pages).
+        const int t0 = a.lists ? 0 : lo >> 5;
+        const int nt = a.lists ? a.n_sel << tshift : (hi >> 5) - t0 + 1;
+        const int parts = a.ps * W, me = part * W + wave;
+        int v = (int)((long long)nt * me / parts);
+        const int v1 = (int)((long long)nt * (me + 1) / parts);
+        const int32_t *list = a.lists ? a.lists + ((size_t)(r0 + first) * kc.n_kv + kv) * a.n_sel : nullptr;
+        const int32_t *table = kc.table + (size_t)sq * kc.max_pages;
+        int b0 = -64, my_page = 0, my_id = -1;  // pages b0 .. b0 + 63 of the run, one a lane
+        // The next tile that there is; its words' loads are queued.
+        auto next = [&](T &x) {
+            x.ok = 0;
+            for (; v < v1; v++) {
+                const int t = t0 + v, i = t >> tshift;
+                if (i >= b0 + 64 || i < b0) {
+                    b0 = i;
+                    const int j = b0 + lane;
+                    my_page = j;
+                    bool there = true;
+                    if (list) {
+                        my_page = j < a.n_sel ? gload(list + j) : -1;
+                        const int prev = j > 0 && j <= a.n_sel ? gload(list + j - 1) : -1;
+                        there = my_page > prev;
+                    }
+                    there = there && my_page >= 0 && my_page < kc.max_pages;
+                    my_id = there ? gload(table + my_page) : -1;
+                }
+                const int pid = __builtin_amdgcn_readlane(my_id, i - b0);
+                if ((unsigned)pid >= (unsigned)kc.n_pages) continue;
+                const int in = t & ((1 << tshift) - 1);
+                const int base = (__builtin_amdgcn_readlane(my_page, i - b0) << kc.page_shift) + in * kTile;
+                if (base > hi || base + kTile <= lo) continue;
+                x.base = base, x.ok = 1;
+                const uint8_t *p = kc.head(pid, kv) + (size_t)in * kc.tile_bytes;
+                load_words<QC, EX>(x.k, p, nq, lane);
+                load_words<VC, EX>(x.v, p + kc.v_codes(), nv, lane);
+                const int ns = (nq + nv) * 16;
+#pragma unroll
+                for (int e = 0; e < T::NS; e++)
+                    x.s[e] = gload((const uint32_t *)(p + kc.k_scales()) + min(lane + 64 * e, ns - 1));
+                v++;
+                return;
+            }
+        };
+
+        f32x4 o[C][VC][2];
+        float ref[C], lim[C], l[C];
+        int E = -24;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            ref[c] = 0.0f, lim[c] = -INFINITY, l[c] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < VC; b++) o[c][b][0] = o[c][b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+
+        auto step = [&](const T &x) {
+            // Scales through LDS (the wave's own: in order, no barrier): every
+            // lane reads its four positions of both halves, 16 bytes.
+            uint32_t top = 0;  // the largest finite value scale of the lane's, f16 bits
+            bool inf = false;
+#pragma unroll
+            for (int e = 0; e < T::NS; e++) {
+                ssc[wave][lane + 64 * e] = x.s[e];
+                const int at = lane + 64 * e;
+                const uint32_t y = at >= nq * 16 && at < (nq + nv) * 16 ? x.s[e] & 0x7fff7fffu : 0;
+                const uint32_t y0 = y & 0xffffu, y1 = y >> 16;
+                inf |= y0 >= 0x7c00u || y1 >= 0x7c00u;
+                top = max(top, max(y0 >= 0x7c00u ? 0 : y0, y1 >= 0x7c00u ? 0 : y1));
+            }
+            const u32x4 *sc = (const u32x4 *)ssc[wave];
+            f32x4 s[C][2];
+#pragma unroll
+            for (int c = 0; c < C; c++) s[c][0] = s[c][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int b = 0; b < QC; b++) {
+                if (!EX && b >= nq) break;
+                const half8 d = __builtin_bit_cast(half8, sc[b * 4 + g]);
+                const half8 k0 = codes_lo_hi(x.k[2 * b]), k1 = codes_lo_hi(x.k[2 * b + 1]);
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    const half8 qh = C == 1 ? qr[2 * b] : __builtin_bit_cast(half8, sm[((c * QC + b) * 2) * 64 + lane]);
+                    const half8 ql = C == 1 ? qr[2 * b + 1] : __builtin_bit_cast(half8, sm[((c * QC + b) * 2 + 1) * 64 + lane]);
+                    const f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+                    f32x4 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql, z, 0, 0, 0);
+                    f32x4 t = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql, z, 0, 0, 0);
+                    r = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh, r, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh, t, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        s[c][0][i] = fmaf((float)d[i], r[i], s[c][0][i]);
+                        s[c][1][i] = fmaf((float)d[4 + i], t[i], s[c][1][i]);
+                    }
+                }
+            }
+            // Positions a column does not see.
+            bool some = false;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                s[c][0] *= ck[c];
+                s[c][1] *= ck[c];
+                some |= cv[c] && (x.base < cl[c] || x.base + kTile - 1 > cp[c]);
+            }
+            if (__any(some)) {
+#pragma unroll
+                for (int c = 0; c < C; c++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int at = x.base + (i >> 2) * 16 + 4 * g + (i & 3);
+                        if (at < cl[c] || at > cp[c]) s[c][i >> 2][i & 3] = -INFINITY;
+                    }
+            }
+            // The references move: a score too far above, or a larger scale.
+            float mx[C];
+            bool move = false;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                mx[c] = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; i++) mx[c] = fmaxf(mx[c], s[c][i >> 2][i & 3]);
+                move |= mx[c] > lim[c];
+            }
+            const bool odd = __any(inf);
+            const bool grow = __any((int)(top >> 10) - 14 > E);  // not below 2^E
+            if (__any(move) || grow) {
+                int ne = (int)(top >> 10) - 14;
+#pragma unroll
+                for (int w = 32; w >= 1; w >>= 1) ne = max(ne, __shfl_xor(ne, w, 64));
+                ne = max(ne, E);
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    float y = fmaxf(mx[c], __shfl_xor(mx[c], 16, 64));
+                    y = fmaxf(y, __shfl_xor(y, 32, 64));
+                    const float m = lim[c] - 6.0f;
+                    const float mn = y > lim[c] ? y : m;
+                    const float nref = mn == -INFINITY ? 0.0f : mn + (float)(ne - 9);
+                    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref[c] - nref);
+                    lim[c] = mn + 6.0f, ref[c] = nref;
+                    l[c] *= f;
+#pragma unroll
+                    for (int b = 0; b < VC; b++) o[c][b][0] *= f, o[c][b][1] *= f;
+                }
+                E = __builtin_amdgcn_readfirstlane(ne);
+            }
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float p = __builtin_amdgcn_exp2f(s[c][i >> 2][i & 3] - ref[c]);
+                    s[c][i >> 2][i & 3] = p;
+                    l[c] += p;
+                }
+#pragma unroll
+            for (int b = 0; b < VC; b++) {
+                if (!EX && b >= nv) break;
+                const half8 d = __builtin_bit_cast(half8, sc[(nq + b) * 4 + g]);
+                const half8 v0 = codes_of<false>(x.v[2 * b], x.v[2 * b + 1]);
+                const half8 v1 = codes_of<true>(x.v[2 * b], x.v[2 * b + 1]);
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    float w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        // Order of the codes: bytes 0, 2, 1, 3 of each half.
+                        const int e = (i & 4) | (i & 1) << 1 | (i >> 1 & 1);
+                        const float p = s[c][e >> 2][e & 3];
+                        w[i] = p * (float)d[e];
+                        // A position of weight 0 may hold an infinity or a NaN.
+                        if (odd) w[i] = p == 0.0f ? 0.0f : w[i];
+                    }
+                    half8 ph, pl;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) ph[i] = (_Float16)w[i];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) pl[i] = (_Float16)(w[i] - (float)ph[i]);
+                    o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph, o[c][b][0], 0, 0, 0);
+                    o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph, o[c][b][1], 0, 0, 0);
+                    o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl, o[c][b][0], 0, 0, 0);
+                    o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl, o[c][b][1], 0, 0, 0);
+                }
+            }
+        };
+        T x, y;
+        next(x);
+        while (x.ok) {
+            next(y);
+            step(x);
+            if (!y.ok) break;
+            next(x);
+            step(y);
+        }
+
+        // Merge the waves: everyone to the block's largest reference, then sums
+        // by halves.
+        __syncthreads();  // reads of Q
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            l[c] += __shfl_xor(l[c], 16, 64);
+            l[c] += __shfl_xor(l[c], 32, 64);
+            if (lim[c] == -INFINITY && l[c] == 0.0f) ref[c] = -INFINITY;  // saw nothing
+            if (g == 0) sm_r[wave][c * 16 + col] = ref[c], sm_l[wave][c * 16 + col] = l[c];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            float rr = -INFINITY, ll = 0.0f;
+            for (int w = 0; w < W; w++) rr = fmaxf(rr, sm_r[w][c * 16 + col]);
+            for (int w = 0; w < W; w++) {
+                const float rw = sm_r[w][c * 16 + col];
+                if (rw != -INFINITY) ll += sm_l[w][c * 16 + col] * __builtin_amdgcn_exp2f(rw - rr);
+            }
+            const float f = ref[c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref[c] - rr);
+            l[c] = ll, ref[c] = rr;
+#pragma unroll
+            for (int b = 0; b < VC; b++) o[c][b][0] *= f, o[c][b][1] *= f;
+        }
+        f32x4 *mrg = (f32x4 *)sm;
+#pragma unroll
+        for (int h = W / 2; h >= 1; h /= 2) {
+            if (wave >= h && wave < 2 * h) {
+#pragma unroll
+                for (int c = 0; c < C; c++)
+#pragma unroll
+                    for (int b = 0; b < VC * 2; b++)
+                        mrg[(((wave - h) * C + c) * VC * 2 + b) * 64 + lane] = o[c][b >> 1][b & 1];
+            }
+            __syncthreads();
+            if (wave < h) {
+#pragma unroll
+                for (int c = 0; c < C; c++)
+#pragma unroll
+                    for (int b = 0; b < VC * 2; b++)
+                        o[c][b >> 1][b & 1] += mrg[((wave * C + c) * VC * 2 + b) * 64 + lane];
+            }
+            __syncthreads();
+        }
+        if (wave != 0) continue;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            if (!cv[c]) continue;
+            const int cc = c * 16 + col;
+            const size_t row = r0 + first + cc / hn, head = h0 + cc % hn;
+            float *dst = a.out + row * a.out_stride + head * kc.vd;
+            float f = l[c] == 0.0f ? 0.0f : 1.0f / l[c];
+            if (a.ps > 1) {
+                const size_t at = (row * a.heads + head) * a.ps + part;
+                dst = a.part + at * kc.vd;
+                if (g == 0) a.part_ml[2 * at] = ref[c], a.part_ml[2 * at + 1] = l[c];
+                f = 1.0f;
+            }
+            // Lane (column, g) holds dims 32 b + 16 h + 4 g + i.
+#pragma unroll
+            for (int b = 0; b < VC; b++) {
+                if (!EX && b >= nv) break;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    f32x4 z = o[c][b][h];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) gstore(dst + 32 * b + 16 * h + 4 * g + i, z[i] * f);
+                }
+            }
+        }
     }
+}
+
+// The parts of rows whose tiles several blocks shared, in part order: a
+// wavefront per (row, head).
+__global__ __launch_bounds__(256) void kv4_join_kernel(const Args a) {
+    const int lane = threadIdx.x & 63, vd = a.c.vd;
+    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= (int64_t)a.rows * a.heads) return;
+    const int row = (int)(at / a.heads), head = (int)(at % a.heads);
+    if (a.pos[row] < 0 || (unsigned)a.seq[row] >= (unsigned)a.c.n_seq) return;
+    const float *ml = a.part_ml + at * a.ps * 2, *part = a.part + at * a.ps * vd;
+    float rr = -INFINITY;
+    for (int p = lane; p < a.ps; p += 64) rr = fmaxf(rr, ml[2 * p]);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) rr = fmaxf(rr, __shfl_xor(rr, o, 64));
+    float l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p = 0; p < a.ps; p++) {
+        const float ref = ml[2 * p];
+        if (ref == -INFINITY) continue;
+        const float f = __builtin_amdgcn_exp2f(ref - rr);
+        l = fmaf(ml[2 * p + 1], f, l);
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (lane + 64 * k < vd) acc[k] = fmaf(part[(size_t)p * vd + lane + 64 * k], f, acc[k]);
+    }
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    float *dst = a.out + (int64_t)row * a.out_stride + (int64_t)head * vd;
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        if (lane + 64 * k < vd) dst[lane + 64 * k] = acc[k] * f;
+}
+
+// How a call is cut up: see Args.
+struct Plan {
+    int C, rc, chunks, tt, groups, split, ps;
+    uint64_t bytes;
+};
+
+Plan plan_of(const Kv4 &c, int rows, int heads, int max_pos, int window, int n_sel) {
+    Plan p{};
+    const int rep = heads / c.n_kv;
+    // Two column tiles halve the unpacking and the cache's traffic where rows
+    // come in runs; 256 groups of 32 columns fill the chip.
+    const long long wide = ((long long)rows * rep + 31) / 32 * c.n_kv;
+    p.C = n_sel == 0 && c.qd <= 192 && c.vd <= 128 && wide >= 256 ? 2 : 1;
+    p.rc = std::min(rep, 16 * p.C);
+    p.chunks = (rep + p.rc - 1) / p.rc;
+    // Rows with lists of their own share nothing.
+    p.tt = n_sel ? 1 : 16 * p.C / p.rc;
+    p.groups = (rows + p.tt - 1) / p.tt;
+    const long long base = (long long)p.groups * p.chunks * c.n_kv;
+    p.split = (int)std::max<long long>(1, std::min<long long>(p.tt, (2048 + base - 1) / base));
+    const long long tiles = n_sel ? (long long)n_sel * c.tiles()
+                                  : (window > 0 ? std::min((long long)window + p.tt, (long long)max_pos + 1) : max_pos + 1LL) / 32 + 1;
+    const long long units = base * p.split;
+    p.ps = (int)std::max<long long>(1, std::min<long long>({(1024 + units - 1) / units, tiles / 16, 256}));
+    p.bytes = p.ps > 1 ? (uint64_t)rows * heads * p.ps * (c.vd + 2) * 4 : 0;
+    return p;
+}
+
+template <int QC, int VC, bool EX, int C>
+void launch(const Args &a, hipStream_t s) {
+    constexpr int W = 4;
+    const long long blocks = (long long)a.groups * a.split * a.ps * a.chunks * a.c.n_kv;
+    hipLaunchKernelGGL((kv4_attention_kernel<QC, VC, EX, C, W>), dim3((unsigned)blocks), dim3(W * 64), 0, s, a);
 }
 
 }  // namespace
@@ -104,9 +548,11 @@ int moe_kv4_attention_workspace_size(const moe_kv4 *c, int32_t rows, int32_t hea
                                      int32_t n_sel, uint64_t *bytes) {
     Kv4 a;
     if (const int rc = kv4_of("moe_kv4_attention_workspace_size", c, &a)) return rc;
-    if (!bytes || rows < 0 || heads <= 0 || heads % a.n_kv || max_pos < 0 || n_sel < 0)
-        return fail(MOE_EINVAL, "moe_kv4_attention_workspace_size: bad argument");
-    *bytes = 0;
+    if (!bytes || rows < 0 || heads <= 0 || heads % a.n_kv || max_pos < 0 ||
+        max_pos >= (int64_t)a.max_pages << a.page_shift || n_sel < 0)
+        return fail(MOE_EINVAL, "moe_kv4_attention_workspace_size: bad argument (%d rows, %d heads over %d, max position %d"
+                    " of %lld)", rows, heads, a.n_kv, max_pos, (long long)a.max_pages << a.page_shift);
+    *bytes = rows ? plan_of(a, rows, heads, max_pos, window, n_sel).bytes : 0;
     return MOE_OK;
 }
 
@@ -114,15 +560,38 @@ int moe_kv4_attention(const moe_kv4 *c, const float *q, int64_t q_stride, int32_
                       const int32_t *seq, const int32_t *pos, int32_t max_pos, int32_t window, const int32_t *lists,
                       int32_t n_sel, float *out, int64_t out_stride, void *workspace, uint64_t workspace_bytes,
                       void *stream) {
-    Kv4 a;
-    if (const int rc = kv4_of("moe_kv4_attention", c, &a)) return rc;
-    if ((rows > 0 && (!q || !seq || !pos || !out)) || rows < 0 || heads <= 0 || heads % a.n_kv || max_pos < 0 ||
-        max_pos >= (int64_t)a.max_pages << a.page_shift || (lists && n_sel <= 0))
+    Args a{};
+    if (const int rc = kv4_of("moe_kv4_attention", c, &a.c)) return rc;
+    if ((rows > 0 && (!q || !seq || !pos || !out)) || rows < 0 || heads <= 0 || heads % a.c.n_kv || max_pos < 0 ||
+        max_pos >= (int64_t)a.c.max_pages << a.c.page_shift || (lists && n_sel <= 0))
         return fail(MOE_EINVAL, "moe_kv4_attention: bad argument (%d rows, %d heads over %d, max position %d of %lld)",
-                    rows, heads, a.n_kv, max_pos, (long long)a.max_pages << a.page_shift);
+                    rows, heads, a.c.n_kv, max_pos, (long long)a.c.max_pages << a.c.page_shift);
     if (rows == 0) return MOE_OK;
-    hipLaunchKernelGGL(kv4_attention_kernel, dim3(rows, heads), dim3(64), 0, (hipStream_t)stream, a, q, q_stride, heads,
-                       scale, seq, pos, window, lists, n_sel, out, out_stride);
+    const Plan p = plan_of(a.c, rows, heads, max_pos, window, lists ? n_sel : 0);
+    if (p.bytes && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < p.bytes))
+        return fail(MOE_EINVAL, "moe_kv4_attention: workspace of %llu bytes, %llu needed",
+                    (unsigned long long)workspace_bytes, (unsigned long long)p.bytes);
+    a.q = q, a.seq = seq, a.pos = pos, a.lists = lists, a.out = out;
+    a.q_stride = q_stride, a.out_stride = out_stride;
+    a.rows = rows, a.heads = heads, a.rep = heads / a.c.n_kv, a.window = window, a.n_sel = lists ? n_sel : 0;
+    a.scale = scale;
+    a.tt = p.tt, a.groups = p.groups, a.rc = p.rc, a.chunks = p.chunks, a.split = p.split, a.ps = p.ps;
+    a.part = static_cast<float *>(workspace);
+    a.part_ml = a.part + (size_t)rows * heads * p.ps * a.c.vd;
+    if ((long long)a.groups * a.split * a.ps * a.chunks * a.c.n_kv > INT32_MAX)
+        return fail(MOE_EUNSUP, "moe_kv4_attention: %d rows of %d heads are too many blocks", rows, heads);
+    hipStream_t s = (hipStream_t)stream;
+    const int qc = a.c.qd / 32, vc = a.c.vd / 32;
+    // Widths of their own: a power-of-two head and the latent cache's 192/128;
+    // the others count their blocks at run time.
+    if (qc == 2 && vc == 2) p.C == 2 ? launch<2, 2, true, 2>(a, s) : launch<2, 2, true, 1>(a, s);
+    else if (qc == 4 && vc == 4) p.C == 2 ? launch<4, 4, true, 2>(a, s) : launch<4, 4, true, 1>(a, s);
+    else if (qc == 6 && vc == 4) p.C == 2 ? launch<6, 4, true, 2>(a, s) : launch<6, 4, true, 1>(a, s);
+    else if (qc <= 6 && vc <= 4) p.C == 2 ? launch<6, 4, false, 2>(a, s) : launch<6, 4, false, 1>(a, s);
+    else if (qc == 8 && vc == 8) launch<8, 8, true, 1>(a, s);
+    else launch<8, 8, false, 1>(a, s);
+    if (a.ps > 1)
+        hipLaunchKernelGGL(kv4_join_kernel, dim3((unsigned)(((long long)rows * heads + 3) / 4)), dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? MOE_OK : fail(MOE_EHIP, "4-bit attention kernel: %s", hipGetErrorString(e));
 }

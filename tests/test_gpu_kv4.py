@@ -339,6 +339,11 @@ def test_unseen_positions_do_not_matter(shape, bad):
     heads, n_kv, qd, vd = shape
     pool, table = filled(shape, 1, 100, 32)
     seq, pos = [0] * 30, list(range(50, 80))
+    # what lies beside the positions in question is larger than all else
+    for p in (27, 64, 67):
+        for kv in range(n_kv):
+            code = np.random.default_rng(p).integers(1, 16, vd).astype(np.uint8)
+            pool.put(int(table[0, p // 32]) * 32 + p % 32, kv, code, np.full(vd // 32, 3e4, np.float16), False)
     q = np.random.default_rng(1).standard_normal((30, heads * qd)).astype(np.float32)
     want = ref.attend(pool, table, q, seq, pos, heads, qd ** -0.5, 25)
     at = (0, 10, 25, 26, 65, 66, 79, 80, 99)

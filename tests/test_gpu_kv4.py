@@ -486,6 +486,34 @@ def test_select(shape, n_seq, mp, n_sel, sinks, recent):
         assert np.array_equal(lists.cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("n_seq,mp,n_sel", [(1, 5000, 20), (40, 700, 33), (9, 4097, 256)])
+def test_select_many_pages(n_seq, mp, n_sel):
+    """Scores through the workspace, and in LDS up to its end; few distinct
+    scores, so that the last one chosen is one of many equal ones."""
+    import torch
+
+    from moe_amd.paged import KvCache
+
+    heads, n_kv, d, page = 2, 2, 32, 32
+    g = torch.Generator(device="cuda").manual_seed(mp)
+    table = torch.randperm(n_seq * mp, generator=g, device="cuda").to(torch.int32).view(n_seq, mp)
+    means = torch.randint(-2, 3, (n_seq * mp, n_kv, 1), generator=g, device="cuda").half().expand(-1, -1, d).contiguous()
+    pool = torch.zeros(n_seq * mp * n_kv * 18 * 2 * d, dtype=torch.uint8, device="cuda")
+    cache = KvCache(pool, table, n_kv=n_kv, qd=d, vd=d, page=page, means=means)
+    q = torch.ones((n_seq, heads * d), device="cuda")
+    seq, pos = ints(range(n_seq)), ints([mp * page - 1 - 40 * i for i in range(n_seq)])
+    lists = torch.empty((n_seq, n_kv, n_sel), dtype=torch.int32, device="cuda")
+    cache.select(q, seq, pos, lists, max_pos=mp * page - 1, sinks=1, recent=2)
+    got = lists.cpu().numpy()
+    score = means[table.long()].double().sum(-1).cpu().numpy()  # [seq, page, kv]
+    for s in range(n_seq):
+        cur = int(pos[s]) // page
+        for kv in range(n_kv):
+            x = score[s, :cur + 1, kv].copy()
+            x[0] = x[cur - 1:] = np.inf
+            assert got[s, kv].tolist() == sorted(np.argsort(-x, kind="stable")[:n_sel].tolist())
+
+
 # ------------------------------------------- calls together, streams and graphs
 
 

@@ -69,17 +69,26 @@ def test_no_rows_are_no_work(lib, call):
         assert call(lib, kv4(), **{k: None}) == L.MOE_EINVAL
 
 
+LONG = dict(max_pages=2000, max_pos=100000)  # positions that go to several blocks
+
+
 @pytest.mark.parametrize("bad", [dict(heads=7), dict(heads=0), dict(heads=-2), dict(max_pos=-1), dict(max_pos=640),
-                                 dict(lists=P, n_sel=0), dict(lists=P, n_sel=-1)], ids=str)
+                                 dict(lists=P, n_sel=0), dict(lists=P, n_sel=-1), dict(ws=None, **LONG),
+                                 dict(ws=P + 8, **LONG), dict(ws_bytes=1000, **LONG)], ids=str)
 def test_attention_refuses(lib, bad):
-    assert attention(lib, kv4(), **bad) == L.MOE_EINVAL
+    bad = dict(bad)
+    assert attention(lib, kv4(max_pages=bad.pop("max_pages", 10)), **bad) == L.MOE_EINVAL
+
+
+MANY = dict(max_pages=9000, max_pos=64 * 8000)  # pages whose scores go through the workspace
 
 
 @pytest.mark.parametrize("bad", [dict(heads=7), dict(max_pos=-1), dict(max_pos=640), dict(sinks=-1), dict(recent=0),
                                  dict(sinks=3, recent=2), dict(sinks=2 ** 31 - 1, recent=2 ** 31 - 1), dict(n_sel=0),
-                                 dict(ws=None), dict(ws=P + 8), dict(ws_bytes=16)], ids=str)
+                                 dict(ws=None, **MANY), dict(ws=P + 8, **MANY), dict(ws_bytes=16, **MANY)], ids=str)
 def test_select_refuses(lib, bad):
-    assert select(lib, kv4(), **bad) == L.MOE_EINVAL
+    bad = dict(bad)
+    assert select(lib, kv4(max_pages=bad.pop("max_pages", 10)), **bad) == L.MOE_EINVAL
 
 
 def test_select_needs_means(lib):

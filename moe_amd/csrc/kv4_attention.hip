@@ -25,6 +25,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "gmem.h"
 #include "kv4.h"
@@ -56,27 +57,37 @@ struct Args {
 
 __device__ inline half2v as_h2(uint32_t v) { return __builtin_bit_cast(half2v, v); }
 
-// Eight codes minus 8 as f16 from one word: low nibbles of its bytes 0, 2, 1,
-// 3, then high ones.  A nibble becomes the low mantissa bits of 1024 (or, four
-// bits up, of 64); the subtraction is exact.
-__device__ inline half8 codes_lo_hi(uint32_t w) {
-    const uint32_t x = w >> 8;
-    const half2v a = as_h2((w & 0x000f000fu) | 0x64006400u), b = as_h2((x & 0x000f000fu) | 0x64006400u);
-    const half2v c = as_h2((w & 0x00f000f0u) | 0x54005400u), d = as_h2((x & 0x00f000f0u) | 0x54005400u);
-    const half2v k = {(_Float16)1032.0f, (_Float16)1032.0f}, m = {(_Float16)72.0f, (_Float16)72.0f};
-    const half2v r0 = a - k, r1 = b - k, r2 = c - m, r3 = d - m;
-    return half8{r0[0], r0[1], r1[0], r1[1], r2[0], r2[1], r3[0], r3[1]};
+// Constants the compiler may not fold: (w & mask) | one is then one
+// instruction (v_and_or_b32 takes no literal, and one scalar register).
+struct Nibbles {
+    uint32_t lo = 0x000f000fu, hi = 0x00f000f0u, lo1 = 0x64006400u, hi1 = 0x54005400u;
+    __device__ Nibbles() { asm("" : "+s"(lo), "+s"(hi), "+v"(lo1), "+v"(hi1)); }
+};
+
+// Codes minus 8 as f16 pairs, from the low or high nibbles of bytes 0 and 2: a
+// nibble becomes the low mantissa bits of 1024 (or, four bits up, of 64); the
+// subtraction is exact.
+__device__ inline half2v low_pair(uint32_t w, const Nibbles &n) {
+    return as_h2((w & n.lo) | n.lo1) - half2v{(_Float16)1032.0f, (_Float16)1032.0f};
 }
-// The low (high) nibbles of two words' bytes 0, 2, 1, 3.
-template <bool HIGH>
-__device__ inline half8 codes_of(uint32_t w0, uint32_t w1) {
-    const uint32_t mask = HIGH ? 0x00f000f0u : 0x000f000fu, one = HIGH ? 0x54005400u : 0x64006400u;
-    const _Float16 off = HIGH ? 72.0f : 1032.0f;
-    const half2v k = {off, off};
-    const half2v r0 = as_h2((w0 & mask) | one) - k, r1 = as_h2((w0 >> 8 & mask) | one) - k;
-    const half2v r2 = as_h2((w1 & mask) | one) - k, r3 = as_h2((w1 >> 8 & mask) | one) - k;
-    return half8{r0[0], r0[1], r1[0], r1[1], r2[0], r2[1], r3[0], r3[1]};
+__device__ inline half2v high_pair(uint32_t w, const Nibbles &n) {
+    return as_h2((w & n.hi) | n.hi1) - half2v{(_Float16)72.0f, (_Float16)72.0f};
 }
+__device__ inline half8 join8(half2v a, half2v b, half2v c, half2v d) {
+    return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// f16 operands of f32 multiply-adds are read as they lie in half a register
+// (v_fma_mix_f32), which the compiler chooses for fmaf of a widened f16; so a
+// product is written as a multiply-add of 0 and a difference as one of -1,
+// the -1 hidden from it.
+__device__ inline float minus_one() {
+    float m = -1.0f;
+    asm("" : "+s"(m));
+    return m;
+}
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+__device__ inline half2v pack_half(float a, float b) { return __builtin_convertvector((f32x2{a, b}), half2v); }
 
 // A tile's words of a lane.
 template <int QC, int VC>
@@ -114,6 +125,8 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
     __shared__ uint32_t ssc[W][T::NS * 64];
     __shared__ float sm_r[W][C * 16], sm_l[W][C * 16], sm_k[C * 16];
     const Kv4 &kc = a.c;
+    const Nibbles nib;
+    const float less = minus_one();
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
     const int nq = EX ? QC : kc.qd / 32, nv = EX ? VC : kc.vd / 32;
     // Kv heads next to each other go to the XCDs in turn, so that one head's
@@ -263,6 +276,51 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
             for (int b = 0; b < VC; b++) o[c][b][0] = o[c][b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
+        // O^T += the tile's values times the weights p.
+        auto second = [&](const T &x, const f32x4 (&p)[C][2], auto odd) {
+            const u32x4 *sc = (const u32x4 *)ssc[wave];
+            uint32_t keep[C][4];
+            if (odd) {
+#pragma unroll
+                for (int c = 0; c < C; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        keep[c][i] = (p[c][i >> 1][2 * i & 3] == 0.0f ? 0 : 0xffffu) |
+                                     (p[c][i >> 1][(2 * i & 3) + 1] == 0.0f ? 0 : 0xffff0000u);
+            }
+#pragma unroll
+            for (int b = 0; b < VC; b++) {
+                if (!EX && b >= nv) break;
+                const u32x4 ds = sc[(nq + b) * 4 + g];
+                const uint32_t w0 = x.v[2 * b], w1 = x.v[2 * b + 1];
+                const half8 v0 = join8(low_pair(w0, nib), low_pair(w0 >> 8, nib), low_pair(w1, nib), low_pair(w1 >> 8, nib));
+                const half8 v1 = join8(high_pair(w0, nib), high_pair(w0 >> 8, nib), high_pair(w1, nib), high_pair(w1 >> 8, nib));
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    // Weights times scales in the codes' order: bytes 0, 2, 1,
+                    // 3 of each half; both pieces.
+                    half2v ph[4], pl[4];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const half2v d0 = as_h2(odd ? ds[2 * h] & keep[c][2 * h] : ds[2 * h]);
+                        const half2v d1 = as_h2(odd ? ds[2 * h + 1] & keep[c][2 * h + 1] : ds[2 * h + 1]);
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float u = fmaf((float)d0[e], p[c][h][e], 0.0f), w = fmaf((float)d1[e], p[c][h][2 + e], 0.0f);
+                            const half2v z = pack_half(u, w);
+                            ph[2 * h + e] = z;
+                            pl[2 * h + e] = pack_half(fmaf((float)z[0], less, u), fmaf((float)z[1], less, w));
+                        }
+                    }
+                    const half8 h8 = join8(ph[0], ph[1], ph[2], ph[3]), l8 = join8(pl[0], pl[1], pl[2], pl[3]);
+                    o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, h8, o[c][b][0], 0, 0, 0);
+                    o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, h8, o[c][b][1], 0, 0, 0);
+                    o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, l8, o[c][b][0], 0, 0, 0);
+                    o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, l8, o[c][b][1], 0, 0, 0);
+                }
+                if (C > 1) __builtin_amdgcn_sched_barrier(0);
+            }
+        };
         auto step = [&](const T &x) {
             // Scales through LDS (the wave's own: in order, no barrier): every
             // lane reads its four positions of both halves, 16 bytes.
@@ -285,7 +343,9 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
             for (int b = 0; b < QC; b++) {
                 if (!EX && b >= nq) break;
                 const half8 d = __builtin_bit_cast(half8, sc[b * 4 + g]);
-                const half8 k0 = codes_lo_hi(x.k[2 * b]), k1 = codes_lo_hi(x.k[2 * b + 1]);
+                const uint32_t w0 = x.k[2 * b], w1 = x.k[2 * b + 1];
+                const half8 k0 = join8(low_pair(w0, nib), low_pair(w0 >> 8, nib), high_pair(w0, nib), high_pair(w0 >> 8, nib));
+                const half8 k1 = join8(low_pair(w1, nib), low_pair(w1 >> 8, nib), high_pair(w1, nib), high_pair(w1 >> 8, nib));
 #pragma unroll
                 for (int c = 0; c < C; c++) {
                     const half8 qh = C == 1 ? qr[2 * b] : __builtin_bit_cast(half8, sm[((c * QC + b) * 2) * 64 + lane]);
@@ -301,15 +361,12 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                         s[c][1][i] = fmaf((float)d[4 + i], t[i], s[c][1][i]);
                     }
                 }
+                if (C > 1) __builtin_amdgcn_sched_barrier(0);
             }
             // Positions a column does not see.
             bool some = false;
 #pragma unroll
-            for (int c = 0; c < C; c++) {
-                s[c][0] *= ck[c];
-                s[c][1] *= ck[c];
-                some |= cv[c] && (x.base < cl[c] || x.base + kTile - 1 > cp[c]);
-            }
+            for (int c = 0; c < C; c++) some |= cv[c] && (x.base < cl[c] || x.base + kTile - 1 > cp[c]);
             if (__any(some)) {
 #pragma unroll
                 for (int c = 0; c < C; c++)
@@ -324,14 +381,14 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
             bool move = false;
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                mx[c] = -INFINITY;
+                mx[c] = s[c][0][0];
 #pragma unroll
-                for (int i = 0; i < 8; i++) mx[c] = fmaxf(mx[c], s[c][i >> 2][i & 3]);
+                for (int i = 1; i < 8; i++) mx[c] = fmaxf(mx[c], s[c][i >> 2][i & 3]);
+                mx[c] *= ck[c];
                 move |= mx[c] > lim[c];
             }
-            const bool odd = __any(inf);
-            const bool grow = __any((int)(top >> 10) - 14 > E);  // not below 2^E
-            if (__any(move) || grow) {
+            const bool grow = (int)(top >> 10) - 14 > E;  // not below 2^E
+            if (__any(move || grow)) {
                 int ne = (int)(top >> 10) - 14;
 #pragma unroll
                 for (int w = 32; w >= 1; w >>= 1) ne = max(ne, __shfl_xor(ne, w, 64));
@@ -355,39 +412,14 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
             for (int c = 0; c < C; c++)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float p = __builtin_amdgcn_exp2f(s[c][i >> 2][i & 3] - ref[c]);
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[c][i >> 2][i & 3], ck[c], -ref[c]));
                     s[c][i >> 2][i & 3] = p;
                     l[c] += p;
                 }
-#pragma unroll
-            for (int b = 0; b < VC; b++) {
-                if (!EX && b >= nv) break;
-                const half8 d = __builtin_bit_cast(half8, sc[(nq + b) * 4 + g]);
-                const half8 v0 = codes_of<false>(x.v[2 * b], x.v[2 * b + 1]);
-                const half8 v1 = codes_of<true>(x.v[2 * b], x.v[2 * b + 1]);
-#pragma unroll
-                for (int c = 0; c < C; c++) {
-                    float w[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        // Order of the codes: bytes 0, 2, 1, 3 of each half.
-                        const int e = (i & 4) | (i & 1) << 1 | (i >> 1 & 1);
-                        const float p = s[c][e >> 2][e & 3];
-                        w[i] = p * (float)d[e];
-                        // A position of weight 0 may hold an infinity or a NaN.
-                        if (odd) w[i] = p == 0.0f ? 0.0f : w[i];
-                    }
-                    half8 ph, pl;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) ph[i] = (_Float16)w[i];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) pl[i] = (_Float16)(w[i] - (float)ph[i]);
-                    o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph, o[c][b][0], 0, 0, 0);
-                    o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph, o[c][b][1], 0, 0, 0);
-                    o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl, o[c][b][0], 0, 0, 0);
-                    o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl, o[c][b][1], 0, 0, 0);
-                }
-            }
+            // A position of weight 0 may hold an infinity or a NaN: such tiles
+            // read its scales as 0.
+            if (__builtin_expect(__any(inf), 0)) second(x, s, std::true_type{});
+            else second(x, s, std::false_type{});
         };
         T x, y;
         next(x);
@@ -472,34 +504,55 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
     }
 }
 
-// The parts of rows whose tiles several blocks shared, in part order: a
-// wavefront per (row, head).
-__global__ __launch_bounds__(256) void kv4_join_kernel(const Args a) {
-    const int lane = threadIdx.x & 63, vd = a.c.vd;
-    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= (int64_t)a.rows * a.heads) return;
-    const int row = (int)(at / a.heads), head = (int)(at % a.heads);
+// The parts of rows whose tiles several blocks shared: a block of T threads
+// per (row, head), each group of vd / 4 of them every so many-th part; the
+// groups' sums in order.
+template <int T>
+__global__ __launch_bounds__(T) void kv4_join_kernel(const Args a) {
+    __shared__ float w[256], red[2];
+    __shared__ f32x4 sums[T];
+    const int vd = a.c.vd, row = blockIdx.x / a.heads, head = blockIdx.x % a.heads, i = threadIdx.x;
     if (a.pos[row] < 0 || (unsigned)a.seq[row] >= (unsigned)a.c.n_seq) return;
-    const float *ml = a.part_ml + at * a.ps * 2, *part = a.part + at * a.ps * vd;
-    float rr = -INFINITY;
-    for (int p = lane; p < a.ps; p += 64) rr = fmaxf(rr, ml[2 * p]);
+    const float *ml = a.part_ml + (size_t)blockIdx.x * a.ps * 2, *part = a.part + (size_t)blockIdx.x * a.ps * vd;
+    if (i < 64) {
+        float ref[4], l = 0.0f, rr = -INFINITY;
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) rr = fmaxf(rr, __shfl_xor(rr, o, 64));
-    float l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int p = 0; p < a.ps; p++) {
-        const float ref = ml[2 * p];
-        if (ref == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(ref - rr);
-        l = fmaf(ml[2 * p + 1], f, l);
+        for (int k = 0; k < 4; k++) {
+            const int p = i + 64 * k;
+            ref[k] = p < a.ps ? ml[2 * p] : -INFINITY;
+            rr = fmaxf(rr, ref[k]);
+        }
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (lane + 64 * k < vd) acc[k] = fmaf(part[(size_t)p * vd + lane + 64 * k], f, acc[k]);
+        for (int o = 32; o >= 1; o >>= 1) rr = fmaxf(rr, __shfl_xor(rr, o, 64));
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int p = i + 64 * k;
+            if (p >= a.ps) continue;
+            const float f = ref[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref[k] - rr);
+            w[p] = f;
+            l += ref[k] == -INFINITY ? 0.0f : ml[2 * p + 1] * f;
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o, 64);
+        if (i == 0) red[0] = l == 0.0f ? 0.0f : 1.0f / l;
     }
-    const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    float *dst = a.out + (int64_t)row * a.out_stride + (int64_t)head * vd;
+    __syncthreads();
+    const int n = vd / 4, groups = T / n, g = i / n, at = i % n;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (g < groups)
+        for (int p = g; p < a.ps; p += groups) {
+            const f32x4 x = gload((const f32x4 *)(part + (size_t)p * vd) + at);
+            const float f = w[p];
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-        if (lane + 64 * k < vd) dst[lane + 64 * k] = acc[k] * f;
+            for (int k = 0; k < 4; k++) acc[k] = f == 0.0f ? acc[k] : fmaf(x[k], f, acc[k]);
+        }
+    sums[i] = acc;
+    __syncthreads();
+    if (i >= n) return;
+    for (int k = 1; k < groups; k++) acc += sums[k * n + i];
+    float *dst = a.out + (int64_t)row * a.out_stride + (int64_t)head * vd + 4 * i;
+#pragma unroll
+    for (int k = 0; k < 4; k++) dst[k] = acc[k] * red[0];
 }
 
 // How a call is cut up: see Args.
@@ -590,8 +643,8 @@ int moe_kv4_attention(const moe_kv4 *c, const float *q, int64_t q_stride, int32_
     else if (qc <= 6 && vc <= 4) p.C == 2 ? launch<6, 4, false, 2>(a, s) : launch<6, 4, false, 1>(a, s);
     else if (qc == 8 && vc == 8) launch<8, 8, true, 1>(a, s);
     else launch<8, 8, false, 1>(a, s);
-    if (a.ps > 1)
-        hipLaunchKernelGGL(kv4_join_kernel, dim3((unsigned)(((long long)rows * heads + 3) / 4)), dim3(256), 0, s, a);
+    if (a.ps > 16) hipLaunchKernelGGL((kv4_join_kernel<256>), dim3((unsigned)rows * heads), dim3(256), 0, s, a);
+    else if (a.ps > 1) hipLaunchKernelGGL((kv4_join_kernel<64>), dim3((unsigned)rows * heads), dim3(64), 0, s, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? MOE_OK : fail(MOE_EHIP, "4-bit attention kernel: %s", hipGetErrorString(e));
 }

@@ -98,17 +98,25 @@ struct Tile {
     int ok;    // whether there is such a tile
 };
 
+// Loads of a tile go through a buffer descriptor: its base is the wave's, in
+// scalar registers, and a lane's offset the same for every tile, so that a
+// tile's loads need no vector address (temporaries of which made the loop wait
+// for loads in flight).  Reads past `bytes` give 0.
+__device__ inline __amdgpu_buffer_rsrc_t buffer_of(const uint8_t *p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p), 0, bytes, 0x00020000);
+}
+
 template <int NB, bool EX>
-__device__ inline void load_words(uint32_t (&w)[2 * NB], const uint8_t *p, int nb, int lane) {
+__device__ inline void load_words(uint32_t (&w)[2 * NB], __amdgpu_buffer_rsrc_t buf, int at, int nb, int lane) {
 #pragma unroll
     for (int c = 0; c < (NB + 1) / 2; c++) {
         if (EX ? 2 * c + 2 <= NB : 2 * c + 2 <= nb) {
-            const u32x4 x = gload((const u32x4 *)(p + 1024 * c + 16 * lane));
+            const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(buf, 16 * lane, at + 1024 * c, 0);
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 if (4 * c + i < 2 * NB) w[4 * c + i] = x[i];
         } else if (EX || 2 * c < nb) {
-            const u32x2 x = gload((const u32x2 *)(p + 1024 * c + 8 * lane));
+            const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(buf, 8 * lane, at + 1024 * c, 0);
             w[4 * c] = x[0], w[4 * c + 1] = x[1];
         }
     }
@@ -127,7 +135,8 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
     const Kv4 &kc = a.c;
     const Nibbles nib;
     const float less = minus_one();
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g = lane >> 4;
     const int nq = EX ? QC : kc.qd / 32, nv = EX ? VC : kc.vd / 32;
     // Kv heads next to each other go to the XCDs in turn, so that one head's
     // blocks find its tiles in their L2.  Later rows of a prompt see more
@@ -230,10 +239,13 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
         const int32_t *list = a.lists ? a.lists + ((size_t)(r0 + first) * kc.n_kv + kv) * a.n_sel : nullptr;
         const int32_t *table = kc.table + (size_t)sq * kc.max_pages;
         int b0 = -64, my_page = 0, my_id = -1;  // pages b0 .. b0 + 63 of the run, one a lane
-        // The next tile that there is; its words' loads are queued.
-        auto next = [&](T &x) {
+        const uint8_t *at = kc.pool;
+        // Queue the loads of tile v.  Control and addresses are the wave's, and
+        // the loads unconditional (where there is no such tile, those of the one
+        // before again), so that waiting for one tile leaves the next in flight.
+        auto load = [&](T &x) {
             x.ok = 0;
-            for (; v < v1; v++) {
+            if (v < v1) {
                 const int t = t0 + v, i = t >> tshift;
                 if (i >= b0 + 64 || i < b0) {
                     b0 = i;
@@ -247,23 +259,23 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                     }
                     there = there && my_page >= 0 && my_page < kc.max_pages;
                     my_id = there ? gload(table + my_page) : -1;
+                    asm volatile("" : "+v"(my_id), "+v"(my_page));  // waited for here, not at every tile
                 }
                 const int pid = __builtin_amdgcn_readlane(my_id, i - b0);
-                if ((unsigned)pid >= (unsigned)kc.n_pages) continue;
                 const int in = t & ((1 << tshift) - 1);
-                const int base = (__builtin_amdgcn_readlane(my_page, i - b0) << kc.page_shift) + in * kTile;
-                if (base > hi || base + kTile <= lo) continue;
-                x.base = base, x.ok = 1;
-                const uint8_t *p = kc.head(pid, kv) + (size_t)in * kc.tile_bytes;
-                load_words<QC, EX>(x.k, p, nq, lane);
-                load_words<VC, EX>(x.v, p + kc.v_codes(), nv, lane);
-                const int ns = (nq + nv) * 16;
-#pragma unroll
-                for (int e = 0; e < T::NS; e++)
-                    x.s[e] = gload((const uint32_t *)(p + kc.k_scales()) + min(lane + 64 * e, ns - 1));
-                v++;
-                return;
+                x.base = (__builtin_amdgcn_readlane(my_page, i - b0) << kc.page_shift) + in * kTile;
+                if ((unsigned)pid < (unsigned)kc.n_pages && x.base <= hi && x.base + kTile > lo) {
+                    x.ok = 1;
+                    at = kc.head(pid, kv) + (size_t)in * kc.tile_bytes;
+                }
             }
+            v++;
+            const __amdgpu_buffer_rsrc_t buf = buffer_of(at, kc.tile_bytes);
+#pragma unroll
+            for (int e = 0; e < T::NS; e++)
+                x.s[e] = __builtin_amdgcn_raw_buffer_load_b32(buf, 4 * lane, kc.k_scales() + 256 * e, 0);
+            load_words<QC, EX>(x.k, buf, 0, nq, lane);
+            load_words<VC, EX>(x.v, buf, kc.v_codes(), nv, lane);
         };
 
         f32x4 o[C][VC][2];
@@ -421,14 +433,17 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
             if (__builtin_expect(__any(inf), 0)) second(x, s, std::true_type{});
             else second(x, s, std::false_type{});
         };
-        T x, y;
-        next(x);
-        while (x.ok) {
-            next(y);
-            step(x);
-            if (!y.ok) break;
-            next(x);
-            step(y);
+        if (v < v1) {
+            T x, y;
+            load(x);
+            while (true) {
+                load(y);
+                if (x.ok) step(x);
+                if (v > v1) break;
+                load(x);
+                if (y.ok) step(y);
+                if (v > v1) break;
+            }
         }
 
         // Merge the waves: everyone to the block's largest reference, then sums

@@ -36,6 +36,7 @@ int fail(int code, const char *fmt, ...);
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_dw __attribute__((ext_vector_type(4), aligned(4)));  // at any float
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
@@ -125,11 +126,10 @@ __device__ inline void load_words(uint32_t (&w)[2 * NB], __amdgpu_buffer_rsrc_t 
 // QC, VC: blocks of a key and a value (EX) or the most there may be.  C:
 // 16-column tiles.  W: waves.
 template <int QC, int VC, bool EX, int C, int W>
-__global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) {
+__global__ __launch_bounds__(W * 64, QC + VC <= 8 && C == 1 ? 3 : 2) void kv4_attention_kernel(const Args a) {
     typedef Tile<QC, VC> T;
-    constexpr int kQ = C * QC * 2 * 64;  // Q operands: [column tile][block][hi, lo][lane] of 16 bytes
-    constexpr int kMerge = W / 2 * C * VC * 2 * 64;
-    __shared__ u32x4 sm[kQ > kMerge ? kQ : kMerge];
+    __shared__ u32x4 sq_[C * QC * 2 * 64];  // Q operands: [column tile][block][hi, lo][lane]
+    __shared__ f32x4 smo[W * VC * 2 * 64];  // O of the waves: [wave][block][half][lane]
     __shared__ uint32_t ssc[W][T::NS * 64];
     __shared__ float sm_r[W][C * 16], sm_l[W][C * 16], sm_k[C * 16];
     const Kv4 &kc = a.c;
@@ -154,6 +154,32 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
     const int nr = min(a.tt, a.rows - r0);
     const int h0 = kv * a.rep + chunk * a.rc, hn = min(a.rc, a.rep - chunk * a.rc);
     const int my_seq = gload(a.seq + r0 + min(lane, nr - 1)), my_pos = gload(a.pos + r0 + min(lane, nr - 1));
+
+    // Column cc of the block is query head h0 + cc % hn of row r0 + cc / hn,
+    // whatever run it is in: queries load while sequences and tables do.  16
+    // threads a column, four values each at a time.
+    constexpr int kPer = (QC + 1) / 2, kCols = (C * 16 + W * 4 - 1) / (W * 4);
+    f32x4 qv[kCols][kPer];
+    const int qi = threadIdx.x & 15;
+#pragma unroll
+    for (int k = 0; k < kCols; k++) {
+        const int cc = min((int)(threadIdx.x >> 4) + k * W * 4, nr * hn - 1);
+        const float *row = a.q + (size_t)(r0 + cc / hn) * a.q_stride + (size_t)(h0 + cc % hn) * kc.qd;
+#pragma unroll
+        for (int j = 0; j < kPer; j++) {
+            const int d = min(4 * qi + 64 * j, kc.qd - 4);
+            qv[k][j] = __builtin_bit_cast(f32x4, gload_x4((const uint32_t *)(row + d)));
+        }
+    }
+    int crow[C];
+    bool there[C];
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        const int cc = c * 16 + col;
+        there[c] = cc < nr * hn;
+        crow[c] = there[c] ? cc / hn : 0;
+    }
+
     const bool valid = lane < nr && my_pos >= 0 && (unsigned)my_seq < (unsigned)kc.n_seq;
     const int before = __shfl_up(my_seq, 1, 64);
     const bool before_ok = __shfl_up((int)valid, 1, 64);
@@ -161,6 +187,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
     const unsigned long long cuts = __ballot(!valid || lane == 0 || my_seq != before || !before_ok);
     unsigned long long starts = cuts & __ballot(valid);
     const int tshift = kc.page_shift - 5;
+    bool staged = false;
 
     for (int run = 0; starts; run++) {
         const int first = __builtin_ctzll(starts);
@@ -168,7 +195,6 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
         if (run % a.split != sub) continue;
         const unsigned long long after = first < 63 ? cuts >> (first + 1) : 0;
         const int end = min(nr, after ? first + 1 + __builtin_ctzll(after) : 64);
-        const int ncol = (end - first) * hn;
         const bool mine = lane >= first && lane < end;
         int hi = mine ? my_pos : -1;
         int lo = mine ? (a.window > 0 ? max(0, my_pos + 1 - a.window) : 0) : 0x7fffffff;
@@ -179,55 +205,15 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
         }
         hi = __builtin_amdgcn_readfirstlane(hi);
         lo = __builtin_amdgcn_readfirstlane(lo);
-        const int sq = __builtin_amdgcn_readfirstlane(__shfl(my_seq, first, 64));
+        const int sq = __builtin_amdgcn_readlane(my_seq, first);
+        // The run's columns, and what each sees.
         int cp[C], cl[C];
         bool cv[C];
 #pragma unroll
         for (int c = 0; c < C; c++) {
-            const int cc = c * 16 + col;
-            cv[c] = cc < ncol;
-            const int p = __shfl(my_pos, first + (cv[c] ? cc / hn : 0), 64);
-            cp[c] = p;
-            cl[c] = a.window > 0 ? max(0, p + 1 - a.window) : 0;
-        }
-
-        // Q: a column's values times scale log2(e), by a power of two that
-        // brings its largest into [2^14, 2^15), in two f16 pieces.  16 threads a
-        // column, twice over its values.
-        __syncthreads();  // the previous run's reads of sm
-        for (int cc = threadIdx.x >> 4; cc < C * 16; cc += W * 4) {
-            const float *row = a.q + (size_t)(r0 + first + min(cc, ncol - 1) / hn) * a.q_stride +
-                               (size_t)(h0 + min(cc, ncol - 1) % hn) * kc.qd;
-            const float f = cc < ncol ? a.scale * 1.44269504f : 0.0f;
-            const int i = threadIdx.x & 15;
-            float top = 0.0f;
-            for (int d = i; d < kc.qd; d += 16) top = fmaxf(top, fabsf(gload(row + d) * f));
-#pragma unroll
-            for (int o = 8; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-            // 2^(14 - exponent of top), within what both it and its inverse can be.
-            const int k = min(max(127 + 14 - ((int)(__float_as_uint(top) >> 23) - 127), 1), 253);
-            const float up = __uint_as_float((uint32_t)k << 23);
-            if (i == 0) sm_k[cc] = __uint_as_float((uint32_t)(254 - k) << 23);
-            _Float16 *dst = (_Float16 *)sm;
-            for (int d = i; d < kc.qd; d += 16) {
-                const float v = gload(row + d) * f * up;
-                const _Float16 hv = (_Float16)v;
-                // Dim 32 s + 16 h + 4 g + e is element 4 h + {0, 2, 1, 3}[e] of lane (g, column).
-                const int s = d >> 5, e = d & 3, gg = (d >> 2) & 3, el = (d >> 4 & 1) * 4 + (e >> 1) + (e & 1) * 2;
-                const int at = (((cc >> 4) * QC + s) * 2 * 64 + gg * 16 + (cc & 15)) * 8 + el;
-                dst[at] = hv;
-                dst[at + 64 * 8] = (_Float16)(v - (float)hv);
-            }
-        }
-        __syncthreads();
-        float ck[C];
-#pragma unroll
-        for (int c = 0; c < C; c++) ck[c] = sm_k[c * 16 + col];
-        half8 qr[C == 1 ? QC * 2 : 1];
-        if (C == 1) {
-#pragma unroll
-            for (int i = 0; i < QC * 2; i++)
-                if (EX || i < 2 * nq) qr[i] = __builtin_bit_cast(half8, sm[i * 64 + lane]);
+            cv[c] = there[c] && crow[c] >= first && crow[c] < end;
+            cp[c] = __shfl(my_pos, crow[c], 64);
+            cl[c] = a.window > 0 ? max(0, cp[c] + 1 - a.window) : 0;
         }
 
         // This wave's tiles: v0 .. v1 - 1 of the run's (of the lists' pages).
@@ -277,6 +263,48 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
             load_words<QC, EX>(x.k, buf, 0, nq, lane);
             load_words<VC, EX>(x.v, buf, kc.v_codes(), nv, lane);
         };
+        T x, y;
+        const bool any = v < v1;
+        if (any) load(x);
+
+        // Q into LDS, once: a column's values times scale log2(e), by a power of
+        // two that brings its largest into [2^14, 2^15), in two f16 pieces.
+        if (!staged) {
+            staged = true;
+            const float f = a.scale * 1.44269504f;
+#pragma unroll
+            for (int k = 0; k < kCols; k++) {
+                const int cc = (threadIdx.x >> 4) + k * W * 4;
+                float top = 0.0f;
+#pragma unroll
+                for (int j = 0; j < kPer; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) qv[k][j][e] *= f, top = fmaxf(top, fabsf(qv[k][j][e]));
+#pragma unroll
+                for (int o = 8; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+                // 2^(14 - exponent of top), within what both it and its inverse can be.
+                const int ex = min(max(127 + 14 - ((int)(__float_as_uint(top) >> 23) - 127), 1), 253);
+                const float up = __uint_as_float((uint32_t)ex << 23);
+                if (qi == 0) sm_k[cc] = __uint_as_float((uint32_t)(254 - ex) << 23);
+#pragma unroll
+                for (int j = 0; j < kPer; j++) {
+                    const int d = 4 * qi + 64 * j;
+                    if (d >= kc.qd) continue;
+                    // Dims 32 s + 16 h + 4 g + 0, 2, 1, 3 are elements 4 h.. of lane (g, column).
+                    const f32x4 z = qv[k][j] * up;
+                    const half2v h0 = pack_half(z[0], z[2]), h1 = pack_half(z[1], z[3]);
+                    const half2v l0 = pack_half(z[0] - (float)h0[0], z[2] - (float)h0[1]);
+                    const half2v l1 = pack_half(z[1] - (float)h1[0], z[3] - (float)h1[1]);
+                    u32x2 *dst = (u32x2 *)(sq_ + ((cc >> 4) * QC + (d >> 5)) * 2 * 64 + (d >> 2 & 3) * 16 + (cc & 15)) + (d >> 4 & 1);
+                    dst[0] = u32x2{__builtin_bit_cast(uint32_t, h0), __builtin_bit_cast(uint32_t, h1)};
+                    dst[128] = u32x2{__builtin_bit_cast(uint32_t, l0), __builtin_bit_cast(uint32_t, l1)};
+                }
+            }
+            __syncthreads();
+        }
+        float ck[C];
+#pragma unroll
+        for (int c = 0; c < C; c++) ck[c] = sm_k[c * 16 + col];
 
         f32x4 o[C][VC][2];
         float ref[C], lim[C], l[C];
@@ -302,7 +330,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
             }
 #pragma unroll
             for (int b = 0; b < VC; b++) {
-                if (!EX && b >= nv) break;
+                if (!EX && b >= nv) continue;
                 const u32x4 ds = sc[(nq + b) * 4 + g];
                 const uint32_t w0 = x.v[2 * b], w1 = x.v[2 * b + 1];
                 const half8 v0 = join8(low_pair(w0, nib), low_pair(w0 >> 8, nib), low_pair(w1, nib), low_pair(w1 >> 8, nib));
@@ -353,15 +381,15 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
             for (int c = 0; c < C; c++) s[c][0] = s[c][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int b = 0; b < QC; b++) {
-                if (!EX && b >= nq) break;
+                if (!EX && b >= nq) continue;
                 const half8 d = __builtin_bit_cast(half8, sc[b * 4 + g]);
                 const uint32_t w0 = x.k[2 * b], w1 = x.k[2 * b + 1];
                 const half8 k0 = join8(low_pair(w0, nib), low_pair(w0 >> 8, nib), high_pair(w0, nib), high_pair(w0 >> 8, nib));
                 const half8 k1 = join8(low_pair(w1, nib), low_pair(w1 >> 8, nib), high_pair(w1, nib), high_pair(w1 >> 8, nib));
 #pragma unroll
                 for (int c = 0; c < C; c++) {
-                    const half8 qh = C == 1 ? qr[2 * b] : __builtin_bit_cast(half8, sm[((c * QC + b) * 2) * 64 + lane]);
-                    const half8 ql = C == 1 ? qr[2 * b + 1] : __builtin_bit_cast(half8, sm[((c * QC + b) * 2 + 1) * 64 + lane]);
+                    const half8 qh = __builtin_bit_cast(half8, sq_[((c * QC + b) * 2) * 64 + lane]);
+                    const half8 ql = __builtin_bit_cast(half8, sq_[((c * QC + b) * 2 + 1) * 64 + lane]);
                     const f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
                     f32x4 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql, z, 0, 0, 0);
                     f32x4 t = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql, z, 0, 0, 0);
@@ -433,9 +461,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
             if (__builtin_expect(__any(inf), 0)) second(x, s, std::true_type{});
             else second(x, s, std::false_type{});
         };
-        if (v < v1) {
-            T x, y;
-            load(x);
+        if (any) {
             while (true) {
                 load(y);
                 if (x.ok) step(x);
@@ -446,9 +472,9 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
             }
         }
 
-        // Merge the waves: everyone to the block's largest reference, then sums
-        // by halves.
-        __syncthreads();  // reads of Q
+        // Merge the waves, a column tile at a time: sums as they are and their
+        // references through LDS, then every wave takes a share of the output's
+        // dims and brings the parts to the largest reference.
 #pragma unroll
         for (int c = 0; c < C; c++) {
             l[c] += __shfl_xor(l[c], 16, 64);
@@ -456,65 +482,47 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
             if (lim[c] == -INFINITY && l[c] == 0.0f) ref[c] = -INFINITY;  // saw nothing
             if (g == 0) sm_r[wave][c * 16 + col] = ref[c], sm_l[wave][c * 16 + col] = l[c];
         }
-        __syncthreads();
 #pragma unroll
         for (int c = 0; c < C; c++) {
-            float rr = -INFINITY, ll = 0.0f;
+#pragma unroll
+            for (int b = 0; b < VC * 2; b++) smo[(wave * VC * 2 + b) * 64 + lane] = o[c][b >> 1][b & 1];
+            __syncthreads();
+            float rr = -INFINITY, ll = 0.0f, fw[W];
+#pragma unroll
             for (int w = 0; w < W; w++) rr = fmaxf(rr, sm_r[w][c * 16 + col]);
+#pragma unroll
             for (int w = 0; w < W; w++) {
                 const float rw = sm_r[w][c * 16 + col];
-                if (rw != -INFINITY) ll += sm_l[w][c * 16 + col] * __builtin_amdgcn_exp2f(rw - rr);
+                fw[w] = rw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(rw - rr);
+                ll += rw == -INFINITY ? 0.0f : sm_l[w][c * 16 + col] * fw[w];
             }
-            const float f = ref[c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref[c] - rr);
-            l[c] = ll, ref[c] = rr;
+            if (cv[c]) {
+                const size_t row = r0 + crow[c], head = h0 + (c * 16 + col) % hn;
+                float *dst = a.out + row * a.out_stride + head * kc.vd;
+                float f = ll == 0.0f ? 0.0f : 1.0f / ll;
+                if (a.ps > 1) {
+                    const size_t where = (row * a.heads + head) * a.ps + part;
+                    dst = a.part + where * kc.vd;
+                    if (g == 0 && wave == 0) a.part_ml[2 * where] = rr, a.part_ml[2 * where + 1] = ll;
+                    f = 1.0f;
+                }
+                // Lane (column, g) of [block][half] holds dims 32 b + 16 h + 4 g + i.
 #pragma unroll
-            for (int b = 0; b < VC; b++) o[c][b][0] *= f, o[c][b][1] *= f;
-        }
-        f32x4 *mrg = (f32x4 *)sm;
+                for (int bh = 0; bh < VC * 2; bh += W) {
+                    if (bh + wave >= nv * 2) continue;
+                    f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int h = W / 2; h >= 1; h /= 2) {
-            if (wave >= h && wave < 2 * h) {
+                    for (int w = 0; w < W; w++) {
+                        const f32x4 ow = smo[(w * VC * 2 + bh + wave) * 64 + lane];
 #pragma unroll
-                for (int c = 0; c < C; c++)
+                        for (int i = 0; i < 4; i++) z[i] = fw[w] == 0.0f ? z[i] : fmaf(ow[i], fw[w], z[i]);
+                    }
 #pragma unroll
-                    for (int b = 0; b < VC * 2; b++)
-                        mrg[(((wave - h) * C + c) * VC * 2 + b) * 64 + lane] = o[c][b >> 1][b & 1];
-            }
-            __syncthreads();
-            if (wave < h) {
-#pragma unroll
-                for (int c = 0; c < C; c++)
-#pragma unroll
-                    for (int b = 0; b < VC * 2; b++)
-                        o[c][b >> 1][b & 1] += mrg[((wave * C + c) * VC * 2 + b) * 64 + lane];
-            }
-            __syncthreads();
-        }
-        if (wave != 0) continue;
-#pragma unroll
-        for (int c = 0; c < C; c++) {
-            if (!cv[c]) continue;
-            const int cc = c * 16 + col;
-            const size_t row = r0 + first + cc / hn, head = h0 + cc % hn;
-            float *dst = a.out + row * a.out_stride + head * kc.vd;
-            float f = l[c] == 0.0f ? 0.0f : 1.0f / l[c];
-            if (a.ps > 1) {
-                const size_t at = (row * a.heads + head) * a.ps + part;
-                dst = a.part + at * kc.vd;
-                if (g == 0) a.part_ml[2 * at] = ref[c], a.part_ml[2 * at + 1] = l[c];
-                f = 1.0f;
-            }
-            // Lane (column, g) holds dims 32 b + 16 h + 4 g + i.
-#pragma unroll
-            for (int b = 0; b < VC; b++) {
-                if (!EX && b >= nv) break;
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    f32x4 z = o[c][b][h];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) gstore(dst + 32 * b + 16 * h + 4 * g + i, z[i] * f);
+                    for (int i = 0; i < 4; i++) z[i] *= f;
+                    gstore((f32x4_dw *)(dst + 16 * (bh + wave) + 4 * g), __builtin_bit_cast(f32x4_dw, z));
                 }
             }
+            __syncthreads();
         }
     }
 }

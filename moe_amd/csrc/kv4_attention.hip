@@ -126,7 +126,7 @@ __device__ inline void load_words(uint32_t (&w)[2 * NB], __amdgpu_buffer_rsrc_t 
 // QC, VC: blocks of a key and a value (EX) or the most there may be.  C:
 // 16-column tiles.  W: waves.
 template <int QC, int VC, bool EX, int C, int W>
-__global__ __launch_bounds__(W * 64, QC + VC <= 8 && C == 1 ? 3 : 2) void kv4_attention_kernel(const Args a) {
+__global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) {
     typedef Tile<QC, VC> T;
     __shared__ u32x4 sq_[C * QC * 2 * 64];  // Q operands: [column tile][block][hi, lo][lane]
     __shared__ f32x4 smo[W * VC * 2 * 64];  // O of the waves: [wave][block][half][lane]
@@ -171,15 +171,6 @@ __global__ __launch_bounds__(W * 64, QC + VC <= 8 && C == 1 ? 3 : 2) void kv4_at
             qv[k][j] = __builtin_bit_cast(f32x4, gload_x4((const uint32_t *)(row + d)));
         }
     }
-    int crow[C];
-    bool there[C];
-#pragma unroll
-    for (int c = 0; c < C; c++) {
-        const int cc = c * 16 + col;
-        there[c] = cc < nr * hn;
-        crow[c] = there[c] ? cc / hn : 0;
-    }
-
     const bool valid = lane < nr && my_pos >= 0 && (unsigned)my_seq < (unsigned)kc.n_seq;
     const int before = __shfl_up(my_seq, 1, 64);
     const bool before_ok = __shfl_up((int)valid, 1, 64);
@@ -206,15 +197,22 @@ __global__ __launch_bounds__(W * 64, QC + VC <= 8 && C == 1 ? 3 : 2) void kv4_at
         hi = __builtin_amdgcn_readfirstlane(hi);
         lo = __builtin_amdgcn_readfirstlane(lo);
         const int sq = __builtin_amdgcn_readlane(my_seq, first);
-        // The run's columns, and what each sees.
-        int cp[C], cl[C];
+        // The run's columns, and what each sees.  A run of few columns has them
+        // several times over, one copy for each block of a value: see `second`.
+        const int c0 = first * hn, ncol = end * hn - c0;
+        const int wide = ncol > 1 ? 32 - __builtin_clz(ncol - 1) : 0;  // log2 of the columns' room
+        const bool copies = C == 1 && nv << wide <= 16;
+        int cc[C], cp[C], cl[C];
         bool cv[C];
 #pragma unroll
         for (int c = 0; c < C; c++) {
-            cv[c] = there[c] && crow[c] >= first && crow[c] < end;
-            cp[c] = __shfl(my_pos, crow[c], 64);
+            const int x = copies ? col & ((1 << wide) - 1) : c * 16 + col - c0;
+            cv[c] = x >= 0 && x < ncol;
+            cc[c] = c0 + (cv[c] ? x : 0);
+            cp[c] = __shfl(my_pos, cc[c] / hn, 64);
             cl[c] = a.window > 0 ? max(0, cp[c] + 1 - a.window) : 0;
         }
+        const int copy = copies ? min(col >> wide, nv - 1) : 0;
 
         // This wave's tiles: v0 .. v1 - 1 of the run's (of the lists' pages).
         const int t0 = a.lists ? 0 : lo >> 5;
@@ -224,44 +222,62 @@ __global__ __launch_bounds__(W * 64, QC + VC <= 8 && C == 1 ? 3 : 2) void kv4_at
         const int v1 = (int)((long long)nt * (me + 1) / parts);
         const int32_t *list = a.lists ? a.lists + ((size_t)(r0 + first) * kc.n_kv + kv) * a.n_sel : nullptr;
         const int32_t *table = kc.table + (size_t)sq * kc.max_pages;
-        int b0 = -64, my_page = 0, my_id = -1;  // pages b0 .. b0 + 63 of the run, one a lane
+        // Pages b0 .. b0 + 63 of the run, one a lane: first position (-1: no
+        // such page) and where the kv head's tiles are.
+        int b0 = -64, my_base = -1;
+        uint32_t my_at[2] = {0, 0};
         const uint8_t *at = kc.pool;
-        // Queue the loads of tile v.  Control and addresses are the wave's, and
-        // the loads unconditional (where there is no such tile, those of the one
-        // before again), so that waiting for one tile leaves the next in flight.
-        auto load = [&](T &x) {
+        // Find tile v, and queue its loads.  Control and addresses are the wave's,
+        // and the loads unconditional (where there is no such tile, those of the
+        // one before again), so that waiting for one tile leaves the next in
+        // flight.
+        auto find = [&](T &x) __attribute__((always_inline)) {
             x.ok = 0;
             if (v < v1) {
                 const int t = t0 + v, i = t >> tshift;
                 if (i >= b0 + 64 || i < b0) {
                     b0 = i;
                     const int j = b0 + lane;
-                    my_page = j;
+                    int page = j;
                     bool there = true;
                     if (list) {
-                        my_page = j < a.n_sel ? gload(list + j) : -1;
+                        page = j < a.n_sel ? gload(list + j) : -1;
                         const int prev = j > 0 && j <= a.n_sel ? gload(list + j - 1) : -1;
-                        there = my_page > prev;
+                        there = page > prev;
                     }
-                    there = there && my_page >= 0 && my_page < kc.max_pages;
-                    my_id = there ? gload(table + my_page) : -1;
-                    asm volatile("" : "+v"(my_id), "+v"(my_page));  // waited for here, not at every tile
+                    there = there && page >= 0 && page < kc.max_pages;
+                    const int pid = there ? gload(table + page) : -1;
+                    there = (unsigned)pid < (unsigned)kc.n_pages;
+                    my_base = there ? page << kc.page_shift : -1;
+                    const uint64_t p = (uint64_t)kc.head(there ? pid : 0, kv);
+                    my_at[0] = (uint32_t)p, my_at[1] = (uint32_t)(p >> 32);
+                    asm volatile("" : "+v"(my_base), "+v"(my_at[0]), "+v"(my_at[1]));  // waited for here, not at every tile
                 }
-                const int pid = __builtin_amdgcn_readlane(my_id, i - b0);
-                const int in = t & ((1 << tshift) - 1);
-                x.base = (__builtin_amdgcn_readlane(my_page, i - b0) << kc.page_shift) + in * kTile;
-                if ((unsigned)pid < (unsigned)kc.n_pages && x.base <= hi && x.base + kTile > lo) {
+                const int in = t & ((1 << tshift) - 1), page = __builtin_amdgcn_readlane(my_base, i - b0);
+                x.base = page + in * kTile;
+                if (page >= 0 && x.base <= hi && x.base + kTile > lo) {
                     x.ok = 1;
-                    at = kc.head(pid, kv) + (size_t)in * kc.tile_bytes;
+                    const uint64_t p = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(my_at[1], i - b0) << 32 |
+                                       (uint32_t)__builtin_amdgcn_readlane(my_at[0], i - b0);
+                    at = (const uint8_t *)p + (uint32_t)(in * kc.tile_bytes);
                 }
             }
             v++;
+        };
+        auto load_keys = [&](T &x) __attribute__((always_inline)) {
             const __amdgpu_buffer_rsrc_t buf = buffer_of(at, kc.tile_bytes);
 #pragma unroll
             for (int e = 0; e < T::NS; e++)
                 x.s[e] = __builtin_amdgcn_raw_buffer_load_b32(buf, 4 * lane, kc.k_scales() + 256 * e, 0);
             load_words<QC, EX>(x.k, buf, 0, nq, lane);
-            load_words<VC, EX>(x.v, buf, kc.v_codes(), nv, lane);
+        };
+        auto load_values = [&](T &x) __attribute__((always_inline)) {
+            load_words<VC, EX>(x.v, buffer_of(at, kc.tile_bytes), kc.v_codes(), nv, lane);
+        };
+        auto load = [&](T &x) __attribute__((always_inline)) {
+            find(x);
+            load_keys(x);
+            load_values(x);
         };
         T x, y;
         const bool any = v < v1;
@@ -304,7 +320,8 @@ __global__ __launch_bounds__(W * 64, QC + VC <= 8 && C == 1 ? 3 : 2) void kv4_at
         }
         float ck[C];
 #pragma unroll
-        for (int c = 0; c < C; c++) ck[c] = sm_k[c * 16 + col];
+        for (int c = 0; c < C; c++) ck[c] = sm_k[C == 1 ? cc[0] : c * 16 + col];
+        const int ql_at = C == 1 ? g * 16 + cc[0] : lane;
 
         f32x4 o[C][VC][2];
         float ref[C], lim[C], l[C];
@@ -316,11 +333,21 @@ __global__ __launch_bounds__(W * 64, QC + VC <= 8 && C == 1 ? 3 : 2) void kv4_at
             for (int b = 0; b < VC; b++) o[c][b][0] = o[c][b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
-        // O^T += the tile's values times the weights p.
-        auto second = [&](const T &x, const f32x4 (&p)[C][2], auto odd) {
+        // O^T += the tile's values times the weights p.  A block of a value has
+        // its own scales, so its own products of weights and scales: 24
+        // instructions a column tile.  With `once` copy k of the columns takes
+        // block k's scales, all blocks' products are made at once, and of what
+        // comes out only copy b's columns of block b are read.
+        auto second = [&](const T &x, const f32x4 (&p)[C][2], bool inf, auto odd, auto once) __attribute__((always_inline)) {
             const u32x4 *sc = (const u32x4 *)ssc[wave];
-            uint32_t keep[C][4];
+            uint32_t keep[C][4] = {};
             if (odd) {
+                // (one column tile: masks that keep all, where there is nothing
+                // to hide, cost four instructions; two: a path of its own)
+                const bool hide = C > 1 || __any(inf);
+#pragma unroll
+                for (int i = 0; i < 4; i++) keep[0][i] = 0xffffffffu;
+                if (hide)
 #pragma unroll
                 for (int c = 0; c < C; c++)
 #pragma unroll
@@ -328,40 +355,46 @@ __global__ __launch_bounds__(W * 64, QC + VC <= 8 && C == 1 ? 3 : 2) void kv4_at
                         keep[c][i] = (p[c][i >> 1][2 * i & 3] == 0.0f ? 0 : 0xffffu) |
                                      (p[c][i >> 1][(2 * i & 3) + 1] == 0.0f ? 0 : 0xffff0000u);
             }
+            half8 h8[C], l8[C];
+            // Weights times scales in the codes' order, bytes 0, 2, 1, 3 of
+            // each half; both pieces.
+            auto scaled = [&](int c, const u32x4 &ds) __attribute__((always_inline)) {
+                half2v ph[4], pl[4];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const half2v d0 = as_h2(odd ? ds[2 * h] & keep[c][2 * h] : ds[2 * h]);
+                    const half2v d1 = as_h2(odd ? ds[2 * h + 1] & keep[c][2 * h + 1] : ds[2 * h + 1]);
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float u = fmaf((float)d0[e], p[c][h][e], 0.0f), w = fmaf((float)d1[e], p[c][h][2 + e], 0.0f);
+                        const half2v z = pack_half(u, w);
+                        ph[2 * h + e] = z;
+                        pl[2 * h + e] = pack_half(fmaf((float)z[0], less, u), fmaf((float)z[1], less, w));
+                    }
+                }
+                h8[c] = join8(ph[0], ph[1], ph[2], ph[3]), l8[c] = join8(pl[0], pl[1], pl[2], pl[3]);
+            };
+            if (once) scaled(0, sc[(nq + copy) * 4 + g]);
 #pragma unroll
             for (int b = 0; b < VC; b++) {
                 if (!EX && b >= nv) continue;
-                const u32x4 ds = sc[(nq + b) * 4 + g];
                 const uint32_t w0 = x.v[2 * b], w1 = x.v[2 * b + 1];
                 const half8 v0 = join8(low_pair(w0, nib), low_pair(w0 >> 8, nib), low_pair(w1, nib), low_pair(w1 >> 8, nib));
                 const half8 v1 = join8(high_pair(w0, nib), high_pair(w0 >> 8, nib), high_pair(w1, nib), high_pair(w1 >> 8, nib));
+                const u32x4 ds = sc[(nq + b) * 4 + g];
 #pragma unroll
                 for (int c = 0; c < C; c++) {
-                    // Weights times scales in the codes' order: bytes 0, 2, 1,
-                    // 3 of each half; both pieces.
-                    half2v ph[4], pl[4];
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const half2v d0 = as_h2(odd ? ds[2 * h] & keep[c][2 * h] : ds[2 * h]);
-                        const half2v d1 = as_h2(odd ? ds[2 * h + 1] & keep[c][2 * h + 1] : ds[2 * h + 1]);
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const float u = fmaf((float)d0[e], p[c][h][e], 0.0f), w = fmaf((float)d1[e], p[c][h][2 + e], 0.0f);
-                            const half2v z = pack_half(u, w);
-                            ph[2 * h + e] = z;
-                            pl[2 * h + e] = pack_half(fmaf((float)z[0], less, u), fmaf((float)z[1], less, w));
-                        }
-                    }
-                    const half8 h8 = join8(ph[0], ph[1], ph[2], ph[3]), l8 = join8(pl[0], pl[1], pl[2], pl[3]);
-                    o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, h8, o[c][b][0], 0, 0, 0);
-                    o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, h8, o[c][b][1], 0, 0, 0);
-                    o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, l8, o[c][b][0], 0, 0, 0);
-                    o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, l8, o[c][b][1], 0, 0, 0);
+                    if (!once) scaled(c, ds);
+                    o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, h8[c], o[c][b][0], 0, 0, 0);
+                    o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, h8[c], o[c][b][1], 0, 0, 0);
+                    o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, l8[c], o[c][b][0], 0, 0, 0);
+                    o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, l8[c], o[c][b][1], 0, 0, 0);
                 }
                 if (C > 1) __builtin_amdgcn_sched_barrier(0);
             }
         };
-        auto step = [&](const T &x) {
+        // between(): what to do when the keys' words have been read.
+        auto step = [&](const T &x, int base, auto once, auto between) __attribute__((always_inline)) {
             // Scales through LDS (the wave's own: in order, no barrier): every
             // lane reads its four positions of both halves, 16 bytes.
             uint32_t top = 0;  // the largest finite value scale of the lane's, f16 bits
@@ -388,8 +421,8 @@ __global__ __launch_bounds__(W * 64, QC + VC <= 8 && C == 1 ? 3 : 2) void kv4_at
                 const half8 k1 = join8(low_pair(w1, nib), low_pair(w1 >> 8, nib), high_pair(w1, nib), high_pair(w1 >> 8, nib));
 #pragma unroll
                 for (int c = 0; c < C; c++) {
-                    const half8 qh = __builtin_bit_cast(half8, sq_[((c * QC + b) * 2) * 64 + lane]);
-                    const half8 ql = __builtin_bit_cast(half8, sq_[((c * QC + b) * 2 + 1) * 64 + lane]);
+                    const half8 qh = __builtin_bit_cast(half8, sq_[((c * QC + b) * 2) * 64 + ql_at]);
+                    const half8 ql = __builtin_bit_cast(half8, sq_[((c * QC + b) * 2 + 1) * 64 + ql_at]);
                     const f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
                     f32x4 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql, z, 0, 0, 0);
                     f32x4 t = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql, z, 0, 0, 0);
@@ -403,16 +436,17 @@ __global__ __launch_bounds__(W * 64, QC + VC <= 8 && C == 1 ? 3 : 2) void kv4_at
                 }
                 if (C > 1) __builtin_amdgcn_sched_barrier(0);
             }
+            between();
             // Positions a column does not see.
             bool some = false;
 #pragma unroll
-            for (int c = 0; c < C; c++) some |= cv[c] && (x.base < cl[c] || x.base + kTile - 1 > cp[c]);
+            for (int c = 0; c < C; c++) some |= cv[c] && (base < cl[c] || base + kTile - 1 > cp[c]);
             if (__any(some)) {
 #pragma unroll
                 for (int c = 0; c < C; c++)
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const int at = x.base + (i >> 2) * 16 + 4 * g + (i & 3);
+                        const int at = base + (i >> 2) * 16 + 4 * g + (i & 3);
                         if (at < cl[c] || at > cp[c]) s[c][i >> 2][i & 3] = -INFINITY;
                     }
             }
@@ -458,19 +492,34 @@ __global__ __launch_bounds__(W * 64, QC + VC <= 8 && C == 1 ? 3 : 2) void kv4_at
                 }
             // A position of weight 0 may hold an infinity or a NaN: such tiles
             // read its scales as 0.
-            if (__builtin_expect(__any(inf), 0)) second(x, s, std::true_type{});
-            else second(x, s, std::false_type{});
+            if (C == 1) second(x, s, inf, std::true_type{}, once);
+            else if (__builtin_expect(__any(inf), 0)) second(x, s, inf, std::true_type{}, once);
+            else second(x, s, inf, std::false_type{}, once);
         };
-        if (any) {
-            while (true) {
+        auto none = [] {};
+        auto walk = [&](auto once) __attribute__((always_inline)) {
+            // One column tile: two sets of words, a whole tile ahead.  Two, whose
+            // sums need the registers: one set, the next tile's keys queued when
+            // this one's have been read, its values at the end.
+            while (C == 1 && any) {
                 load(y);
-                if (x.ok) step(x);
+                if (x.ok) step(x, x.base, once, none);
                 if (v > v1) break;
                 load(x);
-                if (y.ok) step(y);
+                if (y.ok) step(y, y.base, once, none);
                 if (v > v1) break;
             }
-        }
+            while (C > 1 && any) {
+                // (a tile that is none: positions that no column sees)
+                const int base = x.ok ? x.base : 1 << 30;
+                find(x);
+                step(x, base, once, [&] { load_keys(x); });
+                load_values(x);
+                if (v > v1) break;
+            }
+        };
+        if (C == 1 && copies) walk(std::integral_constant<bool, C == 1>{});
+        else walk(std::false_type{});
 
         // Merge the waves, a column tile at a time: sums as they are and their
         // references through LDS, then every wave takes a share of the output's
@@ -497,19 +546,20 @@ __global__ __launch_bounds__(W * 64, QC + VC <= 8 && C == 1 ? 3 : 2) void kv4_at
                 ll += rw == -INFINITY ? 0.0f : sm_l[w][c * 16 + col] * fw[w];
             }
             if (cv[c]) {
-                const size_t row = r0 + crow[c], head = h0 + (c * 16 + col) % hn;
+                const size_t row = r0 + cc[c] / hn, head = h0 + cc[c] % hn;
                 float *dst = a.out + row * a.out_stride + head * kc.vd;
                 float f = ll == 0.0f ? 0.0f : 1.0f / ll;
                 if (a.ps > 1) {
                     const size_t where = (row * a.heads + head) * a.ps + part;
                     dst = a.part + where * kc.vd;
-                    if (g == 0 && wave == 0) a.part_ml[2 * where] = rr, a.part_ml[2 * where + 1] = ll;
+                    if (g == 0 && wave == 0 && (!copies || col >> wide == 0)) a.part_ml[2 * where] = rr, a.part_ml[2 * where + 1] = ll;
                     f = 1.0f;
                 }
                 // Lane (column, g) of [block][half] holds dims 32 b + 16 h + 4 g + i.
 #pragma unroll
                 for (int bh = 0; bh < VC * 2; bh += W) {
-                    if (bh + wave >= nv * 2) continue;
+                    const int b = (bh + wave) >> 1;
+                    if (b >= nv || (copies && col >> wide != b)) continue;
                     f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int w = 0; w < W; w++) {
@@ -519,7 +569,7 @@ __global__ __launch_bounds__(W * 64, QC + VC <= 8 && C == 1 ? 3 : 2) void kv4_at
                     }
 #pragma unroll
                     for (int i = 0; i < 4; i++) z[i] *= f;
-                    gstore((f32x4_dw *)(dst + 16 * (bh + wave) + 4 * g), __builtin_bit_cast(f32x4_dw, z));
+                    *(__attribute__((address_space(1))) f32x4_dw *)(dst + 16 * (bh + wave) + 4 * g) = __builtin_bit_cast(f32x4_dw, z);
                 }
             }
             __syncthreads();

@@ -68,23 +68,33 @@ __device__ inline uint8_t *tile_of(const Kv4 &c, int64_t slot, int kv, int &p) {
     return c.head((int)(slot >> c.page_shift), kv) + (size_t)(off >> 5) * c.tile_bytes;
 }
 
+typedef float f32x4_dw __attribute__((ext_vector_type(4), aligned(4)));  // at any float
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Row of a block: the rows of a tile, 32 in turn in a prompt, go to one XCD, so
+// that the bytes of a line that different rows write meet in one L2 instead of
+// being written back by several.
+__device__ inline int row_of(unsigned block) { return (int)(((block >> 3 >> 5) * 8 + (block & 7)) * 32 + (block >> 3 & 31)); }
+unsigned row_blocks(int rows) { return ((unsigned)rows + 255) / 256 * 256; }
+
 // Eight lanes per 32-value block, four values each; a block of threads takes
 // 32 blocks of a row's keys and values.
 __global__ __launch_bounds__(256) void kv4_store_kernel(const Kv4 c, const float *__restrict__ k, int64_t ks,
-                                                        const float *__restrict__ v, int64_t vs,
+                                                        const float *__restrict__ v, int64_t vs, int rows,
                                                         const int64_t *__restrict__ slots) {
-    const int row = blockIdx.x;
-    const int64_t slot = slots[row];
-    if (!slot_ok(c, slot)) return;
+    const int row = row_of(blockIdx.x);
+    if (row >= rows) return;
+    const int64_t slot = gload(slots + row);
     const int nk = c.qd / 32, nv = c.vd / 32, i = threadIdx.x & 7;
     const int at = blockIdx.y * 32 + (threadIdx.x >> 3);
-    if (at >= c.n_kv * (nk + nv)) return;
+    if (!slot_ok(c, slot) || at >= c.n_kv * (nk + nv)) return;
     const bool key = at < c.n_kv * nk;
     const int blk = key ? at : at - c.n_kv * nk, nb = key ? nk : nv, kv = blk / nb, s = blk % nb;
     const float *src = (key ? k + (size_t)row * ks : v + (size_t)row * vs) + (size_t)blk * 32 + 4 * i;
-    float x[4], top = 0.0f;
+    const f32x4_dw x = *(const __attribute__((address_space(1))) f32x4_dw *)src;
+    float top = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 4; e++) x[e] = src[e], top = fmaxf(top, fabsf(x[e]));  // fmaxf drops NaNs
+    for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[e]));  // fmaxf drops NaNs
 #pragma unroll
     for (int o = 4; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
     const float d = top / 7.0f;
@@ -97,49 +107,89 @@ __global__ __launch_bounds__(256) void kv4_store_kernel(const Kv4 c, const float
     int p;
     uint8_t *tile = tile_of(c, slot, kv, p);
     if (i == 0)
-        *(uint16_t *)(tile + (key ? c.k_scales() : c.v_scales()) + 2 * kv4_scale_at(p, s)) = (uint16_t)h;
+        gstore((uint16_t *)(tile + (key ? c.k_scales() : c.v_scales()) + 2 * kv4_scale_at(p, s)), (uint16_t)h);
     if (i >= 4) return;
     if (key) {
-        *(uint32_t *)(tile + kv4_key_byte(nk, p, s, 4 * i)) = w;
+        gstore((uint32_t *)(tile + kv4_key_byte(nk, p, s, 4 * i)), w);
     } else {
+        uint8_t *dst = tile + c.v_codes() + kv4_value_byte(nv, p, s, 4 * i);
+        const int step = kv4_value_byte(nv, 0, s, 1) - kv4_value_byte(nv, 0, s, 0);
 #pragma unroll
-        for (int e = 0; e < 4; e++) tile[c.v_codes() + kv4_value_byte(nv, p, s, 4 * i + e)] = (uint8_t)(w >> (8 * e));
+        for (int e = 0; e < 4; e++) gstore(dst + e * step, (uint8_t)(w >> (8 * e)));
     }
 }
 
-__device__ inline float value_at(const Kv4 &c, const uint8_t *tile, bool key, int p, int d) {
-    const int nb = (key ? c.qd : c.vd) / 32, s = d >> 5, j = d & 15;
-    const uint8_t b = key ? tile[kv4_key_byte(nb, p, s, j)] : tile[c.v_codes() + kv4_value_byte(nb, p, s, j)];
-    const __half h = ((const __half *)(tile + (key ? c.k_scales() : c.v_scales())))[kv4_scale_at(p, s)];
-    return __half2float(h) * (float)((int)(d & 16 ? b >> 4 : b & 15) - 8);
+// The mean keys of pages whose last position is among the rows: a block looks
+// at 64 rows for one kv head, its waves take the dims' blocks of 32.  A word of
+// the keys' region is eight dims of a position, so a lane sums eight dims over
+// its positions and 16 lanes are added up.  In 64 bits the sums are exact for
+// scales within 2^30 of each other, whatever their order.
+__global__ __launch_bounds__(256) void kv4_means_kernel(const Kv4 c, const int64_t *__restrict__ slots, int rows) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, kv = blockIdx.y;
+    const int64_t last = (1 << c.page_shift) - 1, row = (int64_t)blockIdx.x * 64 + lane;
+    const int64_t mine = row < rows ? gload(slots + row) : -1;
+    const int nq = c.qd / 32, g = lane >> 4, col = lane & 15;
+    for (unsigned long long full = __ballot(slot_ok(c, mine) && (mine & last) == last); full; full &= full - 1) {
+        const int page = (int)(__shfl(mine, __builtin_ctzll(full), 64) >> c.page_shift);
+        const uint8_t *head = c.head(page, kv);
+        for (int s = wave; s < nq; s += 4) {
+            double sum[8] = {};
+#pragma unroll 4
+            for (int t = 0; t < 2 * c.tiles(); t++) {
+                const uint8_t *tile = head + (size_t)(t >> 1) * c.tile_bytes;
+                const int half = t & 1;
+                const uint32_t w = gload((const uint32_t *)(tile + kv4_word(nq, 2 * s + half, lane)));
+                const uint16_t hb = gload((const uint16_t *)(tile + c.k_scales()) + kv4_scale_at(16 * half + col, s));
+                const float d = __half2float(__ushort_as_half(hb));
+#pragma unroll
+                for (int e = 0; e < 8; e++)  // bytes' low nibbles: dims 4 g + e; high: 16 + 4 g + e - 4
+                    sum[e] += (double)(d * (float)((int)(w >> (8 * (e & 3) + (e & 4)) & 15) - 8));
+            }
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1)
+#pragma unroll
+                for (int e = 0; e < 8; e++) sum[e] += __shfl_xor(sum[e], o, 64);
+            if (col == 0)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    float m = (float)(sum[e] / (double)(last + 1));
+                    m = m > 65504.0f ? 65504.0f : m < -65504.0f ? -65504.0f : m;
+                    c.means[((size_t)page * c.n_kv + kv) * c.qd + 32 * s + (e & 4) * 4 + 4 * g + (e & 3)] = __float2half_rn(m);
+                }
+        }
+    }
 }
 
-// The mean key of pages whose last position a row of this call wrote.
-__global__ __launch_bounds__(256) void kv4_means_kernel(const Kv4 c, const int64_t *__restrict__ slots) {
-    const int64_t slot = slots[blockIdx.x];
-    const int kv = blockIdx.y, last = (1 << c.page_shift) - 1, d = threadIdx.x;
-    if (!slot_ok(c, slot) || (slot & last) != last || d >= c.qd) return;
-    const int page = (int)(slot >> c.page_shift);
-    const uint8_t *head = c.head(page, kv);
-    double sum = 0.0;
-    for (int j = 0; j <= last; j++) sum += (double)value_at(c, head + (size_t)(j >> 5) * c.tile_bytes, true, j & 31, d);
-    float m = (float)(sum / (double)(last + 1));
-    m = m > 65504.0f ? 65504.0f : m < -65504.0f ? -65504.0f : m;
-    c.means[((size_t)page * c.n_kv + kv) * c.qd + d] = __float2half_rn(m);
-}
-
-__global__ __launch_bounds__(256) void kv4_load_kernel(const Kv4 c, const int64_t *__restrict__ slots,
+// As the write: eight lanes per block of 32, four values each.
+__global__ __launch_bounds__(256) void kv4_load_kernel(const Kv4 c, const int64_t *__restrict__ slots, int rows,
                                                        float *__restrict__ k, int64_t ks, float *__restrict__ v,
                                                        int64_t vs) {
-    const int64_t slot = slots[blockIdx.x];
-    if (!slot_ok(c, slot)) return;
+    const int row = row_of(blockIdx.x);
+    if (row >= rows) return;
+    const int64_t slot = gload(slots + row);
+    const int nk = k ? c.qd / 32 : 0, nv = v ? c.vd / 32 : 0, i = threadIdx.x & 7;
+    const int at = blockIdx.y * 32 + (threadIdx.x >> 3);
+    if (!slot_ok(c, slot) || at >= c.n_kv * (nk + nv)) return;
+    const bool key = at < c.n_kv * nk;
+    const int blk = key ? at : at - c.n_kv * nk, nb = key ? nk : nv, kv = blk / nb, s = blk % nb;
     int p;
-    if (k)
-        for (int i = threadIdx.x; i < c.n_kv * c.qd; i += 256)
-            k[(size_t)blockIdx.x * ks + i] = value_at(c, tile_of(c, slot, i / c.qd, p), true, (int)slot & 31, i % c.qd);
-    if (v)
-        for (int i = threadIdx.x; i < c.n_kv * c.vd; i += 256)
-            v[(size_t)blockIdx.x * vs + i] = value_at(c, tile_of(c, slot, i / c.vd, p), false, (int)slot & 31, i % c.vd);
+    const uint8_t *tile = tile_of(c, slot, kv, p);
+    const uint16_t hb = gload((const uint16_t *)(tile + (key ? c.k_scales() : c.v_scales())) + kv4_scale_at(p, s));
+    uint32_t w = 0;
+    if (key) {
+        w = gload((const uint32_t *)(tile + kv4_key_byte(nk, p, s, 4 * (i & 3))));
+    } else {
+        const uint8_t *src = tile + c.v_codes() + kv4_value_byte(nv, p, s, 4 * (i & 3));
+        const int step = kv4_value_byte(nv, 0, s, 1) - kv4_value_byte(nv, 0, s, 0);
+#pragma unroll
+        for (int e = 0; e < 4; e++) w |= (uint32_t)gload(src + e * step) << (8 * e);
+    }
+    const float d = __half2float(__ushort_as_half(hb));
+    f32x4_dw x;
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] = d * (float)((int)(w >> (8 * e + (i & 4)) & 15) - 8);
+    float *dst = (key ? k + (size_t)row * ks : v + (size_t)row * vs) + (size_t)blk * 32 + 4 * i;
+    *(__attribute__((address_space(1))) f32x4_dw *)dst = x;
 }
 
 int rc_of(const char *what) {
@@ -176,9 +226,9 @@ int moe_kv4_store(const moe_kv4 *c, const float *k, int64_t k_stride, const floa
     if (rows == 0) return MOE_OK;
     hipStream_t s = (hipStream_t)stream;
     const int blocks = a.n_kv * (a.qd + a.vd) / 32;
-    hipLaunchKernelGGL(kv4_store_kernel, dim3(rows, (blocks + 31) / 32), dim3(256), 0, s, a, k, k_stride, v, v_stride,
-                       slots);
-    if (a.means) hipLaunchKernelGGL(kv4_means_kernel, dim3(rows, a.n_kv), dim3(256), 0, s, a, slots);
+    hipLaunchKernelGGL(kv4_store_kernel, dim3(row_blocks(rows), (blocks + 31) / 32), dim3(256), 0, s, a, k, k_stride, v,
+                       v_stride, rows, slots);
+    if (a.means) hipLaunchKernelGGL(kv4_means_kernel, dim3((rows + 63) / 64, a.n_kv), dim3(256), 0, s, a, slots, rows);
     return rc_of("cache write kernel");
 }
 
@@ -188,8 +238,9 @@ int moe_kv4_load(const moe_kv4 *c, const int64_t *slots, int32_t rows, float *k,
     if (const int rc = kv4_of("moe_kv4_load", c, &a)) return rc;
     if (rows < 0 || (rows > 0 && !slots)) return fail(MOE_EINVAL, "moe_kv4_load: bad argument (%d rows)", rows);
     if (rows == 0 || (!k && !v)) return MOE_OK;
-    hipLaunchKernelGGL(kv4_load_kernel, dim3(rows), dim3(256), 0, (hipStream_t)stream, a, slots, k, k_stride, v,
-                       v_stride);
+    const int blocks = a.n_kv * ((k ? a.qd : 0) + (v ? a.vd : 0)) / 32;
+    hipLaunchKernelGGL(kv4_load_kernel, dim3(row_blocks(rows), (blocks + 31) / 32), dim3(256), 0, (hipStream_t)stream, a,
+                       slots, rows, k, k_stride, v, v_stride);
     return rc_of("cache read kernel");
 }
 

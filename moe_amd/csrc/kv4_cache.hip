@@ -69,53 +69,113 @@ __device__ inline uint8_t *tile_of(const Kv4 &c, int64_t slot, int kv, int &p) {
 }
 
 typedef float f32x4_dw __attribute__((ext_vector_type(4), aligned(4)));  // at any float
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-// Row of a block: the rows of a tile, 32 in turn in a prompt, go to one XCD, so
-// that the bytes of a line that different rows write meet in one L2 instead of
-// being written back by several.
-__device__ inline int row_of(unsigned block) { return (int)(((block >> 3 >> 5) * 8 + (block & 7)) * 32 + (block >> 3 & 31)); }
-unsigned row_blocks(int rows) { return ((unsigned)rows + 255) / 256 * 256; }
+// First of the R rows of a block.  The rows of a tile, 32 in turn in a prompt,
+// go to one XCD, so that the bytes of a line that different rows write meet in
+// one L2 instead of being written back by several.
+template <int R>
+__device__ inline int first_row(unsigned block) {
+    constexpr unsigned per = 32 / R;
+    return (int)(((block >> 3) / per * 8 + (block & 7)) * per + (block >> 3) % per) * R;
+}
+template <int R>
+unsigned row_blocks(int rows) {
+    return ((unsigned)rows + 255) / 256 * (256 / R);
+}
 
-// Eight lanes per 32-value block, four values each; a block of threads takes
-// 32 blocks of a row's keys and values.
+// Quantise and write one 32-value block, eight lanes, four values each, of N
+// rows whose slots follow one another from `slot` on: of one row, or of four
+// that begin at a slot divisible by four, whose values' bytes then make whole
+// words and whose scales lie together.
+template <int N>
+__device__ inline void store_block(const Kv4 &c, const float *src, int64_t stride, int64_t slot, bool key, int kv, int s) {
+    const int i = threadIdx.x & 7, nb = (key ? c.qd : c.vd) / 32;
+    f32x4_dw x[N];
+#pragma unroll
+    for (int r = 0; r < N; r++) x[r] = *(const __attribute__((address_space(1))) f32x4_dw *)(src + r * stride + 4 * i);
+    uint32_t w[N], h[N];
+#pragma unroll
+    for (int r = 0; r < N; r++) {
+        float top = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[r][e]));  // fmaxf drops NaNs
+#pragma unroll
+        for (int o = 4; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        const float d = top / 7.0f;
+        h[r] = half_bits(d);
+        const float inv = d > 0.0f ? 1.0f / __half2float(__ushort_as_half((unsigned short)h[r])) : 0.0f;
+        w[r] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[r] |= code_of(x[r][e], inv) << (8 * e);
+        w[r] |= (uint32_t)__shfl_down((int)w[r], 4, 64) << 4;  // dims j + 16 into the high nibbles (lanes 0..3)
+    }
+    int p;
+    uint8_t *tile = tile_of(c, slot, kv, p);
+    if (i == 4) {
+        uint16_t *dst = (uint16_t *)(tile + (key ? c.k_scales() : c.v_scales())) + kv4_scale_at(p, s);
+        if (N == 4) gstore((u32x2 *)dst, u32x2{h[0] | h[N > 1 ? 1 : 0] << 16, h[N > 2 ? 2 : 0] | h[N > 3 ? 3 : 0] << 16});
+        else gstore(dst, (uint16_t)h[0]);
+    }
+    if (i >= 4) return;
+    if (key) {
+#pragma unroll
+        for (int r = 0; r < N; r++) gstore((uint32_t *)(tile + kv4_key_byte(nb, p + r, s, 4 * i)), w[r]);
+        return;
+    }
+    uint8_t *dst = tile + c.v_codes() + kv4_value_byte(nb, p, s, 4 * i);
+    const int step = kv4_value_byte(nb, 0, s, 1) - kv4_value_byte(nb, 0, s, 0);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if (N == 4) {
+            uint32_t y = 0;
+#pragma unroll
+            for (int r = 0; r < N; r++) y |= (w[r] >> (8 * e) & 255) << (8 * r);
+            gstore((uint32_t *)(dst + e * step), y);
+        } else {
+            gstore(dst + e * step, (uint8_t)(w[0] >> (8 * e)));
+        }
+    }
+}
+
+// A block of threads takes 32 blocks of 32 values of R rows.  R = 4: four rows
+// in turn whose slots are too, from one divisible by four on, are written by
+// the block that has the first of them; other rows one by one.
+template <int R>
 __global__ __launch_bounds__(256) void kv4_store_kernel(const Kv4 c, const float *__restrict__ k, int64_t ks,
                                                         const float *__restrict__ v, int64_t vs, int rows,
                                                         const int64_t *__restrict__ slots) {
-    const int row = row_of(blockIdx.x);
-    if (row >= rows) return;
-    const int64_t slot = gload(slots + row);
-    const int nk = c.qd / 32, nv = c.vd / 32, i = threadIdx.x & 7;
+    const int r0 = first_row<R>(blockIdx.x);
+    const int nk = c.qd / 32, nv = c.vd / 32;
     const int at = blockIdx.y * 32 + (threadIdx.x >> 3);
-    if (!slot_ok(c, slot) || at >= c.n_kv * (nk + nv)) return;
+    if (r0 >= rows || at >= c.n_kv * (nk + nv)) return;
     const bool key = at < c.n_kv * nk;
     const int blk = key ? at : at - c.n_kv * nk, nb = key ? nk : nv, kv = blk / nb, s = blk % nb;
-    const float *src = (key ? k + (size_t)row * ks : v + (size_t)row * vs) + (size_t)blk * 32 + 4 * i;
-    const f32x4_dw x = *(const __attribute__((address_space(1))) f32x4_dw *)src;
-    float top = 0.0f;
+    const float *src = (key ? k : v) + (size_t)blk * 32;
+    const int64_t stride = key ? ks : vs;
+    if (R == 1) {
+        const int64_t slot = gload(slots + r0);
+        if (slot_ok(c, slot)) store_block<1>(c, src + (int64_t)r0 * stride, stride, slot, key, kv, s);
+        return;
+    }
+    // Slots of rows r0 - 3 .. r0 + 6, and which of them begin such a four.
+    int64_t sl[10];
 #pragma unroll
-    for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[e]));  // fmaxf drops NaNs
+    for (int i = 0; i < 10; i++) {
+        const int r = r0 - 3 + i;
+        sl[i] = r >= 0 && r < rows ? gload(slots + r) : -1;
+    }
+    bool four[7];
 #pragma unroll
-    for (int o = 4; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    const float d = top / 7.0f;
-    const uint32_t h = half_bits(d);
-    const float inv = d > 0.0f ? 1.0f / __half2float(__ushort_as_half((unsigned short)h)) : 0.0f;
-    uint32_t w = 0;
+    for (int i = 0; i < 7; i++)
+        four[i] = slot_ok(c, sl[i]) && (sl[i] & 3) == 0 && sl[i + 1] == sl[i] + 1 && sl[i + 2] == sl[i] + 2 &&
+                  sl[i + 3] == sl[i] + 3;
 #pragma unroll
-    for (int e = 0; e < 4; e++) w |= code_of(x[e], inv) << (8 * e);
-    w |= (uint32_t)__shfl_down((int)w, 4, 64) << 4;  // dims j + 16 into the high nibbles (lanes 0..3)
-    int p;
-    uint8_t *tile = tile_of(c, slot, kv, p);
-    if (i == 0)
-        gstore((uint16_t *)(tile + (key ? c.k_scales() : c.v_scales()) + 2 * kv4_scale_at(p, s)), (uint16_t)h);
-    if (i >= 4) return;
-    if (key) {
-        gstore((uint32_t *)(tile + kv4_key_byte(nk, p, s, 4 * i)), w);
-    } else {
-        uint8_t *dst = tile + c.v_codes() + kv4_value_byte(nv, p, s, 4 * i);
-        const int step = kv4_value_byte(nv, 0, s, 1) - kv4_value_byte(nv, 0, s, 0);
-#pragma unroll
-        for (int e = 0; e < 4; e++) gstore(dst + e * step, (uint8_t)(w >> (8 * e)));
+    for (int i = 3; i < 7; i++) {
+        const int64_t row = r0 - 3 + i;
+        if (four[i]) store_block<4>(c, src + row * stride, stride, sl[i], key, kv, s);
+        else if (!(four[i - 1] || four[i - 2] || four[i - 3]) && slot_ok(c, sl[i]))
+            store_block<1>(c, src + row * stride, stride, sl[i], key, kv, s);
     }
 }
 
@@ -164,7 +224,7 @@ __global__ __launch_bounds__(256) void kv4_means_kernel(const Kv4 c, const int64
 __global__ __launch_bounds__(256) void kv4_load_kernel(const Kv4 c, const int64_t *__restrict__ slots, int rows,
                                                        float *__restrict__ k, int64_t ks, float *__restrict__ v,
                                                        int64_t vs) {
-    const int row = row_of(blockIdx.x);
+    const int row = first_row<1>(blockIdx.x);
     if (row >= rows) return;
     const int64_t slot = gload(slots + row);
     const int nk = k ? c.qd / 32 : 0, nv = v ? c.vd / 32 : 0, i = threadIdx.x & 7;
@@ -226,8 +286,16 @@ int moe_kv4_store(const moe_kv4 *c, const float *k, int64_t k_stride, const floa
     if (rows == 0) return MOE_OK;
     hipStream_t s = (hipStream_t)stream;
     const int blocks = a.n_kv * (a.qd + a.vd) / 32;
-    hipLaunchKernelGGL(kv4_store_kernel, dim3(row_blocks(rows), (blocks + 31) / 32), dim3(256), 0, s, a, k, k_stride, v,
-                       v_stride, rows, slots);
+    // Word stores of four rows pay where there are prompts (16376 rows of 8 heads
+    // of 128: 59 -> 41 us); a few rows are latency, one row a block (32 rows:
+    // 5.7 -> 3.0 us, 999 rows of 16 heads of 192/128 13.3 -> 12.0).
+    const unsigned y = (unsigned)(blocks + 31) / 32;
+    if (rows >= 4096)
+        hipLaunchKernelGGL((kv4_store_kernel<4>), dim3(row_blocks<4>(rows), y), dim3(256), 0, s, a, k, k_stride, v, v_stride,
+                           rows, slots);
+    else
+        hipLaunchKernelGGL((kv4_store_kernel<1>), dim3(row_blocks<1>(rows), y), dim3(256), 0, s, a, k, k_stride, v, v_stride,
+                           rows, slots);
     if (a.means) hipLaunchKernelGGL(kv4_means_kernel, dim3((rows + 63) / 64, a.n_kv), dim3(256), 0, s, a, slots, rows);
     return rc_of("cache write kernel");
 }
@@ -239,7 +307,7 @@ int moe_kv4_load(const moe_kv4 *c, const int64_t *slots, int32_t rows, float *k,
     if (rows < 0 || (rows > 0 && !slots)) return fail(MOE_EINVAL, "moe_kv4_load: bad argument (%d rows)", rows);
     if (rows == 0 || (!k && !v)) return MOE_OK;
     const int blocks = a.n_kv * ((k ? a.qd : 0) + (v ? a.vd : 0)) / 32;
-    hipLaunchKernelGGL(kv4_load_kernel, dim3(row_blocks(rows), (blocks + 31) / 32), dim3(256), 0, (hipStream_t)stream, a,
+    hipLaunchKernelGGL(kv4_load_kernel, dim3(row_blocks<1>(rows), (blocks + 31) / 32), dim3(256), 0, (hipStream_t)stream, a,
                        slots, rows, k, k_stride, v, v_stride);
     return rc_of("cache read kernel");
 }

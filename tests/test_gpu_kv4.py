@@ -226,6 +226,34 @@ def test_store_and_load(shape, page):
             assert np.array_equal(vb[r, kv * vd:(kv + 1) * vd], pool.get(s, kv, False).astype(np.float32))
 
 
+@pytest.mark.parametrize("page", [32, 64])
+def test_store_runs_of_rows(page):
+    """Runs that begin at any offset, follow one another, break off, go
+    backwards: rows that are written four at a time beside single ones."""
+    n_kv, qd, vd = 1, 64, 96
+    g = np.random.default_rng(page)
+    for trial in range(6):
+        n_pages = [6, 300, 400, 5, 350, 320][trial] * 32 // page  # few rows, and enough for the kernel of four
+        free = g.permutation(n_pages * page // 8)
+        slots = []
+        for b in free[:len(free) - 2]:
+            run = list(range(b * 8, b * 8 + 8))
+            how = int(g.integers(0, 5))
+            slots += [run, run[int(g.integers(0, 8)):], run[::-1], run[:int(g.integers(1, 8))],
+                      [run[i] for i in g.permutation(8)]][how]
+            if g.random() < 0.2:
+                slots.append(-1)
+        k = g.standard_normal((len(slots), n_kv * qd)).astype(np.float32)
+        v = g.standard_normal((len(slots), n_kv * vd)).astype(np.float32)
+        pool = ref.Pool(n_pages, n_kv, qd, vd, page, g.integers(0, 255, n_pages * n_kv * page // 32 * 18 * (qd + vd)).astype(np.uint8))
+        cache = on_gpu(pool, np.zeros((1, 1), np.int32))
+        import torch
+
+        cache.store(torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), ints(slots, "int64"))
+        pool.store(slots, k, v)
+        assert np.array_equal(cache.pool.cpu().numpy(), pool.raw)
+
+
 def test_store_as_the_host_quantiser():
     """Codes and scales equal moe_quantize_rows(Q4_0)'s, over the range of
     f32: subnormal and overflowing scales, zeros, infinities, NaNs."""

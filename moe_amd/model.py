@@ -31,6 +31,7 @@ import numpy as np
 
 from . import _lib as L
 from .layer import Context, Mlp, MoeLayer, MoeSpec, Rec, Region, Store, View, _stream_ptr, row_bytes
+from .paged import KvCache, PageTable, Rows
 
 try:
     import torch
@@ -398,6 +399,99 @@ class State:
         self.v = [torch.zeros((n_seq, ctx, vd), dtype=torch.float32, device=dev) for _ in range(s.layers)]
 
 
+@dataclass
+class Sparse:
+    """Which pages a decode step's rows read: `pages` of them, the first
+    `sinks`, the last `recent`, then those whose mean key scores highest."""
+
+    pages: int
+    sinks: int = 1
+    recent: int = 2
+
+
+class PagedBatch:
+    """Batch for a PagedState: the host sends how many tokens each sequence
+    has and the rows' ids; sequences, positions and slots are made on the
+    device (PageTable.advance), rows in the order of the sequences' numbers."""
+
+    def __init__(self, st: "PagedState", seqs: list, counts: list, ids: list, device, sp: int, queued: bool):
+        if queued and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a model step cannot be captured into a graph: its rows' ids are copied from the host")
+        t, n = sum(counts), st.n_seq
+        self.t = t
+        host = torch.zeros(n + t, dtype=torch.int32, pin_memory=queued)
+        a = host.numpy()
+        a[seqs] = counts
+        a[n:] = ids
+        dev = host.to(device, non_blocking=queued)
+        self.ids = dev[n:]
+        # The new lengths and the free pages' state are the state's only when
+        # the step is queued (commit): one that fails half-way is as if not made.
+        old = st.table
+        self.table = PageTable(old.table, torch.empty_like(old.length), old.ring, torch.empty_like(old.state), st.page)
+        rows = old.advance(dev[:n], Rows.new(n, t, device), out=self.table, stream=sp)
+        self.seq, self.pos, self.dst = rows.seq, rows.pos, rows.slot
+        self.max_pos = max(st.pos[q] + c for q, c in zip(seqs, counts)) - 1
+        self.sparse = st.sparse is not None and max(counts) == 1
+        self.ends = None  # each token list's last row
+
+
+class PagedState:
+    """State with the cache in 4 bits, in pages (moe_amd.paged): n_seq
+    sequences of up to ctx positions share `pages` pages, which they take as
+    they grow and end() gives back.  With `sparse`, decode steps (one token a
+    sequence) read only the pages they choose; prompts read everything."""
+
+    def __init__(self, model: "Model", n_seq: int, ctx: int, page: int, pages: Optional[int], sparse: Optional[Sparse]):
+        s = model.spec
+        n_kv, qd, vd = model.kv_heads()
+        each = -(-ctx // page)
+        pages = n_seq * each if pages is None else pages
+        if sparse is not None and not (sparse.sinks >= 0 and sparse.recent >= 1
+                                       and sparse.sinks + sparse.recent <= sparse.pages):
+            raise ValueError(f"{sparse.sinks} first and {sparse.recent} last pages of {sparse.pages}")
+        KvCache.page_bytes(n_kv, qd, vd, page)  # refuses widths and pages the cache does not hold
+        if n_seq < 1 or ctx < 1 or pages < 1:
+            raise ValueError(f"{n_seq} sequences of {ctx} positions over {pages} pages")
+        self.ctx, self.n_seq, self.page, self.pages, self.sparse = ctx, n_seq, page, pages, sparse
+        self.pos = [0] * n_seq
+        self.table = PageTable.new(n_seq, each, pages, page, model.device)
+        self.kv = [KvCache.new(pages, self.table.table, n_kv=n_kv, qd=qd, vd=vd, page=page, means=sparse is not None)
+                   for _ in range(s.layers)]
+
+    def free_pages(self) -> int:
+        return self.pages - sum(-(-p // self.page) for p in self.pos)
+
+    def batch(self, seqs: list, tokens: list, device, sp: int, queued: bool) -> PagedBatch:
+        if len(set(seqs)) != len(seqs) or any(not 0 <= q < self.n_seq for q in seqs):
+            raise ValueError(f"sequences {seqs} of {self.n_seq}: each once")
+        counts = [len(t) for t in tokens]
+        if not any(counts):
+            raise ValueError("a step without tokens")
+        need = sum(-(-(self.pos[q] + c) // self.page) - -(-self.pos[q] // self.page) for q, c in zip(seqs, counts))
+        if need > self.free_pages():
+            raise ValueError(f"{need} pages wanted, {self.free_pages()} free")
+        order = sorted(range(len(seqs)), key=lambda i: seqs[i])
+        b = PagedBatch(self, [seqs[i] for i in order], [counts[i] for i in order],
+                       [int(t) for i in order for t in tokens[i]], device, sp, queued)
+        b.ends, r = [0] * len(seqs), 0
+        for i in order:
+            r += counts[i]
+            b.ends[i] = r - 1
+        return b
+
+    def end(self, seqs: list, stream=None) -> None:
+        """Empty these sequences; their pages are free for the next step."""
+        if any(not 0 <= q < self.n_seq for q in seqs):
+            raise ValueError(f"sequences {seqs} of {self.n_seq}")
+        add = torch.zeros(self.n_seq, dtype=torch.int32)
+        add[list(seqs)] = -1
+        dev = self.table.device
+        self.table.advance(add.to(dev), Rows.new(self.n_seq, 0, dev), stream=stream)
+        for q in seqs:
+            self.pos[q] = 0
+
+
 class Model:
     """Model (src/model.rs:192-209, 336-834) over weights in one device
     region, bound by the reference's tensor names."""
@@ -466,7 +560,22 @@ class Model:
             return s.heads * (s.mla.qk_nope + s.mla.qk_rope), s.heads * s.mla.v_head
         return s.kv_heads * s.head_dim, s.kv_heads * s.head_dim
 
-    def new_state(self, n_seq: int, ctx: int) -> State:
+    def kv_heads(self):
+        """(heads, key width, value width) of the cache."""
+        s = self.spec
+        if s.mla:
+            return s.heads, s.mla.qk_nope + s.mla.qk_rope, s.mla.v_head
+        return s.kv_heads, s.head_dim, s.head_dim
+
+    def new_state(self, n_seq: int, ctx: int, cache: str = "f32", page: int = 64, pages: Optional[int] = None,
+                  sparse: Optional[Sparse] = None):
+        """State for n_seq sequences of up to ctx positions; with cache="q4"
+        a PagedState (head widths that are multiples of 32, up to 256), whose
+        contexts may be of any length."""
+        if cache == "q4":
+            return PagedState(self, n_seq, ctx, page, pages, sparse)
+        if cache != "f32" or pages is not None or sparse is not None:
+            raise ValueError(f"cache {cache!r}: f32, or q4 for pages and sparse steps")
         # moe_attention keeps one row's scores in LDS: at most
         # ATTN_MAX_POSITIONS positions per row (the window, where a layer
         # has one).  A longer context is refused here, before any step.
@@ -527,7 +636,11 @@ class Model:
             if p + n > st.ctx:
                 raise ValueError("context window exhausted")
         sp = _stream_ptr(stream)
-        b = Batch(seq_of, pos_of, st.ctx, self.device, ids, queued=stream is None or sp == _stream_ptr(None))
+        queued = stream is None or sp == _stream_ptr(None)
+        if isinstance(st, PagedState):
+            b = st.batch(seqs, tokens, self.device, sp, queued)
+        else:
+            b = Batch(seq_of, pos_of, st.ctx, self.device, ids, queued=queued)
         t, H = b.t, s.hidden
         lib = L.lib()
         ws = self._workspace(t)
@@ -551,6 +664,8 @@ class Model:
             if rc:
                 L.check(rc, "moe_rmsnorm")
             self._ffn(lay).feed_forward(norm, out, residual=x, stream=sp, workspace=mws)
+        if isinstance(st, PagedState):
+            st.table = b.table
         for q, toks in zip(seqs, tokens):
             st.pos[q] += len(toks)
         return x, b
@@ -599,6 +714,8 @@ class Model:
                     self._rmsnorm(proj, nrm, tmp, sp, rows=proj.numel() // span, n=span, xs=span, os_=span)
                     proj.copy_(tmp)
                 self._rope(proj, t, proj.shape[1], heads, qd, 0, qd, b, sp)
+            if isinstance(st, PagedState):
+                return self._attend_paged(li, lay, q, k, v, b, st, resid, ws, sp, take)
             kd, vdim, dst = n_kv * qd, n_kv * vd, b.dst.data_ptr()
             rc = lib.moe_scatter_rows(k.data_ptr(), t, kd, kd, st.k[li].data_ptr(), kd, dst, sp)
             rc = rc or lib.moe_scatter_rows(v.data_ptr(), t, vdim, vdim, st.v[li].data_ptr(), vdim, dst, sp)
@@ -621,6 +738,17 @@ class Model:
             kv = lay["kv_b"](cn, take("kv", s.heads * (m.qk_nope + m.v_head)), ws, stream=sp)
             self._rope(c, t, ca, 1, 0, m.kv_lora, m.qk_rope, b, sp)
             self._rope(q, t, s.heads * qd, s.heads, qd, m.qk_nope, m.qk_rope, b, sp)
+            if isinstance(st, PagedState):
+                # Rows as they would lie in an f32 cache, then the 4-bit write.
+                k, v = take("k", s.heads * qd), take("v", s.heads * vd)
+                rows = buf.get("rows")
+                if rows is None:
+                    rows = buf["rows"] = torch.arange(t, dtype=torch.int64, device=self.device)
+                rc = lib.moe_mla_kv_store(kv.data_ptr(), c.data_ptr(), ca, m.kv_lora, t, s.heads, m.qk_nope, m.qk_rope,
+                                          m.v_head, k.data_ptr(), v.data_ptr(), rows.data_ptr(), sp)
+                if rc:
+                    L.check(rc, "moe_mla_kv_store")
+                return self._attend_paged(li, lay, q, k, v, b, st, resid, ws, sp, take)
             rc = lib.moe_mla_kv_store(kv.data_ptr(), c.data_ptr(), ca, m.kv_lora, t, s.heads, m.qk_nope, m.qk_rope,
                                       m.v_head, st.k[li].data_ptr(), st.v[li].data_ptr(), b.dst.data_ptr(), sp)
             if rc:
@@ -632,6 +760,36 @@ class Model:
         if rc:
             L.check(rc, "moe_attention")
         lay["o"](ctxv, take("y", s.hidden), ws, residual=resid, stream=sp)
+
+    def _attend_paged(self, li, lay, q, k, v, b: PagedBatch, st: PagedState, resid, ws, sp, take):
+        """The cache write and attention of _attention over a PagedState."""
+        cache, lib, t = st.kv[li], L.lib(), b.t
+        heads, seq, pos, window = self.spec.heads, b.seq.data_ptr(), b.pos.data_ptr(), lay["window"] or 0
+        rc = lib.moe_kv4_store(cache._c, k.data_ptr(), k.shape[1], v.data_ptr(), v.shape[1], t, b.dst.data_ptr(), sp)
+        if rc:
+            L.check(rc, "moe_kv4_store")
+
+        def scratch(name, *args):
+            n = cache._size(name, t, *args)
+            return (take("scratch " + name, -(-n // (4 * t))).data_ptr() if n else None), n
+
+        lists, n_sel = None, 0
+        # (a window's layer reads its window)
+        if b.sparse and not window and b.max_pos // st.page >= st.sparse.pages:
+            n_sel = st.sparse.pages
+            lists = take("lists", cache.n_kv * n_sel).data_ptr()  # 32-bit whole numbers
+            buf, n = scratch("moe_kv4_select_workspace_size", b.max_pos)
+            rc = lib.moe_kv4_select(cache._c, q.data_ptr(), q.shape[1], t, heads, seq, pos, b.max_pos, st.sparse.sinks,
+                                    st.sparse.recent, n_sel, lists, buf, n, sp)
+            if rc:
+                L.check(rc, "moe_kv4_select")
+        out = take("ctx", heads * cache.vd)
+        buf, n = scratch("moe_kv4_attention_workspace_size", heads, b.max_pos, window, n_sel)
+        rc = lib.moe_kv4_attention(cache._c, q.data_ptr(), q.shape[1], t, heads, self.attn_scale, seq, pos, b.max_pos,
+                                   window, lists, n_sel, out.data_ptr(), out.shape[1], buf, n, sp)
+        if rc:
+            L.check(rc, "moe_kv4_attention")
+        lay["o"](out, take("y", self.spec.hidden), ws, residual=resid, stream=sp)
 
     def head(self, x, rows, stream=None):
         """Model::head (src/model.rs:636-642) for the chosen rows of the
@@ -661,7 +819,8 @@ class Model:
         for toks in tokens:
             r += len(toks)
             ends.append(r - 1)
-        return self.head(x, ends, stream)
+        # (a paged batch has its rows in the order of the sequences' numbers)
+        return self.head(x, getattr(b, "ends", None) or ends, stream)
 
     def forward_all(self, tokens: list, st: State, stream=None):
         """Model::forward_all (src/model.rs:572-589) for one sequence: logits

@@ -18,9 +18,12 @@ from __future__ import annotations
 import ctypes as C
 from typing import Optional
 
-import torch
-
 from . import _lib as L
+
+try:
+    import torch
+except ImportError:  # pragma: no cover - torch is part of the image
+    torch = None
 
 
 def _need(ok: bool, what: str) -> None:
@@ -42,7 +45,7 @@ def _rows(t, rows: int, cols: int, name: str) -> None:
 class _OnDevice:
     """Where a call's kernels and scratch go."""
 
-    device: torch.device
+    device: "torch.device"
 
     def _call(self, tensors, run, stream):
         """run(stream handle, scratch) on this object's device; scratch(n)

@@ -16,6 +16,7 @@ raise ValueError before anything is queued.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional
 
 from . import _lib as L
@@ -26,20 +27,29 @@ except ImportError:  # pragma: no cover - torch is part of the image
     torch = None
 
 
+# A step of few rows is as long as its calls take to queue, so what a call has
+# to check is checked in few steps, and the addresses of an object's own tensors
+# are taken when it is made.
+
+
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
 
 
 def _ids(t, dtype, n: int, name: str) -> None:
-    _need(t.dtype == dtype and t.dim() == 1 and t.is_contiguous() and t.shape[0] == n,
-          f"{name} must be a contiguous {str(dtype)[6:]} tensor of {n}")
+    if t.dtype != dtype or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {str(dtype)[6:]} tensor of {n}")
 
 
-def _rows(t, rows: int, cols: int, name: str) -> None:
-    _need(t.dtype == torch.float32 and t.dim() == 2 and t.shape[0] == rows and t.shape[1] == cols
-          and (cols == 1 or t.stride(1) == 1) and (rows <= 1 or t.stride(0) >= 0),
-          f"{name} must be float32 [{rows}, {cols}] with contiguous rows")
+def _rows(t, rows: int, cols: int, name: str) -> int:
+    """The row stride of float32 [rows, cols] with contiguous rows."""
+    if t.dtype != torch.float32 or t.shape != (rows, cols):
+        raise ValueError(f"{name} must be float32 [{rows}, {cols}]")
+    st = t.stride()
+    if (st[1] != 1 and cols > 1) or (st[0] < cols and rows > 1):
+        raise ValueError(f"{name} must have contiguous rows that do not overlap: strides {st}")
+    return st[0]
 
 
 class _OnDevice:
@@ -47,32 +57,43 @@ class _OnDevice:
 
     device: "torch.device"
 
-    def _call(self, tensors, run, stream):
-        """run(stream handle, scratch) on this object's device; scratch(n)
-        gives n bytes that the call's stream owns."""
-        dev = self.device
+    def _check_device(self, *tensors) -> None:
+        index = self._index
         for t in tensors:
-            if t is not None and t.device != dev:
-                raise ValueError(f"a tensor on {t.device}; the cache is on {dev}")
-        if dev.type != "cuda":
-            raise ValueError(f"a cache on {dev}: the kernels run on the GPU")
-        if torch.cuda.current_device() != dev.index:
-            with torch.cuda.device(dev):
-                return self._call(tensors, run, stream)
-        mine = torch.cuda.current_stream().cuda_stream
-        sp = mine if stream is None else stream if type(stream) is int else stream.cuda_stream
+            if t.get_device() != index:
+                raise ValueError(f"a tensor on {t.device}; this is on {self.device}")
+        if index < 0:
+            raise ValueError(f"tensors on {self.device}: the kernels run on the GPU")
 
-        def scratch(n: int):
-            # The caching allocator hands a freed block to later work of the
-            # stream it was allocated on: the call's own, whichever is current.
-            # Inside a capture it comes from the graph's own pool.
-            if sp == mine:
-                return torch.empty(n, dtype=torch.uint8, device=dev)
-            s = torch.cuda.ExternalStream(sp, device=dev) if sp else torch.cuda.default_stream(dev)
-            with torch.cuda.stream(s):
-                return torch.empty(n, dtype=torch.uint8, device=dev)
+    def _on(self, stream) -> int:
+        """The call's stream handle: torch's current one of this object's
+        device when None."""
+        if stream is None:
+            return torch._C._cuda_getCurrentRawStream(self._index)
+        return stream if type(stream) is int else stream.cuda_stream
 
-        return run(sp, scratch)
+    def _scratch(self, n: int, sp: int):
+        """n bytes that stream sp owns.  The caching allocator hands a freed
+        block to later work of the stream it was allocated on: the call's own,
+        whichever is current.  Inside a capture it comes from the graph's own
+        pool."""
+        if sp == torch._C._cuda_getCurrentRawStream(self._index):
+            return torch.empty(n, dtype=torch.uint8, device=self.device)
+        s = torch.cuda.ExternalStream(sp, device=self.device) if sp else torch.cuda.default_stream(self.device)
+        with torch.cuda.stream(s):
+            return torch.empty(n, dtype=torch.uint8, device=self.device)
+
+
+def _on_its_device(call):
+    """Run a method with its object's device current."""
+    @functools.wraps(call)
+    def run(self, *args, **kw):
+        index = self._index
+        if index < 0 or torch._C._cuda_getDevice() == index:
+            return call(self, *args, **kw)
+        with torch.cuda.device(index):
+            return call(self, *args, **kw)
+    return run
 
 
 class Rows:
@@ -88,6 +109,10 @@ class Rows:
         _ids(row_start, torch.int32, status.shape[0] + 1, "row_start")
         _ids(status, torch.int32, status.shape[0], "status")
         self.row_start, self.seq, self.pos, self.slot, self.status = row_start, seq, pos, slot, status
+        self.device, self._index = seq.device, seq.get_device()
+        _need(all(t.device == self.device for t in (pos, slot, row_start, status)), "rows on several devices")
+        self._args = (n, row_start.data_ptr(), seq.data_ptr(), pos.data_ptr(), slot.data_ptr(), status.data_ptr())
+        self.n_seq = status.shape[0]
 
     @staticmethod
     def new(n_seq: int, rows: int, device) -> "Rows":
@@ -107,8 +132,11 @@ class PageTable(_OnDevice):
         _ids(ring, torch.int32, ring.shape[0], "ring")
         _ids(state, torch.int32, 2, "state")
         self.table, self.length, self.ring, self.state, self.page = table, length, ring, state, page
-        self.device = table.device
-        self._scratch = 0
+        self.device, self._index = table.device, table.get_device()
+        _need(all(t.device == self.device for t in (length, ring, state)), "a table on several devices")
+        self._where = (table.data_ptr(), table.shape[1], page, ring.data_ptr(), ring.shape[0])
+        self._now = (length.data_ptr(), state.data_ptr())
+        self._bytes = 0
 
     @staticmethod
     def new(n_seq: int, max_pages: int, n_pages: int, page: int, device) -> "PageTable":
@@ -118,6 +146,7 @@ class PageTable(_OnDevice):
                          torch.arange(n_pages, dtype=torch.int32, device=device),
                          torch.tensor([0, n_pages], dtype=torch.int32, device=device), page)
 
+    @_on_its_device
     def advance(self, add, rows: Rows, out: Optional["PageTable"] = None, stream=None) -> Rows:
         """Give sequence i add[i] more positions (int32; below 0: end it and
         free its pages) and fill `rows` (moe_pages_advance).  The new lengths
@@ -126,27 +155,19 @@ class PageTable(_OnDevice):
         out = self if out is None else out
         n = self.table.shape[0]
         _ids(add, torch.int32, n, "add")
-        _need(rows.status.shape[0] == n, f"rows of {rows.status.shape[0]} sequences, the table has {n}")
-        _need(out is self or (out.table.data_ptr() == self.table.data_ptr() and out.page == self.page
-                              and out.table.shape == self.table.shape and out.ring.shape == self.ring.shape
-                              and out.ring.data_ptr() == self.ring.data_ptr()), "out has another table or ring")
-        if not self._scratch:
+        _need(rows.n_seq == n, f"rows of {rows.n_seq} sequences, the table has {n}")
+        _need(out._where == self._where, "out has another table or ring")
+        self._check_device(add, rows.seq)
+        if not self._bytes:
             b = C.c_uint64()
             L.check(L.lib().moe_pages_workspace_size(n, C.byref(b)), "moe_pages_workspace_size")
-            self._scratch = b.value
-
-        def run(sp, scratch):
-            ws = scratch(self._scratch)
-            rc = L.lib().moe_pages_advance(
-                n, self.length.data_ptr(), add.data_ptr(), out.length.data_ptr(), self.table.data_ptr(),
-                self.table.shape[1], self.page, self.ring.data_ptr(), self.ring.shape[0], self.state.data_ptr(),
-                out.state.data_ptr(), rows.seq.shape[0], rows.row_start.data_ptr(), rows.seq.data_ptr(),
-                rows.pos.data_ptr(), rows.slot.data_ptr(), rows.status.data_ptr(), ws.data_ptr(), self._scratch, sp)
-            if rc:
-                L.check(rc, "moe_pages_advance")
-
-        self._call((add, rows.seq, rows.pos, rows.slot, rows.row_start, rows.status, self.length, self.ring, self.state,
-                    out.length, out.state), run, stream)
+            self._bytes = b.value
+        sp = self._on(stream)
+        ws = self._scratch(self._bytes, sp)
+        rc = L.lib().moe_pages_advance(n, self._now[0], add.data_ptr(), out._now[0], *self._where, self._now[1],
+                                       out._now[1], *rows._args, ws.data_ptr(), self._bytes, sp)
+        if rc:
+            L.check(rc, "moe_pages_advance")
         return rows
 
 
@@ -167,7 +188,9 @@ class KvCache(_OnDevice):
                   f"means must be a contiguous float16 [{n_pages}, {n_kv}, {qd}] tensor")
         self.pool, self.table, self.means = pool, table, means
         self.n_kv, self.qd, self.vd, self.page, self.n_pages = n_kv, qd, vd, page, n_pages
-        self.device = pool.device
+        self.device, self._index = pool.device, pool.get_device()
+        _need(table.device == pool.device and (means is None or means.device == pool.device),
+              "a cache on several devices")
         self.c = L.Kv4C(pool=pool.data_ptr(), pool_bytes=pool.shape[0], table=table.data_ptr(),
                         means=None if means is None else means.data_ptr(), n_seq=table.shape[0],
                         max_pages=table.shape[1], n_pages=n_pages, page=page, n_kv=n_kv, qd=qd, vd=vd)
@@ -202,52 +225,51 @@ class KvCache(_OnDevice):
             n = self._sizes[name, args] = b.value
         return n
 
+    @_on_its_device
     def store(self, k, v, slots, stream=None) -> None:
         """Write rows k [rows, kv heads * key width], v [rows, kv heads *
         value width] (float32) into `slots` (int64, distinct; rows of negative
         slots are skipped)."""
         n = k.shape[0]
-        _rows(k, n, self.n_kv * self.qd, "k")
-        _rows(v, n, self.n_kv * self.vd, "v")
+        ks, vs = _rows(k, n, self.n_kv * self.qd, "k"), _rows(v, n, self.n_kv * self.vd, "v")
         _ids(slots, torch.int64, n, "slots")
+        self._check_device(k, v, slots)
+        rc = L.lib().moe_kv4_store(self._c, k.data_ptr(), ks, v.data_ptr(), vs, n, slots.data_ptr(), self._on(stream))
+        if rc:
+            L.check(rc, "moe_kv4_store")
 
-        def run(sp, scratch):
-            rc = L.lib().moe_kv4_store(self._c, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), n,
-                                       slots.data_ptr(), sp)
-            if rc:
-                L.check(rc, "moe_kv4_store")
-
-        self._call((k, v, slots, self.table, self.means), run, stream)
-
+    @_on_its_device
     def load(self, slots, k=None, v=None, stream=None) -> None:
         """Read the rows of `slots` into k and v (float32, either may be
         None); rows of negative slots are left as they were."""
         n = slots.shape[0]
         _ids(slots, torch.int64, n, "slots")
-        if k is not None:
-            _rows(k, n, self.n_kv * self.qd, "k")
-        if v is not None:
-            _rows(v, n, self.n_kv * self.vd, "v")
+        ks = 0 if k is None else _rows(k, n, self.n_kv * self.qd, "k")
+        vs = 0 if v is None else _rows(v, n, self.n_kv * self.vd, "v")
+        self._check_device(slots, *(t for t in (k, v) if t is not None))
+        rc = L.lib().moe_kv4_load(self._c, slots.data_ptr(), n, None if k is None else k.data_ptr(), ks,
+                                  None if v is None else v.data_ptr(), vs, self._on(stream))
+        if rc:
+            L.check(rc, "moe_kv4_load")
 
-        def run(sp, scratch):
-            rc = L.lib().moe_kv4_load(self._c, slots.data_ptr(), n, None if k is None else k.data_ptr(),
-                                      0 if k is None else k.stride(0), None if v is None else v.data_ptr(),
-                                      0 if v is None else v.stride(0), sp)
-            if rc:
-                L.check(rc, "moe_kv4_load")
-
-        self._call((slots, k, v, self.table), run, stream)
-
-    def _query(self, q, seq, pos) -> int:
-        n = q.shape[0]
-        heads = q.shape[1] // self.qd
-        _need(heads >= 1 and heads % self.n_kv == 0, f"queries of {q.shape[1]} values: not a multiple of {self.n_kv} kv "
-              f"heads of {self.qd}")
-        _rows(q, n, heads * self.qd, "q")
+    def _query(self, q, seq, pos):
+        """(rows, heads, row stride) of a call's queries."""
+        n, width = q.shape if q.dim() == 2 else (-1, 0)
+        heads = width // self.qd
+        if heads < 1 or heads % self.n_kv:
+            raise ValueError(f"queries of {tuple(q.shape)}: rows of a multiple of {self.n_kv} heads of {self.qd}")
+        qs = _rows(q, n, heads * self.qd, "q")
         _ids(seq, torch.int32, n, "seq")
         _ids(pos, torch.int32, n, "pos")
-        return heads
+        return n, heads, qs
 
+    def _lists(self, t, n: int, name: str) -> int:
+        if t.dtype != torch.int32 or t.dim() != 3 or t.shape[:2] != (n, self.n_kv) or t.shape[2] < 1 or \
+                not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 [{n}, {self.n_kv}, pages] tensor")
+        return t.shape[2]
+
+    @_on_its_device
     def attend(self, q, seq, pos, out, *, max_pos: int, scale: float, window: int = 0, pages=None, stream=None) -> None:
         """Causal attention of rows q [rows, heads * key width] into out
         [rows, heads * value width] (moe_kv4_attention): row r of sequence
@@ -255,49 +277,39 @@ class KvCache(_OnDevice):
         max_pos, over the last `window` positions when that is above 0, over
         the pages `pages` lists (select's int32 [rows, kv heads, n]) when
         given."""
-        heads = self._query(q, seq, pos)
-        n = q.shape[0]
-        _rows(out, n, heads * self.vd, "out")
-        n_sel = 0
-        if pages is not None:
-            _need(pages.dtype == torch.int32 and pages.dim() == 3 and pages.is_contiguous()
-                  and pages.shape[0] == n and pages.shape[1] == self.n_kv and pages.shape[2] >= 1,
-                  f"pages must be a contiguous int32 [{n}, {self.n_kv}, pages] tensor")
-            n_sel = pages.shape[2]
+        n, heads, qs = self._query(q, seq, pos)
+        os = _rows(out, n, heads * self.vd, "out")
+        if pages is None:
+            n_sel, lists = 0, None
+            self._check_device(q, seq, pos, out)
+        else:
+            n_sel, lists = self._lists(pages, n, "pages"), pages.data_ptr()
+            self._check_device(q, seq, pos, out, pages)
         need = self._size("moe_kv4_attention_workspace_size", n, heads, max_pos, window, n_sel)
+        sp = self._on(stream)
+        ws = self._scratch(need, sp) if need else None
+        rc = L.lib().moe_kv4_attention(self._c, q.data_ptr(), qs, n, heads, scale, seq.data_ptr(), pos.data_ptr(), max_pos,
+                                       window, lists, n_sel, out.data_ptr(), os, ws.data_ptr() if need else None, need, sp)
+        if rc:
+            L.check(rc, "moe_kv4_attention")
 
-        def run(sp, scratch):
-            ws = scratch(need) if need else None
-            rc = L.lib().moe_kv4_attention(self._c, q.data_ptr(), q.stride(0), n, heads, scale, seq.data_ptr(),
-                                           pos.data_ptr(), max_pos, window, None if pages is None else pages.data_ptr(),
-                                           n_sel, out.data_ptr(), out.stride(0), None if ws is None else ws.data_ptr(),
-                                           need, sp)
-            if rc:
-                L.check(rc, "moe_kv4_attention")
-
-        self._call((q, seq, pos, out, pages, self.table), run, stream)
-
+    @_on_its_device
     def select(self, q, seq, pos, lists, *, max_pos: int, sinks: int = 1, recent: int = 1, stream=None):
         """Fill lists (int32 [rows, kv heads, n]) with the n pages each row
         and kv head reads (moe_kv4_select): the first `sinks`, the last
         `recent`, then by score; -1 behind the last."""
-        _need(self.means is not None, "the cache keeps no mean keys")
-        heads = self._query(q, seq, pos)
-        n = q.shape[0]
-        _need(lists.dtype == torch.int32 and lists.dim() == 3 and lists.is_contiguous()
-              and lists.shape[0] == n and lists.shape[1] == self.n_kv and lists.shape[2] >= 1,
-              f"lists must be a contiguous int32 [{n}, {self.n_kv}, pages] tensor")
-        _need(sinks >= 0 and recent >= 1 and sinks + recent <= lists.shape[2],
-              f"{sinks} first and {recent} last pages of {lists.shape[2]}")
+        if self.means is None:
+            raise ValueError("the cache keeps no mean keys")
+        n, heads, qs = self._query(q, seq, pos)
+        n_sel = self._lists(lists, n, "lists")
+        if sinks < 0 or recent < 1 or sinks + recent > n_sel:
+            raise ValueError(f"{sinks} first and {recent} last pages of {n_sel}")
+        self._check_device(q, seq, pos, lists)
         need = self._size("moe_kv4_select_workspace_size", n, max_pos)
-
-        def run(sp, scratch):
-            ws = scratch(max(need, 16))
-            rc = L.lib().moe_kv4_select(self._c, q.data_ptr(), q.stride(0), n, heads, seq.data_ptr(), pos.data_ptr(),
-                                        max_pos, sinks, recent, lists.shape[2], lists.data_ptr(), ws.data_ptr(), need,
-                                        sp)
-            if rc:
-                L.check(rc, "moe_kv4_select")
-
-        self._call((q, seq, pos, lists, self.table, self.means), run, stream)
+        sp = self._on(stream)
+        ws = self._scratch(need, sp) if need else None
+        rc = L.lib().moe_kv4_select(self._c, q.data_ptr(), qs, n, heads, seq.data_ptr(), pos.data_ptr(), max_pos, sinks,
+                                    recent, n_sel, lists.data_ptr(), ws.data_ptr() if need else None, need, sp)
+        if rc:
+            L.check(rc, "moe_kv4_select")
         return lists

@@ -651,7 +651,17 @@ Plan plan_of(const Kv4 &c, int rows, int heads, int max_pos, int window, int n_s
     const long long tiles = n_sel ? (long long)n_sel * c.tiles()
                                   : (window > 0 ? std::min((long long)window + p.tt, (long long)max_pos + 1) : max_pos + 1LL) / 32 + 1;
     const long long units = base * p.split;
-    p.ps = (int)std::max<long long>(1, std::min<long long>({(1024 + units - 1) / units, tiles / 16, 256}));
+    // Parts of a run's tiles.  A block costs about as much as 8 tiles of a wave
+    // before its first and after its last, and parts a launch that joins them
+    // (5 us): with a block for every CU they pay for long runs only, below that
+    // from 12 tiles a wave on.  (Kernel + join: 512 blocks of 19 to 38 tiles
+    // 28.2 us, in two parts 34 + 4.6; 488 of 64 tiles 34.5, 39.4 + 4.8; 512 of
+    // 190 to 375 152.6, 152.3 + 4.8; 8 of 3126 tiles in 64, 128, 256 parts 60.8 +
+    // 5.7, 36.8 + 5.0, 32.4 + 5.6.)
+    const long long ps = units >= 256 ? std::min((512 + units - 1) / units, tiles / 64)
+                         : tiles < 48 ? 1
+                                      : std::min<long long>({(2048 + units - 1) / units, tiles / 12, 256});
+    p.ps = (int)std::max<long long>(1, ps);
     p.bytes = p.ps > 1 ? (uint64_t)rows * heads * p.ps * (c.vd + 2) * 4 : 0;
     return p;
 }

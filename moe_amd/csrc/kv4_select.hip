@@ -29,6 +29,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef double f64x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 
+constexpr int kThreads = 512;
 constexpr int kHeads = 4;        // query heads scored at once
 constexpr int kLdsPages = 4096;  // scores a block keeps in LDS (32 KiB)
 
@@ -50,7 +51,7 @@ __device__ inline uint64_t order_of(double s) {
     return b < 0 ? ~(uint64_t)b : (uint64_t)b | 0x8000000000000000ull;
 }
 
-// The keys of pages [j0, j1) of a (row, kv head) by 256 threads into out[j -
+// The keys of pages [j0, j1) of a (row, kv head) by the block into out[j -
 // j0].  cur: the row's own page.  qs: LDS of kHeads * qd doubles.
 template <int QC>
 __device__ inline void score_pages(const Args &a, int row, int kv, int sid, int cur, int j0, int j1, double *qs,
@@ -61,26 +62,47 @@ __device__ inline void score_pages(const Args &a, int row, int kv, int sid, int 
     for (int h0 = 0; h0 < a.rep; h0 += kHeads) {
         const int hn = min(kHeads, a.rep - h0);
         __syncthreads();  // the reads of the heads before
-        for (int i = threadIdx.x; i < kHeads * c.qd; i += 256) {
+        for (int i = threadIdx.x; i < kHeads * c.qd; i += kThreads) {
             const int h = min(i / c.qd, hn - 1), d = i % c.qd;  // past the last head: the last again
             qs[i] = (double)gload(a.q + (size_t)row * a.q_stride + (size_t)(kv * a.rep + h0 + h) * c.qd + d);
         }
         __syncthreads();
-        // 16 pages a wave, twice.
-        for (int base = j0 + wave * 32; base < j1; base += 128) {
-            const int j[2] = {base + (lane >> 2), base + 16 + (lane >> 2)};
-            half8 m[2][QC];
-            bool has[2];
+        // 16 pages a wave, twice.  The means of the next 32 load while these are
+        // scored, the table's entries of those after them before.
+        constexpr int kStep = kThreads / 64 * 32;
+        int id[2];
+        half8 m[2][QC], mn[2][QC];
+        bool has[2], hasn[2];
+        auto load_ids = [&](int base) __attribute__((always_inline)) {
 #pragma unroll
             for (int p = 0; p < 2; p++) {
-                const bool want = j[p] < j1 && j[p] <= cur && j[p] >= a.sinks && j[p] <= cur - a.recent;
-                const int id = want ? gload(table + j[p]) : -1;
-                has[p] = (unsigned)id < (unsigned)c.n_pages;
-                const __half *mean = c.means + ((size_t)(has[p] ? id : 0) * c.n_kv + kv) * c.qd;
+                const int j = base + 16 * p + (lane >> 2);
+                id[p] = j < j1 && j >= a.sinks && j <= cur - a.recent ? gload(table + j) : -1;
+            }
+        };
+        auto load_means = [&](half8 (&m)[2][QC], bool (&has)[2]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                has[p] = (unsigned)id[p] < (unsigned)c.n_pages;
+                const __half *mean = c.means + ((size_t)(has[p] ? id[p] : 0) * c.n_kv + kv) * c.qd;
 #pragma unroll
                 for (int s = 0; s < QC; s++)
                     if (s < nq) m[p][s] = gload((const half8 *)(mean + 32 * s + 8 * e));
             }
+        };
+        load_ids(j0 + wave * 32);
+        load_means(mn, hasn);
+        load_ids(j0 + wave * 32 + kStep);
+        for (int base = j0 + wave * 32; base < j1; base += kStep) {
+            const int j[2] = {base + (lane >> 2), base + 16 + (lane >> 2)};
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                has[p] = hasn[p];
+#pragma unroll
+                for (int s = 0; s < QC; s++) m[p][s] = mn[p][s];
+            }
+            load_means(mn, hasn);
+            load_ids(base + 2 * kStep);
             double acc[2][kHeads];
 #pragma unroll
             for (int h = 0; h < kHeads; h++) acc[0][h] = acc[1][h] = 0.0;
@@ -124,18 +146,18 @@ __device__ inline void score_pages(const Args &a, int row, int kv, int sid, int 
 }
 
 // The first n_sel of n keys in their order, equal ones by index, as ascending
-// indices into list; 256 threads.
+// indices into list.
 __device__ inline void pick(const uint64_t *keys, int n, int n_sel, int32_t *list) {
-    __shared__ int hist[256], found[4];
+    __shared__ int hist[256], found[kThreads / 64];
     __shared__ int s_digit, s_above, s_here;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint64_t prefix = 0, mask = 0;
     int want = n_sel;  // how many of those that agree with prefix
     bool all = false;  // every one that does
     for (int shift = 56; shift >= 0 && !all; shift -= 8) {
-        hist[threadIdx.x] = 0;
+        if (threadIdx.x < 256) hist[threadIdx.x] = 0;
         __syncthreads();
-        for (int j = threadIdx.x; j < n; j += 256) {
+        for (int j = threadIdx.x; j < n; j += kThreads) {
             const uint64_t k = keys[j];
             if (k != 0 && (k & mask) == prefix) atomicAdd(hist + (int)(k >> shift & 255), 1);
         }
@@ -174,7 +196,7 @@ __device__ inline void pick(const uint64_t *keys, int n, int n_sel, int32_t *lis
         }
     }
     int before = 0, ties = 0;  // chosen pages and those equal to the last one, so far
-    for (int base = 0; base < n; base += 256) {
+    for (int base = 0; base < n; base += kThreads) {
         const int j = base + threadIdx.x;
         const uint64_t k = j < n ? keys[j] : 0;
         const bool edge = k != 0 && (k & mask) == prefix;
@@ -189,7 +211,7 @@ __device__ inline void pick(const uint64_t *keys, int n, int n_sel, int32_t *lis
             int at = ties + __popcll(b & ((1ull << lane) - 1));
             for (int w = 0; w < wave; w++) at += found[w];
             in |= edge && at < want;
-            ties += found[0] + found[1] + found[2] + found[3];
+            for (int w = 0; w < kThreads / 64; w++) ties += found[w];
         }
         const unsigned long long b = __ballot(in);
         __syncthreads();
@@ -198,26 +220,26 @@ __device__ inline void pick(const uint64_t *keys, int n, int n_sel, int32_t *lis
         int at = before + __popcll(b & ((1ull << lane) - 1));
         for (int w = 0; w < wave; w++) at += found[w];
         if (in && at < n_sel) list[at] = j;
-        before += found[0] + found[1] + found[2] + found[3];
+        for (int w = 0; w < kThreads / 64; w++) before += found[w];
     }
-    for (int i = before + (int)threadIdx.x; i < n_sel; i += 256) list[i] = -1;
+    for (int i = before + (int)threadIdx.x; i < n_sel; i += kThreads) list[i] = -1;
 }
 
 // FUSED: score and pick; otherwise pick from the workspace's keys.
 template <int QC, bool FUSED>
-__global__ __launch_bounds__(256) void kv4_select_kernel(const Args a) {
+__global__ __launch_bounds__(kThreads) void kv4_select_kernel(const Args a) {
     __shared__ uint64_t keys[FUSED ? kLdsPages : 1];
     __shared__ double qs[FUSED ? kHeads * QC * 32 : 1];
     const int row = blockIdx.x / a.n_kv, kv = blockIdx.x % a.n_kv;
     int32_t *list = a.lists + (size_t)blockIdx.x * a.n_sel;
     const int sid = gload(a.seq + row), top = gload(a.pos + row);
     if (top < 0 || (unsigned)sid >= (unsigned)a.c.n_seq) {
-        for (int i = threadIdx.x; i < a.n_sel; i += 256) list[i] = -1;
+        for (int i = threadIdx.x; i < a.n_sel; i += kThreads) list[i] = -1;
         return;
     }
     const int cur = min(top >> a.c.page_shift, a.n - 1);
     if (cur < a.n_sel) {  // every page
-        for (int i = threadIdx.x; i < a.n_sel; i += 256) list[i] = i <= cur ? i : -1;
+        for (int i = threadIdx.x; i < a.n_sel; i += kThreads) list[i] = i <= cur ? i : -1;
         return;
     }
     if (FUSED) {
@@ -230,7 +252,7 @@ __global__ __launch_bounds__(256) void kv4_select_kernel(const Args a) {
 
 constexpr int kScorePages = 256;  // pages of a block of kv4_score_kernel
 template <int QC>
-__global__ __launch_bounds__(256) void kv4_score_kernel(const Args a) {
+__global__ __launch_bounds__(kThreads) void kv4_score_kernel(const Args a) {
     __shared__ double qs[kHeads * QC * 32];
     const int row = blockIdx.x / a.n_kv, kv = blockIdx.x % a.n_kv;
     const int sid = gload(a.seq + row), top = gload(a.pos + row);
@@ -248,10 +270,10 @@ template <int QC>
 void launch(const Args &a, int rows, hipStream_t s) {
     const unsigned pairs = (unsigned)rows * a.n_kv;
     if (apart(pairs, a.n)) {
-        hipLaunchKernelGGL((kv4_score_kernel<QC>), dim3(pairs, (a.n + kScorePages - 1) / kScorePages), dim3(256), 0, s, a);
-        hipLaunchKernelGGL((kv4_select_kernel<QC, false>), dim3(pairs), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((kv4_score_kernel<QC>), dim3(pairs, (a.n + kScorePages - 1) / kScorePages), dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL((kv4_select_kernel<QC, false>), dim3(pairs), dim3(kThreads), 0, s, a);
     } else {
-        hipLaunchKernelGGL((kv4_select_kernel<QC, true>), dim3(pairs), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((kv4_select_kernel<QC, true>), dim3(pairs), dim3(kThreads), 0, s, a);
     }
 }
 

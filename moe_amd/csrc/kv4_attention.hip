@@ -338,57 +338,53 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
         // instructions a column tile.  With `once` copy k of the columns takes
         // block k's scales, all blocks' products are made at once, and of what
         // comes out only copy b's columns of block b are read.
-        auto second = [&](const T &x, const f32x4 (&p)[C][2], bool inf, auto odd, auto once) __attribute__((always_inline)) {
+        auto second = [&](const T &x, const f32x4 (&p)[C][2], auto once) __attribute__((always_inline)) {
             const u32x4 *sc = (const u32x4 *)ssc[wave];
-            uint32_t keep[C][4] = {};
-            if (odd) {
-                // (one column tile: masks that keep all, where there is nothing
-                // to hide, cost four instructions; two: a path of its own)
-                const bool hide = C > 1 || __any(inf);
-#pragma unroll
-                for (int i = 0; i < 4; i++) keep[0][i] = 0xffffffffu;
-                if (hide)
-#pragma unroll
-                for (int c = 0; c < C; c++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        keep[c][i] = (p[c][i >> 1][2 * i & 3] == 0.0f ? 0 : 0xffffu) |
-                                     (p[c][i >> 1][(2 * i & 3) + 1] == 0.0f ? 0 : 0xffff0000u);
-            }
-            half8 h8[C], l8[C];
+            half8 h8[C], l8[C], v0, v1;
             // Weights times scales in the codes' order, bytes 0, 2, 1, 3 of
             // each half; both pieces.
-            auto scaled = [&](int c, const u32x4 &ds) __attribute__((always_inline)) {
-                half2v ph[4], pl[4];
+            auto scaled = [&](const u32x4 &ds) __attribute__((always_inline)) {
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const half2v d0 = as_h2(odd ? ds[2 * h] & keep[c][2 * h] : ds[2 * h]);
-                    const half2v d1 = as_h2(odd ? ds[2 * h + 1] & keep[c][2 * h + 1] : ds[2 * h + 1]);
+                for (int c = 0; c < C; c++) {
+                    half2v ph[4], pl[4];
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const float u = fmaf((float)d0[e], p[c][h][e], 0.0f), w = fmaf((float)d1[e], p[c][h][2 + e], 0.0f);
-                        const half2v z = pack_half(u, w);
-                        ph[2 * h + e] = z;
-                        pl[2 * h + e] = pack_half(fmaf((float)z[0], less, u), fmaf((float)z[1], less, w));
+                    for (int h = 0; h < 2; h++) {
+                        const half2v d0 = as_h2(ds[2 * h]), d1 = as_h2(ds[2 * h + 1]);
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float u = fmaf((float)d0[e], p[c][h][e], 0.0f), w = fmaf((float)d1[e], p[c][h][2 + e], 0.0f);
+                            const half2v z = pack_half(u, w);
+                            ph[2 * h + e] = z;
+                            pl[2 * h + e] = pack_half(fmaf((float)z[0], less, u), fmaf((float)z[1], less, w));
+                        }
                     }
+                    h8[c] = join8(ph[0], ph[1], ph[2], ph[3]), l8[c] = join8(pl[0], pl[1], pl[2], pl[3]);
                 }
-                h8[c] = join8(ph[0], ph[1], ph[2], ph[3]), l8[c] = join8(pl[0], pl[1], pl[2], pl[3]);
             };
-            if (once) scaled(0, sc[(nq + copy) * 4 + g]);
+            auto unpack = [&](int b) __attribute__((always_inline)) {
+                const uint32_t w0 = x.v[2 * b], w1 = x.v[2 * b + 1];
+                v0 = join8(low_pair(w0, nib), low_pair(w0 >> 8, nib), low_pair(w1, nib), low_pair(w1 >> 8, nib));
+                v1 = join8(high_pair(w0, nib), high_pair(w0 >> 8, nib), high_pair(w1, nib), high_pair(w1 >> 8, nib));
+            };
+            scaled(sc[(nq + (once ? copy : 0)) * 4 + g]);
+            unpack(0);
 #pragma unroll
             for (int b = 0; b < VC; b++) {
                 if (!EX && b >= nv) continue;
-                const uint32_t w0 = x.v[2 * b], w1 = x.v[2 * b + 1];
-                const half8 v0 = join8(low_pair(w0, nib), low_pair(w0 >> 8, nib), low_pair(w1, nib), low_pair(w1 >> 8, nib));
-                const half8 v1 = join8(high_pair(w0, nib), high_pair(w0 >> 8, nib), high_pair(w1, nib), high_pair(w1 >> 8, nib));
-                const u32x4 ds = sc[(nq + b) * 4 + g];
 #pragma unroll
                 for (int c = 0; c < C; c++) {
-                    if (!once) scaled(c, ds);
                     o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, h8[c], o[c][b][0], 0, 0, 0);
                     o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, h8[c], o[c][b][1], 0, 0, 0);
+                }
+#pragma unroll
+                for (int c = 0; c < C; c++) {
                     o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, l8[c], o[c][b][0], 0, 0, 0);
                     o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, l8[c], o[c][b][1], 0, 0, 0);
+                }
+                // The next block's operands while these products run.
+                if (b + 1 < VC && (EX || b + 1 < nv)) {
+                    unpack(b + 1);
+                    if (!once) scaled(sc[(nq + b + 1) * 4 + g]);
                 }
                 if (C > 1) __builtin_amdgcn_sched_barrier(0);
             }
@@ -412,6 +408,18 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
             f32x4 s[C][2];
 #pragma unroll
             for (int c = 0; c < C; c++) s[c][0] = s[c][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            // A block's sums are scaled while the next block's products run.
+            half8 dp;
+            f32x4 rp[C][2];
+            auto scale = [&] __attribute__((always_inline)) {
+#pragma unroll
+                for (int c = 0; c < C; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        s[c][0][i] = fmaf((float)dp[i], rp[c][0][i], s[c][0][i]);
+                        s[c][1][i] = fmaf((float)dp[4 + i], rp[c][1][i], s[c][1][i]);
+                    }
+            };
 #pragma unroll
             for (int b = 0; b < QC; b++) {
                 if (!EX && b >= nq) continue;
@@ -419,23 +427,23 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                 const uint32_t w0 = x.k[2 * b], w1 = x.k[2 * b + 1];
                 const half8 k0 = join8(low_pair(w0, nib), low_pair(w0 >> 8, nib), high_pair(w0, nib), high_pair(w0 >> 8, nib));
                 const half8 k1 = join8(low_pair(w1, nib), low_pair(w1 >> 8, nib), high_pair(w1, nib), high_pair(w1 >> 8, nib));
+                f32x4 r[C][2];
 #pragma unroll
-                for (int c = 0; c < C; c++) {
-                    const half8 qh = __builtin_bit_cast(half8, sq_[((c * QC + b) * 2) * 64 + ql_at]);
-                    const half8 ql = __builtin_bit_cast(half8, sq_[((c * QC + b) * 2 + 1) * 64 + ql_at]);
-                    const f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
-                    f32x4 r = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql, z, 0, 0, 0);
-                    f32x4 t = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql, z, 0, 0, 0);
-                    r = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh, r, 0, 0, 0);
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh, t, 0, 0, 0);
+                for (int i = 0; i < 2; i++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        s[c][0][i] = fmaf((float)d[i], r[i], s[c][0][i]);
-                        s[c][1][i] = fmaf((float)d[4 + i], t[i], s[c][1][i]);
+                    for (int c = 0; c < C; c++) {
+                        const half8 q = __builtin_bit_cast(half8, sq_[((c * QC + b) * 2 + 1 - i) * 64 + ql_at]);
+                        const f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+                        r[c][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q, i ? r[c][0] : z, 0, 0, 0);
+                        r[c][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q, i ? r[c][1] : z, 0, 0, 0);
                     }
-                }
+                if (b > 0) scale();
+                dp = d;
+#pragma unroll
+                for (int c = 0; c < C; c++) rp[c][0] = r[c][0], rp[c][1] = r[c][1];
                 if (C > 1) __builtin_amdgcn_sched_barrier(0);
             }
+            scale();
             between();
             // Positions a column does not see.
             bool some = false;
@@ -490,11 +498,36 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                     s[c][i >> 2][i & 3] = p;
                     l[c] += p;
                 }
-            // A position of weight 0 may hold an infinity or a NaN: such tiles
-            // read its scales as 0.
-            if (C == 1) second(x, s, inf, std::true_type{}, once);
-            else if (__builtin_expect(__any(inf), 0)) second(x, s, inf, std::true_type{}, once);
-            else second(x, s, inf, std::false_type{}, once);
+            // Scales that are infinite or NaN (rare): positions of weight 0 may
+            // hold them, so they become 0, and what a column does see of them
+            // makes the block's 32 values NaN.
+            if (__builtin_expect(__any(inf), 0)) {
+#pragma unroll
+                for (int b = 0; b < VC; b++) {
+                    if (!EX && b >= nv) continue;
+                    const u32x4 y = sc[(nq + (once ? copy : b)) * 4 + g];
+#pragma unroll
+                    for (int c = 0; c < C; c++) {
+                        int bad = 0;
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            bad |= (y[i >> 1] >> (16 * (i & 1)) & 0x7c00u) == 0x7c00u && s[c][i >> 2][i & 3] != 0.0f;
+                        bad |= __shfl_xor(bad, 16, 64);
+                        bad |= __shfl_xor(bad, 32, 64);
+                        const float nan = bad ? __uint_as_float(0x7fc00000u) : 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) o[c][b][0][i] += nan, o[c][b][1][i] += nan;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < T::NS; e++) {
+                    uint32_t y = x.s[e];
+                    if ((y & 0x7c00u) == 0x7c00u) y &= 0xffff0000u;
+                    if ((y & 0x7c000000u) == 0x7c000000u) y &= 0xffffu;
+                    if (lane + 64 * e >= nq * 16) ssc[wave][lane + 64 * e] = y;
+                }
+            }
+            second(x, s, once);
         };
         auto none = [] {};
         auto walk = [&](auto once) __attribute__((always_inline)) {

@@ -90,6 +90,13 @@ __device__ inline float minus_one() {
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ inline half2v pack_half(float a, float b) { return __builtin_convertvector((f32x2{a, b}), half2v); }
 
+// Lanes of a wave hand each other values through LDS: its LDS operations run in
+// order, so only the compiler has to keep them so.
+__device__ inline void lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // A tile's words of a lane.
 template <int QC, int VC>
 struct Tile {
@@ -367,6 +374,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                 v1 = join8(high_pair(w0, nib), high_pair(w0 >> 8, nib), high_pair(w1, nib), high_pair(w1 >> 8, nib));
             };
             scaled(sc[(nq + (once ? copy : 0)) * 4 + g]);
+            u32x4 ds = sc[(nq + min(1, nv - 1)) * 4 + g];  // the next block's, read one ahead
             unpack(0);
 #pragma unroll
             for (int b = 0; b < VC; b++) {
@@ -384,7 +392,11 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                 // The next block's operands while these products run.
                 if (b + 1 < VC && (EX || b + 1 < nv)) {
                     unpack(b + 1);
-                    if (!once) scaled(sc[(nq + b + 1) * 4 + g]);
+                    if (!once) {
+                        const u32x4 y = ds;
+                        if (b + 2 < VC && (EX || b + 2 < nv)) ds = sc[(nq + b + 2) * 4 + g];
+                        scaled(y);
+                    }
                 }
                 if (C > 1) __builtin_amdgcn_sched_barrier(0);
             }
@@ -393,6 +405,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
         auto step = [&](const T &x, int base, auto once, auto between) __attribute__((always_inline)) {
             // Scales through LDS (the wave's own: in order, no barrier): every
             // lane reads its four positions of both halves, 16 bytes.
+            lds_order();       // the reads of the tile before
             uint32_t top = 0;  // the largest finite value scale of the lane's, f16 bits
             bool inf = false;
 #pragma unroll
@@ -404,6 +417,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                 inf |= y0 >= 0x7c00u || y1 >= 0x7c00u;
                 top = max(top, max(y0 >= 0x7c00u ? 0 : y0, y1 >= 0x7c00u ? 0 : y1));
             }
+            lds_order();
             const u32x4 *sc = (const u32x4 *)ssc[wave];
             f32x4 s[C][2];
 #pragma unroll
@@ -420,10 +434,25 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                         s[c][1][i] = fmaf((float)dp[4 + i], rp[c][1][i], s[c][1][i]);
                     }
             };
+            // (reads of LDS one block ahead)
+            u32x4 qn[C][2], dn;
+            auto operands = [&](int b) __attribute__((always_inline)) {
+                dn = sc[b * 4 + g];
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    qn[c][0] = sq_[((c * QC + b) * 2 + 1) * 64 + ql_at];
+                    qn[c][1] = sq_[((c * QC + b) * 2) * 64 + ql_at];
+                }
+            };
+            operands(0);
 #pragma unroll
             for (int b = 0; b < QC; b++) {
                 if (!EX && b >= nq) continue;
-                const half8 d = __builtin_bit_cast(half8, sc[b * 4 + g]);
+                const half8 d = __builtin_bit_cast(half8, dn);
+                u32x4 q[C][2];
+#pragma unroll
+                for (int c = 0; c < C; c++) q[c][0] = qn[c][0], q[c][1] = qn[c][1];
+                if (b + 1 < QC && (EX || b + 1 < nq)) operands(b + 1);
                 const uint32_t w0 = x.k[2 * b], w1 = x.k[2 * b + 1];
                 const half8 k0 = join8(low_pair(w0, nib), low_pair(w0 >> 8, nib), high_pair(w0, nib), high_pair(w0 >> 8, nib));
                 const half8 k1 = join8(low_pair(w1, nib), low_pair(w1 >> 8, nib), high_pair(w1, nib), high_pair(w1 >> 8, nib));
@@ -432,10 +461,10 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                 for (int i = 0; i < 2; i++)
 #pragma unroll
                     for (int c = 0; c < C; c++) {
-                        const half8 q = __builtin_bit_cast(half8, sq_[((c * QC + b) * 2 + 1 - i) * 64 + ql_at]);
+                        const half8 qq = __builtin_bit_cast(half8, q[c][i]);
                         const f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
-                        r[c][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q, i ? r[c][0] : z, 0, 0, 0);
-                        r[c][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q, i ? r[c][1] : z, 0, 0, 0);
+                        r[c][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qq, i ? r[c][0] : z, 0, 0, 0);
+                        r[c][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qq, i ? r[c][1] : z, 0, 0, 0);
                     }
                 if (b > 0) scale();
                 dp = d;
@@ -519,13 +548,15 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                         for (int i = 0; i < 4; i++) o[c][b][0][i] += nan, o[c][b][1][i] += nan;
                     }
                 }
+                lds_order();
 #pragma unroll
                 for (int e = 0; e < T::NS; e++) {
-                    uint32_t y = x.s[e];
+                    uint32_t y = ssc[wave][lane + 64 * e];
                     if ((y & 0x7c00u) == 0x7c00u) y &= 0xffff0000u;
                     if ((y & 0x7c000000u) == 0x7c000000u) y &= 0xffffu;
                     if (lane + 64 * e >= nq * 16) ssc[wave][lane + 64 * e] = y;
                 }
+                lds_order();
             }
             second(x, s, once);
         };
@@ -680,7 +711,7 @@ Plan plan_of(const Kv4 &c, int rows, int heads, int max_pos, int window, int n_s
     p.tt = n_sel ? 1 : 16 * p.C / p.rc;
     p.groups = (rows + p.tt - 1) / p.tt;
     const long long base = (long long)p.groups * p.chunks * c.n_kv;
-    p.split = (int)std::max<long long>(1, std::min<long long>(p.tt, (2048 + base - 1) / base));
+    p.split = (int)std::max<long long>(1, std::min<long long>(p.tt, (1024 + base - 1) / base));
     const long long tiles = n_sel ? (long long)n_sel * c.tiles()
                                   : (window > 0 ? std::min((long long)window + p.tt, (long long)max_pos + 1) : max_pos + 1LL) / 32 + 1;
     const long long units = base * p.split;

@@ -388,6 +388,36 @@ def test_unseen_positions_do_not_matter(shape, bad):
     assert not np.isfinite(got[sees]).all(axis=1).any()
 
 
+def test_unseen_positions_do_not_matter_to_many_rows():
+    """The same where the rows fill the wide groups: 600 rows, an infinity and
+    a NaN at positions that the earlier rows do not see, in tiles the others'
+    scales follow at once."""
+    shape = (32, 8, 128, 128)
+    cache, k, v = device_pool(shape, 1, 640, 64)
+    import torch
+
+    q = torch.randn((600, 32 * 128), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    seq, pos = [0] * 600, list(range(600))
+    clean = run_attend(cache, q.cpu().numpy(), seq, pos, 32, 128 ** -0.5)
+    pick = list(range(0, 600, 17)) + [399, 400, 401, 431, 432]
+    close(clean[pick], attend64(k, v, q[pick], [0] * len(pick), pick, 32, 128 ** -0.5))
+    pool = ref.Pool(10, 8, 128, 128, 64, cache.pool.cpu().numpy().copy())
+    table = cache.table.cpu().numpy()
+    bad = np.array([np.inf, 1, np.nan, -np.inf], np.float16)
+    for p in (400, 431):
+        slot = int(table[0, p // 64]) * 64 + p % 64
+        for kv in range(8):
+            for keys in (True, False):
+                pool.put(slot, kv, np.full(128, 11, np.uint8), bad, keys)
+    cache.pool.copy_(torch.from_numpy(pool.raw))
+    got = run_attend(cache, q.cpu().numpy(), seq, pos, 32, 128 ** -0.5)
+    # The finite scale beside them (1, above every other) moves the power of two
+    # that the weights are held under, so their two pieces round elsewhere: by
+    # up to 2^-22 of a weight, within TOL.
+    close(got[:400], clean[:400])
+    assert not np.isfinite(got[400:]).all(axis=1).any()
+
+
 def test_large_and_small_values():
     """Values from 1e-6 to 1e5 in one cache, scores hundreds apart."""
     shape = (8, 2, 64, 64)

@@ -131,19 +131,21 @@ __device__ inline void load_words(uint32_t (&w)[2 * NB], __amdgpu_buffer_rsrc_t 
 }
 
 // QC, VC: blocks of a key and a value (EX) or the most there may be.  C:
-// 16-column tiles.  W: waves.
-template <int QC, int VC, bool EX, int C, int W>
+// 16-column tiles of a wave.  W waves: S sets of columns, W / S parts of the
+// positions.
+template <int QC, int VC, bool EX, int C, int S, int W>
 __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) {
     typedef Tile<QC, VC> T;
-    __shared__ u32x4 sq_[C * QC * 2 * 64];  // Q operands: [column tile][block][hi, lo][lane]
+    constexpr int P = W / S;
+    __shared__ u32x4 sq_[S * C * QC * 2 * 64];  // Q operands: [column tile][block][hi, lo][lane]
     __shared__ f32x4 smo[W * VC * 2 * 64];  // O of the waves: [wave][block][half][lane]
     __shared__ uint32_t ssc[W][T::NS * 64];
-    __shared__ float sm_r[W][C * 16], sm_l[W][C * 16], sm_k[C * 16];
+    __shared__ float sm_r[W][C * 16], sm_l[W][C * 16], sm_k[S * C * 16];
     const Kv4 &kc = a.c;
     const Nibbles nib;
     const float less = minus_one();
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, g = lane >> 4;
+    const int col = lane & 15, g = lane >> 4, set = wave % S, share = wave / S;
     const int nq = EX ? QC : kc.qd / 32, nv = EX ? VC : kc.vd / 32;
     // Kv heads next to each other go to the XCDs in turn, so that one head's
     // blocks find its tiles in their L2.  Later rows of a prompt see more
@@ -165,7 +167,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
     // Column cc of the block is query head h0 + cc % hn of row r0 + cc / hn,
     // whatever run it is in: queries load while sequences and tables do.  16
     // threads a column, four values each at a time.
-    constexpr int kPer = (QC + 1) / 2, kCols = (C * 16 + W * 4 - 1) / (W * 4);
+    constexpr int kPer = (QC + 1) / 2, kCols = S * C * 16 / (W * 4);
     f32x4 qv[kCols][kPer];
     const int qi = threadIdx.x & 15;
 #pragma unroll
@@ -213,7 +215,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
         bool cv[C];
 #pragma unroll
         for (int c = 0; c < C; c++) {
-            const int x = copies ? col & ((1 << wide) - 1) : c * 16 + col - c0;
+            const int x = copies ? col & ((1 << wide) - 1) : (set * C + c) * 16 + col - c0;
             cv[c] = x >= 0 && x < ncol;
             cc[c] = c0 + (cv[c] ? x : 0);
             cp[c] = __shfl(my_pos, cc[c] / hn, 64);
@@ -224,7 +226,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
         // This wave's tiles: v0 .. v1 - 1 of the run's (of the lists' pages).
         const int t0 = a.lists ? 0 : lo >> 5;
         const int nt = a.lists ? a.n_sel << tshift : (hi >> 5) - t0 + 1;
-        const int parts = a.ps * W, me = part * W + wave;
+        const int parts = a.ps * P, me = part * P + share;
         int v = (int)((long long)nt * me / parts);
         const int v1 = (int)((long long)nt * (me + 1) / parts);
         const int32_t *list = a.lists ? a.lists + ((size_t)(r0 + first) * kc.n_kv + kv) * a.n_sel : nullptr;
@@ -327,7 +329,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
         }
         float ck[C];
 #pragma unroll
-        for (int c = 0; c < C; c++) ck[c] = sm_k[C == 1 ? cc[0] : c * 16 + col];
+        for (int c = 0; c < C; c++) ck[c] = sm_k[C == 1 ? cc[0] : (set * C + c) * 16 + col];
         const int ql_at = C == 1 ? g * 16 + cc[0] : lane;
 
         f32x4 o[C][VC][2];
@@ -440,8 +442,8 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                 dn = sc[b * 4 + g];
 #pragma unroll
                 for (int c = 0; c < C; c++) {
-                    qn[c][0] = sq_[((c * QC + b) * 2 + 1) * 64 + ql_at];
-                    qn[c][1] = sq_[((c * QC + b) * 2) * 64 + ql_at];
+                    qn[c][0] = sq_[(((set * C + c) * QC + b) * 2 + 1) * 64 + ql_at];
+                    qn[c][1] = sq_[(((set * C + c) * QC + b) * 2) * 64 + ql_at];
                 }
             };
             operands(0);
@@ -600,14 +602,14 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
 #pragma unroll
             for (int b = 0; b < VC * 2; b++) smo[(wave * VC * 2 + b) * 64 + lane] = o[c][b >> 1][b & 1];
             __syncthreads();
-            float rr = -INFINITY, ll = 0.0f, fw[W];
+            float rr = -INFINITY, ll = 0.0f, fw[P];
 #pragma unroll
-            for (int w = 0; w < W; w++) rr = fmaxf(rr, sm_r[w][c * 16 + col]);
+            for (int w = 0; w < P; w++) rr = fmaxf(rr, sm_r[w * S + set][c * 16 + col]);
 #pragma unroll
-            for (int w = 0; w < W; w++) {
-                const float rw = sm_r[w][c * 16 + col];
+            for (int w = 0; w < P; w++) {
+                const float rw = sm_r[w * S + set][c * 16 + col];
                 fw[w] = rw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(rw - rr);
-                ll += rw == -INFINITY ? 0.0f : sm_l[w][c * 16 + col] * fw[w];
+                ll += rw == -INFINITY ? 0.0f : sm_l[w * S + set][c * 16 + col] * fw[w];
             }
             if (cv[c]) {
                 const size_t row = r0 + cc[c] / hn, head = h0 + cc[c] % hn;
@@ -616,24 +618,24 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                 if (a.ps > 1) {
                     const size_t where = (row * a.heads + head) * a.ps + part;
                     dst = a.part + where * kc.vd;
-                    if (g == 0 && wave == 0 && (!copies || col >> wide == 0)) a.part_ml[2 * where] = rr, a.part_ml[2 * where + 1] = ll;
+                    if (g == 0 && share == 0 && (!copies || col >> wide == 0)) a.part_ml[2 * where] = rr, a.part_ml[2 * where + 1] = ll;
                     f = 1.0f;
                 }
                 // Lane (column, g) of [block][half] holds dims 32 b + 16 h + 4 g + i.
 #pragma unroll
-                for (int bh = 0; bh < VC * 2; bh += W) {
-                    const int b = (bh + wave) >> 1;
+                for (int bh = 0; bh < VC * 2; bh += P) {
+                    const int b = (bh + share) >> 1;
                     if (b >= nv || (copies && col >> wide != b)) continue;
                     f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int w = 0; w < W; w++) {
-                        const f32x4 ow = smo[(w * VC * 2 + bh + wave) * 64 + lane];
+                    for (int w = 0; w < P; w++) {
+                        const f32x4 ow = smo[((w * S + set) * VC * 2 + bh + share) * 64 + lane];
 #pragma unroll
                         for (int i = 0; i < 4; i++) z[i] = fw[w] == 0.0f ? z[i] : fmaf(ow[i], fw[w], z[i]);
                     }
 #pragma unroll
                     for (int i = 0; i < 4; i++) z[i] *= f;
-                    *(__attribute__((address_space(1))) f32x4_dw *)(dst + 16 * (bh + wave) + 4 * g) = __builtin_bit_cast(f32x4_dw, z);
+                    *(__attribute__((address_space(1))) f32x4_dw *)(dst + 16 * (bh + share) + 4 * g) = __builtin_bit_cast(f32x4_dw, z);
                 }
             }
             __syncthreads();
@@ -694,24 +696,26 @@ __global__ __launch_bounds__(T) void kv4_join_kernel(const Args a) {
 
 // How a call is cut up: see Args.
 struct Plan {
-    int C, rc, chunks, tt, groups, split, ps;
+    int C, cols, rc, chunks, tt, groups, split, ps;  // cols: columns of a block
     uint64_t bytes;
 };
 
 Plan plan_of(const Kv4 &c, int rows, int heads, int max_pos, int window, int n_sel) {
     Plan p{};
     const int rep = heads / c.n_kv;
-    // Two column tiles halve the unpacking and the cache's traffic where rows
-    // come in runs; 256 groups of 32 columns fill the chip.
-    const long long wide = ((long long)rows * rep + 31) / 32 * c.n_kv;
+    // Two column tiles a wave halve the unpacking, and two sets of them a block
+    // halve what comes before the first tile and after the last, where rows come
+    // in runs; from two blocks of 64 columns a CU on.
+    const long long wide = ((long long)rows * rep + 63) / 64 * c.n_kv;
     p.C = n_sel == 0 && c.qd <= 192 && c.vd <= 128 && wide >= 256 ? 2 : 1;
-    p.rc = std::min(rep, 16 * p.C);
+    p.cols = p.C == 2 ? 64 : 16;
+    p.rc = std::min(rep, p.cols);
     p.chunks = (rep + p.rc - 1) / p.rc;
     // Rows with lists of their own share nothing.
-    p.tt = n_sel ? 1 : 16 * p.C / p.rc;
+    p.tt = n_sel ? 1 : p.cols / p.rc;
     p.groups = (rows + p.tt - 1) / p.tt;
     const long long base = (long long)p.groups * p.chunks * c.n_kv;
-    p.split = (int)std::max<long long>(1, std::min<long long>(p.tt, (1024 + base - 1) / base));
+    p.split = (int)std::max<long long>(1, std::min<long long>(p.tt, 1024 / base));
     const long long tiles = n_sel ? (long long)n_sel * c.tiles()
                                   : (window > 0 ? std::min((long long)window + p.tt, (long long)max_pos + 1) : max_pos + 1LL) / 32 + 1;
     const long long units = base * p.split;
@@ -734,7 +738,7 @@ template <int QC, int VC, bool EX, int C>
 void launch(const Args &a, hipStream_t s) {
     constexpr int W = 4;
     const long long blocks = (long long)a.groups * a.split * a.ps * a.chunks * a.c.n_kv;
-    hipLaunchKernelGGL((kv4_attention_kernel<QC, VC, EX, C, W>), dim3((unsigned)blocks), dim3(W * 64), 0, s, a);
+    hipLaunchKernelGGL((kv4_attention_kernel<QC, VC, EX, C, C, W>), dim3((unsigned)blocks), dim3(W * 64), 0, s, a);
 }
 
 }  // namespace

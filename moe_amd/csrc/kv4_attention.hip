@@ -576,8 +576,8 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                 if (v > v1) break;
             }
             while (C > 1 && any) {
-                // (a tile that is none: positions that no column sees)
-                const int base = x.ok ? x.base : 1 << 30;
+                // (a tile that is none: behind the last position there can be)
+                const int base = x.ok ? x.base : 0x7fffffff - (kTile - 1);
                 find(x);
                 step(x, base, once, [&] { load_keys(x); });
                 load_values(x);

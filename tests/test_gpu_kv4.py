@@ -509,6 +509,26 @@ def test_long_contexts_and_prompts(shape, ctx, rows):
             close(got[pick], want, 2 * TOL)
 
 
+@pytest.mark.parametrize("rows", [5, 1024])
+def test_positions_past_2_30(rows):
+    """A sequence of more than 2^30 positions, a page in the middle of the
+    window missing: few rows, and enough of them for the wide groups."""
+    import torch
+
+    from moe_amd.paged import KvCache
+
+    shape, page, mid = (16, 2, 64, 64), 4096, 1 << 18
+    few, k, v = device_pool(shape, 1, 2 * page, page)
+    table = torch.full((1, mid + 1), -1, dtype=torch.int32, device="cuda")
+    table[0, mid - 2], table[0, mid] = few.table[0, 0], few.table[0, 1]
+    cache = KvCache(few.pool, table, n_kv=2, qd=64, vd=64, page=page)
+    q = torch.randn((rows, 16 * 64), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    got = run_attend(cache, q.cpu().numpy(), [0] * rows, [mid * page + r for r in range(rows)], 16, 0.125, 2 * page)
+    pick = list(range(0, rows, max(1, rows // 20)))
+    # without the missing page the rows are at 4096 + r, with a window of 4096
+    close(got[pick], attend64(k, v, q[pick], [0] * len(pick), [page + r for r in pick], 16, 0.125, page))
+
+
 # ------------------------------------------------------------- choice of pages
 
 

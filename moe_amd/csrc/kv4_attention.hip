@@ -410,14 +410,26 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
             lds_order();       // the reads of the tile before
             uint32_t top = 0;  // the largest finite value scale of the lane's, f16 bits
             bool inf = false;
+            auto largest = [&](uint32_t seen) __attribute__((always_inline)) {
 #pragma unroll
-            for (int e = 0; e < T::NS; e++) {
-                ssc[wave][lane + 64 * e] = x.s[e];
-                const int at = lane + 64 * e;
-                const uint32_t y = at >= nq * 16 && at < (nq + nv) * 16 ? x.s[e] & 0x7fff7fffu : 0;
-                const uint32_t y0 = y & 0xffffu, y1 = y >> 16;
-                inf |= y0 >= 0x7c00u || y1 >= 0x7c00u;
-                top = max(top, max(y0 >= 0x7c00u ? 0 : y0, y1 >= 0x7c00u ? 0 : y1));
+                for (int e = 0; e < T::NS; e++) {
+                    const int at = lane + 64 * e;
+                    const uint32_t y = at >= nq * 16 && at < (nq + nv) * 16 ? x.s[e] & seen : 0;
+                    const uint32_t y0 = y & 0xffffu, y1 = y >> 16;
+                    inf |= y0 >= 0x7c00u || y1 >= 0x7c00u;
+                    top = max(top, max(y0 >= 0x7c00u ? 0 : y0, y1 >= 0x7c00u ? 0 : y1));
+                }
+            };
+#pragma unroll
+            for (int e = 0; e < T::NS; e++) ssc[wave][lane + 64 * e] = x.s[e];
+            largest(0x7fff7fffu);
+            if (__builtin_expect(base < lo || base + kTile - 1 > hi, 0)) {
+                // Of positions that the run sees: what lies in a page's rest or
+                // before the window must not set the weights' power of two.  A
+                // lane's pair of scales is the same two positions in every block.
+                const int w = 2 * col, p = base + 4 * (w >> 3) + 16 * (w >> 2 & 1) + (w & 3);
+                top = 0;
+                largest((p >= lo && p <= hi ? 0x7fffu : 0) | (p + 1 >= lo && p + 1 <= hi ? 0x7fff0000u : 0));
             }
             lds_order();
             const u32x4 *sc = (const u32x4 *)ssc[wave];

@@ -529,6 +529,41 @@ def test_positions_past_2_30(rows):
     close(got[pick], attend64(k, v, q[pick], [0] * len(pick), [page + r for r in pick], 16, 0.125, page))
 
 
+@pytest.mark.parametrize("shape,rows", [((8, 2, 64, 64), 3), ((6, 2, 96, 96), 40), ((16, 2, 64, 64), 1024), ((16, 2, 96, 64), 1024)],
+                         ids=str)
+def test_unseen_sizes_do_not_matter(shape, rows):
+    """Values 10^11 times those that the rows see, before their window and in
+    the rest of the last page: outputs keep their relative precision."""
+    import torch
+
+    heads, n_kv, qd, vd = shape
+    first, window, page = 100, 45, 64
+    cache, k, v = device_pool(shape, 1, first + rows + 60, page)
+    top = first + rows - 1
+    h = torch.rand((cache.table.shape[1] * page, n_kv, vd // 32), generator=torch.Generator(device="cuda").manual_seed(2),
+                   device="cuda")
+    size = torch.full_like(h, 6e-7)  # f16 subnormals
+    size[:first + 1 - window] = 6e4
+    size[top + 1:] = 6e4
+    scale = ((0.5 + 0.5 * h) * size).half()
+    # Into the tiles: number 32 b + 8 (p % 16 / 4) + 4 (p / 16) + p % 4 of the region, page by page.
+    tiles = cache.pool.view(-1, n_kv, page // 32, 18 * (qd + vd))
+    p = torch.arange(32, device="cuda")
+    at = 8 * (p % 16 // 4) + 4 * (p // 16) + p % 4
+    new = torch.empty((len(tiles), n_kv, page // 32, vd // 32, 32), dtype=torch.float16, device="cuda")
+    new[cache.table[0].long()] = scale.view(-1, page // 32, 32, n_kv, vd // 32).permute(0, 3, 1, 4, 2)[..., at.argsort()]
+    tiles[..., 18 * qd + 16 * vd:] = new.view(*new.shape[:3], -1).view(torch.uint8)
+    slots = (cache.table[0].long()[:, None] * page + torch.arange(page, device="cuda")).view(-1)
+    kb, vb = torch.empty((len(slots), n_kv * qd), device="cuda"), torch.empty((len(slots), n_kv * vd), device="cuda")
+    cache.load(slots, kb, vb)
+    assert vb[first + 1 - window:top + 1].abs().max() < 1e-5 and vb[top + 1:].abs().max() > 1e5
+    q = torch.randn((rows, heads * qd), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    got = run_attend(cache, q.cpu().numpy(), [0] * rows, [first + r for r in range(rows)], heads, qd ** -0.5, window)
+    pick = list(range(0, rows, max(1, rows // 20)))
+    close(got[pick], attend64(kb.view(1, -1, n_kv, qd).double(), vb.view(1, -1, n_kv, vd).double(), q[pick], [0] * len(pick),
+                              [first + r for r in pick], heads, qd ** -0.5, window))
+
+
 # ------------------------------------------------------------- choice of pages
 
 

@@ -420,7 +420,7 @@ typedef struct moe_kv4 {
     void *means;           /* device f16 [n_pages][n_kv][qd], or NULL */
     int32_t n_seq, max_pages, n_pages;
     int32_t page;          /* positions of a page: 32, 64, 128 ... 4096 */
-    int32_t n_kv, qd, vd;  /* kv heads, key and value widths: multiples of 32 up to 256 */
+    int32_t n_kv, qd, vd;  /* kv heads (up to 65535), key and value widths: multiples of 32 up to 256 */
     int32_t _reserved;
 } moe_kv4;
 
@@ -449,7 +449,8 @@ int moe_kv4_pool_size(const moe_kv4 *c, uint64_t *bytes);
  * state_out may be length and state themselves.  Table entries behind a
  * sequence's pages are left as they were.  Lengths outside 0 ... max_pages *
  * page count as the nearest of the two; sequences of pages that are in use
- * elsewhere are the caller's mistake and are not found.  `workspace`: device,
+ * elsewhere are the caller's mistake and are not found.  At most 2^24
+ * sequences, 2^30 pages and fewer than 2^30 rows.  `workspace`: device,
  * 8-byte aligned, moe_pages_workspace_size bytes.  No counterpart in the
  * reference, whose sequences own whole caches. */
 int moe_pages_workspace_size(int32_t n_seq, uint64_t *bytes);
@@ -463,7 +464,7 @@ int moe_pages_advance(int32_t n_seq, const int32_t *length, const int32_t *add, 
  * v_stride floats apart, quantised as moe_quantize_rows(Q4_0) does, NaNs (read
  * as 0) and infinities (their block reads as NaN) included.  slots: device
  * int64 [rows], distinct; rows whose slot is negative or past the pool are
- * skipped.  With c->means, a page whose last position is among the rows gets
+ * skipped; at most 2^24 - 256 rows (also moe_kv4_load's).  With c->means, a page whose last position is among the rows gets
  * its mean key: the sum over its positions in 64 bits, divided, rounded to f32,
  * bounded by the largest f16 and rounded to it. */
 int moe_kv4_store(const moe_kv4 *c, const float *k, int64_t k_stride, const float *v, int64_t v_stride, int32_t rows,
@@ -483,7 +484,12 @@ int moe_kv4_load(const moe_kv4 *c, const int64_t *slots, int32_t rows, float *k,
  * before it is skipped).  max_pos bounds every pos[r].  A row with pos[r] < 0
  * or seq[r] outside 0 ... n_seq - 1 is left as it was; pages outside the pool
  * and behind max_pages hold no positions; a row that sees no position at all
- * is 0.  What positions a row does not see hold does not matter.  `workspace`:
+ * is 0, as is one whose scores are all minus infinity; a block of a value that
+ * reads as infinite or NaN makes its 32 values NaN in the rows that see it.
+ * What positions hold that no row sees does not matter.  Sums are f32 and
+ * weights have 22 bits; a value smaller than 2^-12 of those that other rows of
+ * the call see beside it (in its 32 positions, or before its row's window) has
+ * fewer.  `workspace`:
  * device, 16-byte aligned, moe_kv4_attention_workspace_size bytes (its
  * arguments as the call's; it may be 0 bytes).  Calls that share one must be
  * ordered. */

@@ -57,6 +57,9 @@ struct Kv4 {
     __host__ __device__ int v_scales() const { return 18 * qd + 16 * vd; }
 };
 
+// A launch is at most 2^32 - 1 threads.
+constexpr long long kMostThreads = 0xffffffffll;
+
 // Checks a caller's cache and turns it into the kernels' form: 0 or a
 // MOE_E* code with its message set.
 int kv4_of(const char *what, const moe_kv4 *c, Kv4 *out);

@@ -725,7 +725,7 @@ Plan plan_of(const Kv4 &c, int rows, int heads, int max_pos, int window, int n_s
     p.chunks = (rep + p.rc - 1) / p.rc;
     // Rows with lists of their own share nothing.
     p.tt = n_sel ? 1 : p.cols / p.rc;
-    p.groups = (rows + p.tt - 1) / p.tt;
+    p.groups = (int)(((long long)rows + p.tt - 1) / p.tt);
     const long long base = (long long)p.groups * p.chunks * c.n_kv;
     p.split = (int)std::max<long long>(1, std::min<long long>(p.tt, 1024 / base));
     const long long tiles = n_sel ? (long long)n_sel * c.tiles()
@@ -765,7 +765,7 @@ int moe_kv4_attention_workspace_size(const moe_kv4 *c, int32_t rows, int32_t hea
     Kv4 a;
     if (const int rc = kv4_of("moe_kv4_attention_workspace_size", c, &a)) return rc;
     if (!bytes || rows < 0 || heads <= 0 || heads % a.n_kv || max_pos < 0 ||
-        max_pos >= (int64_t)a.max_pages << a.page_shift || n_sel < 0)
+        max_pos >= (int64_t)a.max_pages << a.page_shift || n_sel < 0 || (int64_t)n_sel << a.page_shift > INT32_MAX)
         return fail(MOE_EINVAL, "moe_kv4_attention_workspace_size: bad argument (%d rows, %d heads over %d, max position %d"
                     " of %lld)", rows, heads, a.n_kv, max_pos, (long long)a.max_pages << a.page_shift);
     *bytes = rows ? plan_of(a, rows, heads, max_pos, window, n_sel).bytes : 0;
@@ -779,9 +779,10 @@ int moe_kv4_attention(const moe_kv4 *c, const float *q, int64_t q_stride, int32_
     Args a{};
     if (const int rc = kv4_of("moe_kv4_attention", c, &a.c)) return rc;
     if ((rows > 0 && (!q || !seq || !pos || !out)) || rows < 0 || heads <= 0 || heads % a.c.n_kv || max_pos < 0 ||
-        max_pos >= (int64_t)a.c.max_pages << a.c.page_shift || (lists && n_sel <= 0))
-        return fail(MOE_EINVAL, "moe_kv4_attention: bad argument (%d rows, %d heads over %d, max position %d of %lld)",
-                    rows, heads, a.c.n_kv, max_pos, (long long)a.c.max_pages << a.c.page_shift);
+        max_pos >= (int64_t)a.c.max_pages << a.c.page_shift ||
+        (lists && (n_sel <= 0 || (int64_t)n_sel << a.c.page_shift > INT32_MAX)))
+        return fail(MOE_EINVAL, "moe_kv4_attention: bad argument (%d rows, %d heads over %d, max position %d of %lld, %d pages)",
+                    rows, heads, a.c.n_kv, max_pos, (long long)a.c.max_pages << a.c.page_shift, n_sel);
     if (rows == 0) return MOE_OK;
     const Plan p = plan_of(a.c, rows, heads, max_pos, window, lists ? n_sel : 0);
     if (p.bytes && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < p.bytes))
@@ -794,7 +795,7 @@ int moe_kv4_attention(const moe_kv4 *c, const float *q, int64_t q_stride, int32_
     a.tt = p.tt, a.groups = p.groups, a.rc = p.rc, a.chunks = p.chunks, a.split = p.split, a.ps = p.ps;
     a.part = static_cast<float *>(workspace);
     a.part_ml = a.part + (size_t)rows * heads * p.ps * a.c.vd;
-    if ((long long)a.groups * a.split * a.ps * a.chunks * a.c.n_kv > INT32_MAX)
+    if ((long long)a.groups * a.split * a.ps * a.chunks * a.c.n_kv > kMostThreads / 256)
         return fail(MOE_EUNSUP, "moe_kv4_attention: %d rows of %d heads are too many blocks", rows, heads);
     hipStream_t s = (hipStream_t)stream;
     const int qc = a.c.qd / 32, vc = a.c.vd / 32;

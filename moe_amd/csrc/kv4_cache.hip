@@ -22,6 +22,7 @@ int kv4_of(const char *what, const moe_kv4 *c, Kv4 *out) {
                     what, c->page, c->max_pages);
     if (c->qd <= 0 || c->vd <= 0 || c->qd % 32 || c->vd % 32 || c->qd > 256 || c->vd > 256)
         return fail(MOE_EUNSUP, "%s: key width %d, value width %d (multiples of 32 up to 256)", what, c->qd, c->vd);
+    if (c->n_kv > 65535) return fail(MOE_EUNSUP, "%s: %d kv heads (up to 65535)", what, c->n_kv);  // a grid's second size
     Kv4 k{};
     k.pool = static_cast<uint8_t *>(c->pool), k.table = c->table, k.means = static_cast<__half *>(c->means);
     k.n_seq = c->n_seq, k.max_pages = c->max_pages, k.n_pages = c->n_pages, k.n_kv = c->n_kv, k.qd = c->qd, k.vd = c->vd;
@@ -252,6 +253,8 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(const Kv4 c, const int64_
     *(__attribute__((address_space(1))) f32x4_dw *)dst = x;
 }
 
+constexpr int kMostRows = (1 << 24) - 256;  // a block of 256 threads a row
+
 int rc_of(const char *what) {
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? MOE_OK : fail(MOE_EHIP, "%s: %s", what, hipGetErrorString(e));
@@ -283,6 +286,7 @@ int moe_kv4_store(const moe_kv4 *c, const float *k, int64_t k_stride, const floa
     if (const int rc = kv4_of("moe_kv4_store", c, &a)) return rc;
     if (rows < 0 || (rows > 0 && (!k || !v || !slots)))
         return fail(MOE_EINVAL, "moe_kv4_store: bad argument (%d rows)", rows);
+    if (rows > kMostRows) return fail(MOE_EUNSUP, "moe_kv4_store: %d rows, up to %d at once", rows, kMostRows);
     if (rows == 0) return MOE_OK;
     hipStream_t s = (hipStream_t)stream;
     const int blocks = a.n_kv * (a.qd + a.vd) / 32;
@@ -305,6 +309,7 @@ int moe_kv4_load(const moe_kv4 *c, const int64_t *slots, int32_t rows, float *k,
     Kv4 a;
     if (const int rc = kv4_of("moe_kv4_load", c, &a)) return rc;
     if (rows < 0 || (rows > 0 && !slots)) return fail(MOE_EINVAL, "moe_kv4_load: bad argument (%d rows)", rows);
+    if (rows > kMostRows) return fail(MOE_EUNSUP, "moe_kv4_load: %d rows, up to %d at once", rows, kMostRows);
     if (rows == 0 || (!k && !v)) return MOE_OK;
     const int blocks = a.n_kv * ((k ? a.qd : 0) + (v ? a.vd : 0)) / 32;
     hipLaunchKernelGGL(kv4_load_kernel, dim3(row_blocks<1>(rows), (blocks + 31) / 32), dim3(256), 0, (hipStream_t)stream, a,

@@ -309,10 +309,13 @@ int moe_kv4_select(const moe_kv4 *c, const float *q, int64_t q_stride, int32_t r
         max_pos >= (int64_t)a.c.max_pages << a.c.page_shift)
         return fail(MOE_EINVAL, "moe_kv4_select: bad argument (%d rows, %d heads over %d, max position %d of %lld)", rows,
                     heads, a.c.n_kv, max_pos, (long long)a.c.max_pages << a.c.page_shift);
-    if (sinks < 0 || recent < 1 || n_sel < 1 || (int64_t)sinks + recent > n_sel)
+    if (sinks < 0 || recent < 1 || n_sel < 1 || (int64_t)n_sel << a.c.page_shift > INT32_MAX || (int64_t)sinks + recent > n_sel)
         return fail(MOE_EINVAL, "moe_kv4_select: %d first and %d last pages of %d", sinks, recent, n_sel);
     if (rows == 0) return MOE_OK;
-    if ((int64_t)rows * a.c.n_kv > INT32_MAX) return fail(MOE_EUNSUP, "moe_kv4_select: %d rows are too many blocks", rows);
+    const int64_t pages = (max_pos >> a.c.page_shift) + 1;
+    if ((int64_t)rows * a.c.n_kv * kThreads > kMostThreads || pages > 65535ll * kScorePages)
+        return fail(MOE_EUNSUP, "moe_kv4_select: %d rows of %d kv heads and %lld pages are too many blocks", rows, a.c.n_kv,
+                    (long long)pages);
     const uint64_t need = workspace_of(a.c, rows, max_pos);
     if (need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need))
         return fail(MOE_EINVAL, "moe_kv4_select: workspace of %llu bytes, %llu needed", (unsigned long long)workspace_bytes,

@@ -31,6 +31,7 @@ int fail(int code, const char *fmt, ...);
 namespace {
 
 constexpr int kMost = 1 << 30;
+constexpr int kMostSeq = 1 << 24;  // blocks of the second launch: 2^22 for them and for the rows
 
 struct Pages {
     const int32_t *length, *add, *state;
@@ -250,7 +251,7 @@ int moe_pages_advance(int32_t n_seq, const int32_t *length, const int32_t *add, 
                       int64_t *slot, int32_t *status, void *workspace, uint64_t workspace_bytes, void *stream) {
     if (!length || !add || !length_out || !table || !ring || !state || !state_out || !row_start || !status ||
         (max_rows > 0 && (!seq || !pos || !slot)) || n_seq <= 0 || max_pages <= 0 || n_pages <= 0 || max_rows < 0 ||
-        n_seq > kMost || n_pages > kMost || max_rows >= kMost)
+        n_seq > kMostSeq || n_pages > kMost || max_rows >= kMost)
         return fail(MOE_EINVAL, "moe_pages_advance: bad argument (%d sequences of %d pages, pool of %d, %d rows)", n_seq,
                     max_pages, n_pages, max_rows);
     if (page < 32 || page > 4096 || (page & (page - 1)) || (int64_t)max_pages * page > INT32_MAX)

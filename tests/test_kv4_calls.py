@@ -201,3 +201,36 @@ def test_wrong_tables(lib):
             pt.advance(add, rows, out=out)
     with pytest.raises(ValueError, match="GPU"):
         pt.advance(i(3), Rows.new(3, 5, "cpu"))
+
+
+BIG = 2 ** 31 - 1
+
+
+def test_refuses_what_no_launch_holds(lib):
+    """Sizes whose blocks are more than a launch's: refused, nothing queued."""
+    one = dict(n_kv=1, qd=32, vd=32, page=32, pool_bytes=1 << 60)
+    for rows in (2 ** 24 - 255, BIG):
+        assert store(lib, kv4(**one), rows=rows) == L.MOE_EUNSUP
+        assert load(lib, kv4(**one), rows=rows) == L.MOE_EUNSUP
+    assert attention(lib, kv4(**one), rows=BIG, heads=16) == L.MOE_EUNSUP
+    assert attention(lib, kv4(**one), rows=2 ** 24, heads=16, lists=P, n_sel=1) == L.MOE_EUNSUP
+    assert select(lib, kv4(**one), rows=2 ** 23, heads=1, ws_bytes=1 << 62) == L.MOE_EUNSUP
+    for call in (attention, select, store, load):
+        assert call(lib, kv4(n_kv=65536, pool_bytes=1 << 60)) != L.MOE_OK
+    long = dict(one, max_pages=2 ** 26 - 1)
+    assert select(lib, kv4(**long), rows=1, heads=1, max_pos=2 ** 31 - 33, ws_bytes=1 << 62) == L.MOE_EUNSUP
+
+
+def test_refuses_lists_of_too_many_pages(lib):
+    """More pages than positions have numbers."""
+    n = C.c_uint64()
+    for n_sel in (2 ** 25, BIG):
+        assert attention(lib, kv4(), lists=P, n_sel=n_sel) == L.MOE_EINVAL
+        assert select(lib, kv4(), n_sel=n_sel) == L.MOE_EINVAL
+        assert lib.moe_kv4_attention_workspace_size(C.byref(kv4()), 3, 8, 100, 0, n_sel, C.byref(n)) == L.MOE_EINVAL
+
+
+@pytest.mark.parametrize("bad", [dict(n=2 ** 24 + 1), dict(n=BIG), dict(n_pages=2 ** 30 + 1), dict(rows=2 ** 30), dict(rows=BIG)],
+                         ids=str)
+def test_advance_refuses_sizes_past_its_sums(lib, bad):
+    assert advance(lib, ws_bytes=1 << 40, **bad) == L.MOE_EINVAL

@@ -409,6 +409,15 @@ class Sparse:
     recent: int = 2
 
 
+def _keep_for(sp: int, queued: bool, *tensors) -> None:
+    """Memory that stream sp reads though another one is current: freed, it
+    goes to no other work before sp is done with it."""
+    if not queued and tensors[0].is_cuda:
+        s = torch.cuda.ExternalStream(sp) if sp else torch.cuda.default_stream()
+        for t in tensors:
+            t.record_stream(s)
+
+
 class PagedBatch:
     """Batch for a PagedState: the host sends how many tokens each sequence
     has and the rows' ids; sequences, positions and slots are made on the
@@ -430,6 +439,8 @@ class PagedBatch:
         old = st.table
         self.table = PageTable(old.table, torch.empty_like(old.length), old.ring, torch.empty_like(old.state), st.page)
         rows = old.advance(dev[:n], Rows.new(n, t, device), out=self.table, stream=sp)
+        _keep_for(sp, queued, dev, rows.seq, rows.pos, rows.slot, rows.row_start, rows.status, old.length, old.state,
+                  self.table.length, self.table.state)
         self.seq, self.pos, self.dst = rows.seq, rows.pos, rows.slot
         self.max_pos = max(st.pos[q] + c for q, c in zip(seqs, counts)) - 1
         self.sparse = st.sparse is not None and max(counts) == 1
@@ -451,7 +462,7 @@ class PagedState:
                                        and sparse.sinks + sparse.recent <= sparse.pages):
             raise ValueError(f"{sparse.sinks} first and {sparse.recent} last pages of {sparse.pages}")
         KvCache.page_bytes(n_kv, qd, vd, page)  # refuses widths and pages the cache does not hold
-        if n_seq < 1 or ctx < 1 or pages < 1:
+        if n_seq < 1 or ctx < 1 or pages < 1 or each * page >= 2 ** 31:
             raise ValueError(f"{n_seq} sequences of {ctx} positions over {pages} pages")
         self.ctx, self.n_seq, self.page, self.pages, self.sparse = ctx, n_seq, page, pages, sparse
         self.pos = [0] * n_seq
@@ -487,7 +498,10 @@ class PagedState:
         add = torch.zeros(self.n_seq, dtype=torch.int32)
         add[list(seqs)] = -1
         dev = self.table.device
-        self.table.advance(add.to(dev), Rows.new(self.n_seq, 0, dev), stream=stream)
+        add, rows = add.to(dev), Rows.new(self.n_seq, 0, dev)
+        self.table.advance(add, rows, stream=stream)
+        if stream is not None:
+            _keep_for(_stream_ptr(stream), False, add, rows.row_start, rows.status)
         for q in seqs:
             self.pos[q] = 0
 

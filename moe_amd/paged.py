@@ -70,7 +70,12 @@ class _OnDevice:
         device when None."""
         if stream is None:
             return torch._C._cuda_getCurrentRawStream(self._index)
-        return stream if type(stream) is int else stream.cuda_stream
+        if type(stream) is int:
+            return stream
+        index = getattr(stream, "device_index", self._index)
+        if index != self._index:
+            raise ValueError(f"a stream of cuda:{index}; this is on {self.device}")
+        return stream.cuda_stream
 
     def _scratch(self, n: int, sp: int):
         """n bytes that stream sp owns.  The caching allocator hands a freed

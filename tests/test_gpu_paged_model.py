@@ -209,3 +209,25 @@ def test_a_context_past_the_f32_limit(ctx):
     x = m.forward([[1]], st)
     assert st.pos == [17001] and np.isfinite(x.cpu().numpy()).all()
     m.close()
+
+
+def test_ends_and_steps_on_a_stream_that_is_not_current(ctx):
+    """What such a call leaves to its stream is not given to the current
+    stream's next tensors while the stream is still behind."""
+    import torch
+
+    m, shape = build(ctx, "tiny_mixtral", **SMALL["tiny_mixtral"])
+    st = m.new_state(4, 128, cache="q4", page=32)
+    m.forward([ids(40, shape.vocab, 1), ids(33, shape.vocab, 2)], st)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(100_000_000)
+    st.end([0], stream=s)
+    b = st.batch([1, 2], [[1, 2], [3]], m.device, s.cuda_stream, False)
+    junk = [torch.full((n,), 5, dtype=torch.int32, device="cuda") for n in (4, 5, 2, 3) for _ in range(50)]
+    torch.cuda.synchronize()
+    assert all((j == 5).all().item() for j in junk)
+    assert st.table.length.tolist() == [0, 33, 0, 0] and b.table.length.tolist() == [0, 35, 1, 0]
+    assert b.seq.tolist() == [1, 1, 2] and b.pos.tolist() == [33, 34, 0]
+    m.close()

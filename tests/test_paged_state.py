@@ -1,5 +1,7 @@
 """PagedState on the CPU: which rows a step has and which steps are refused,
 with the device's tables replaced by a record of the calls."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -79,3 +81,13 @@ def test_steps_are_not_captured(state, monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="captured"):
         state.batch([0], [[1]], torch.device("cpu"), 0, True)
+
+
+def test_positions_have_numbers():
+    with pytest.raises(ValueError):
+        fake_model().new_state(1, 2 ** 31 - 1, cache="q4", pages=4)
+
+
+def test_streams_of_another_device(state):
+    with pytest.raises(ValueError, match="stream of cuda:1"):
+        state.table._on(SimpleNamespace(device_index=1, cuda_stream=5))

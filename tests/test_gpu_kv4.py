@@ -564,6 +564,73 @@ def test_unseen_sizes_do_not_matter(shape, rows):
                               [first + r for r in pick], heads, qd ** -0.5, window))
 
 
+@pytest.mark.parametrize("window", [0, 90])
+@pytest.mark.parametrize("shape", [(100, 1, 64, 64), (96, 2, 96, 32), (32, 8, 128, 128), (16, 16, 192, 128), (90, 3, 224, 64)],
+                         ids=str)
+def test_ragged_batches_of_many_rows(shape, window):
+    """Sequences of different lengths, rows that are none between them, rows in
+    no order, more query heads a kv head than a block's columns."""
+    import torch
+
+    heads, n_kv, qd, vd = shape
+    cache, k, v = device_pool(shape, 5, 700, 64)
+    g = np.random.default_rng(0)
+    rows = ([(0, p) for p in range(299)] + [(0, -1)] * 3 + [(3, p) for p in range(651, 700)] + [(7, 20)] * 5 +
+            [(1, p) for p in range(5, 250)] + [(-1, 9)] + [(2, int(p)) for p in g.integers(0, 700, 50)] + [(4, 699)])
+    seq, pos = zip(*rows)
+    q = torch.randn((len(rows), heads * qd), generator=torch.Generator(device="cuda").manual_seed(7), device="cuda")
+    got = run_attend(cache, q.cpu().numpy(), seq, pos, heads, qd ** -0.5, window)
+    none = [i for i, (a, p) in enumerate(rows) if p < 0 or not 0 <= a < 5]
+    assert (got[none] == 7.0).all()
+    pick = [i for i in range(len(rows)) if i not in none and (i % 9 == 0 or i > len(rows) - 40)]
+    close(got[pick], attend64(k, v, q[pick], [seq[i] for i in pick], [pos[i] for i in pick], heads, qd ** -0.5, window))
+
+
+def test_load_of_keys_or_values_alone():
+    import torch
+
+    cache, k, v = device_pool((6, 3, 96, 160), 1, 100, 32)
+    slots = torch.tensor([5, -1, 70, 31, 10 ** 9], device="cuda")
+    whole = [torch.full((5, 3 * d), 7.0, device="cuda") for d in (96, 160)]
+    cache.load(slots, *whole)
+    for i in range(2):
+        one = torch.full_like(whole[i], 7.0)
+        cache.load(slots, *((one, None) if i == 0 else (None, one)))
+        assert torch.equal(one, whole[i]) and (one[[1, 4]] == 7.0).all() and (one[0] != 7.0).any()
+    cache.load(slots)
+
+
+def test_a_pool_past_4_gib():
+    """Pages whose bytes, and rows' slots, lie past 32 bits: written, read,
+    attended to and chosen as the same rows are in a small pool."""
+    import torch
+
+    from moe_amd.paged import KvCache
+
+    heads, n_kv, d, page, ctx = 32, 8, 128, 64, 1000
+    near, k, v = device_pool((heads, n_kv, d, d), 1, ctx, page)
+    mp = near.table.shape[1]
+    n_pages = (5 << 30) // KvCache.page_bytes(n_kv, d, d, page)
+    table = (n_pages - 1 - torch.arange(mp, dtype=torch.int32, device="cuda")).view(1, mp)
+    far = KvCache.new(n_pages, table, n_kv=n_kv, qd=d, vd=d, page=page, means=True)
+    slot = lambda c: (c.table[0].long()[:, None] * page + torch.arange(page, device="cuda")).view(-1)  # noqa: E731
+    kv = [torch.randn((mp * page, n_kv * d), generator=torch.Generator(device="cuda").manual_seed(i), device="cuda")
+          for i in range(2)]
+    q = torch.randn((3, heads * d), generator=torch.Generator(device="cuda").manual_seed(5), device="cuda")
+    seq, pos = ints([0] * 3), ints([999, 700, 998])
+    got = []
+    for c in (near, far):
+        c.store(*kv, slot(c))
+        back = [torch.empty_like(x) for x in kv]
+        c.load(slot(c), *back)
+        lists, out = torch.empty((3, n_kv, 5), dtype=torch.int32, device="cuda"), torch.empty_like(q)
+        c.select(q, seq, pos, lists, max_pos=999)
+        c.attend(q, seq, pos, out, max_pos=999, scale=d ** -0.5, pages=lists)
+        got.append([*back, lists, out])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 # ------------------------------------------------------------- choice of pages
 
 

@@ -694,6 +694,48 @@ def test_select_many_pages(n_seq, mp, n_sel):
             assert got[s, kv].tolist() == sorted(np.argsort(-x, kind="stable")[:n_sel].tolist())
 
 
+@pytest.mark.parametrize("size,spread", [(1.0, 0.0), (1e-30, 0.0), (1e25, 0.0), (1.0, 20.0)])
+@pytest.mark.parametrize("near", [2, 40, 200, 500])
+@pytest.mark.parametrize("shape", [(32, 8, 128, 128), (6, 2, 96, 96), (40, 2, 64, 32), (4, 2, 256, 256), (8, 2, 192, 128)], ids=str)
+def test_select_near_scores(shape, near, size, spread):
+    """Pages whose scores differ by less than f32 sums resolve around the last
+    one chosen, few of them and more than are settled together; mean keys among
+    f16's subnormals; queries of any size, heads e^20 apart."""
+    import torch
+
+    from moe_amd.paged import KvCache
+
+    heads, n_kv, qd, vd = shape
+    page, mp, n_sel, n_seq = 32, 600, 20, 3
+    g = np.random.default_rng(near)
+    means = (g.standard_normal((n_seq * mp, n_kv, qd)) * np.array([1, 6e-6, 1e4]).repeat(mp)[:, None, None]).astype(np.float16)
+    table = np.stack([g.permutation(mp) + s * mp for s in range(n_seq)]).astype(np.int32)
+    q = (g.standard_normal((n_seq, heads, qd)) * size * np.exp(spread * g.standard_normal((n_seq, heads, 1)))).astype(np.float32)
+    for s in range(n_seq):
+        at = g.permutation(np.arange(5, mp - 5))[:near]
+        top = means[table[s, at[0]]]
+        for kv in range(n_kv):  # along the first head: well above the others
+            qq = q[s, kv * (heads // n_kv)]
+            top[kv] = (qq / np.abs(qq).max() * 4 * np.array([1, 6e-6, 1e4])[s]).astype(np.float16)
+        bits = np.broadcast_to(top.view(np.uint16), (near, n_kv, qd)).copy()
+        bits[np.arange(near), :, g.integers(0, qd, near)] += g.integers(0, 2, (near, 1), dtype=np.uint16)
+        means[table[s, at]] = bits.view(np.float16)
+    pool = torch.zeros(len(means) * n_kv * 18 * (qd + vd), dtype=torch.uint8, device="cuda")
+    d = lambda x: torch.from_numpy(x).cuda()  # noqa: E731
+    cache = KvCache(pool, d(table), n_kv=n_kv, qd=qd, vd=vd, page=page, means=d(means))
+    pos = [mp * page - 1, mp * page - 40, mp * page - 1]
+    lists = torch.empty((n_seq, n_kv, n_sel), dtype=torch.int32, device="cuda")
+    cache.select(d(q.reshape(n_seq, -1)), ints(range(n_seq)), ints(pos), lists, max_pos=mp * page - 1, sinks=1, recent=2)
+    got = lists.cpu().numpy()
+    for s in range(n_seq):
+        cur = pos[s] // page
+        for kv in range(n_kv):
+            qq = q[s].reshape(n_kv, -1, qd)[kv].astype(np.float64)
+            x = (means[table[s, :cur + 1], kv].astype(np.float64) @ qq.T).max(-1)
+            x[0] = x[cur - 1:] = np.inf
+            assert got[s, kv].tolist() == sorted(np.argsort(-x, kind="stable")[:n_sel].tolist())
+
+
 # ------------------------------------------- calls together, streams and graphs
 
 

@@ -21,6 +21,17 @@
 // m a running maximum (it moves when a score exceeds it by 6) and 2^E above
 // every value scale seen, so P d_v stays below 2^15 and mostly above 2^-10.
 // Sums are f32; the two pieces' rounding is 2^-22, as f32 dot products' own.
+//
+// Decode reads the cache once and is bound by it: 64 sequences of 6000 to 12000
+// positions, 8 kv heads of 128, 147 us (4.5 TB/s of tiles); 32 sequences of up to
+// 1200 with 16 heads of 192/128 27.5 (3 TB/s: two blocks a CU, a start and a merge
+// beside 19 to 38 tiles each); one sequence of 100001 positions in 256 parts 31 +
+// 5.4 for the joining launch.  Prompts are bound by instruction issue: a tile's
+// products (two f16 passes) take about a third of the slots that scaling block by
+// block, exponentials and the two pieces of the weights take beside them; 2000
+// rows of 32 heads of 128 120 us in a loop, 136 alone (270 and 240 TFLOP/s of the
+// attention's own operations), 8000 rows 357 TFLOP/s, against 1220 of a large f16
+// product.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -717,7 +728,9 @@ Plan plan_of(const Kv4 &c, int rows, int heads, int max_pos, int window, int n_s
     const int rep = heads / c.n_kv;
     // Two column tiles a wave halve the unpacking, and two sets of them a block
     // halve what comes before the first tile and after the last, where rows come
-    // in runs; from two blocks of 64 columns a CU on.
+    // in runs; from one such block a CU on (2000 rows of 32 heads over 8 of 128:
+    // 281 us with one tile and set, 161 with two tiles, 130 with two sets of them;
+    // below it one tile in blocks of 16 columns fills more CUs).
     const long long wide = ((long long)rows * rep + 63) / 64 * c.n_kv;
     p.C = n_sel == 0 && c.qd <= 192 && c.vd <= 128 && wide >= 256 ? 2 : 1;
     p.cols = p.C == 2 ? 64 : 16;

@@ -1,6 +1,13 @@
 // kv4_cache.hip — writing and reading rows of the paged 4-bit cache
 // (moe_kv4_store, moe_kv4_load): layout in kv4.h, quantiser as
 // moe_quantize_rows(Q4_0) (src/quant.rs:304-365).
+//
+// Both are streams of f32 rows, eight lanes a 32-value block: 16376 rows of 8 kv
+// heads of 128 are written in 40.5 us (152 MB, 3.8 TB/s; the byte-wide stores of
+// a value's lanes are what keeps it off the copy's 4.9) and read in 31.4 (4.8),
+// their 255 full pages' mean keys taken in 10.8; 999 rows of 16 heads of 192/128
+// 11.5, 8.4 and 9 (the mean keys' pages are few, so latency); 32 rows 3.0, 2.3
+// and 5.1.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

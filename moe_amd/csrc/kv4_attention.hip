@@ -728,11 +728,14 @@ Plan plan_of(const Kv4 &c, int rows, int heads, int max_pos, int window, int n_s
     const int rep = heads / c.n_kv;
     // Two column tiles a wave halve the unpacking, and two sets of them a block
     // halve what comes before the first tile and after the last, where rows come
-    // in runs; from one such block a CU on (2000 rows of 32 heads over 8 of 128:
-    // 281 us with one tile and set, 161 with two tiles, 130 with two sets of them;
-    // below it one tile in blocks of 16 columns fills more CUs).
+    // in runs; but blocks of 64 columns are a quarter as many.  At 128 dims they
+    // pay from about two such blocks a CU on (one tile and 16 columns beside them:
+    // 520 rows of 32 heads over 8 26.7 and 34.5 us, 1000 54 and 54, 1200 71 and 64,
+    // 2000 155 and 129).  Wider heads lose a wave of every SIMD to the registers
+    // (4000 rows of 16 heads of 192/128 298 and 359), 96 dims gain nothing (4000
+    // rows of 6 heads 194 and 222), nor do 64 below 16000 rows.
     const long long wide = ((long long)rows * rep + 63) / 64 * c.n_kv;
-    p.C = n_sel == 0 && c.qd <= 192 && c.vd <= 128 && wide >= 256 ? 2 : 1;
+    p.C = n_sel == 0 && c.qd == 128 && c.vd == 128 && wide >= 512 ? 2 : 1;
     p.cols = p.C == 2 ? 64 : 16;
     p.rc = std::min(rep, p.cols);
     p.chunks = (rep + p.rc - 1) / p.rc;
@@ -814,10 +817,10 @@ int moe_kv4_attention(const moe_kv4 *c, const float *q, int64_t q_stride, int32_
     const int qc = a.c.qd / 32, vc = a.c.vd / 32;
     // Widths of their own: a power-of-two head and the latent cache's 192/128;
     // the others count their blocks at run time.
-    if (qc == 2 && vc == 2) p.C == 2 ? launch<2, 2, true, 2>(a, s) : launch<2, 2, true, 1>(a, s);
+    if (qc == 2 && vc == 2) launch<2, 2, true, 1>(a, s);
     else if (qc == 4 && vc == 4) p.C == 2 ? launch<4, 4, true, 2>(a, s) : launch<4, 4, true, 1>(a, s);
-    else if (qc == 6 && vc == 4) p.C == 2 ? launch<6, 4, true, 2>(a, s) : launch<6, 4, true, 1>(a, s);
-    else if (qc <= 6 && vc <= 4) p.C == 2 ? launch<6, 4, false, 2>(a, s) : launch<6, 4, false, 1>(a, s);
+    else if (qc == 6 && vc == 4) launch<6, 4, true, 1>(a, s);
+    else if (qc <= 6 && vc <= 4) launch<6, 4, false, 1>(a, s);
     else if (qc == 8 && vc == 8) launch<8, 8, true, 1>(a, s);
     else launch<8, 8, false, 1>(a, s);
     if (a.ps > 16) hipLaunchKernelGGL((kv4_join_kernel<256>), dim3((unsigned)rows * heads), dim3(256), 0, s, a);

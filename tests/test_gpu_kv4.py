@@ -388,19 +388,20 @@ def test_unseen_positions_do_not_matter(shape, bad):
     assert not np.isfinite(got[sees]).all(axis=1).any()
 
 
-def test_unseen_positions_do_not_matter_to_many_rows():
+@pytest.mark.parametrize("heads", [32, 64])
+def test_unseen_positions_do_not_matter_to_many_rows(heads):
     """The same where the rows fill the wide groups: 600 rows, an infinity and
     a NaN at positions that the earlier rows do not see, in tiles the others'
     scales follow at once."""
-    shape = (32, 8, 128, 128)
+    shape = (heads, 8, 128, 128)
     cache, k, v = device_pool(shape, 1, 640, 64)
     import torch
 
-    q = torch.randn((600, 32 * 128), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    q = torch.randn((600, heads * 128), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
     seq, pos = [0] * 600, list(range(600))
-    clean = run_attend(cache, q.cpu().numpy(), seq, pos, 32, 128 ** -0.5)
+    clean = run_attend(cache, q.cpu().numpy(), seq, pos, heads, 128 ** -0.5)
     pick = list(range(0, 600, 17)) + [399, 400, 401, 431, 432]
-    close(clean[pick], attend64(k, v, q[pick], [0] * len(pick), pick, 32, 128 ** -0.5))
+    close(clean[pick], attend64(k, v, q[pick], [0] * len(pick), pick, heads, 128 ** -0.5))
     pool = ref.Pool(10, 8, 128, 128, 64, cache.pool.cpu().numpy().copy())
     table = cache.table.cpu().numpy()
     bad = np.array([np.inf, 1, np.nan, -np.inf], np.float16)
@@ -410,7 +411,7 @@ def test_unseen_positions_do_not_matter_to_many_rows():
             for keys in (True, False):
                 pool.put(slot, kv, np.full(128, 11, np.uint8), bad, keys)
     cache.pool.copy_(torch.from_numpy(pool.raw))
-    got = run_attend(cache, q.cpu().numpy(), seq, pos, 32, 128 ** -0.5)
+    got = run_attend(cache, q.cpu().numpy(), seq, pos, heads, 128 ** -0.5)
     # The finite scale beside them (1, above every other) moves the power of two
     # that the weights are held under, so their two pieces round elsewhere: by
     # up to 2^-22 of a weight, within TOL.
@@ -490,6 +491,7 @@ def attend64(k, v, q, seq, pos, heads, scale, window=0):
     ((4, 2, 256, 256), 20001, [(0, 20000)]),
     ((32, 8, 128, 128), 3000, [(0, p) for p in range(2500, 3000)]),
     ((32, 32, 128, 128), 900, [(0, p) for p in range(900)]),
+    ((32, 8, 128, 128), 2000, [(0, p) for p in range(700, 2000)]),
 ])
 def test_long_contexts_and_prompts(shape, ctx, rows):
     """One sequence far along (its positions go to many blocks), and long runs
@@ -509,28 +511,29 @@ def test_long_contexts_and_prompts(shape, ctx, rows):
             close(got[pick], want, 2 * TOL)
 
 
-@pytest.mark.parametrize("rows", [5, 1024])
-def test_positions_past_2_30(rows):
+@pytest.mark.parametrize("shape,rows", [((16, 2, 64, 64), 5), ((16, 2, 64, 64), 1024), ((32, 8, 128, 128), 1100)], ids=str)
+def test_positions_past_2_30(shape, rows):
     """A sequence of more than 2^30 positions, a page in the middle of the
     window missing: few rows, and enough of them for the wide groups."""
     import torch
 
     from moe_amd.paged import KvCache
 
-    shape, page, mid = (16, 2, 64, 64), 4096, 1 << 18
+    heads, n_kv, d, _ = shape
+    page, mid = 4096, 1 << 18
     few, k, v = device_pool(shape, 1, 2 * page, page)
     table = torch.full((1, mid + 1), -1, dtype=torch.int32, device="cuda")
     table[0, mid - 2], table[0, mid] = few.table[0, 0], few.table[0, 1]
-    cache = KvCache(few.pool, table, n_kv=2, qd=64, vd=64, page=page)
-    q = torch.randn((rows, 16 * 64), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
-    got = run_attend(cache, q.cpu().numpy(), [0] * rows, [mid * page + r for r in range(rows)], 16, 0.125, 2 * page)
+    cache = KvCache(few.pool, table, n_kv=n_kv, qd=d, vd=d, page=page)
+    q = torch.randn((rows, heads * d), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    got = run_attend(cache, q.cpu().numpy(), [0] * rows, [mid * page + r for r in range(rows)], heads, 0.125, 2 * page)
     pick = list(range(0, rows, max(1, rows // 20)))
     # without the missing page the rows are at 4096 + r, with a window of 4096
-    close(got[pick], attend64(k, v, q[pick], [0] * len(pick), [page + r for r in pick], 16, 0.125, page))
+    close(got[pick], attend64(k, v, q[pick], [0] * len(pick), [page + r for r in pick], heads, 0.125, page))
 
 
-@pytest.mark.parametrize("shape,rows", [((8, 2, 64, 64), 3), ((6, 2, 96, 96), 40), ((16, 2, 64, 64), 1024), ((16, 2, 96, 64), 1024)],
-                         ids=str)
+@pytest.mark.parametrize("shape,rows", [((8, 2, 64, 64), 3), ((6, 2, 96, 96), 40), ((16, 2, 64, 64), 1024), ((16, 2, 96, 64), 1024),
+                                        ((32, 8, 128, 128), 1100)], ids=str)
 def test_unseen_sizes_do_not_matter(shape, rows):
     """Values 10^11 times those that the rows see, before their window and in
     the rest of the last page: outputs keep their relative precision."""
@@ -565,8 +568,8 @@ def test_unseen_sizes_do_not_matter(shape, rows):
 
 
 @pytest.mark.parametrize("window", [0, 90])
-@pytest.mark.parametrize("shape", [(100, 1, 64, 64), (96, 2, 96, 32), (32, 8, 128, 128), (16, 16, 192, 128), (90, 3, 224, 64)],
-                         ids=str)
+@pytest.mark.parametrize("shape", [(100, 1, 64, 64), (96, 2, 96, 32), (32, 8, 128, 128), (16, 16, 192, 128), (90, 3, 224, 64),
+                                   (128, 8, 128, 128), (100, 1, 128, 128)], ids=str)
 def test_ragged_batches_of_many_rows(shape, window):
     """Sequences of different lengths, rows that are none between them, rows in
     no order, more query heads a kv head than a block's columns."""

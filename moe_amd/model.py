@@ -667,6 +667,8 @@ class Model:
         if rc:
             L.check(rc, "moe_embed_rows")
         buf = {"norm": torch.empty((t, H), dtype=f32, device=dev), "out": torch.empty((t, H), dtype=f32, device=dev)}
+        if isinstance(st, PagedState):
+            buf["work"] = self._paged_workspace(b, st)
         norm, out = buf["norm"], buf["out"]
         px, pn = x.data_ptr(), norm.data_ptr()
         for li, lay in enumerate(self.layers):
@@ -729,7 +731,7 @@ class Model:
                     proj.copy_(tmp)
                 self._rope(proj, t, proj.shape[1], heads, qd, 0, qd, b, sp)
             if isinstance(st, PagedState):
-                return self._attend_paged(li, lay, q, k, v, b, st, resid, ws, sp, take)
+                return self._attend_paged(li, lay, q, k, v, b, st, resid, ws, sp, take, buf["work"])
             kd, vdim, dst = n_kv * qd, n_kv * vd, b.dst.data_ptr()
             rc = lib.moe_scatter_rows(k.data_ptr(), t, kd, kd, st.k[li].data_ptr(), kd, dst, sp)
             rc = rc or lib.moe_scatter_rows(v.data_ptr(), t, vdim, vdim, st.v[li].data_ptr(), vdim, dst, sp)
@@ -762,7 +764,7 @@ class Model:
                                           m.v_head, k.data_ptr(), v.data_ptr(), rows.data_ptr(), sp)
                 if rc:
                     L.check(rc, "moe_mla_kv_store")
-                return self._attend_paged(li, lay, q, k, v, b, st, resid, ws, sp, take)
+                return self._attend_paged(li, lay, q, k, v, b, st, resid, ws, sp, take, buf["work"])
             rc = lib.moe_mla_kv_store(kv.data_ptr(), c.data_ptr(), ca, m.kv_lora, t, s.heads, m.qk_nope, m.qk_rope,
                                       m.v_head, st.k[li].data_ptr(), st.v[li].data_ptr(), b.dst.data_ptr(), sp)
             if rc:
@@ -775,30 +777,42 @@ class Model:
             L.check(rc, "moe_attention")
         lay["o"](ctxv, take("y", s.hidden), ws, residual=resid, stream=sp)
 
-    def _attend_paged(self, li, lay, q, k, v, b: PagedBatch, st: PagedState, resid, ws, sp, take):
+    @staticmethod
+    def _reads(lay, b: PagedBatch, st: PagedState):
+        """(window or 0, pages its rows choose or 0) of a layer's attention: a
+        window's layer reads its window."""
+        window = lay["window"] or 0
+        choose = b.sparse and not window and b.max_pos // st.page >= st.sparse.pages
+        return window, st.sparse.pages if choose else 0
+
+    def _paged_workspace(self, b: PagedBatch, st: PagedState):
+        """The workspace that a step's page choices and attentions run on in
+        turn: what the layer whose call needs most needs."""
+        need = 0
+        for window, n_sel in {self._reads(lay, b, st) for lay in self.layers}:
+            size = st.kv[0]._size  # (one of every layer's cache)
+            need = max(need, size("moe_kv4_attention_workspace_size", b.t, self.spec.heads, b.max_pos, window, n_sel),
+                       size("moe_kv4_select_workspace_size", b.t, b.max_pos) if n_sel else 0)
+        return torch.empty(need, dtype=torch.uint8, device=self.device)
+
+    def _attend_paged(self, li, lay, q, k, v, b: PagedBatch, st: PagedState, resid, ws, sp, take, work):
         """The cache write and attention of _attention over a PagedState."""
         cache, lib, t = st.kv[li], L.lib(), b.t
-        heads, seq, pos, window = self.spec.heads, b.seq.data_ptr(), b.pos.data_ptr(), lay["window"] or 0
+        heads, seq, pos = self.spec.heads, b.seq.data_ptr(), b.pos.data_ptr()
         rc = lib.moe_kv4_store(cache._c, k.data_ptr(), k.shape[1], v.data_ptr(), v.shape[1], t, b.dst.data_ptr(), sp)
         if rc:
             L.check(rc, "moe_kv4_store")
 
-        def scratch(name, *args):
-            n = cache._size(name, t, *args)
-            return (take("scratch " + name, -(-n // (4 * t))).data_ptr() if n else None), n
-
-        lists, n_sel = None, 0
-        # (a window's layer reads its window)
-        if b.sparse and not window and b.max_pos // st.page >= st.sparse.pages:
-            n_sel = st.sparse.pages
+        buf, n = work.data_ptr() or None, work.numel()
+        window, n_sel = self._reads(lay, b, st)
+        lists = None
+        if n_sel:
             lists = take("lists", cache.n_kv * n_sel).data_ptr()  # 32-bit whole numbers
-            buf, n = scratch("moe_kv4_select_workspace_size", b.max_pos)
             rc = lib.moe_kv4_select(cache._c, q.data_ptr(), q.shape[1], t, heads, seq, pos, b.max_pos, st.sparse.sinks,
                                     st.sparse.recent, n_sel, lists, buf, n, sp)
             if rc:
                 L.check(rc, "moe_kv4_select")
         out = take("ctx", heads * cache.vd)
-        buf, n = scratch("moe_kv4_attention_workspace_size", heads, b.max_pos, window, n_sel)
         rc = lib.moe_kv4_attention(cache._c, q.data_ptr(), q.shape[1], t, heads, self.attn_scale, seq, pos, b.max_pos,
                                    window, lists, n_sel, out.data_ptr(), out.shape[1], buf, n, sp)
         if rc:

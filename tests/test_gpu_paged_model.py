@@ -231,3 +231,54 @@ def test_ends_and_steps_on_a_stream_that_is_not_current(ctx):
     assert st.table.length.tolist() == [0, 33, 0, 0] and b.table.length.tolist() == [0, 35, 1, 0]
     assert b.seq.tolist() == [1, 1, 2] and b.pos.tolist() == [33, 34, 0]
     m.close()
+
+
+class Taking(Rounding):
+    """The library with every row that goes into an f32 cache taken from a
+    paged state's caches instead, as they read back: both attend over the same
+    values, in any layer."""
+
+    def __init__(self, lib, model, st):
+        super().__init__(lib, model)
+        self.st, self.calls = st, 0
+
+    def moe_scatter_rows(self, src, rows, n, ss, dst, ds, dst_rows, sp):
+        import torch
+
+        st = self.st
+        at = _view(dst_rows, (rows,), "<i8").long()
+        cache, keys = st.kv[self.calls // 2], self.calls % 2 == 0
+        self.calls += 1
+        seq, pos = at // st.ctx, at % st.ctx
+        slots = st.table.table[seq, pos // st.page].long() * st.page + pos % st.page
+        x = torch.empty((rows, n), device="cuda")
+        cache.load(slots, *((x, None) if keys else (None, x)))
+        _view(dst, (int(at.max()) + 1, n), "<f4")[at] = x
+        torch.cuda.synchronize()
+        return 0
+
+
+@pytest.mark.parametrize("windows", [(2048, None, 100), (None, 2600, 1500)], ids=str)
+def test_layers_of_different_windows(ctx, monkeypatch, windows):
+    """Decode steps past 3000 positions over layers whose windows differ, so
+    that their positions are shared among differing numbers of blocks: logits as
+    with an f32 cache of the same values."""
+    from moe_amd import model as M
+    from moe_amd import synth
+    from moe_amd.model import Model, Spec, upload_store
+
+    cfg, ck = synth.build_host_model(synth.model_shape("tiny_mixtral", layers=3, vocab=1000), 0)
+    spec = Spec.derive(cfg, {n: t.shape for n, t in ck.items()})
+    spec.windows = list(windows)
+    m = Model(ctx, spec, upload_store(ctx, ck))
+    paged, plain = m.new_state(1, 3200, cache="q4", page=32), m.new_state(1, 3200)
+    lib = M.L.lib()
+    for toks in [ids(3010, 1000, 3), [5], [6], ids(4, 1000, 4), [7]]:
+        got = m.forward([toks], paged).cpu().numpy()
+        with monkeypatch.context() as p:
+            taking = Taking(lib, m, paged)
+            p.setattr(M.L, "lib", lambda: taking)
+            want = m.forward([toks], plain).cpu().numpy()
+        assert taking.calls == 2 * len(windows)
+        assert rel_err(got, want) < MODEL_TOL
+    m.close()

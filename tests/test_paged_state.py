@@ -91,3 +91,91 @@ def test_positions_have_numbers():
 def test_streams_of_another_device(state):
     with pytest.raises(ValueError, match="stream of cuda:1"):
         state.table._on(SimpleNamespace(device_index=1, cuda_stream=5))
+
+
+class Sizes:
+    """The library's sizes, its launches recorded: every workspace with the
+    bytes that the call declares it to have."""
+
+    def __init__(self, lib):
+        self.lib, self.calls = lib, []
+
+    def __getattr__(self, name):
+        if name.endswith("_size"):
+            return getattr(self.lib, name)
+        if name in ("moe_kv4_attention", "moe_kv4_select"):
+            return lambda *a: self.calls.append((name, *((a[14], a[15], a[9]) if "att" in name else (a[12], a[13], 0)))) or 0
+        return lambda *a: 0
+
+
+class Told:
+    """A projection that does nothing."""
+
+    def __call__(self, x, y, *a, **kw):
+        return y
+
+    def workspace_size(self, t):
+        return 256
+
+    feed_forward = __call__
+
+
+def steps_of(monkeypatch, windows, sparse=None, pos=20000, rows=1):
+    """Workspaces of one step's calls over layers with these windows: (call,
+    declared bytes, bytes there are from its address on, window)."""
+    from moe_amd import _lib as L
+
+    m = fake_model(layers=len(windows), windows=windows)
+    m.spec = Spec(hidden=64, layers=len(windows), heads=32, kv_heads=8, head_dim=128, vocab=10, windows=list(windows))
+    st = m.new_state(1, pos + 64, cache="q4", sparse=sparse)
+    st.pos[0] = pos
+    m.embed = SimpleNamespace(offset=0, dt=0, rows=10, cols=64)
+    m.store = SimpleNamespace(region=SimpleNamespace(device_ptr=lambda: 0))
+    m.lm_head, m._ws, m._mws, m._ws_t, m.attn_scale, m.inv_freq = Told(), None, None, 0, 1.0, torch.zeros(64)
+    m.layers = [dict(ln1=torch.ones(64), ln2=torch.ones(64), moe=Told(), q=Told(), k=Told(), v=Told(), o=Told(),
+                     bias=[None] * 3, q_norm=None, k_norm=None, window=w) for w in windows]
+    m._ffn_workspace = lambda t: torch.empty(256)
+    lib, made = Sizes(L.lib()), []
+    empty = torch.empty
+
+    def record(*a, **kw):
+        t = empty(*a, **kw)
+        made.append(t)
+        return t
+
+    with monkeypatch.context() as p:
+        p.setattr(M.L, "lib", lambda: lib)
+        p.setattr(M, "_stream_ptr", lambda s: 0 if s is None else s)
+        p.setattr(M.PageTable, "advance", lambda self, add, r, out=None, stream=None: r)
+        p.setattr(torch, "empty", record)
+        M.Model.trunk(m, [[1] * rows], st, stream=7)
+    there = lambda at: max((t.data_ptr() + t.numel() * t.element_size() - at for t in made  # noqa: E731
+                            if t.data_ptr() <= at < t.data_ptr() + t.numel() * t.element_size()), default=0)
+    return [(name, n, there(at) if at else 0, w) for name, at, n, w in lib.calls], m, st
+
+
+@pytest.mark.parametrize("windows", [(4096, None), (None, 4096), (2048, None), (1500, 9000, None, 64), (64, 64)], ids=str)
+@pytest.mark.parametrize("sparse", [None, Sparse(16), Sparse(200, recent=3)], ids=str)
+@pytest.mark.parametrize("rows", [1, 3])
+def test_layers_of_different_windows_have_the_scratch_they_declare(monkeypatch, windows, sparse, rows):
+    """A layer's workspace depends on its window and on lists: what a call
+    says it has is there, and is what the call needs."""
+    import ctypes as C
+
+    from moe_amd import _lib as L
+
+    calls, m, st = steps_of(monkeypatch, windows, sparse, rows=rows)
+    assert [w for name, _, _, w in calls if "att" in name] == [w or 0 for w in windows]
+    chosen = 0
+    for name, declared, there, window in calls:
+        assert declared <= there, f"{name}: {declared} bytes declared, {there} there (window {window})"
+        need = C.c_uint64()
+        if name == "moe_kv4_select":
+            chosen = sparse.pages
+            L.check(L.lib().moe_kv4_select_workspace_size(st.kv[0]._c, rows, 20000 + rows - 1, C.byref(need)))
+        else:
+            L.check(L.lib().moe_kv4_attention_workspace_size(st.kv[0]._c, rows, 32, 20000 + rows - 1, window, chosen,
+                                                             C.byref(need)))
+            chosen = 0
+        assert declared >= need.value
+    assert any(d for _, d, _, _ in calls) == (windows != (64, 64))

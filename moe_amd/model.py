@@ -436,11 +436,9 @@ class PagedBatch:
         self.ids = dev[n:]
         # The new lengths and the free pages' state are the state's only when
         # the step is queued (commit): one that fails half-way is as if not made.
-        old = st.table
-        self.table = PageTable(old.table, torch.empty_like(old.length), old.ring, torch.empty_like(old.state), st.page)
-        rows = old.advance(dev[:n], Rows.new(n, t, device), out=self.table, stream=sp)
-        _keep_for(sp, queued, dev, rows.seq, rows.pos, rows.slot, rows.row_start, rows.status, old.length, old.state,
-                  self.table.length, self.table.state)
+        self.table = st.next
+        rows = st.table.advance(dev[:n], Rows.new(n, t, device), out=self.table, stream=sp)
+        _keep_for(sp, queued, dev, rows.seq, rows.pos, rows.slot, rows.row_start, rows.status)
         self.seq, self.pos, self.dst = rows.seq, rows.pos, rows.slot
         self.max_pos = max(st.pos[q] + c for q, c in zip(seqs, counts)) - 1
         self.sparse = st.sparse is not None and max(counts) == 1
@@ -466,7 +464,10 @@ class PagedState:
             raise ValueError(f"{n_seq} sequences of {ctx} positions over {pages} pages")
         self.ctx, self.n_seq, self.page, self.pages, self.sparse = ctx, n_seq, page, pages, sparse
         self.pos = [0] * n_seq
-        self.table = PageTable.new(n_seq, each, pages, page, model.device)
+        # Lengths and free pages twice: a step reads the one and writes the
+        # other (next), so that no step frees what a stream has yet to read.
+        self.table = t = PageTable.new(n_seq, each, pages, page, model.device)
+        self.next = PageTable(t.table, torch.empty_like(t.length), t.ring, torch.empty_like(t.state), page)
         self.kv = [KvCache.new(pages, self.table.table, n_kv=n_kv, qd=qd, vd=vd, page=page, means=sparse is not None)
                    for _ in range(s.layers)]
 
@@ -681,7 +682,7 @@ class Model:
                 L.check(rc, "moe_rmsnorm")
             self._ffn(lay).feed_forward(norm, out, residual=x, stream=sp, workspace=mws)
         if isinstance(st, PagedState):
-            st.table = b.table
+            st.table, st.next = b.table, st.table
         for q, toks in zip(seqs, tokens):
             st.pos[q] += len(toks)
         return x, b

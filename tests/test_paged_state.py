@@ -179,3 +179,41 @@ def test_layers_of_different_windows_have_the_scratch_they_declare(monkeypatch, 
             chosen = 0
         assert declared >= need.value
     assert any(d for _, d, _, _ in calls) == (windows != (64, 64))
+
+
+def test_steps_free_no_lengths(monkeypatch):
+    """A step's new lengths and free pages go to memory that the state keeps:
+    what one stream has yet to read is not freed for another to write."""
+    from moe_amd import _lib as L
+
+    m = fake_model()
+    st = m.new_state(2, 100, cache="q4", page=32)
+    where = lambda: (st.table.length.data_ptr(), st.table.state.data_ptr(), st.table.table.data_ptr(),  # noqa: E731
+                     st.table.ring.data_ptr())
+    m.spec.layers, m.layers = 0, []
+    m.embed = SimpleNamespace(offset=0, dt=0, rows=10, cols=64)
+    m.store = SimpleNamespace(region=SimpleNamespace(device_ptr=lambda: 0))
+    m._workspace = m._ffn_workspace = lambda t: torch.empty(256)
+    reads, writes = [], []
+
+    def advance(self, add, r, out=None, stream=None):
+        reads.append(self.length.data_ptr())
+        writes.append(out.length.data_ptr())
+        return r
+
+    lib = Sizes(L.lib())
+    monkeypatch.setattr(M.L, "lib", lambda: lib)
+    monkeypatch.setattr(M, "_stream_ptr", lambda s: 0 if s is None else s)
+    monkeypatch.setattr(M.PageTable, "advance", advance)
+    seen = []
+    for i in range(6):
+        seen.append(where())
+        kept = st.table.length
+        M.Model.trunk(m, [[1], [2]], st, stream=7)
+        assert st.table.length is not kept and reads[-1] == seen[-1][0] and writes[-1] == where()[0]
+        del kept
+    assert seen[0] != seen[1] and seen[0] == seen[2] == seen[4] and seen[1] == seen[3] == seen[5]
+    assert seen[0][2:] == seen[1][2:]
+    # a step that fails half-way leaves the state's own
+    st.batch([0], [[1]], m.device, 7, False)
+    assert where() == seen[0]

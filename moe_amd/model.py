@@ -23,6 +23,8 @@ weights are bound by the Hugging Face names the reference reads
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import inspect
 import math
 from dataclasses import dataclass, field
 from typing import Optional, Sequence
@@ -409,6 +411,34 @@ class Sparse:
     recent: int = 2
 
 
+def _as_current(sp: int, device):
+    """Stream sp as torch's current one: tensors made meanwhile are sp's, and
+    so are torch's own copies and fills."""
+    return torch.cuda.stream(torch.cuda.ExternalStream(sp, device=device) if sp else torch.cuda.default_stream(device))
+
+
+def _on_its_stream(call):
+    """Run a Model method with its `stream` current, where it is another: what
+    the call allocates for a moment goes back to the stream that reads it, and
+    what torch copies or fills waits for the kernels before it.  What it returns
+    is kept for the caller's stream too."""
+    at = list(inspect.signature(call).parameters).index("stream") - 1
+
+    @functools.wraps(call)
+    def run(self, *args, **kw):
+        stream = args[at] if len(args) > at else kw.get("stream")
+        if stream is None or self.device.type != "cuda" or _stream_ptr(stream) == _stream_ptr(None):
+            return call(self, *args, **kw)
+        caller = torch.cuda.current_stream()
+        with _as_current(_stream_ptr(stream), self.device):
+            got = call(self, *args, **kw)
+        for t in got if isinstance(got, tuple) else (got,):
+            if isinstance(t, torch.Tensor):
+                t.record_stream(caller)
+        return got
+    return run
+
+
 def _keep_for(sp: int, queued: bool, *tensors) -> None:
     """Memory that stream sp reads though another one is current: freed, it
     goes to no other work before sp is done with it."""
@@ -611,11 +641,19 @@ class Model:
                 lins += [v for k, v in lay.items() if isinstance(v, Linear)]
             need = max(l.workspace_size(t) for l in lins)
             if self._ws is None or self._ws.numel() < need:
+                self._last_read(self._ws)
                 buf = torch.empty(need + 256, dtype=torch.uint8, device=self.device)
                 off = (-buf.data_ptr()) % 256
                 self._ws = buf[off:off + need]
             self._ws_t = t
         return self._ws
+
+    @staticmethod
+    def _last_read(ws):
+        """A workspace that a larger one replaces may be another stream's
+        memory: it goes to nothing else before the steps so far are done."""
+        if ws is not None and ws.is_cuda:
+            ws.record_stream(torch.cuda.current_stream())
 
     @staticmethod
     def _ffn(lay):
@@ -628,6 +666,7 @@ class Model:
         zero)."""
         need = max(self._ffn(lay).workspace_size(t) for lay in self.layers)
         if self._mws is None or self._mws.numel() < need:
+            self._last_read(self._mws)
             self._mws = MoeLayer.new_workspace(need, device=self.device)
         return self._mws
 
@@ -636,10 +675,12 @@ class Model:
     # layer), so what a call does not need is done once: the stream handle per
     # forward, the buffers per forward (every layer reuses them, in stream
     # order), raw addresses instead of ctypes objects.
+    @_on_its_stream
     def trunk(self, tokens: list, st: State, seqs: Optional[list] = None, stream=None):
         """Model::trunk (src/model.rs:646-684) for tokens[i] (a list per
         sequence, sequence seqs[i] of the state); returns the residual
-        stream [rows, H] and the batch."""
+        stream [rows, H] and the batch.  Calls of one model share its
+        workspaces: the caller orders their streams."""
         s = self.spec
         seqs = list(range(len(tokens))) if seqs is None else seqs
         seq_of, pos_of, ids = [], [], []
@@ -651,7 +692,7 @@ class Model:
             if p + n > st.ctx:
                 raise ValueError("context window exhausted")
         sp = _stream_ptr(stream)
-        queued = stream is None or sp == _stream_ptr(None)
+        queued = self.device.type == "cuda"  # (sp is the current stream)
         if isinstance(st, PagedState):
             b = st.batch(seqs, tokens, self.device, sp, queued)
         else:
@@ -820,6 +861,7 @@ class Model:
             L.check(rc, "moe_kv4_attention")
         lay["o"](out, take("y", self.spec.hidden), ws, residual=resid, stream=sp)
 
+    @_on_its_stream
     def head(self, x, rows, stream=None):
         """Model::head (src/model.rs:636-642) for the chosen rows of the
         residual stream: logits [len(rows), vocab]."""
@@ -838,6 +880,7 @@ class Model:
         logits = torch.empty((n, s.vocab), dtype=torch.float32, device=self.device)
         return self.lm_head(nx, logits, self._workspace(n), stream=stream)
 
+    @_on_its_stream
     def forward(self, tokens: list, st: State, seqs: Optional[list] = None, stream=None):
         """Model::forward (src/model.rs:565-570) for each sequence: the
         logits of its last token, [len(tokens), vocab]."""
@@ -851,18 +894,21 @@ class Model:
         # (a paged batch has its rows in the order of the sequences' numbers)
         return self.head(x, getattr(b, "ends", None) or ends, stream)
 
+    @_on_its_stream
     def forward_all(self, tokens: list, st: State, stream=None):
         """Model::forward_all (src/model.rs:572-589) for one sequence: logits
         at every position."""
         x, b = self.trunk([tokens], st, [0], stream)
         return self.head(x, list(range(len(tokens))), stream)
 
+    @_on_its_stream
     def argmax(self, logits, stream=None):
         out = torch.empty(logits.shape[0], dtype=torch.int32, device=self.device)
         L.check(L.lib().moe_argmax(C.c_void_p(logits.data_ptr()), logits.shape[0], logits.shape[1],
                                    C.c_void_p(out.data_ptr()), C.c_void_p(_stream_ptr(stream))), "moe_argmax")
         return out
 
+    @_on_its_stream
     def generate_greedy(self, prompts: list, max_tokens: int, st: Optional[State] = None, stream=None) -> list:
         """Greedy generation (Sampler::default, temp 0: src/sample.rs:87-95;
         the loop of src/generate.rs:142-320 without stop tokens) for every

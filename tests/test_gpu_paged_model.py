@@ -282,3 +282,34 @@ def test_layers_of_different_windows(ctx, monkeypatch, windows):
         assert taking.calls == 2 * len(windows)
         assert rel_err(got, want) < MODEL_TOL
     m.close()
+
+
+@pytest.mark.parametrize("cache", ["f32", "q4"])
+@pytest.mark.parametrize("late", ["current", "own"])
+def test_steps_and_another_stream_do_not_wait_for_each_other(model, cache, late):
+    """Prompts, decode steps and greedy tokens with stream= while the current
+    stream, or that one, is behind: as without a stream, and the current
+    stream's tensors as they were."""
+    import torch
+
+    m, shape = model
+    prompts = [ids(40, shape.vocab, 1), ids(33, shape.vocab, 2)]
+    kw = dict(cache="q4", page=32) if cache == "q4" else {}
+    a, b = (m.new_state(2, 128, **kw) for _ in range(2))
+    want = [m.forward(t, a).cpu().numpy() for t in (prompts, [[3], [4]])]
+    tokens = m.generate_greedy(prompts, 4, m.new_state(2, 128, **kw))
+    c = m.new_state(2, 128, **kw)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s if late == "own" else torch.cuda.current_stream()):
+        torch.cuda._sleep(100_000_000)
+    got = [m.forward(t, b, stream=s) for t in (prompts, [[3], [4]])]
+    junk = [torch.full((n,), 5, dtype=torch.int32, device="cuda") for n in (4, 64, 5000, 100000) for _ in range(20)]
+    assert m.generate_greedy(prompts, 4, c, stream=s.cuda_stream) == tokens
+    s.synchronize()
+    with torch.cuda.stream(s):
+        got = [x.cpu().numpy() for x in got]
+    for x, y in zip(got, want):
+        assert np.array_equal(x, y)
+    torch.cuda.synchronize()
+    assert all((j == 5).all().item() for j in junk)

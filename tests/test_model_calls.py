@@ -108,3 +108,64 @@ def test_rows_are_not_copied_inside_a_capture(monkeypatch):
         Batch([0], [0], 8, "cpu", [1], queued=True)
     b = Batch([0, 2], [3, 1], 8, "cpu", [1, 7])
     assert b.dst.tolist() == [3, 17] and b.ids.tolist() == [1, 7] and b.max_pos == 3
+
+
+def test_calls_on_another_stream_allocate_and_copy_there(monkeypatch):
+    """With stream=7 everything that a call allocates, and every copy of
+    torch's own, is made while 7 is the current stream; what it returns is kept
+    for the caller's stream as well."""
+    from types import SimpleNamespace
+
+    from moe_amd import model as M
+
+    now, made, kept = [0], [], []
+
+    class Current:
+        def __init__(self, sp):
+            self.sp = sp
+
+        def __enter__(self):
+            self.before, now[0] = now[0], self.sp
+
+        def __exit__(self, *a):
+            now[0] = self.before
+
+    def on_cpu(f):
+        def go(*a, device=None, pin_memory=None, **kw):
+            made.append((f.__name__, now[0]))
+            return f(*a, **kw)
+        return go
+
+    monkeypatch.setattr(M.L, "lib", Ok)
+    monkeypatch.setattr(M, "_stream_ptr", lambda s: now[0] if s is None else s)
+    monkeypatch.setattr(M, "_as_current", lambda sp, device: Current(sp))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: f"stream {now[0]}")
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: kept.append((tuple(t.shape), s)))
+    for f in (torch.empty, torch.zeros, torch.arange, torch.empty_like):
+        monkeypatch.setattr(torch, f.__name__, on_cpu(f))
+    cpu = torch.Tensor.cpu
+    monkeypatch.setattr(torch.Tensor, "cpu", lambda t: (made.append(("cpu", now[0])), cpu(t).zero_())[1])
+    monkeypatch.setattr(M, "Batch", lambda seq, pos, ctx, device, ids, queued: (
+        made.append(("rows", now[0])), SimpleNamespace(t=len(seq), ids=torch.tensor(ids)))[1])
+    m = Reads()
+    m.device = SimpleNamespace(type="cuda")
+    m.embed = SimpleNamespace(offset=0, dt=0, rows=4, cols=8)
+    m.store = SimpleNamespace(region=SimpleNamespace(device_ptr=lambda: 0))
+    m._attention = lambda *args: None
+    m._mws = None
+    m.layers = [dict(ln1=torch.ones(8), ln2=torch.ones(8), moe=Layer())]
+    m.trunk = lambda *a, **kw: M.Model.trunk(m, *a, **kw)
+    st = SimpleNamespace(pos=[0], ctx=16)
+    for call, shape in ((lambda: m.forward([[1, 2, 3]], st, stream=7), (1, 8)), (lambda: m.trunk([[1]], st, None, 7), (1, 8)),
+                        (lambda: m.head(torch.ones(5, 8), [2, 3], 7), (2, 8)), (lambda: m.argmax(torch.ones(3, 4), 7), (3,))):
+        made.clear(), kept.clear()
+        call()
+        assert made and {s for _, s in made} == {7} and now == [0]
+        assert (shape, "stream 0") in kept
+    m.lm_head = lambda nx, logits, ws, stream=None: logits
+    made.clear()
+    assert m.generate_greedy([[1, 2]], 3, SimpleNamespace(pos=[0], ctx=16), stream=7) == [[0, 0, 0]]
+    assert [n for n, _ in made].count("cpu") == 3 and {s for _, s in made} == {7}
+    made.clear()
+    m.forward([[1]], st)  # the current one: as it is
+    assert {s for _, s in made} == {0}

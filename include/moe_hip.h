@@ -487,12 +487,12 @@ int moe_kv4_load(const moe_kv4 *c, const int64_t *slots, int32_t rows, float *k,
  * is 0, as is one whose scores are all minus infinity; a block of a value that
  * reads as infinite or NaN makes its 32 values NaN in the rows that see it.
  * What positions hold that no row sees does not matter.  Sums are f32 and
- * weights have 22 bits; a value smaller than 2^-12 of those that other rows of
- * the call see beside it (in its 32 positions, or before its row's window) has
- * fewer.  `workspace`:
- * device, 16-byte aligned, moe_kv4_attention_workspace_size bytes (its
- * arguments as the call's; it may be 0 bytes).  Calls that share one must be
- * ordered. */
+ * weights have 22 bits, whatever the sizes of the values beside them (products
+ * of weights and values down to 2^-70 of a head's largest; scales that lie
+ * more than 2^8 apart cost a second pass over the positions); a query's values
+ * are held to 2^-38 of its head's largest.  `workspace`: device, 16-byte
+ * aligned, moe_kv4_attention_workspace_size bytes (its arguments as the
+ * call's; it may be 0 bytes).  Calls that share one must be ordered. */
 int moe_kv4_attention_workspace_size(const moe_kv4 *c, int32_t rows, int32_t heads, int32_t max_pos, int32_t window,
                                      int32_t n_sel, uint64_t *bytes);
 int moe_kv4_attention(const moe_kv4 *c, const float *q, int64_t q_stride, int32_t rows, int32_t heads, float scale,

@@ -17,10 +17,17 @@
 // second product, whose sum runs over positions with a scale each:
 //   O^T += C (P d_v)_hi + C (P d_v)_lo
 // The weights P = 2^(s - ref) are kept so large that two f16 pieces hold
-// their products with the scales to 2^-30 of the largest: ref = m + E - 9 with
+// their products with the scales to 2^-34 of the largest: ref = m + E - 9 with
 // m a running maximum (it moves when a score exceeds it by 6) and 2^E above
 // every value scale seen, so P d_v stays below 2^15 and mostly above 2^-10.
 // Sums are f32; the two pieces' rounding is 2^-22, as f32 dot products' own.
+// Where all value scales of a wave's tiles lie within 2^8 of each other, the
+// position of weight 2^9 and more alone makes every block's sum 2 or more, of
+// which what the pieces leave is less than 2^-22 (2^-25 a product).  Where they
+// do not (a block of small values beside large ones, a far larger value that
+// hardly weighs, a 0 that takes all weight), the wave goes over its tiles once
+// more with the references it has found and four pieces: a block's precision
+// is then its own down to 2^-70 of the largest product.
 //
 // Decode reads the cache once and is bound by it: 64 sequences of 6000 to 12000
 // positions, 8 kv heads of 128, 147 us (4.5 TB/s of tiles); 32 sequences of up to
@@ -48,6 +55,7 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4_dw __attribute__((ext_vector_type(4), aligned(4)));  // at any float
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
@@ -238,7 +246,8 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
         const int t0 = a.lists ? 0 : lo >> 5;
         const int nt = a.lists ? a.n_sel << tshift : (hi >> 5) - t0 + 1;
         const int parts = a.ps * P, me = part * P + share;
-        int v = (int)((long long)nt * me / parts);
+        const int v0 = (int)((long long)nt * me / parts);
+        int v = v0;
         const int v1 = (int)((long long)nt * (me + 1) / parts);
         const int32_t *list = a.lists ? a.lists + ((size_t)(r0 + first) * kc.n_kv + kv) * a.n_sel : nullptr;
         const int32_t *table = kc.table + (size_t)sq * kc.max_pages;
@@ -346,6 +355,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
         f32x4 o[C][VC][2];
         float ref[C], lim[C], l[C];
         int E = -24;
+        int low = 0x7c00;  // the smallest value scale seen (f16 bits), of this lane's
 #pragma unroll
         for (int c = 0; c < C; c++) {
             ref[c] = 0.0f, lim[c] = -INFINITY, l[c] = 0.0f;
@@ -360,7 +370,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
         // comes out only copy b's columns of block b are read.
         auto second = [&](const T &x, const f32x4 (&p)[C][2], auto once) __attribute__((always_inline)) {
             const u32x4 *sc = (const u32x4 *)ssc[wave];
-            half8 h8[C], l8[C], v0, v1;
+            half8 h8[C], l8[C], w0, w1;
             // Weights times scales in the codes' order, bytes 0, 2, 1, 3 of
             // each half; both pieces.
             auto scaled = [&](const u32x4 &ds) __attribute__((always_inline)) {
@@ -382,9 +392,9 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                 }
             };
             auto unpack = [&](int b) __attribute__((always_inline)) {
-                const uint32_t w0 = x.v[2 * b], w1 = x.v[2 * b + 1];
-                v0 = join8(low_pair(w0, nib), low_pair(w0 >> 8, nib), low_pair(w1, nib), low_pair(w1 >> 8, nib));
-                v1 = join8(high_pair(w0, nib), high_pair(w0 >> 8, nib), high_pair(w1, nib), high_pair(w1 >> 8, nib));
+                const uint32_t y0 = x.v[2 * b], y1 = x.v[2 * b + 1];
+                w0 = join8(low_pair(y0, nib), low_pair(y0 >> 8, nib), low_pair(y1, nib), low_pair(y1 >> 8, nib));
+                w1 = join8(high_pair(y0, nib), high_pair(y0 >> 8, nib), high_pair(y1, nib), high_pair(y1 >> 8, nib));
             };
             scaled(sc[(nq + (once ? copy : 0)) * 4 + g]);
             u32x4 ds = sc[(nq + min(1, nv - 1)) * 4 + g];  // the next block's, read one ahead
@@ -394,13 +404,13 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                 if (!EX && b >= nv) continue;
 #pragma unroll
                 for (int c = 0; c < C; c++) {
-                    o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, h8[c], o[c][b][0], 0, 0, 0);
-                    o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, h8[c], o[c][b][1], 0, 0, 0);
+                    o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w0, h8[c], o[c][b][0], 0, 0, 0);
+                    o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w1, h8[c], o[c][b][1], 0, 0, 0);
                 }
 #pragma unroll
                 for (int c = 0; c < C; c++) {
-                    o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, l8[c], o[c][b][0], 0, 0, 0);
-                    o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, l8[c], o[c][b][1], 0, 0, 0);
+                    o[c][b][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w0, l8[c], o[c][b][0], 0, 0, 0);
+                    o[c][b][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w1, l8[c], o[c][b][1], 0, 0, 0);
                 }
                 // The next block's operands while these products run.
                 if (b + 1 < VC && (EX || b + 1 < nv)) {
@@ -414,34 +424,89 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                 if (C > 1) __builtin_amdgcn_sched_barrier(0);
             }
         };
-        // between(): what to do when the keys' words have been read.
-        auto step = [&](const T &x, int base, auto once, auto between) __attribute__((always_inline)) {
+        // O^T += what second()'s two pieces leave of products below 1: steps of
+        // 2^-24 are all that f16 has there.  In two pieces again, 2^39 times as
+        // large, and through sums of their own.
+        auto rest = [&](const T &x, const f32x4 (&p)[C][2], auto once) __attribute__((always_inline)) {
+            const u32x4 *sc = (const u32x4 *)ssc[wave];
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                half8 h8, l8;
+#pragma unroll
+                for (int b = 0; b < VC; b++) {
+                    if (!EX && b >= nv) continue;
+                    if (!once || b == 0) {
+                        const u32x4 ds = sc[(nq + (once ? copy : b)) * 4 + g];
+                        half2v ph[4], pl[4];
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                // (as second() has them)
+                                const float u0 = fmaf((float)as_h2(ds[2 * h])[e], p[c][h][e], 0.0f);
+                                const float u1 = fmaf((float)as_h2(ds[2 * h + 1])[e], p[c][h][2 + e], 0.0f);
+                                const half2v a = pack_half(u0, u1);
+                                const float v0 = u0 - (float)a[0], v1 = u1 - (float)a[1];
+                                const half2v b = pack_half(v0, v1);
+                                const float r0 = fabsf(u0) < 1.0f ? (v0 - (float)b[0]) * 0x1p39f : 0.0f;
+                                const float r1 = fabsf(u1) < 1.0f ? (v1 - (float)b[1]) * 0x1p39f : 0.0f;
+                                const half2v z = pack_half(r0, r1);
+                                ph[2 * h + e] = z;
+                                pl[2 * h + e] = pack_half(r0 - (float)z[0], r1 - (float)z[1]);
+                            }
+                        h8 = join8(ph[0], ph[1], ph[2], ph[3]), l8 = join8(pl[0], pl[1], pl[2], pl[3]);
+                    }
+                    const uint32_t y0 = x.v[2 * b], y1 = x.v[2 * b + 1];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const half8 w = h ? join8(high_pair(y0, nib), high_pair(y0 >> 8, nib), high_pair(y1, nib), high_pair(y1 >> 8, nib))
+                                          : join8(low_pair(y0, nib), low_pair(y0 >> 8, nib), low_pair(y1, nib), low_pair(y1 >> 8, nib));
+                        f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+                        r = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, h8, r, 0, 0, 0);
+                        r = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, l8, r, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) o[c][b][h][i] = fmaf(r[i], 0x1p-39f, o[c][b][h][i]);
+                    }
+                }
+            }
+        };
+        // between(): what to do when the keys' words have been read.  again: with
+        // the references that a walk before has found.
+        auto step = [&](const T &x, int base, auto once, auto again, auto between) __attribute__((always_inline)) {
             // Scales through LDS (the wave's own: in order, no barrier): every
             // lane reads its four positions of both halves, 16 bytes.
-            lds_order();       // the reads of the tile before
-            uint32_t top = 0;  // the largest finite value scale of the lane's, f16 bits
-            bool inf = false;
-            auto largest = [&](uint32_t seen) __attribute__((always_inline)) {
+            lds_order();  // the reads of the tile before
+            u16x2 top = {0, 0}, least = {0x7fff, 0x7fff};  // of the lane's value scales, f16 bits
+#pragma unroll
+            for (int e = 0; e < T::NS; e++) {
+                ssc[wave][lane + 64 * e] = x.s[e];
+                const int at = lane + 64 * e;
+                const bool value = at >= nq * 16 && at < (nq + nv) * 16;
+                const uint32_t y = x.s[e] & 0x7fff7fffu;
+                top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, value ? y : 0u));
+                least = __builtin_elementwise_min(least, __builtin_bit_cast(u16x2, value ? y : 0x7fff7fffu));
+            }
+            const bool inf = __any(max(top[0], top[1]) >= 0x7c00);
+            if (__builtin_expect(inf || base < lo || base + kTile - 1 > hi, 0)) {
+                // Finite ones of positions that the run sees: what lies in a
+                // page's rest or before the window must not set the weights'
+                // power of two.  A lane's pair of scales is the same two positions
+                // in every block.
+                const int w = 2 * col, p = base + 4 * (w >> 3) + 16 * (w >> 2 & 1) + (w & 3);
+                top = u16x2{0, 0}, least = u16x2{0x7fff, 0x7fff};
 #pragma unroll
                 for (int e = 0; e < T::NS; e++) {
                     const int at = lane + 64 * e;
-                    const uint32_t y = at >= nq * 16 && at < (nq + nv) * 16 ? x.s[e] & seen : 0;
-                    const uint32_t y0 = y & 0xffffu, y1 = y >> 16;
-                    inf |= y0 >= 0x7c00u || y1 >= 0x7c00u;
-                    top = max(top, max(y0 >= 0x7c00u ? 0 : y0, y1 >= 0x7c00u ? 0 : y1));
-                }
-            };
 #pragma unroll
-            for (int e = 0; e < T::NS; e++) ssc[wave][lane + 64 * e] = x.s[e];
-            largest(0x7fff7fffu);
-            if (__builtin_expect(base < lo || base + kTile - 1 > hi, 0)) {
-                // Of positions that the run sees: what lies in a page's rest or
-                // before the window must not set the weights' power of two.  A
-                // lane's pair of scales is the same two positions in every block.
-                const int w = 2 * col, p = base + 4 * (w >> 3) + 16 * (w >> 2 & 1) + (w & 3);
-                top = 0;
-                largest((p >= lo && p <= hi ? 0x7fffu : 0) | (p + 1 >= lo && p + 1 <= hi ? 0x7fff0000u : 0));
+                    for (int k = 0; k < 2; k++) {
+                        const uint16_t y = x.s[e] >> (16 * k) & 0x7fff;
+                        if (at < nq * 16 || at >= (nq + nv) * 16 || y >= 0x7c00 || p + k < lo || p + k > hi) continue;
+                        top[k] = max(top[k], y), least[k] = min(least[k], y);
+                    }
+                }
             }
+            const int most = max(top[0], top[1]);
+            low = min(low, (int)min(least[0], least[1]));
             lds_order();
             const u32x4 *sc = (const u32x4 *)ssc[wave];
             f32x4 s[C][2];
@@ -523,9 +588,9 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                 mx[c] *= ck[c];
                 move |= mx[c] > lim[c];
             }
-            const bool grow = (int)(top >> 10) - 14 > E;  // not below 2^E
-            if (__any(move || grow)) {
-                int ne = (int)(top >> 10) - 14;
+            const bool grow = (most >> 10) - 14 > E;  // not below 2^E
+            if (!again && __any(move || grow)) {
+                int ne = (most >> 10) - 14;
 #pragma unroll
                 for (int w = 32; w >= 1; w >>= 1) ne = max(ne, __shfl_xor(ne, w, 64));
                 ne = max(ne, E);
@@ -555,7 +620,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
             // Scales that are infinite or NaN (rare): positions of weight 0 may
             // hold them, so they become 0, and what a column does see of them
             // makes the block's 32 values NaN.
-            if (__builtin_expect(__any(inf), 0)) {
+            if (__builtin_expect(inf, 0)) {
 #pragma unroll
                 for (int b = 0; b < VC; b++) {
                     if (!EX && b >= nv) continue;
@@ -584,6 +649,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
                 lds_order();
             }
             second(x, s, once);
+            if (again) rest(x, s, once);
         };
         auto none = [] {};
         auto walk = [&](auto once) __attribute__((always_inline)) {
@@ -592,19 +658,34 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
             // this one's have been read, its values at the end.
             while (C == 1 && any) {
                 load(y);
-                if (x.ok) step(x, x.base, once, none);
+                if (x.ok) step(x, x.base, once, std::false_type{}, none);
                 if (v > v1) break;
                 load(x);
-                if (y.ok) step(y, y.base, once, none);
+                if (y.ok) step(y, y.base, once, std::false_type{}, none);
                 if (v > v1) break;
             }
             while (C > 1 && any) {
                 // (a tile that is none: behind the last position there can be)
                 const int base = x.ok ? x.base : 0x7fffffff - (kTile - 1);
                 find(x);
-                step(x, base, once, [&] { load_keys(x); });
+                step(x, base, once, std::false_type{}, [&] { load_keys(x); });
                 load_values(x);
                 if (v > v1) break;
+            }
+            // Scales 2^-8 of the largest and less (or subnormal ones, or 0): what
+            // they scale may be all that has weight in a block of a value, below
+            // what two pieces under one power of two hold.  The same tiles again,
+            // with what those leave.
+            if (__builtin_expect(!__any(low < max((E + 6) << 10, 0x400)), 1)) return;
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                l[c] = 0.0f;
+#pragma unroll
+                for (int b = 0; b < VC; b++) o[c][b][0] = o[c][b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+            for (v = v0; v < v1;) {
+                load(x);
+                if (x.ok) step(x, x.base, once, std::true_type{}, none);
             }
         };
         if (C == 1 && copies) walk(std::integral_constant<bool, C == 1>{});

@@ -567,6 +567,88 @@ def test_unseen_sizes_do_not_matter(shape, rows):
                               [first + r for r in pick], heads, qd ** -0.5, window))
 
 
+def blocks_close(got, cache, table_slots, q, seq, pos, heads, scale, tol, window=0):
+    """Per row, head and 32-value block: the largest error against the largest
+    of the block's sums of |weight value|, which is what f32 sums are off by a
+    share of.  The cache's values as they read back, in 64 bits."""
+    import torch
+
+    n_seq, ctx = table_slots.shape
+    n_kv, qd, vd, rep = cache.n_kv, cache.qd, cache.vd, heads // cache.n_kv
+    kb, vb = (torch.empty((n_seq * ctx, n_kv * d), device="cuda") for d in (qd, vd))
+    cache.load(table_slots.reshape(-1), kb, vb)
+    k, v = kb.view(n_seq, ctx, n_kv, qd).double(), vb.view(n_seq, ctx, n_kv, vd).double()
+    errors = []
+    for r, (s, p) in enumerate(zip(seq, pos)):
+        lo = max(0, p + 1 - window) if window else 0
+        qq = q[r].double().view(n_kv, rep, qd)
+        kk, vv = (x[s, lo:p + 1].permute(1, 0, 2).contiguous() for x in (k, v))
+        w = torch.softmax(torch.matmul(qq, kk.transpose(1, 2).contiguous()) * scale, -1)
+        want, size = torch.matmul(w, vv).view(heads, -1, 32), torch.matmul(w, vv.abs()).view(heads, -1, 32).amax(-1)
+        err = (torch.from_numpy(got[r]).cuda().double().view(heads, -1, 32) - want).abs().amax(-1)
+        assert bool(torch.isfinite(size).all()) and bool((err[size == 0] == 0).all())
+        errors.append(float((err / size.clamp(min=1e-300)).max()))
+    assert np.max(errors) < tol, np.max(errors)  # (a NaN is none)
+
+
+UNEVEN = {  # shape, positions, rows
+    "one_row": ((8, 2, 64, 64), 200, [190]), "rows": ((8, 2, 64, 64), 200, range(150, 190)),
+    "latent": ((16, 16, 192, 128), 150, range(130, 140)), "96": ((6, 2, 96, 96), 150, range(100, 140)),
+    "224": ((1, 1, 224, 64), 100, [60, 99]), "256": ((4, 2, 256, 256), 100, range(80, 90)),
+    "parts": ((32, 8, 128, 128), 9000, [8990]), "prompt": ((32, 8, 128, 128), 1200, range(20, 1200)),
+    "wide": ((32, 32, 128, 128), 1200, range(60, 1200))}
+
+
+@pytest.mark.parametrize("how", ["block", "early", "late", "silent", "mixed", "subnormal"])
+@pytest.mark.parametrize("name", list(UNEVEN))
+def test_uneven_values_keep_their_precision(name, how):
+    """What is small among a head's values is as exact as if it were alone:
+    one block of 32 dims 2^-16 of the others (or a subnormal scale's size); a
+    position whose values are 2^20 times the others' and that hardly weighs
+    anything, before or behind them; one that takes nearly all weight and is 0;
+    every block of a size of its own.
+
+    Tolerance: sums of up to 9000 products in f32, sqrt(9000) 2^-24 and 2^-22
+    of the two pieces, are within TOL.  A score S is off by 2^-22 S (the query's
+    two pieces) and 2^-24 S (its sum in f32), and a weight by as much; scores
+    that weigh are below 6 but for the silent position's 13."""
+    import torch
+
+    from moe_amd.paged import KvCache
+
+    (heads, n_kv, qd, vd), ctx, rows = UNEVEN[name]
+    page = 64
+    mp = -(-ctx // page)
+    g = torch.Generator(device="cuda").manual_seed(len(name))
+    table = torch.randperm(mp, generator=g, device="cuda").to(torch.int32).view(1, mp)
+    cache = KvCache.new(mp, table, n_kv=n_kv, qd=qd, vd=vd, page=page)
+    slots = (table.long()[:, :, None] * page + torch.arange(page, device="cuda")).view(1, -1)
+    k = torch.randn((mp * page, n_kv, qd), generator=g, device="cuda")
+    v = torch.randn((mp * page, n_kv, vd), generator=g, device="cuda")
+    q = torch.randn((len(rows), heads, qd), generator=g, device="cuda")
+    scale, S = qd ** -0.5, 6.0
+    q[..., 0], k[..., 0] = 2.0, 0.0
+    at = {"early": 3, "late": min(rows) - 2, "silent": 0}.get(how)
+    if how == "block":
+        v[..., -32:] *= 2.0 ** -16
+    elif how == "subnormal":
+        v[..., :32] *= 2.0 ** -18
+    elif how == "mixed":
+        v *= torch.exp2(torch.randint(-11, 12, (mp * page, n_kv, vd // 32, 1), generator=g, device="cuda").float()) \
+            .expand(-1, -1, -1, 32).reshape(v.shape)
+    else:
+        k[at], q[..., 1:32] = 0.0, 0.0
+        k[at, :, 0] = (13.0 if how == "silent" else -28.0) / scale / 2.0
+        v *= 2.0 ** -8
+        v[at] *= 0.0 if how == "silent" else 2.0 ** 20
+        S = 13.0
+    cache.store(k.view(len(k), -1), v.view(len(v), -1), slots.view(-1))
+    got = run_attend(cache, q.view(len(rows), -1).cpu().numpy(), [0] * len(rows), list(rows), heads, scale)
+    pick = list(range(0, len(rows), max(1, len(rows) // 25)))
+    blocks_close(got[pick], cache, slots, q.view(len(rows), -1)[pick], [0] * len(pick), [rows[i] for i in pick], heads, scale,
+                 TOL + S * (2.0 ** -22 + 2.0 ** -24))
+
+
 @pytest.mark.parametrize("window", [0, 90])
 @pytest.mark.parametrize("shape", [(100, 1, 64, 64), (96, 2, 96, 32), (32, 8, 128, 128), (16, 16, 192, 128), (90, 3, 224, 64),
                                    (128, 8, 128, 128), (100, 1, 128, 128)], ids=str)

@@ -4,7 +4,7 @@
 // Rows find their sequence and position on the device, so one kernel serves
 // decode steps, prompts and chunks.  A block takes a group of consecutive rows
 // and one kv head, splits the group into runs of one sequence and makes each
-// run's (row, query head) pairs the 16 or 32 columns of its products on the
+// run's (row, query head) pairs the 16 or 64 columns of its products on the
 // f16 matrix cores; its waves (and, where there are few rows, several blocks)
 // split the run's tiles of 32 positions and merge at the end.
 //
@@ -71,7 +71,7 @@ struct Args {
     float scale;
     int tt, groups;  // rows of a group, groups
     int rc, chunks;  // query heads of a block, blocks that share a kv head's
-    int split;       // blocks that share a group's runs
+    int split;       // blocks that share a group's runs (of 64 columns: its groups of 16)
     int ps;          // blocks that share a run's tiles
 };
 
@@ -149,40 +149,55 @@ __device__ inline void load_words(uint32_t (&w)[2 * NB], __amdgpu_buffer_rsrc_t 
     }
 }
 
+// What a block shares.
+template <int QC, int VC, int C, int S, int W>
+struct Lds {
+    u32x4 sq_[S * C * QC * 2 * 64];  // Q operands: [column tile][block][hi, lo][lane]
+    f32x4 smo[W * VC * 2 * 64];      // O of the waves: [wave][block][half][lane]
+    uint32_t ssc[W][Tile<QC, VC>::NS * 64];
+    float sm_r[W][C * 16], sm_l[W][C * 16], sm_k[S * C * 16];
+};
+
+// Lanes of my_seq and my_pos that begin a run of one sequence's rows or are
+// none; the runs' first lanes.
+struct Runs {
+    unsigned long long cuts, starts, valid;
+};
+__device__ inline Runs runs_of(const Kv4 &c, int my_seq, int my_pos, int nr) {
+    const int lane = threadIdx.x & 63;
+    const bool valid = lane < nr && my_pos >= 0 && (unsigned)my_seq < (unsigned)c.n_seq;
+    const int before = __shfl_up(my_seq, 1, 64);
+    const bool before_ok = __shfl_up((int)valid, 1, 64);
+    Runs r;
+    r.valid = __ballot(valid);
+    r.cuts = __ballot(!valid || lane == 0 || my_seq != before || !before_ok);
+    r.starts = r.cuts & r.valid;
+    return r;
+}
+
+// A block's work: rows r0 .. r0 + nr - 1 (whose sequences and positions the
+// lanes hold), heads h0 .. h0 + hn - 1; of the rows' runs every split-th from
+// `sub` on, of their tiles the part-th part.
 // QC, VC: blocks of a key and a value (EX) or the most there may be.  C:
 // 16-column tiles of a wave.  W waves: S sets of columns, W / S parts of the
 // positions.
 template <int QC, int VC, bool EX, int C, int S, int W>
-__global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) {
+__device__ __attribute__((always_inline)) inline void attend(const Args &a, Lds<QC, VC, C, S, W> &lds, int kv, int part, int r0,
+                                                             int nr, int h0, int hn, int my_seq, int my_pos, int sub,
+                                                             int split) {
     typedef Tile<QC, VC> T;
     constexpr int P = W / S;
-    __shared__ u32x4 sq_[S * C * QC * 2 * 64];  // Q operands: [column tile][block][hi, lo][lane]
-    __shared__ f32x4 smo[W * VC * 2 * 64];  // O of the waves: [wave][block][half][lane]
-    __shared__ uint32_t ssc[W][T::NS * 64];
-    __shared__ float sm_r[W][C * 16], sm_l[W][C * 16], sm_k[S * C * 16];
+    auto &sq_ = lds.sq_;
+    auto &smo = lds.smo;
+    auto &ssc = lds.ssc;
+    auto &sm_r = lds.sm_r, &sm_l = lds.sm_l;
+    auto &sm_k = lds.sm_k;
     const Kv4 &kc = a.c;
     const Nibbles nib;
     const float less = minus_one();
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4, set = wave % S, share = wave / S;
     const int nq = EX ? QC : kc.qd / 32, nv = EX ? VC : kc.vd / 32;
-    // Kv heads next to each other go to the XCDs in turn, so that one head's
-    // blocks find its tiles in their L2.  Later rows of a prompt see more
-    // positions: the last groups go first.  A group's blocks that find no run
-    // of their own leave at once, so the first ones come together.
-    int id = blockIdx.x;
-    const int kv = id % kc.n_kv;
-    id /= kc.n_kv;
-    const int chunk = id % a.chunks;
-    id /= a.chunks;
-    const int part = id % a.ps;
-    id /= a.ps;
-    const int sub = id / a.groups;
-    const int r0 = (a.groups - 1 - id % a.groups) * a.tt;
-    const int nr = min(a.tt, a.rows - r0);
-    const int h0 = kv * a.rep + chunk * a.rc, hn = min(a.rc, a.rep - chunk * a.rc);
-    const int my_seq = gload(a.seq + r0 + min(lane, nr - 1)), my_pos = gload(a.pos + r0 + min(lane, nr - 1));
-
     // Column cc of the block is query head h0 + cc % hn of row r0 + cc / hn,
     // whatever run it is in: queries load while sequences and tables do.  16
     // threads a column, four values each at a time.
@@ -199,19 +214,16 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
             qv[k][j] = __builtin_bit_cast(f32x4, gload_x4((const uint32_t *)(row + d)));
         }
     }
-    const bool valid = lane < nr && my_pos >= 0 && (unsigned)my_seq < (unsigned)kc.n_seq;
-    const int before = __shfl_up(my_seq, 1, 64);
-    const bool before_ok = __shfl_up((int)valid, 1, 64);
-    // Lanes that begin a run or are none; the runs' first lanes.
-    const unsigned long long cuts = __ballot(!valid || lane == 0 || my_seq != before || !before_ok);
-    unsigned long long starts = cuts & __ballot(valid);
+    const Runs runs = runs_of(kc, my_seq, my_pos, nr);
+    const unsigned long long cuts = runs.cuts;
+    unsigned long long starts = runs.starts;
     const int tshift = kc.page_shift - 5;
     bool staged = false;
 
     for (int run = 0; starts; run++) {
         const int first = __builtin_ctzll(starts);
         starts &= starts - 1;
-        if (run % a.split != sub) continue;
+        if (run % split != sub) continue;
         const unsigned long long after = first < 63 ? cuts >> (first + 1) : 0;
         const int end = min(nr, after ? first + 1 + __builtin_ctzll(after) : 64);
         const bool mine = lane >= first && lane < end;
@@ -747,6 +759,54 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) 
     }
 }
 
+// C tiles of 16 columns a wave and S sets of them pay where one run fills them:
+// a group of 64 columns with several runs (sequences that decode, ends of
+// prompts), or with no more than 16 columns, is dealt to its blocks in groups of
+// 16 instead.  (1024 sequences of 32 heads over 8 that decode at 500 positions:
+// 499 us with 64 columns a block, 191 with 16; a prompt of 2000 rows 124 and 144;
+// that prompt beside 512 that decode 1402 and 387.)
+template <int QC, int VC, bool EX, int C, int S, int W>
+__global__ __launch_bounds__(W * 64, 2) void kv4_attention_kernel(const Args a) {
+    union Both {
+        Lds<QC, VC, C, S, W> wide;
+        Lds<QC, VC, 1, 1, W> narrow;
+    };
+    __shared__ Both lds;
+    const Kv4 &kc = a.c;
+    const int lane = threadIdx.x & 63;
+    // Kv heads next to each other go to the XCDs in turn, so that one head's
+    // blocks find its tiles in their L2.  Later rows of a prompt see more
+    // positions: the last groups go first.  A group's blocks that find no run
+    // of their own leave at once, so the first ones come together.
+    int id = blockIdx.x;
+    const int kv = id % kc.n_kv;
+    id /= kc.n_kv;
+    const int chunk = id % a.chunks;
+    id /= a.chunks;
+    const int part = id % a.ps;
+    id /= a.ps;
+    const int sub = id / a.groups;
+    const int r0 = (a.groups - 1 - id % a.groups) * a.tt;
+    const int nr = min(a.tt, a.rows - r0);
+    const int h0 = kv * a.rep + chunk * a.rc, hn = min(a.rc, a.rep - chunk * a.rc);
+    const int my_seq = gload(a.seq + r0 + min(lane, nr - 1)), my_pos = gload(a.pos + r0 + min(lane, nr - 1));
+    if (C == 1) {
+        attend<QC, VC, EX, 1, 1, W>(a, lds.narrow, kv, part, r0, nr, h0, hn, my_seq, my_pos, sub, a.split);
+        return;
+    }
+    const Runs runs = runs_of(kc, my_seq, my_pos, nr);
+    if (__popcll(runs.starts) == 1 && __popcll(runs.valid) * hn > 16) {
+        if (sub == 0) attend<QC, VC, EX, C, S, W>(a, lds.wide, kv, 0, r0, nr, h0, hn, my_seq, my_pos, 0, 1);
+        return;
+    }
+    const int chunks = (hn + 15) / 16, rc = min(hn, 16), tt = 16 / rc;
+    const int r1 = sub / chunks * tt, h1 = sub % chunks * 16;
+    if (r1 >= nr) return;
+    const int n1 = min(tt, nr - r1), from = r1 + min(lane, n1 - 1);
+    attend<QC, VC, EX, 1, 1, W>(a, lds.narrow, kv, 0, r0 + r1, n1, h0 + h1, min(rc, hn - h1), __shfl(my_seq, from, 64),
+                                __shfl(my_pos, from, 64), 0, 1);
+}
+
 // The parts of rows whose tiles several blocks shared: a block of T threads
 // per (row, head), each group of vd / 4 of them every so many-th part; the
 // groups' sums in order.
@@ -824,7 +884,9 @@ Plan plan_of(const Kv4 &c, int rows, int heads, int max_pos, int window, int n_s
     p.tt = n_sel ? 1 : p.cols / p.rc;
     p.groups = (int)(((long long)rows + p.tt - 1) / p.tt);
     const long long base = (long long)p.groups * p.chunks * c.n_kv;
-    p.split = (int)std::max<long long>(1, std::min<long long>(p.tt, 1024 / base));
+    const int narrow = std::min(p.rc, 16);  // query heads of a group of 16 columns
+    p.split = p.C == 2 ? (p.tt + 16 / narrow - 1) / (16 / narrow) * ((p.rc + 15) / 16)
+                       : (int)std::max<long long>(1, std::min<long long>(p.tt, 1024 / base));
     const long long tiles = n_sel ? (long long)n_sel * c.tiles()
                                   : (window > 0 ? std::min((long long)window + p.tt, (long long)max_pos + 1) : max_pos + 1LL) / 32 + 1;
     const long long units = base * p.split;

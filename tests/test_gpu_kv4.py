@@ -671,6 +671,70 @@ def test_ragged_batches_of_many_rows(shape, window):
     close(got[pick], attend64(k, v, q[pick], [seq[i] for i in pick], [pos[i] for i in pick], heads, qd ** -0.5, window))
 
 
+@pytest.mark.parametrize("window", [0, 70])
+@pytest.mark.parametrize("shape", [(32, 8, 128, 128), (32, 32, 128, 128), (21, 3, 128, 128), (36, 3, 128, 128), (40, 2, 128, 128),
+                                   (64, 2, 128, 128), (80, 1, 128, 128)], ids=str)
+def test_wide_groups_of_mixed_rows(shape, window):
+    """So many rows that groups of 64 columns are formed, of which some are one
+    run (prompts), some several (sequences that decode, a prompt's end, rows that
+    are none), some one of few columns: 1 to 80 query heads a kv head."""
+    heads, n_kv, d, _ = shape
+    n_seq = 40
+    cache, k, v = device_pool(shape, n_seq, 200, 64)
+    g = np.random.default_rng(1)
+    # enough for 512 groups of 64 columns
+    rows, want = [], 512 // n_kv * 64 // (heads // n_kv) + 70
+    for i in range(n_seq):
+        rows += [(i, int(g.integers(0, 200)))]
+    rows += [(0, -1)] * 70 + [(5, 199)] + [(-1, 3)] * 70
+    while len(rows) < want:
+        n, s = int(g.integers(2, 200)), int(g.integers(0, n_seq))
+        rows += [(s, p) for p in range(200 - n, 200)]
+        rows += [(int(g.integers(0, n_seq)), int(g.integers(0, 200))) for _ in range(int(g.integers(0, 20)))]
+    seq, pos = zip(*rows)
+    import torch
+
+    q = torch.randn((len(rows), heads * d), generator=torch.Generator(device="cuda").manual_seed(7), device="cuda")
+    got = run_attend(cache, q.cpu().numpy(), seq, pos, heads, d ** -0.5, window)
+    none = [i for i, (a, p) in enumerate(rows) if p < 0 or not 0 <= a < n_seq]
+    assert (got[none] == 7.0).all()
+    there = [i for i in range(len(rows)) if i not in set(none)]
+    pick = there[:60] + there[60::max(1, len(there) // 300)] + there[-20:]
+    close(got[pick], attend64(k, v, q[pick], [seq[i] for i in pick], [pos[i] for i in pick], heads, d ** -0.5, window))
+    # and each row as it is in a call of few rows
+    few = pick[::40]
+    part = run_attend(cache, q[few].cpu().numpy(), [seq[i] for i in few], [pos[i] for i in few], heads, d ** -0.5, window)
+    close(part, got[few])
+
+
+def test_many_sequences_cost_what_their_halves_do():
+    """A decode step of 1024 sequences in one call, against two calls of 512,
+    each the shortest of several: groups of 64 columns are for runs that fill
+    them (in such groups the one call took 2.5 times the two)."""
+    import torch
+
+    heads, n_kv, d, n, ctx = 32, 8, 128, 1024, 320
+    cache, _, _ = device_pool((heads, n_kv, d, d), n, ctx, 64)
+    q = torch.randn((n, heads * d), device="cuda")
+    out = torch.empty_like(q)
+    seq, pos = ints(range(n)), ints([ctx - 1 - i % 50 for i in range(n)])
+
+    def time_of(*parts):
+        best = 1e9
+        for _ in range(8):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(4):
+                for lo, hi in parts:
+                    cache.attend(q[lo:hi], seq[lo:hi], pos[lo:hi], out[lo:hi], max_pos=ctx - 1, scale=d ** -0.5)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    assert time_of((0, n)) < 1.5 * time_of((0, n // 2), (n // 2, n))
+
+
 def test_load_of_keys_or_values_alone():
     import torch
 

@@ -823,7 +823,7 @@ class Model:
     def _reads(lay, b: PagedBatch, st: PagedState):
         """(window or 0, pages its rows choose or 0) of a layer's attention: a
         window's layer reads its window."""
-        window = lay["window"] or 0
+        window = min(lay["window"] or 0, 2 ** 31 - 1)  # (no context is longer)
         choose = b.sparse and not window and b.max_pos // st.page >= st.sparse.pages
         return window, st.sparse.pages if choose else 0
 

@@ -37,6 +37,23 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
+def _fits(**numbers) -> None:
+    """Numbers that the library takes in 32 bits: ctypes would drop the rest."""
+    for name, n in numbers.items():
+        if not -2 ** 31 <= n < 2 ** 31:
+            raise ValueError(f"{name} {n}: a number of 32 bits")
+
+
+def _refused(rc: int, what: str) -> None:
+    """The error of a call that the library did not make."""
+    try:
+        L.check(rc, what)
+    except L.MoeError as e:
+        if e.code in (L.MOE_EINVAL, L.MOE_EUNSUP):
+            raise ValueError(str(e)) from None
+        raise
+
+
 def _ids(t, dtype, n: int, name: str) -> None:
     if t.dtype != dtype or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {str(dtype)[6:]} tensor of {n}")
@@ -108,6 +125,7 @@ class Rows:
 
     def __init__(self, row_start, seq, pos, slot, status):
         n = seq.shape[0]
+        _fits(rows=n, sequences=status.shape[0])
         _ids(seq, torch.int32, n, "seq")
         _ids(pos, torch.int32, n, "pos")
         _ids(slot, torch.int64, n, "slot")
@@ -133,6 +151,7 @@ class PageTable(_OnDevice):
     def __init__(self, table, length, ring, state, page: int):
         _need(table.dtype == torch.int32 and table.dim() == 2 and table.is_contiguous(),
               "table must be a contiguous int32 [sequences, pages] tensor")
+        _fits(page=page, sequences=table.shape[0], pages=table.shape[1], pool=ring.shape[0])
         _ids(length, torch.int32, table.shape[0], "length")
         _ids(ring, torch.int32, ring.shape[0], "ring")
         _ids(state, torch.int32, 2, "state")
@@ -165,14 +184,14 @@ class PageTable(_OnDevice):
         self._check_device(add, rows.seq)
         if not self._bytes:
             b = C.c_uint64()
-            L.check(L.lib().moe_pages_workspace_size(n, C.byref(b)), "moe_pages_workspace_size")
+            _refused(L.lib().moe_pages_workspace_size(n, C.byref(b)), "moe_pages_workspace_size")
             self._bytes = b.value
         sp = self._on(stream)
         ws = self._scratch(self._bytes, sp)
         rc = L.lib().moe_pages_advance(n, self._now[0], add.data_ptr(), out._now[0], *self._where, self._now[1],
                                        out._now[1], *rows._args, ws.data_ptr(), self._bytes, sp)
         if rc:
-            L.check(rc, "moe_pages_advance")
+            _refused(rc, "moe_pages_advance")
         return rows
 
 
@@ -188,6 +207,7 @@ class KvCache(_OnDevice):
               "table must be a contiguous int32 [sequences, pages] tensor")
         n_pages = pool.shape[0] // self.page_bytes(n_kv, qd, vd, page)
         _need(n_pages >= 1, f"a pool of {pool.shape[0]} bytes holds no page")
+        _fits(sequences=table.shape[0], pages=table.shape[1], pool=n_pages)
         if means is not None:
             _need(means.dtype == torch.float16 and means.is_contiguous() and tuple(means.shape) == (n_pages, n_kv, qd),
                   f"means must be a contiguous float16 [{n_pages}, {n_kv}, {qd}] tensor")
@@ -200,17 +220,16 @@ class KvCache(_OnDevice):
                         means=None if means is None else means.data_ptr(), n_seq=table.shape[0],
                         max_pages=table.shape[1], n_pages=n_pages, page=page, n_kv=n_kv, qd=qd, vd=vd)
         self._c = C.byref(self.c)
+        self._positions = table.shape[1] * page
         self._sizes = {}
 
     @staticmethod
     def page_bytes(n_kv: int, qd: int, vd: int, page: int) -> int:
         """Bytes of a page; ValueError for sizes the cache does not hold."""
+        _fits(page=page, n_kv=n_kv, qd=qd, vd=vd)
         one = L.Kv4C(n_pages=1, page=page, n_kv=n_kv, qd=qd, vd=vd)
         b = C.c_uint64()
-        try:
-            L.check(L.lib().moe_kv4_pool_size(C.byref(one), C.byref(b)), "moe_kv4_pool_size")
-        except L.MoeError as e:
-            raise ValueError(str(e)) from None
+        _refused(L.lib().moe_kv4_pool_size(C.byref(one), C.byref(b)), "moe_kv4_pool_size")
         return b.value
 
     @staticmethod
@@ -224,7 +243,7 @@ class KvCache(_OnDevice):
         n = self._sizes.get((name, args))
         if n is None:
             b = C.c_uint64()
-            L.check(getattr(L.lib(), name)(self._c, *args, C.byref(b)), name)
+            _refused(getattr(L.lib(), name)(self._c, *args, C.byref(b)), name)
             if len(self._sizes) > 256:
                 self._sizes.clear()
             n = self._sizes[name, args] = b.value
@@ -236,18 +255,20 @@ class KvCache(_OnDevice):
         value width] (float32) into `slots` (int64, distinct; rows of negative
         slots are skipped)."""
         n = k.shape[0]
+        _fits(rows=n)
         ks, vs = _rows(k, n, self.n_kv * self.qd, "k"), _rows(v, n, self.n_kv * self.vd, "v")
         _ids(slots, torch.int64, n, "slots")
         self._check_device(k, v, slots)
         rc = L.lib().moe_kv4_store(self._c, k.data_ptr(), ks, v.data_ptr(), vs, n, slots.data_ptr(), self._on(stream))
         if rc:
-            L.check(rc, "moe_kv4_store")
+            _refused(rc, "moe_kv4_store")
 
     @_on_its_device
     def load(self, slots, k=None, v=None, stream=None) -> None:
         """Read the rows of `slots` into k and v (float32, either may be
         None); rows of negative slots are left as they were."""
         n = slots.shape[0]
+        _fits(rows=n)
         _ids(slots, torch.int64, n, "slots")
         ks = 0 if k is None else _rows(k, n, self.n_kv * self.qd, "k")
         vs = 0 if v is None else _rows(v, n, self.n_kv * self.vd, "v")
@@ -255,10 +276,12 @@ class KvCache(_OnDevice):
         rc = L.lib().moe_kv4_load(self._c, slots.data_ptr(), n, None if k is None else k.data_ptr(), ks,
                                   None if v is None else v.data_ptr(), vs, self._on(stream))
         if rc:
-            L.check(rc, "moe_kv4_load")
+            _refused(rc, "moe_kv4_load")
 
-    def _query(self, q, seq, pos):
+    def _query(self, q, seq, pos, max_pos):
         """(rows, heads, row stride) of a call's queries."""
+        if not 0 <= max_pos < self._positions:
+            raise ValueError(f"max_pos {max_pos}: the table has {self._positions} positions a sequence")
         n, width = q.shape if q.dim() == 2 else (-1, 0)
         heads = width // self.qd
         if heads < 1 or heads % self.n_kv:
@@ -282,7 +305,9 @@ class KvCache(_OnDevice):
         max_pos, over the last `window` positions when that is above 0, over
         the pages `pages` lists (select's int32 [rows, kv heads, n]) when
         given."""
-        n, heads, qs = self._query(q, seq, pos)
+        n, heads, qs = self._query(q, seq, pos, max_pos)
+        if not -2 ** 31 <= window < 2 ** 31:
+            _fits(window=window)
         os = _rows(out, n, heads * self.vd, "out")
         if pages is None:
             n_sel, lists = 0, None
@@ -296,7 +321,7 @@ class KvCache(_OnDevice):
         rc = L.lib().moe_kv4_attention(self._c, q.data_ptr(), qs, n, heads, scale, seq.data_ptr(), pos.data_ptr(), max_pos,
                                        window, lists, n_sel, out.data_ptr(), os, ws.data_ptr() if need else None, need, sp)
         if rc:
-            L.check(rc, "moe_kv4_attention")
+            _refused(rc, "moe_kv4_attention")
 
     @_on_its_device
     def select(self, q, seq, pos, lists, *, max_pos: int, sinks: int = 1, recent: int = 1, stream=None):
@@ -305,7 +330,7 @@ class KvCache(_OnDevice):
         `recent`, then by score; -1 behind the last."""
         if self.means is None:
             raise ValueError("the cache keeps no mean keys")
-        n, heads, qs = self._query(q, seq, pos)
+        n, heads, qs = self._query(q, seq, pos, max_pos)
         n_sel = self._lists(lists, n, "lists")
         if sinks < 0 or recent < 1 or sinks + recent > n_sel:
             raise ValueError(f"{sinks} first and {recent} last pages of {n_sel}")
@@ -316,5 +341,5 @@ class KvCache(_OnDevice):
         rc = L.lib().moe_kv4_select(self._c, q.data_ptr(), qs, n, heads, seq.data_ptr(), pos.data_ptr(), max_pos, sinks,
                                     recent, n_sel, lists.data_ptr(), ws.data_ptr() if need else None, need, sp)
         if rc:
-            L.check(rc, "moe_kv4_select")
+            _refused(rc, "moe_kv4_select")
         return lists

@@ -234,3 +234,59 @@ def test_refuses_lists_of_too_many_pages(lib):
                          ids=str)
 def test_advance_refuses_sizes_past_its_sums(lib, bad):
     assert advance(lib, ws_bytes=1 << 40, **bad) == L.MOE_EINVAL
+
+
+@pytest.mark.parametrize("bad", [dict(max_pos=-1), dict(max_pos=128), dict(max_pos=2 ** 32 + 5), dict(max_pos=-2 ** 32 + 7)], ids=str)
+def test_positions_past_the_table(lib, bad):
+    """Refused as they are, not as what 32 bits hold of them."""
+    c, a = cpu_cache(), ok_args()
+    for call in (lambda **kw: c.attend(a["q"], a["seq"], a["pos"], a["out"], scale=1.0, **kw),
+                 lambda **kw: c.select(a["q"], a["seq"], a["pos"], a["lists"], **kw)):
+        with pytest.raises(ValueError, match="max_pos"):
+            call(**bad)
+        with pytest.raises(ValueError, match="GPU"):
+            call(max_pos=127)
+
+
+@pytest.mark.parametrize("window", [2 ** 31, 2 ** 32 + 16, -2 ** 31 - 1])
+def test_windows_past_32_bits(lib, window):
+    c, a = cpu_cache(), ok_args()
+    with pytest.raises(ValueError, match="window"):
+        c.attend(a["q"], a["seq"], a["pos"], a["out"], max_pos=7, scale=1.0, window=window)
+    with pytest.raises(ValueError, match="GPU"):
+        c.attend(a["q"], a["seq"], a["pos"], a["out"], max_pos=7, scale=1.0, window=2 ** 31 - 1)
+
+
+def test_sizes_past_32_bits(lib):
+    for bad in (dict(page=2 ** 32 + 32), dict(n_kv=2 ** 32 + 2), dict(qd=2 ** 32 + 64), dict(vd=-2 ** 32 + 64)):
+        with pytest.raises(ValueError):
+            KvCache.page_bytes(**{**dict(n_kv=2, qd=64, vd=32, page=32), **bad})
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(ValueError, match="page"):
+        PageTable(i(3, 4), i(3), i(9), i(2), 2 ** 32 + 32)
+
+
+def test_what_the_library_refuses_is_a_value_error(lib, monkeypatch):
+    """Too many rows, pages of an odd size ...: as the module promises; a
+    failure of the device stays what it is."""
+    from moe_amd import paged
+
+    with pytest.raises(ValueError):
+        cpu_cache()._size("moe_kv4_attention_workspace_size", 3, 7, 10, 0, 0)
+    monkeypatch.setattr(paged._OnDevice, "_check_device", lambda self, *t: None)
+    monkeypatch.setattr(paged._OnDevice, "_on", lambda self, stream: 0)
+    monkeypatch.setattr(paged._OnDevice, "_scratch", lambda self, n, sp: torch.empty(n, dtype=torch.uint8))
+    for code, error in ((L.MOE_EINVAL, ValueError), (L.MOE_EUNSUP, ValueError), (L.MOE_EHIP, L.MoeError)):
+        class Refuses:
+            def __getattr__(self, name):
+                return getattr(lib, name) if "last_error" in name or name.endswith("_size") else lambda *a: code
+
+        with monkeypatch.context() as p:
+            p.setattr(paged.L, "lib", Refuses)
+            c, a = cpu_cache(), ok_args()
+            for call in calls(c, a).values():
+                with pytest.raises(error):
+                    call()
+            table = PageTable.new(3, 4, 9, 32, "cpu")
+            with pytest.raises(error):
+                table.advance(torch.zeros(3, dtype=torch.int32), Rows.new(3, 5, "cpu"))

@@ -217,3 +217,8 @@ def test_steps_free_no_lengths(monkeypatch):
     # a step that fails half-way leaves the state's own
     st.batch([0], [[1]], m.device, 7, False)
     assert where() == seen[0]
+
+
+def test_windows_past_32_bits_are_as_wide_as_positions_go(monkeypatch):
+    calls, _, _ = steps_of(monkeypatch, (2 ** 32 + 16, 64))
+    assert [w for _, _, _, w in calls] == [2 ** 31 - 1, 64]

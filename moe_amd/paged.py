@@ -69,7 +69,18 @@ def _rows(t, rows: int, cols: int, name: str) -> int:
     return st[0]
 
 
-class _OnDevice:
+class _Fixed:
+    """An object whose tensors' addresses are taken when it is made: its
+    attributes stay what they were.  (Their contents may change; memory that
+    another tensor should take needs another object.)"""
+
+    def __setattr__(self, name, value):
+        if name in self.__dict__ and name[0] != "_":
+            raise AttributeError(f"{type(self).__name__}.{name} is fixed: its address is taken when the object is made")
+        object.__setattr__(self, name, value)
+
+
+class _OnDevice(_Fixed):
     """Where a call's kernels and scratch go."""
 
     device: "torch.device"
@@ -118,7 +129,7 @@ def _on_its_device(call):
     return run
 
 
-class Rows:
+class Rows(_Fixed):
     """What PageTable.advance says of a step's rows: `row_start` int32
     [sequences + 1], `seq`, `pos` int32 and `slot` int64 [rows], `status` int32
     [sequences].  Their number of rows is what a step has room for."""

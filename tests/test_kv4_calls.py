@@ -290,3 +290,19 @@ def test_what_the_library_refuses_is_a_value_error(lib, monkeypatch):
             table = PageTable.new(3, 4, 9, 32, "cpu")
             with pytest.raises(error):
                 table.advance(torch.zeros(3, dtype=torch.int32), Rows.new(3, 5, "cpu"))
+
+
+def test_what_addresses_are_taken_of_is_not_replaced(lib):
+    """The kernels work on the tensors an object was made with: another one
+    in their place would not be seen, so it is refused."""
+    c, t, r = cpu_cache(), PageTable.new(3, 4, 9, 32, "cpu"), Rows.new(3, 5, "cpu")
+    for x, names in ((c, ("pool", "table", "means", "n_kv", "qd", "vd", "page", "n_pages", "c", "device")),
+                     (t, ("table", "length", "ring", "state", "page", "device")),
+                     (r, ("row_start", "seq", "pos", "slot", "status", "n_seq", "device"))):
+        for name in names:
+            now = getattr(x, name)
+            with pytest.raises(AttributeError):
+                setattr(x, name, now)
+            assert getattr(x, name) is now
+    t.length.fill_(3)  # their contents are the caller's
+    assert t.length.tolist() == [3, 3, 3]

@@ -27,18 +27,23 @@
 // do not (a block of small values beside large ones, a far larger value that
 // hardly weighs, a 0 that takes all weight), the wave goes over its tiles once
 // more with the references it has found and four pieces: a block's precision
-// is then its own down to 2^-70 of the largest product.
+// is then its own down to 2^-70 of the largest product.  (One block of four
+// 2^-12 of the others: 32-sequence decode 28 -> 53 us, 64 x 12000 164 -> 354,
+// prompt of 2000 rows 134 -> 299, one row at 100001 37 -> 66.)
 //
 // Decode reads the cache once and is bound by it: 64 sequences of 6000 to 12000
-// positions, 8 kv heads of 128, 147 us (4.5 TB/s of tiles); 32 sequences of up to
-// 1200 with 16 heads of 192/128 27.5 (3 TB/s: two blocks a CU, a start and a merge
-// beside 19 to 38 tiles each); one sequence of 100001 positions in 256 parts 31 +
-// 5.4 for the joining launch.  Prompts are bound by instruction issue: a tile's
-// products (two f16 passes) take about a third of the slots that scaling block by
-// block, exponentials and the two pieces of the weights take beside them; 2000
-// rows of 32 heads of 128 120 us in a loop, 136 alone (270 and 240 TFLOP/s of the
-// attention's own operations), 8000 rows 357 TFLOP/s, against 1220 of a large f16
-// product.
+// positions, 8 kv heads of 128, 152 us (4.4 TB/s of tiles); 32 sequences of up to
+// 1200 with 16 heads of 192/128 28 (3 TB/s: all blocks resident at once, two a
+// CU, with 19 to 38 tiles, so the longest sets the time; beside them a start, in
+// which each block of a group loads and stages the group's 16 queries, and a
+// merge); one sequence of 100001 positions in 256 parts 32 + 5.5 for the joining
+// launch.  Prompts are bound by nothing alone: a wave issues in 45% of its time,
+// waits for loads and LDS in 29% and to be issued in 26%, at 1.5 waves a SIMD
+// (256 registers, 35 spilled); vector instructions, 9.4 to a product (scaling
+// block by block, exponentials, the weights' two pieces), are issued in 52% of
+// the cycles, the matrix pipe is busy in 19%.  2000 rows of 32 heads of 128 113 us
+// in a loop, 130 alone (290 and 252 TFLOP/s of the attention's own operations),
+// 8000 rows 390 TFLOP/s, against 1200 of a large f16 product.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -870,11 +875,12 @@ Plan plan_of(const Kv4 &c, int rows, int heads, int max_pos, int window, int n_s
     // Two column tiles a wave halve the unpacking, and two sets of them a block
     // halve what comes before the first tile and after the last, where rows come
     // in runs; but blocks of 64 columns are a quarter as many.  At 128 dims they
-    // pay from about two such blocks a CU on (one tile and 16 columns beside them:
-    // 520 rows of 32 heads over 8 26.7 and 34.5 us, 1000 54 and 54, 1200 71 and 64,
-    // 2000 155 and 129).  Wider heads lose a wave of every SIMD to the registers
-    // (4000 rows of 16 heads of 192/128 298 and 359), 96 dims gain nothing (4000
-    // rows of 6 heads 194 and 222), nor do 64 below 16000 rows.
+    // pay from about two such blocks a CU on (blocks of 16 columns and of 64: 520
+    // rows of 32 heads over 8 26.1 and 29.4 us, 700 33.5 and 34.5, 1000 52.8 and
+    // 48.5, 1200 68.6 and 59.2, 2000 149 and 122, 8000 1715 and 1355).  Wider heads
+    // lose a wave of every SIMD to the registers (4000 rows of 16 heads of 192/128
+    // 298 and 359), 96 dims gain nothing (4000 rows of 6 heads 194 and 222), nor do
+    // 64 below 16000 rows.
     const long long wide = ((long long)rows * rep + 63) / 64 * c.n_kv;
     p.C = n_sel == 0 && c.qd == 128 && c.vd == 128 && wide >= 512 ? 2 : 1;
     p.cols = p.C == 2 ? 64 : 16;
@@ -897,7 +903,8 @@ Plan plan_of(const Kv4 &c, int rows, int heads, int max_pos, int window, int n_s
     // 28.2 us, in two parts 34 + 4.6; 488 of 64 tiles 34.5, 39.4 + 4.8; 512 of
     // 190 to 375 152.6, 152.3 + 4.8; 8 of 3126 tiles in 64, 128, 256 parts 60.8 +
     // 5.7, 36.8 + 5.0, 32.4 + 5.6.)
-    const long long ps = units >= 256 ? std::min((512 + units - 1) / units, tiles / 64)
+    const long long ps = p.C == 2       ? 1  // (512 blocks and more: nothing to share)
+                         : units >= 256 ? std::min((512 + units - 1) / units, tiles / 64)
                          : tiles < 48 ? 1
                                       : std::min<long long>({(2048 + units - 1) / units, tiles / 12, 256});
     p.ps = (int)std::max<long long>(1, ps);

@@ -297,9 +297,12 @@ int moe_kv4_store(const moe_kv4 *c, const float *k, int64_t k_stride, const floa
     if (rows == 0) return MOE_OK;
     hipStream_t s = (hipStream_t)stream;
     const int blocks = a.n_kv * (a.qd + a.vd) / 32;
-    // Word stores of four rows pay where there are prompts (16376 rows of 8 heads
-    // of 128: 59 -> 41 us); a few rows are latency, one row a block (32 rows:
-    // 5.7 -> 3.0 us, 999 rows of 16 heads of 192/128 13.3 -> 12.0).
+    // Word stores of four rows pay where there are prompts, one row a block where
+    // a few rows are latency (32 rows of 8 heads of 128: 5.7 -> 3.0 us).  One row
+    // and four, back to back: 4096 rows of 8 heads of 128 14.4 and 11.2 us, of 16
+    // of 192/128 29.3 and 22.9, of 2 of 64 5.7 and 6.3; 16376 rows 49.5 and 33.4,
+    // 120 and 90.5, 10.2 and 8.8.  At 2048 rows it is 8.7 and 7.8, 16.2 and 13.4,
+    // 5.7 and 6.1, at 1024 5.9 and 6.4, 9.2 and 8.4, 5.7 and 6.4.
     const unsigned y = (unsigned)(blocks + 31) / 32;
     if (rows >= 4096)
         hipLaunchKernelGGL((kv4_store_kernel<4>), dim3(row_blocks<4>(rows), y), dim3(256), 0, s, a, k, k_stride, v, v_stride,

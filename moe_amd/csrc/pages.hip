@@ -1,7 +1,7 @@
 // pages.hip — block tables and slot maps from request lengths, on the device
 // (moe_pages_advance).
 //
-// plan_pages, one block, four sequences a thread: three running sums over
+// plan_pages, one block, four sequences a thread: five running sums over
 // them (rows wanted; pages wanted; then rows, pages given back and pages taken
 // of those not refused) settle what every sequence gets.  Rows and pages are
 // refused by their running sums with the refused ones counted, so those that
@@ -17,7 +17,7 @@
 // 1024 sequences and rows is one launch of one block: 32 sequences 5.4 us (two
 // launches, a 1024-thread block and 64-bit sums: 21.5).  Beyond that the rows
 // are a launch of their own: 4096 sequences and 100000 rows 14.3 + 6.2 us, the
-// first one's four passes of scans and barriers on one CU.
+// first one's five scans, one after the other, and their barriers on one CU.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -567,7 +567,7 @@ def test_unseen_sizes_do_not_matter(shape, rows):
                               [first + r for r in pick], heads, qd ** -0.5, window))
 
 
-def blocks_close(got, cache, table_slots, q, seq, pos, heads, scale, tol, window=0):
+def blocks_close(got, cache, table_slots, q, seq, pos, heads, scale, tol, window=0, lists=None):
     """Per row, head and 32-value block: the largest error against the largest
     of the block's sums of |weight value|, which is what f32 sums are off by a
     share of.  The cache's values as they read back, in 64 bits."""
@@ -583,7 +583,10 @@ def blocks_close(got, cache, table_slots, q, seq, pos, heads, scale, tol, window
         lo = max(0, p + 1 - window) if window else 0
         qq = q[r].double().view(n_kv, rep, qd)
         kk, vv = (x[s, lo:p + 1].permute(1, 0, 2).contiguous() for x in (k, v))
-        w = torch.softmax(torch.matmul(qq, kk.transpose(1, 2).contiguous()) * scale, -1)
+        score = torch.matmul(qq, kk.transpose(1, 2).contiguous()) * scale
+        if lists is not None:  # [row, kv head, page]: whether it is listed
+            score.masked_fill_(~lists[r][:, torch.arange(lo, p + 1, device="cuda") // cache.page][:, None], -math.inf)
+        w = torch.softmax(score, -1)
         want, size = torch.matmul(w, vv).view(heads, -1, 32), torch.matmul(w, vv.abs()).view(heads, -1, 32).amax(-1)
         err = (torch.from_numpy(got[r]).cuda().double().view(heads, -1, 32) - want).abs().amax(-1)
         assert bool(torch.isfinite(size).all()) and bool((err[size == 0] == 0).all())
@@ -647,6 +650,74 @@ def test_uneven_values_keep_their_precision(name, how):
     pick = list(range(0, len(rows), max(1, len(rows) // 25)))
     blocks_close(got[pick], cache, slots, q.view(len(rows), -1)[pick], [0] * len(pick), [rows[i] for i in pick], heads, scale,
                  TOL + S * (2.0 ** -22 + 2.0 ** -24))
+
+
+@pytest.mark.parametrize("shape", [(8, 2, 64, 64), (16, 16, 192, 128), (32, 8, 128, 128), (6, 2, 96, 96)], ids=str)
+@pytest.mark.parametrize("window", [0, 45, 2 ** 31 - 1])
+def test_uneven_values_in_windows_and_lists(shape, window):
+    """Every block of a size of its own, 2^22 between them, read through a
+    window, or through lists of pages that differ from row to row."""
+    import torch
+
+    from moe_amd.paged import KvCache
+
+    heads, n_kv, qd, vd = shape
+    ctx, page = 400, 32
+    mp = -(-ctx // page)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    table = torch.randperm(mp, generator=g, device="cuda").to(torch.int32).view(1, mp)
+    cache = KvCache.new(mp, table, n_kv=n_kv, qd=qd, vd=vd, page=page)
+    slots = (table.long()[:, :, None] * page + torch.arange(page, device="cuda")).view(1, -1)
+    size = torch.exp2(torch.randint(-11, 12, (mp * page, n_kv * vd // 32, 1), generator=g, device="cuda").float())
+    v = (torch.randn((mp * page, n_kv * vd // 32, 32), generator=g, device="cuda") * size).view(mp * page, -1)
+    cache.store(torch.randn((mp * page, n_kv * qd), generator=g, device="cuda"), v, slots.view(-1))
+    rows = list(range(130, 400, 7))
+    q = torch.randn((len(rows), heads * qd), generator=g, device="cuda")
+    listed = torch.rand((len(rows), n_kv, mp), generator=g, device="cuda") < 0.4
+    listed[..., 0] = True
+    lists = torch.full((len(rows), n_kv, mp), -1, dtype=torch.int32, device="cuda")
+    at = torch.where(listed, torch.arange(mp, device="cuda"), mp).sort(-1).values
+    lists.copy_(torch.where(at < mp, at, -1))
+    # scores below 6, as above
+    tol = TOL + 6 * (2.0 ** -22 + 2.0 ** -24)
+    got = run_attend(cache, q.cpu().numpy(), [0] * len(rows), rows, heads, qd ** -0.5, window)
+    blocks_close(got, cache, slots, q, [0] * len(rows), rows, heads, qd ** -0.5, tol, window)
+    if window != 45:  # (a row's pages might all lie before it)
+        got = run_attend(cache, q.cpu().numpy(), [0] * len(rows), rows, heads, qd ** -0.5, window, lists.cpu().numpy())
+        blocks_close(got, cache, slots, q, [0] * len(rows), rows, heads, qd ** -0.5, tol, window, listed)
+
+
+@pytest.mark.parametrize("used", [3, 40, 700])
+def test_room_for_more_rows_than_there_are(used):
+    """A captured step has room for many rows, of which most are none: so many
+    that groups of 64 columns are formed around a few sequences that decode."""
+    import torch
+
+    shape, room = (32, 8, 128, 128), 1500
+    heads, n_kv, d, _ = shape
+    cache, k, v = device_pool(shape, 40, 320, 64)
+    rows = [(i % 40, 319 - i % 90) for i in range(min(used, 40))] + [(7, p) for p in range(used - 40)][:320]
+    rows += [(3, p) for p in range(used - len(rows))][:320]
+    assert max(p for _, p in rows) < 320
+    seq, pos = zip(*(rows + [(-1, -1)] * (room - len(rows))))
+    q = torch.randn((room, heads * d), generator=torch.Generator(device="cuda").manual_seed(7), device="cuda")
+    out = torch.full((room, heads * d), 7.0, device="cuda")
+    args = q, ints(seq), ints(pos), out
+    call = lambda: cache.attend(*args, max_pos=cache.table.shape[1] * 64 - 1, scale=d ** -0.5)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for _ in range(3):
+        out.fill_(7.0)
+        q.normal_(generator=torch.Generator(device="cuda").manual_seed(9))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.cpu().numpy()
+        assert (got[len(rows):] == 7.0).all()
+        pick = list(range(0, len(rows), max(1, len(rows) // 60)))
+        close(got[pick], attend64(k, v, q[pick], [seq[i] for i in pick], [pos[i] for i in pick], heads, d ** -0.5))
 
 
 @pytest.mark.parametrize("window", [0, 90])

@@ -513,6 +513,125 @@ int moe_kv4_select(const moe_kv4 *c, const float *q, int64_t q_stride, int32_t r
                    const int32_t *pos, int32_t max_pos, int32_t sinks, int32_t recent, int32_t n_sel, int32_t *lists,
                    void *workspace, uint64_t workspace_bytes, void *stream);
 
+/* ------------------------------------------ the paged 8-bit key/value cache
+ * The same pages (moe_pages_advance) with keys and values in 8 bits: 16
+ * positions of a kv head, a block, share one f32 scale for their keys and one
+ * for their values, s = max|v| / 127, and are held as codes round(v * (127 /
+ * max|v|)), halves to even, each step rounded to f32.  A block whose largest
+ * value is below 2^-100 is held as zeros; one with an infinity or a NaN reads
+ * as NaN.  A tile is 64 positions of one kv head:
+ *   codes   int8 [page][kv head][page / 64 tiles][64 (qd + vd)], a tile's
+ *           keys [block][qd / 16][position][16 dims], then its values
+ *           [vd / 16][g 4][16 dims][block][i 4] of position 16 block + 4 g + i
+ *   scales  f32 [page][kv head][page / 64 tiles][keys, values][block]
+ *   open    per sequence and kv head, the f32 values of blocks that are not
+ *           full yet (two of them, 128 (qd + vd) bytes) and which ones they are
+ *           (32 bytes); zeros: none.  A block's codes are therefore those of its
+ *           positions' values, however the steps that wrote them were cut.
+ * No counterpart in the reference, which keeps f32 (src/model.rs:93-114). */
+typedef struct moe_kv8 {
+    void *codes;           /* device, 16-byte aligned, as scales and open */
+    float *scales;
+    void *open;
+    const int32_t *table;  /* device [n_seq][max_pages]: the page holding a sequence's positions page * i ... */
+    uint64_t codes_bytes, scales_bytes, open_bytes;
+    int32_t n_seq, max_pages, n_pages;
+    int32_t page;          /* positions of a page: 64, 128 ... 4096 */
+    int32_t n_kv, qd, vd;  /* kv heads (up to 65535), key and value widths: multiples of 32 up to 256 */
+    int32_t _reserved;
+} moe_kv8;
+
+/* Bytes of codes, scales and open blocks of c->n_pages pages and c->n_seq
+ * sequences (of c's page, n_kv, qd and vd). */
+int moe_kv8_sizes(const moe_kv8 *c, uint64_t *codes, uint64_t *scales, uint64_t *open);
+
+/* Write a step's rows into their slots (src/model.rs:732-733, 773-787): k
+ * [rows, n_kv * qd] and v [rows, n_kv * vd] f32, k_stride and v_stride floats
+ * apart.  row_start, seq, pos and slots are moe_pages_advance's: sequence i's
+ * rows are row_start[i] to row_start[i + 1] - 1, its next positions in order.
+ * Rows whose slot is negative or past the pool, whose seq is outside 0 ...
+ * n_seq - 1 or whose position is negative are skipped.  Where a sequence goes
+ * on behind a block that `open` does not hold (its caller took it back to an
+ * earlier position), that block's earlier positions are taken as they read.
+ * The same step made again writes the same.  At most 2^24 - 256 rows (also
+ * moe_kv8_load's). */
+int moe_kv8_store(const moe_kv8 *c, const float *k, int64_t k_stride, const float *v, int64_t v_stride, int32_t rows,
+                  const int32_t *row_start, const int32_t *seq, const int32_t *pos, const int64_t *slots, void *stream);
+
+/* The rows of slots as f32 (k or v may be NULL); rows whose slot is negative
+ * or past the pool are left as they were. */
+int moe_kv8_load(const moe_kv8 *c, const int64_t *slots, int32_t rows, float *k, int64_t k_stride, float *v,
+                 int64_t v_stride, void *stream);
+
+/* Causal attention over the cache (src/model.rs:790-831): as moe_attention,
+ * row r of q (heads x qd values) belonging to sequence seq[r] at position
+ * pos[r], with the sequence's positions found through its table row.  heads is
+ * a multiple of c->n_kv.  max_pos bounds every pos[r].  A row with pos[r] < 0
+ * or seq[r] outside 0 ... n_seq - 1 is left as it was; pages outside the pool
+ * hold no positions; a row that sees no position is 0.  A row that sees a
+ * position of a block whose keys or values read as NaN, or whose query is not
+ * finite, is NaN; what positions hold that no row sees does not matter.
+ * `workspace`: device, 16-byte aligned, moe_kv8_attention_workspace_size bytes
+ * (its arguments as the call's; it may be 0 bytes).  Calls that share one must
+ * be ordered. */
+int moe_kv8_attention_workspace_size(const moe_kv8 *c, int32_t rows, int32_t heads, int32_t max_pos, int32_t window,
+                                     uint64_t *bytes);
+int moe_kv8_attention(const moe_kv8 *c, const float *q, int64_t q_stride, int32_t rows, int32_t heads, float scale,
+                      const int32_t *seq, const int32_t *pos, int32_t max_pos, int32_t window, float *out,
+                      int64_t out_stride, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* -------------------------------------- products in 8-bit integers
+ * y = x W^T with a scale for each token and each channel: rows of x and of W are
+ * held as the 8-bit cache's blocks are (scale max / 127, codes by the rule
+ * above), the sum of the codes' products is exact in 32 bits and
+ *   y[t][n] = sum * (scale_x[t] * scale_w[n]).
+ * Beside moe_linear (src/quant.rs:482-506), which keeps f32 precision: this
+ * halves a Q8_0 matrix's work on the matrix cores at the precision of 8-bit
+ * activations.  Weights are packed once into memory of the caller's. */
+
+/* Bytes of n channels of k values (at most 131072), packed. */
+int moe_int8_pack_size(int32_t n, int32_t k, uint64_t *bytes);
+/* Quantise `rows` rows of k values in format dt (F32, F16, BF16, Q8_0, Q4_0,
+ * Q5_0), row_bytes apart in device memory, into channels row0 ... of a packed
+ * matrix of n channels (256-byte aligned).  Several matrices over the same
+ * input, packed one behind the other, are one product.  Channels that no call
+ * has packed hold what the memory holds. */
+int moe_int8_pack(const void *w, int32_t dt, int64_t row_bytes, int32_t rows, int32_t row0, int32_t n, int32_t k,
+                  void *packed, uint64_t packed_bytes, void *stream);
+/* y [t, n] (y_stride floats apart) = x [t, k] (x_stride) W^T; residual (or
+ * NULL, residual_stride) += y.  y and residual must not lie in x's memory.  At
+ * most 2^20 tokens.  `workspace`: device, 256-byte aligned,
+ * moe_int8_linear_workspace_size bytes; calls that share one must be ordered. */
+int moe_int8_linear_workspace_size(int32_t n, int32_t k, int32_t t, uint64_t *bytes);
+int moe_int8_linear(const void *packed, int32_t n, int32_t k, const float *x, int64_t x_stride, int32_t t, float *y,
+                    int64_t y_stride, float *residual, int64_t residual_stride, void *workspace, uint64_t workspace_bytes,
+                    void *stream);
+
+/* ------------------------- biases, head norms and rotation in one pass
+ * What the reference's attention does to its projections before the cache
+ * write (src/model.rs:707-730), bit for bit what moe_add_bias, moe_rmsnorm over
+ * each head (or the whole projection) and moe_rope give in turn. */
+typedef struct moe_head_rope {
+    const float *q_bias, *k_bias, *v_bias;  /* device [heads * width], [n_kv * width], [v_width], or NULL */
+    const float *q_norm, *k_norm;           /* device [span * width], or NULL: no norm */
+    const float *inv_freq;                  /* device f32 [n_inv] */
+    int32_t heads, n_kv, width;             /* query heads, key heads (up to 30000), values of a head */
+    int32_t q_span, k_span;                 /* heads that one norm spans: 1, or all of them */
+    int32_t offset, dim;                    /* values offset ... offset + dim - 1 of a head rotate pairwise (i, i + dim / 2) */
+    int32_t n_inv;                          /* pairs past n_inv stay */
+    int32_t v_width;
+    float eps;
+} moe_head_rope;
+/* Rows q [rows, heads * width], k [rows, n_kv * width] and v [rows, v_width] (or
+ * NULL: no values), their strides in floats, to q_out, k_out and v_out, which
+ * may be their inputs (same address and stride) and otherwise do not overlap
+ * them.  pos: device int32 [rows]; the angle is (float)pos * inv_freq[i] in f32.
+ * At most 2^24 - 1 rows. */
+int moe_head_rope_rows(const moe_head_rope *h, const float *q, int64_t q_stride, const float *k, int64_t k_stride,
+                       const float *v, int64_t v_stride, int32_t rows, const int32_t *pos, float *q_out,
+                       int64_t q_out_stride, float *k_out, int64_t k_out_stride, float *v_out, int64_t v_out_stride,
+                       void *stream);
+
 /* --------------------------------------------------- checkpoint containers */
 
 /* One tensor of a single-file checkpoint: Store's Rec (src/store.rs:25-47).

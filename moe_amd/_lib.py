@@ -63,6 +63,20 @@ class Kv4C(C.Structure):
                 ("n_kv", C.c_int32), ("qd", C.c_int32), ("vd", C.c_int32), ("_reserved", C.c_int32)]
 
 
+class Kv8C(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("open", C.c_void_p), ("table", C.c_void_p),
+                ("codes_bytes", C.c_uint64), ("scales_bytes", C.c_uint64), ("open_bytes", C.c_uint64),
+                ("n_seq", C.c_int32), ("max_pages", C.c_int32), ("n_pages", C.c_int32), ("page", C.c_int32),
+                ("n_kv", C.c_int32), ("qd", C.c_int32), ("vd", C.c_int32), ("_reserved", C.c_int32)]
+
+
+class HeadRopeC(C.Structure):
+    _fields_ = [("q_bias", C.c_void_p), ("k_bias", C.c_void_p), ("v_bias", C.c_void_p), ("q_norm", C.c_void_p),
+                ("k_norm", C.c_void_p), ("inv_freq", C.c_void_p), ("heads", C.c_int32), ("n_kv", C.c_int32),
+                ("width", C.c_int32), ("q_span", C.c_int32), ("k_span", C.c_int32), ("offset", C.c_int32),
+                ("dim", C.c_int32), ("n_inv", C.c_int32), ("v_width", C.c_int32), ("eps", C.c_float)]
+
+
 DT_Q6_REF = -2
 
 
@@ -154,6 +168,25 @@ PROTOTYPES = {
     "moe_kv4_select": (C.c_int, [C.POINTER(Kv4C), C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p,
                                  C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_uint64,
                                  C.c_void_p]),
+    "moe_kv8_sizes": (C.c_int, [C.POINTER(Kv8C), C.POINTER(C.c_uint64), C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]),
+    "moe_kv8_store": (C.c_int, [C.POINTER(Kv8C), C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p,
+                                C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "moe_kv8_load": (C.c_int, [C.POINTER(Kv8C), C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                               C.c_void_p]),
+    "moe_kv8_attention_workspace_size": (C.c_int, [C.POINTER(Kv8C), C.c_int32, C.c_int32, C.c_int32, C.c_int32,
+                                                   C.POINTER(C.c_uint64)]),
+    "moe_kv8_attention": (C.c_int, [C.POINTER(Kv8C), C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_float,
+                                    C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p,
+                                    C.c_uint64, C.c_void_p]),
+    "moe_int8_pack_size": (C.c_int, [C.c_int32, C.c_int32, C.POINTER(C.c_uint64)]),
+    "moe_int8_pack": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
+                                C.c_void_p, C.c_uint64, C.c_void_p]),
+    "moe_int8_linear_workspace_size": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_uint64)]),
+    "moe_int8_linear": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p,
+                                  C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "moe_head_rope_rows": (C.c_int, [C.POINTER(HeadRopeC), C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
+                                     C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                     C.c_void_p, C.c_int64, C.c_void_p]),
 }
 
 STAGES = ("router", "gating", "dispatch", "expert_up", "expert_down", "combine", "encode")

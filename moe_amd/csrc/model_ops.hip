@@ -25,49 +25,13 @@
 
 #include "gmem.h"
 #include "moe_internal.h"
+#include "row_value.h"
+#include "rotate.h"
 
 namespace moe {
 int fail(int code, const char *fmt, ...);
 
 namespace {
-
-__device__ inline float half_at(const uint8_t *p) {
-    return __half2float(__ushort_as_half((unsigned short)(p[0] | (p[1] << 8))));
-}
-
-// Value c of a stored row (src/quant.rs:177-227).
-__device__ inline float row_value(const uint8_t *row, int dt, int c) {
-    const int b = c >> 5, i = c & 31;
-    switch (dt) {
-    case MOE_DT_F32: {
-        float v;
-        __builtin_memcpy(&v, row + 4 * (size_t)c, 4);
-        return v;
-    }
-    case MOE_DT_F16: return half_at(row + 2 * (size_t)c);
-    case MOE_DT_BF16: {
-        const uint32_t u = (uint32_t)(row[2 * (size_t)c] | (row[2 * (size_t)c + 1] << 8)) << 16;
-        return __uint_as_float(u);
-    }
-    case MOE_DT_Q8_0: {
-        const uint8_t *blk = row + 34 * (size_t)b;
-        return half_at(blk) * (float)(int8_t)blk[2 + i];
-    }
-    case MOE_DT_Q4_0: {
-        const uint8_t *blk = row + 18 * (size_t)b;
-        const uint32_t v = blk[2 + (i & 15)];
-        const int nib = i < 16 ? (int)(v & 15) : (int)(v >> 4);
-        return half_at(blk) * (float)(nib - 8);
-    }
-    default: {  // Q5_0
-        const uint8_t *blk = row + 22 * (size_t)b;
-        const uint32_t v = blk[6 + (i & 15)];
-        const int nib = i < 16 ? (int)(v & 15) : (int)(v >> 4);
-        const int hb = (blk[2 + i / 8] >> (i % 8)) & 1;
-        return half_at(blk) * (float)((nib | (hb << 4)) - 16);
-    }
-    }
-}
 
 __global__ __launch_bounds__(256) void embed_rows_kernel(const uint8_t *__restrict__ table, int dt, uint32_t rows,
                                                          int cols, size_t row_bytes,
@@ -113,9 +77,7 @@ __global__ __launch_bounds__(256) void rope_kernel(float *__restrict__ x, int64_
         float *hx = row + (size_t)h * hs;
         const float ang = p * inv[i];
         const float s = sinf(ang), c = cosf(ang);
-        const float a = hx[i], b = hx[i + half];
-        hx[i] = a * c - b * s;
-        hx[i + half] = a * s + b * c;
+        rotate(hx[i], hx[i + half], c, s, hx[i], hx[i + half]);
     }
 }
 

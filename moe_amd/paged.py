@@ -356,3 +356,102 @@ class KvCache(_OnDevice):
         if rc:
             _refused(rc, "moe_kv4_select")
         return lists
+
+
+class KvCache8(_OnDevice):
+    """One layer's keys and values in 8 bits, a scale for every block of 16
+    positions of a kv head: `codes` and `open` uint8, `scales` float32 (sizes()
+    says how many of each), pages found through `table` (a PageTable's)."""
+
+    def __init__(self, codes, scales, open_blocks, table, *, n_kv: int, qd: int, vd: int, page: int):
+        for t, dtype, name in ((codes, torch.uint8, "codes"), (scales, torch.float32, "scales"),
+                               (open_blocks, torch.uint8, "open_blocks")):
+            _need(t.dtype == dtype and t.dim() == 1 and t.is_contiguous(),
+                  f"{name} must be a contiguous one-dimensional {str(dtype)[6:]} tensor")
+        _need(table.dtype == torch.int32 and table.dim() == 2 and table.is_contiguous(),
+              "table must be a contiguous int32 [sequences, pages] tensor")
+        n_seq = table.shape[0]
+        each, _, _ = self.sizes(1, max(1, n_seq), n_kv=n_kv, qd=qd, vd=vd, page=page)
+        n_pages = codes.shape[0] // each
+        _need(n_pages >= 1, f"codes of {codes.shape[0]} bytes hold no page")
+        _fits(sequences=n_seq, pages=table.shape[1], pool=n_pages)
+        need = self.sizes(n_pages, max(1, n_seq), n_kv=n_kv, qd=qd, vd=vd, page=page)
+        _need(scales.shape[0] * 4 >= need[1] and open_blocks.shape[0] >= need[2],
+              f"{scales.shape[0]} scales and {open_blocks.shape[0]} bytes of open blocks: {need[1] // 4} and {need[2]} needed")
+        self.codes, self.scales, self.open_blocks, self.table = codes, scales, open_blocks, table
+        self.n_kv, self.qd, self.vd, self.page, self.n_pages = n_kv, qd, vd, page, n_pages
+        self.device, self._index = codes.device, codes.get_device()
+        _need(all(t.device == codes.device for t in (scales, open_blocks, table)), "a cache on several devices")
+        self.c = L.Kv8C(codes=codes.data_ptr(), scales=scales.data_ptr(), open=open_blocks.data_ptr(), table=table.data_ptr(),
+                        codes_bytes=codes.shape[0], scales_bytes=4 * scales.shape[0], open_bytes=open_blocks.shape[0],
+                        n_seq=n_seq, max_pages=table.shape[1], n_pages=n_pages, page=page, n_kv=n_kv, qd=qd, vd=vd)
+        self._c = C.byref(self.c)
+        self._positions = table.shape[1] * page
+        self._sizes = {}
+
+    @staticmethod
+    def sizes(n_pages: int, n_seq: int, *, n_kv: int, qd: int, vd: int, page: int):
+        """Bytes of codes, of scales and of open blocks; ValueError for sizes
+        the cache does not hold."""
+        _fits(pool=n_pages, sequences=n_seq, page=page, n_kv=n_kv, qd=qd, vd=vd)
+        one = L.Kv8C(n_seq=n_seq, n_pages=n_pages, page=page, n_kv=n_kv, qd=qd, vd=vd)
+        b = [C.c_uint64() for _ in range(3)]
+        _refused(L.lib().moe_kv8_sizes(C.byref(one), *map(C.byref, b)), "moe_kv8_sizes")
+        return tuple(x.value for x in b)
+
+    @staticmethod
+    def new(n_pages: int, table, *, n_kv: int, qd: int, vd: int, page: int) -> "KvCache8":
+        codes, scales, open_blocks = KvCache8.sizes(n_pages, table.shape[0], n_kv=n_kv, qd=qd, vd=vd, page=page)
+        z = lambda n, t=torch.uint8: torch.zeros(n, dtype=t, device=table.device)  # noqa: E731
+        return KvCache8(z(codes), z(scales // 4, torch.float32), z(open_blocks), table, n_kv=n_kv, qd=qd, vd=vd, page=page)
+
+    _size = KvCache._size
+    _query = KvCache._query
+
+    @_on_its_device
+    def store(self, k, v, rows: Rows, stream=None) -> None:
+        """Write a step's rows k [rows, kv heads * key width], v [rows, kv
+        heads * value width] (float32): `rows` as PageTable.advance fills it
+        (moe_kv8_store).  Rows of negative slots are skipped; the same step made
+        again writes the same."""
+        n, start, seq, pos, slot, _ = rows._args
+        ks, vs = _rows(k, n, self.n_kv * self.qd, "k"), _rows(v, n, self.n_kv * self.vd, "v")
+        _need(rows.n_seq == self.table.shape[0], f"rows of {rows.n_seq} sequences, the table has {self.table.shape[0]}")
+        self._check_device(k, v, rows.seq)
+        rc = L.lib().moe_kv8_store(self._c, k.data_ptr(), ks, v.data_ptr(), vs, n, start, seq, pos, slot, self._on(stream))
+        if rc:
+            _refused(rc, "moe_kv8_store")
+
+    @_on_its_device
+    def load(self, slots, k=None, v=None, stream=None) -> None:
+        """Read the rows of `slots` (int64) into k and v (float32, either may
+        be None); rows of negative slots are left as they were."""
+        n = slots.shape[0]
+        _fits(rows=n)
+        _ids(slots, torch.int64, n, "slots")
+        ks = 0 if k is None else _rows(k, n, self.n_kv * self.qd, "k")
+        vs = 0 if v is None else _rows(v, n, self.n_kv * self.vd, "v")
+        self._check_device(slots, *(t for t in (k, v) if t is not None))
+        rc = L.lib().moe_kv8_load(self._c, slots.data_ptr(), n, None if k is None else k.data_ptr(), ks,
+                                  None if v is None else v.data_ptr(), vs, self._on(stream))
+        if rc:
+            _refused(rc, "moe_kv8_load")
+
+    @_on_its_device
+    def attend(self, q, seq, pos, out, *, max_pos: int, scale: float, window: int = 0, stream=None) -> None:
+        """Causal attention of rows q [rows, heads * key width] into out
+        [rows, heads * value width] (moe_kv8_attention): row r of sequence
+        seq[r] at position pos[r] (-1: left as it was), no position above
+        max_pos, over the last `window` positions when that is above 0."""
+        n, heads, qs = self._query(q, seq, pos, max_pos)
+        if not -2 ** 31 <= window < 2 ** 31:
+            _fits(window=window)
+        os = _rows(out, n, heads * self.vd, "out")
+        self._check_device(q, seq, pos, out)
+        need = self._size("moe_kv8_attention_workspace_size", n, heads, max_pos, window)
+        sp = self._on(stream)
+        ws = self._scratch(need, sp) if need else None
+        rc = L.lib().moe_kv8_attention(self._c, q.data_ptr(), qs, n, heads, scale, seq.data_ptr(), pos.data_ptr(), max_pos,
+                                       window, out.data_ptr(), os, ws.data_ptr() if need else None, need, sp)
+        if rc:
+            _refused(rc, "moe_kv8_attention")

@@ -32,8 +32,10 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import _lib as L
+from .heads import HeadRope
+from .int8 import Int8Linear
 from .layer import Context, Mlp, MoeLayer, MoeSpec, Rec, Region, Store, View, _stream_ptr, row_bytes
-from .paged import KvCache, PageTable, Rows
+from .paged import KvCache, KvCache8, PageTable, Rows
 
 try:
     import torch
@@ -362,6 +364,13 @@ class Linear:
             self.handle = None
 
 
+def _project(linear, x, y, ws, residual=None, stream=None):
+    """A Linear on the model's workspace, or an Int8Linear."""
+    if isinstance(linear, Int8Linear):
+        return linear(x, y, residual=residual, stream=stream)
+    return linear(x, y, ws, residual=residual, stream=stream)
+
+
 class Batch:
     """Which sequence and position each row of a forward call belongs to, and
     the rows' token ids: one block of host memory, one copy to the device.
@@ -469,6 +478,7 @@ class PagedBatch:
         self.table = st.next
         rows = st.table.advance(dev[:n], Rows.new(n, t, device), out=self.table, stream=sp)
         _keep_for(sp, queued, dev, rows.seq, rows.pos, rows.slot, rows.row_start, rows.status)
+        self.rows = rows
         self.seq, self.pos, self.dst = rows.seq, rows.pos, rows.slot
         self.max_pos = max(st.pos[q] + c for q, c in zip(seqs, counts)) - 1
         self.sparse = st.sparse is not None and max(counts) == 1
@@ -476,12 +486,13 @@ class PagedBatch:
 
 
 class PagedState:
-    """State with the cache in 4 bits, in pages (moe_amd.paged): n_seq
+    """State with the cache in 4 or 8 bits, in pages (moe_amd.paged): n_seq
     sequences of up to ctx positions share `pages` pages, which they take as
     they grow and end() gives back.  With `sparse`, decode steps (one token a
     sequence) read only the pages they choose; prompts read everything."""
 
-    def __init__(self, model: "Model", n_seq: int, ctx: int, page: int, pages: Optional[int], sparse: Optional[Sparse]):
+    def __init__(self, model: "Model", n_seq: int, ctx: int, page: int, pages: Optional[int], sparse: Optional[Sparse],
+                 cache: str = "q4"):
         s = model.spec
         n_kv, qd, vd = model.kv_heads()
         each = -(-ctx // page)
@@ -489,7 +500,13 @@ class PagedState:
         if sparse is not None and not (sparse.sinks >= 0 and sparse.recent >= 1
                                        and sparse.sinks + sparse.recent <= sparse.pages):
             raise ValueError(f"{sparse.sinks} first and {sparse.recent} last pages of {sparse.pages}")
-        KvCache.page_bytes(n_kv, qd, vd, page)  # refuses widths and pages the cache does not hold
+        # (both refuse widths and pages that the cache does not hold)
+        if cache == "int8":
+            if sparse is not None:
+                raise ValueError("the 8-bit cache keeps no mean keys: no sparse steps")
+            KvCache8.sizes(1, max(1, n_seq), n_kv=n_kv, qd=qd, vd=vd, page=page)
+        else:
+            KvCache.page_bytes(n_kv, qd, vd, page)
         if n_seq < 1 or ctx < 1 or pages < 1 or each * page >= 2 ** 31:
             raise ValueError(f"{n_seq} sequences of {ctx} positions over {pages} pages")
         self.ctx, self.n_seq, self.page, self.pages, self.sparse = ctx, n_seq, page, pages, sparse
@@ -498,8 +515,11 @@ class PagedState:
         # other (next), so that no step frees what a stream has yet to read.
         self.table = t = PageTable.new(n_seq, each, pages, page, model.device)
         self.next = PageTable(t.table, torch.empty_like(t.length), t.ring, torch.empty_like(t.state), page)
-        self.kv = [KvCache.new(pages, self.table.table, n_kv=n_kv, qd=qd, vd=vd, page=page, means=sparse is not None)
-                   for _ in range(s.layers)]
+        kw = dict(n_kv=n_kv, qd=qd, vd=vd, page=page)
+        if cache == "int8":
+            self.kv = [KvCache8.new(pages, self.table.table, **kw) for _ in range(s.layers)]
+        else:
+            self.kv = [KvCache.new(pages, self.table.table, means=sparse is not None, **kw) for _ in range(s.layers)]
 
     def free_pages(self) -> int:
         return self.pages - sum(-(-p // self.page) for p in self.pos)
@@ -539,9 +559,15 @@ class PagedState:
 
 class Model:
     """Model (src/model.rs:192-209, 336-834) over weights in one device
-    region, bound by the reference's tensor names."""
+    region, bound by the reference's tensor names.  projections="int8": the
+    attention's projections as products in 8-bit integers (Int8Linear; q, k and
+    v are one), in place of Linear's f32 precision."""
 
-    def __init__(self, ctx: Context, spec: Spec, store: Store, device="cuda:0"):
+    def __init__(self, ctx: Context, spec: Spec, store: Store, device="cuda:0", projections: str = "f32"):
+        if projections not in ("f32", "int8"):
+            raise ValueError(f"projections {projections!r}: f32 or int8")
+        linear = functools.partial(Int8Linear.of_views, device=device) if projections == "int8" else None
+        one = (lambda v: linear(ctx, [v])) if linear else (lambda v: Linear(ctx, v))
         self.ctx, self.spec, self.store, self.device = ctx, spec, store, torch.device(device)
         s = spec
         p = s.prefix
@@ -556,21 +582,25 @@ class Model:
             a = f"{p}{l}.self_attn."
             lay = dict(ln1=self._vec(f"{p}{l}.input_layernorm.weight"),
                        ln2=self._vec(f"{p}{l}.post_attention_layernorm.weight"),
-                       o=Linear(ctx, g(a + "o_proj.weight")), window=s.windows[l] if l < len(s.windows) else None)
+                       o=one(g(a + "o_proj.weight")), window=s.windows[l] if l < len(s.windows) else None)
             if s.mla is None:
-                lay.update(q=Linear(ctx, g(a + "q_proj.weight")), k=Linear(ctx, g(a + "k_proj.weight")),
-                           v=Linear(ctx, g(a + "v_proj.weight")),
-                           bias=[self._vec(a + f"{m}_proj.bias", optional=True) for m in "qkv"],
+                qkv = [g(a + f"{m}_proj.weight") for m in "qkv"]
+                if linear:
+                    lay["qkv"] = linear(ctx, qkv)
+                else:
+                    lay.update(zip("qkv", map(one, qkv)))
+                lay.update(bias=[self._vec(a + f"{m}_proj.bias", optional=True) for m in "qkv"],
                            q_norm=self._vec(a + "q_norm.weight", optional=True),
                            k_norm=self._vec(a + "k_norm.weight", optional=True))
+                self._heads(lay)
             else:
                 qa = g(a + "q_a_proj.weight")
-                lay.update(q_a=Linear(ctx, qa) if qa is not None else None,
+                lay.update(q_a=one(qa) if qa is not None else None,
                            q_a_norm=self._vec(a + "q_a_layernorm.weight", optional=True),
-                           q_b=Linear(ctx, g(a + "q_b_proj.weight") if qa is not None else g(a + "q_proj.weight")),
-                           kv_a=Linear(ctx, g(a + "kv_a_proj_with_mqa.weight")),
+                           q_b=one(g(a + "q_b_proj.weight") if qa is not None else g(a + "q_proj.weight")),
+                           kv_a=one(g(a + "kv_a_proj_with_mqa.weight")),
                            kv_a_norm=self._vec(a + "kv_a_layernorm.weight"),
-                           kv_b=Linear(ctx, g(a + "kv_b_proj.weight")))
+                           kv_b=one(g(a + "kv_b_proj.weight")))
             m = f"{p}{l}.mlp."
             if g(m + "gate.weight") is not None or g(f"{p}{l}.block_sparse_moe.gate.weight") is not None:
                 from .checkpoint import bind_layer
@@ -614,13 +644,13 @@ class Model:
 
     def new_state(self, n_seq: int, ctx: int, cache: str = "f32", page: int = 64, pages: Optional[int] = None,
                   sparse: Optional[Sparse] = None):
-        """State for n_seq sequences of up to ctx positions; with cache="q4"
-        a PagedState (head widths that are multiples of 32, up to 256), whose
-        contexts may be of any length."""
-        if cache == "q4":
-            return PagedState(self, n_seq, ctx, page, pages, sparse)
+        """State for n_seq sequences of up to ctx positions; with cache="q4" or
+        "int8" (4 or 8 bits a value) a PagedState (head widths that are multiples
+        of 32, up to 256), whose contexts may be of any length."""
+        if cache in ("q4", "int8"):
+            return PagedState(self, n_seq, ctx, page, pages, sparse, cache)
         if cache != "f32" or pages is not None or sparse is not None:
-            raise ValueError(f"cache {cache!r}: f32, or q4 for pages and sparse steps")
+            raise ValueError(f"cache {cache!r}: f32, or q4 and int8 for pages, q4 for sparse steps")
         # moe_attention keeps one row's scores in LDS: at most
         # ATTN_MAX_POSITIONS positions per row (the window, where a layer
         # has one).  A longer context is refused here, before any step.
@@ -742,6 +772,17 @@ class Model:
         if rc:
             L.check(rc, "moe_rope")
 
+    def _heads(self, lay) -> HeadRope:
+        """A layer's biases, norms (one weight across the projection, OLMoE, or
+        one per head, Qwen3) and rotation."""
+        h = lay.get("heads")
+        if h is None:
+            s, bias = self.spec, lay["bias"]
+            h = lay["heads"] = HeadRope(s.heads, s.kv_heads, s.head_dim, self.inv_freq, dim=s.head_dim // 2 * 2, eps=s.eps,
+                                        q_norm=lay["q_norm"], k_norm=lay["k_norm"], q_bias=bias[0], k_bias=bias[1],
+                                        v_bias=bias[2])
+        return h
+
     def _attention(self, li, lay, x, b: Batch, st: State, resid, ws, stream, buf):
         """Model::attention (src/model.rs:686-834); resid += o(ctx).  stream:
         the handle; buf: the forward's scratch by name."""
@@ -757,47 +798,44 @@ class Model:
         if s.mla is None:
             qd = vd = s.head_dim
             n_kv = s.kv_heads
-            q = lay["q"](x, take("q", s.heads * qd), ws, stream=sp)
-            k = lay["k"](x, take("k", n_kv * qd), ws, stream=sp)
-            v = lay["v"](x, take("v", n_kv * vd), ws, stream=sp)
-            for proj, bias in zip((q, k, v), lay["bias"]):
-                if bias is not None:
-                    L.check(lib.moe_add_bias(proj.data_ptr(), proj.numel(), bias.data_ptr(), bias.numel(), sp),
-                            "moe_add_bias")
-            for proj, heads, nrm in ((q, s.heads, lay["q_norm"]), (k, n_kv, lay["k_norm"])):
-                if nrm is not None:
-                    # One weight across the projection (OLMoE) or one per head (Qwen3).
-                    span = proj.shape[1] if nrm.numel() == proj.shape[1] else qd
-                    tmp = torch.empty_like(proj)
-                    self._rmsnorm(proj, nrm, tmp, sp, rows=proj.numel() // span, n=span, xs=span, os_=span)
-                    proj.copy_(tmp)
-                self._rope(proj, t, proj.shape[1], heads, qd, 0, qd, b, sp)
+            nq, nk = s.heads * qd, n_kv * qd
+            if "qkv" in lay:
+                qkv = lay["qkv"](x, take("qkv", nq + 2 * nk), stream=sp)
+                q, k, v = qkv[:, :nq], qkv[:, nq:nq + nk], qkv[:, nq + nk:]
+            else:
+                q, k, v = (lay[m](x, take(m, n), ws, stream=sp) for m, n in (("q", nq), ("k", nk), ("v", nk)))
+            h = self._heads(lay)
+            va = (v.data_ptr(), v.stride(0)) if h.v_bias is not None else (None, 0)
+            qk = (q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0))
+            rc = lib.moe_head_rope_rows(h._c, *qk, *va, t, b.pos.data_ptr(), *qk, *va, sp)
+            if rc:
+                L.check(rc, "moe_head_rope_rows")
             if isinstance(st, PagedState):
                 return self._attend_paged(li, lay, q, k, v, b, st, resid, ws, sp, take, buf["work"])
             kd, vdim, dst = n_kv * qd, n_kv * vd, b.dst.data_ptr()
-            rc = lib.moe_scatter_rows(k.data_ptr(), t, kd, kd, st.k[li].data_ptr(), kd, dst, sp)
-            rc = rc or lib.moe_scatter_rows(v.data_ptr(), t, vdim, vdim, st.v[li].data_ptr(), vdim, dst, sp)
+            rc = lib.moe_scatter_rows(k.data_ptr(), t, kd, k.stride(0), st.k[li].data_ptr(), kd, dst, sp)
+            rc = rc or lib.moe_scatter_rows(v.data_ptr(), t, vdim, v.stride(0), st.v[li].data_ptr(), vdim, dst, sp)
             if rc:
                 L.check(rc, "moe_scatter_rows")
         else:
             m = s.mla
             qd, vd, n_kv = m.qk_nope + m.qk_rope, m.v_head, s.heads
             if lay["q_a"] is not None:
-                cq = lay["q_a"](x, take("cq", m.q_lora), ws, stream=sp)
+                cq = _project(lay["q_a"], x, take("cq", m.q_lora), ws, stream=sp)
                 cqn = take("cqn", m.q_lora)
                 self._rmsnorm(cq, lay["q_a_norm"], cqn, sp)
-                q = lay["q_b"](cqn, take("q", s.heads * qd), ws, stream=sp)
+                q = _project(lay["q_b"], cqn, take("q", s.heads * qd), ws, stream=sp)
             else:
-                q = lay["q_b"](x, take("q", s.heads * qd), ws, stream=sp)
+                q = _project(lay["q_b"], x, take("q", s.heads * qd), ws, stream=sp)
             ca = m.kv_lora + m.qk_rope
-            c = lay["kv_a"](x, take("c", ca), ws, stream=sp)
+            c = _project(lay["kv_a"], x, take("c", ca), ws, stream=sp)
             cn = take("cn", m.kv_lora)
             self._rmsnorm(c, lay["kv_a_norm"], cn, sp, n=m.kv_lora, xs=ca, os_=m.kv_lora)
-            kv = lay["kv_b"](cn, take("kv", s.heads * (m.qk_nope + m.v_head)), ws, stream=sp)
+            kv = _project(lay["kv_b"], cn, take("kv", s.heads * (m.qk_nope + m.v_head)), ws, stream=sp)
             self._rope(c, t, ca, 1, 0, m.kv_lora, m.qk_rope, b, sp)
             self._rope(q, t, s.heads * qd, s.heads, qd, m.qk_nope, m.qk_rope, b, sp)
             if isinstance(st, PagedState):
-                # Rows as they would lie in an f32 cache, then the 4-bit write.
+                # Rows as they would lie in an f32 cache, then the paged write.
                 k, v = take("k", s.heads * qd), take("v", s.heads * vd)
                 rows = buf.get("rows")
                 if rows is None:
@@ -812,12 +850,12 @@ class Model:
             if rc:
                 L.check(rc, "moe_mla_kv_store")
         ctxv = take("ctx", s.heads * vd)
-        rc = lib.moe_attention(q.data_ptr(), q.shape[1], t, s.heads, n_kv, qd, vd, self.attn_scale, st.k[li].data_ptr(),
+        rc = lib.moe_attention(q.data_ptr(), q.stride(0), t, s.heads, n_kv, qd, vd, self.attn_scale, st.k[li].data_ptr(),
                                st.v[li].data_ptr(), st.ctx, b.seq.data_ptr(), b.pos.data_ptr(), b.max_pos,
                                lay["window"] or 0, ctxv.data_ptr(), ctxv.shape[1], sp)
         if rc:
             L.check(rc, "moe_attention")
-        lay["o"](ctxv, take("y", s.hidden), ws, residual=resid, stream=sp)
+        _project(lay["o"], ctxv, take("y", s.hidden), ws, residual=resid, stream=sp)
 
     @staticmethod
     def _reads(lay, b: PagedBatch, st: PagedState):
@@ -833,6 +871,9 @@ class Model:
         need = 0
         for window, n_sel in {self._reads(lay, b, st) for lay in self.layers}:
             size = st.kv[0]._size  # (one of every layer's cache)
+            if isinstance(st.kv[0], KvCache8):
+                need = max(need, size("moe_kv8_attention_workspace_size", b.t, self.spec.heads, b.max_pos, window))
+                continue
             need = max(need, size("moe_kv4_attention_workspace_size", b.t, self.spec.heads, b.max_pos, window, n_sel),
                        size("moe_kv4_select_workspace_size", b.t, b.max_pos) if n_sel else 0)
         return torch.empty(need, dtype=torch.uint8, device=self.device)
@@ -841,25 +882,33 @@ class Model:
         """The cache write and attention of _attention over a PagedState."""
         cache, lib, t = st.kv[li], L.lib(), b.t
         heads, seq, pos = self.spec.heads, b.seq.data_ptr(), b.pos.data_ptr()
-        rc = lib.moe_kv4_store(cache._c, k.data_ptr(), k.shape[1], v.data_ptr(), v.shape[1], t, b.dst.data_ptr(), sp)
+        buf, n = work.data_ptr() or None, work.numel()
+        window, n_sel = self._reads(lay, b, st)
+        if isinstance(cache, KvCache8):
+            cache.store(k, v, b.rows, stream=sp)
+            out = take("ctx", heads * cache.vd)
+            rc = lib.moe_kv8_attention(cache._c, q.data_ptr(), q.stride(0), t, heads, self.attn_scale, seq, pos, b.max_pos,
+                                       window, out.data_ptr(), out.shape[1], buf, n, sp)
+            if rc:
+                L.check(rc, "moe_kv8_attention")
+            return _project(lay["o"], out, take("y", self.spec.hidden), ws, residual=resid, stream=sp)
+        rc = lib.moe_kv4_store(cache._c, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), t, b.dst.data_ptr(), sp)
         if rc:
             L.check(rc, "moe_kv4_store")
 
-        buf, n = work.data_ptr() or None, work.numel()
-        window, n_sel = self._reads(lay, b, st)
         lists = None
         if n_sel:
             lists = take("lists", cache.n_kv * n_sel).data_ptr()  # 32-bit whole numbers
-            rc = lib.moe_kv4_select(cache._c, q.data_ptr(), q.shape[1], t, heads, seq, pos, b.max_pos, st.sparse.sinks,
+            rc = lib.moe_kv4_select(cache._c, q.data_ptr(), q.stride(0), t, heads, seq, pos, b.max_pos, st.sparse.sinks,
                                     st.sparse.recent, n_sel, lists, buf, n, sp)
             if rc:
                 L.check(rc, "moe_kv4_select")
         out = take("ctx", heads * cache.vd)
-        rc = lib.moe_kv4_attention(cache._c, q.data_ptr(), q.shape[1], t, heads, self.attn_scale, seq, pos, b.max_pos,
+        rc = lib.moe_kv4_attention(cache._c, q.data_ptr(), q.stride(0), t, heads, self.attn_scale, seq, pos, b.max_pos,
                                    window, lists, n_sel, out.data_ptr(), out.shape[1], buf, n, sp)
         if rc:
             L.check(rc, "moe_kv4_attention")
-        lay["o"](out, take("y", self.spec.hidden), ws, residual=resid, stream=sp)
+        _project(lay["o"], out, take("y", self.spec.hidden), ws, residual=resid, stream=sp)
 
     @_on_its_stream
     def head(self, x, rows, stream=None):

@@ -1,12 +1,14 @@
-"""The paged 4-bit key/value cache: block tables on the device, the cache
-write and read, attention over it, and the choice of pages for sparse
-attention (include/moe_hip.h, "the paged 4-bit key/value cache").
+"""The paged 4-bit and 8-bit key/value caches: block tables on the device, the
+cache write and read, attention over it, and the choice of pages for sparse
+attention (include/moe_hip.h, "the paged 4-bit key/value cache", "the paged
+8-bit key/value cache").
 
 The reference keeps one f32 cache per sequence, reserved to the context's end
 (State, src/model.rs:93-114, 732-733).  Here sequences take pages of positions
 from a pool as they grow (PageTable), a layer's keys and values are held as
-the reference's Q4 blocks (KvCache: 4.5 bits a value instead of 32), and a
-row may attend to every position or to the pages it scores highest.
+the reference's Q4 blocks (KvCache: 4.5 bits a value instead of 32, whose rows
+may attend to every position or to the pages they score highest) or as blocks
+of 16 positions in 8 bits (KvCache8).
 
 Every method queues its kernels on `stream` (torch's current stream of the
 cache's device when None) and returns; nothing waits for the device, so a

@@ -1,78 +1,553 @@
 // kv8_attention.hip — causal attention over the paged 8-bit cache
 // (moe_kv8_attention), layout in kv8.h.
+//
+// Rows find their sequence and position on the device, so one kernel serves
+// decode steps, prompts and chunks.  A block takes a group of consecutive rows
+// and one kv head, splits the group into runs of one sequence and makes each
+// run's (row, query head) pairs the columns of its products on the 8-bit integer
+// matrix cores, 16 a wave.
+//
+// Codes are the products' operands as they lie in memory; queries and weights
+// meet them as whole numbers of 24 bits in three signed bytes,
+//   q scale = Q 2^(e - 22),  Q = 65536 d2 + 256 d1 + d0,  |Q| <= 2^22
+// (2^e above the head's largest), so a block's scores are
+//   s = s_k 2^(e - 22) (65536 K d2 + (256 K d1 + K d0)),
+// sums of whole numbers, exact, in one f32 rounding.  The result's layout (lane
+// = column, positions 4 g + i of each block) is the second operand of the values'
+// product.  There the weights p = 2^(s - m) meet the values' scales first:
+//   W = p s_v C 2^(m - r),  r the largest s + log2 s_v of the step,  C = 2^23 - ..
+// so W below 2^23 keeps each block's product of weight and scale to 2^-23 of the
+// step's largest, however far apart the scales are.  Multiplied and added to
+// 2^23 + 0x8080 in one instruction, a weight's bits are its three digits (the
+// two low ones with 128 added).  A step's sums are whole numbers too; they join
+// the f32 sums O, which have a reference of their own (R, as r; the weights' sum
+// has m).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "gmem.h"
 #include "kv8.h"
+#include "lds_dma.h"
 
 namespace moe {
 int fail(int code, const char *fmt, ...);
 
 namespace {
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_dw __attribute__((ext_vector_type(4), aligned(4)));  // at any float
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 struct Args {
     Kv8 c;
     const float *q;
     const int32_t *seq, *pos;
-    float *out;
+    float *out, *part, *part_ml;  // part [row][head][ps][vd], part_ml [row][head][ps][m, l, R]
     int64_t q_stride, out_stride;
     int rows, heads, rep, window;
     float scale;
+    int tt, groups;  // rows of a group, groups
+    int rc, chunks;  // query heads of a block, blocks that share a kv head's
+    int split;       // blocks that share a group's runs
+    int ps;          // blocks that share a run's tiles
 };
 
-// A block takes one row's head, a tile at a time: four threads a position for
-// the scores, a thread a dim for the values.
-__global__ __launch_bounds__(256) void kv8_attention_kernel(const Args a) {
-    __shared__ float sq[256], sp[64], part[4][64];
-    const Kv8 &c = a.c;
-    const int row = blockIdx.x, head = blockIdx.y, kv = head / a.rep, i = threadIdx.x, p = i & 63, share = i >> 6;
-    const int pos = gload(a.pos + row), seq = gload(a.seq + row);
-    if (pos < 0 || (unsigned)seq >= (unsigned)c.n_seq) return;
-    const float mine = i < c.qd ? gload(a.q + row * a.q_stride + (int64_t)head * c.qd + i) : 0.0f;
-    sq[i] = mine;
-    const bool lost = __syncthreads_or(!(fabsf(mine) < INFINITY));  // a query that is not finite
-    const int lo = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (int t0 = lo & ~63; t0 <= pos; t0 += 64) {
-        const int page = t0 >> c.page_shift, id = page < c.max_pages ? gload(c.table + (int64_t)seq * c.max_pages + page) : -1;
-        if ((unsigned)id >= (unsigned)c.n_pages) continue;
-        const int64_t tile = c.tile(id, kv, t0 & ((1 << c.page_shift) - 1));
-        const uint8_t *codes = c.at(tile);
-        __syncthreads();
-        float s = 0.0f;
-        for (int d = share; d < c.qd; d += 4) s = fmaf(sq[d], (float)(int8_t)gload(codes + kv8_key_byte(c.qd, p, d)), s);
-        part[share][p] = s;
-        __syncthreads();
-        const bool seen = t0 + p >= lo && t0 + p <= pos;
-        s = seen ? (((part[0][p] + part[1][p]) + (part[2][p] + part[3][p])) * gload(c.scale_at(tile, true, p >> 4))) * a.scale : -INFINITY;
-        float top = s;
-        bool bad = lost || s != s || (seen && gload(c.scale_at(tile, false, p >> 4)) != gload(c.scale_at(tile, false, p >> 4)));
-        for (int x = 32; x >= 1; x >>= 1) {
-            top = fmaxf(top, __shfl_xor(top, x, 64));
-            bad |= (bool)__shfl_xor((int)bad, x, 64);
+constexpr float kNone = -1e30f;          // below every score: where nothing has been seen
+constexpr float kMost = 8355000.0f;      // largest weight (C): its digits' room is 8355711, what exp2 errs by taken off
+constexpr float kLeastLog = -100.0f;     // log2 of a value scale, where it is smaller or 0
+
+__device__ inline i32x4 mfma(i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+
+// The largest of a column's four lanes (16 apart), in each of them.
+__device__ inline float column_max(float x) {
+    const uint32_t u = __float_as_uint(x);
+    auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t v = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Four weights' digits, by digit: 2 (highest), 1, 0.
+struct Digits {
+    uint32_t d2, d1, d0;
+};
+__device__ inline Digits digits_of(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+    const uint32_t a = __builtin_amdgcn_perm(w1, w0, 0x05010400u), b = __builtin_amdgcn_perm(w3, w2, 0x05010400u);
+    Digits d;
+    d.d0 = __builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u;
+    d.d1 = __builtin_amdgcn_perm(b, a, 0x07060302u) ^ 0x80808080u;
+    d.d2 = __builtin_amdgcn_perm(w1, w0, 0x0c0c0602u) | __builtin_amdgcn_perm(w3, w2, 0x06020c0cu);
+    return d;
+}
+
+// A wave's 16 columns.  Lane (column, g) of o[D] holds dims 16 D + 4 g + i.
+template <int NV>
+struct Columns {
+    f32x4 o[NV];
+    float m, R, l;      // (l: this lane's positions only)
+    float qs;           // 2^(e - 22) |scale| log2(e)
+    int pos, lo;        // what a column sees: positions lo .. pos
+    int first, last;    // of all columns: everything in first .. last is seen by every one
+};
+
+// One step of NT tiles: k(T, c) and v(D, t) give operands, ks and vs the blocks'
+// scales, base[t] the tiles' first positions (negative: no such tile, whose
+// scales are 0).
+template <int NQ, int NV, int NT, bool EX, class K, class V>
+__device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const i32x4 (&q)[3][NQ], K k, V v, float (&ks)[4 * NT],
+                                                           float (&vs)[4 * NT], const int (&base)[NT], int nq, int nv, int g) {
+    f32x4 s[4 * NT];
+#pragma unroll
+    for (int b = 0; b < 4 * NT; b++) {
+        i32x4 kk[NQ], hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < NQ; c++) kk[c] = k(b, c);
+#pragma unroll
+        for (int c = 0; c < NQ; c++) {
+            lo = mfma(kk[c], q[1][c], lo);
+            hi = mfma(kk[c], q[0][c], hi);
         }
-        if (bad) top = __uint_as_float(0x7fc00000u);
-        const float m1 = bad || m != m ? __uint_as_float(0x7fc00000u) : fmaxf(m, top);
-        const float w = m1 == -INFINITY ? 0.0f : expf(s - m1), f = m1 == -INFINITY ? 1.0f : expf(m - m1);
-        m = m1;
-        if (share == 0) sp[p] = w;
-        float sum = w;
-        for (int x = 32; x >= 1; x >>= 1) sum += __shfl_xor(sum, x, 64);
-        l = l * f + sum;
-        __syncthreads();
-        if (i < c.vd) {
-            o *= f;
-            for (int t = 0; t < 64; t++) {
-                if (t0 + t < lo || t0 + t > pos) continue;
-                const float v = gload(c.scale_at(tile, false, t >> 4)) * (float)(int8_t)gload(codes + c.values() + kv8_value_byte(t, i));
-                o = fmaf(sp[t], v, o);
-            }
+        lo = lo << 8;
+#pragma unroll
+        for (int c = 0; c < NQ; c++) lo = mfma(kk[c], q[2][c], lo);
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[b][i] = fmaf((float)hi[i], 65536.0f, (float)lo[i]);
+    }
+    float all = 0.0f, sc[4 * NT];
+#pragma unroll
+    for (int b = 0; b < 4 * NT; b++) all += fabsf(ks[b]) + fabsf(vs[b]);
+    if (__builtin_expect(!(all < INFINITY), 0)) {  // a block that reads as NaN: so are the columns that see it
+#pragma unroll
+        for (int b = 0; b < 4 * NT; b++) {
+            const int p = base[b / 4] + 16 * (b % 4);
+            if (fabsf(ks[b]) < INFINITY && fabsf(vs[b]) < INFINITY) continue;
+            if (base[b / 4] >= 0 && p <= x.pos && p + 15 >= x.lo) x.l = __uint_as_float(0x7fc00000u);
+            ks[b] = vs[b] = 0.0f;
         }
     }
-    if (i < c.vd) gstore(a.out + row * a.out_stride + (int64_t)head * c.vd + i, l == 0.0f ? 0.0f : o / l);
+#pragma unroll
+    for (int b = 0; b < 4 * NT; b++) sc[b] = ks[b] * x.qs;
+    bool whole = true;
+#pragma unroll
+    for (int t = 0; t < NT; t++) whole = whole && base[t] >= x.first && base[t] + 63 <= x.last;
+    if (!whole) {
+#pragma unroll
+        for (int b = 0; b < 4 * NT; b++) {
+            const int p = base[b / 4] + 16 * (b % 4) + 4 * g;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                s[b][i] = base[b / 4] >= 0 && p + i >= x.lo && p + i <= x.pos ? s[b][i] * sc[b] : -INFINITY;
+            sc[b] = 1.0f;
+        }
+    }
+    float top = kNone, ref = kNone;
+#pragma unroll
+    for (int b = 0; b < 4 * NT; b++) {
+        const float t = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])) * sc[b];
+        top = fmaxf(top, t);
+        ref = fmaxf(ref, t + fmaxf(__builtin_amdgcn_logf(vs[b]), kLeastLog));
+    }
+    top = column_max(top), ref = column_max(ref);
+    const float f = __builtin_amdgcn_exp2f(top - ref) * kMost;
+    float sum = 0.0f;
+    i32x4 w[NT][3];
+#pragma unroll
+    for (int b = 0; b < 4 * NT; b++) {
+        const float scaled = fminf(vs[b] * f, 3e38f);  // (p is 0 where it would be more)
+        uint32_t y[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(s[b][i], sc[b], -top));
+            sum += p;
+            y[i] = __float_as_uint(fmaf(p, scaled, 8388608.0f + 32896.0f));
+        }
+        const Digits d = digits_of(y[0], y[1], y[2], y[3]);
+        w[b / 4][0][b % 4] = (int)d.d2, w[b / 4][1][b % 4] = (int)d.d1, w[b / 4][2][b % 4] = (int)d.d0;
+    }
+    const float m = fmaxf(x.m, top), R = fmaxf(x.R, ref);
+    x.l = x.l * __builtin_amdgcn_exp2f(x.m - m) + sum * __builtin_amdgcn_exp2f(top - m);
+    const float keep = __builtin_amdgcn_exp2f(x.R - R), join = __builtin_amdgcn_exp2f(ref - R) * (1.0f / kMost);
+    x.m = m, x.R = R;
+#pragma unroll
+    for (int D = 0; D < NV; D++) {
+        if (!EX && D >= nv) continue;
+        i32x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0}, vv[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++) vv[t] = v(D, t);
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            lo = mfma(vv[t], w[t][1], lo);
+            hi = mfma(vv[t], w[t][0], hi);
+        }
+        lo = lo << 8;
+#pragma unroll
+        for (int t = 0; t < NT; t++) lo = mfma(vv[t], w[t][2], lo);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            x.o[D][i] = fmaf(fmaf((float)hi[i], 65536.0f, (float)lo[i]), join, x.o[D][i] * keep);
+    }
+}
+
+// Lanes of my_seq and my_pos that begin a run of one sequence's rows or are
+// none; the runs' first lanes.
+struct Runs {
+    unsigned long long cuts, starts, valid;
+};
+__device__ inline Runs runs_of(const Kv8 &c, int my_seq, int my_pos, int nr) {
+    const int lane = threadIdx.x & 63;
+    const bool valid = lane < nr && my_pos >= 0 && (unsigned)my_seq < (unsigned)c.n_seq;
+    const int before = __shfl_up(my_seq, 1, 64);
+    const bool before_ok = __shfl_up((int)valid, 1, 64);
+    Runs r;
+    r.valid = __ballot(valid);
+    r.cuts = __ballot(!valid || lane == 0 || my_seq != before || !before_ok);
+    r.starts = r.cuts & r.valid;
+    return r;
+}
+
+// One run of a group: rows first .. end - 1 of it, and what they see.
+struct Run {
+    int first, end, seq, lo, hi;
+};
+__device__ inline bool next_run(const Runs &r, unsigned long long &starts, int nr, int my_seq, int my_pos, int window, Run &x) {
+    if (!starts) return false;
+    const int lane = threadIdx.x & 63;
+    x.first = __builtin_ctzll(starts);
+    starts &= starts - 1;
+    const unsigned long long after = x.first < 63 ? r.cuts >> (x.first + 1) : 0;
+    x.end = min(nr, after ? x.first + 1 + __builtin_ctzll(after) : 64);
+    const bool mine = lane >= x.first && lane < x.end;
+    int hi = mine ? my_pos : -1, lo = mine ? (window > 0 ? max(0, my_pos + 1 - window) : 0) : 0x7fffffff;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        hi = max(hi, __shfl_xor(hi, o, 64));
+        lo = min(lo, __shfl_xor(lo, o, 64));
+    }
+    x.hi = __builtin_amdgcn_readfirstlane(hi), x.lo = __builtin_amdgcn_readfirstlane(lo);
+    x.seq = __builtin_amdgcn_readlane(my_seq, x.first);
+    return true;
+}
+
+// Pages of a run, 64 at a time, one a lane: where the kv head's tiles are (as a
+// tile's number; negative: no such page).
+struct Pages {
+    int b0 = -64;
+    uint32_t lo = 0;
+    int hi = -1;
+    __device__ int64_t tile(const Kv8 &c, const int32_t *table, int kv, int t) {  // of the sequence's tile t
+        const int shift = c.page_shift - 6, i = t >> shift;
+        if (i < b0 || i >= b0 + 64) {
+            b0 = i;
+            const int page = b0 + (threadIdx.x & 63), pid = page < c.max_pages ? gload(table + page) : -1;
+            const int64_t at = (unsigned)pid < (unsigned)c.n_pages ? c.tile(pid, kv, 0) : -1;
+            lo = (uint32_t)at, hi = (int)(at >> 32);
+            asm volatile("" : "+v"(lo), "+v"(hi));  // waited for here, not at every tile
+        }
+        const int h = __builtin_amdgcn_readlane(hi, i - b0);
+        const uint32_t l = (uint32_t)__builtin_amdgcn_readlane((int)lo, i - b0);
+        return h < 0 ? -1 : ((int64_t)h << 32 | l) + (t & ((1 << shift) - 1));
+    }
+};
+
+// Queries' digits into LDS as the product reads them, [digit][chunk][lane], for
+// COLS columns; a column's factor 2^(e - 22) |scale| log2(e), NaN where the query
+// is not finite.  16 threads a column, 16 dims each.
+template <int NQ, int COLS>
+__device__ inline void stage_queries(const Args &a, u32x4 *sq, float *sk, int r0, int h0, int hn, int c0, int c1) {
+    const int u = threadIdx.x & 15, nu = a.c.qd / 16;
+    for (int col = threadIdx.x >> 4; col < COLS; col += blockDim.x >> 4) {
+        const int cc = c0 + col;
+        float x[16];
+        const bool there = cc < c1 && u < nu;
+        const float *src = a.q + (int64_t)(r0 + (there ? cc : c0) / hn) * a.q_stride + (int64_t)(h0 + (there ? cc : c0) % hn) * a.c.qd +
+                           (there ? 16 * u : 0);
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const f32x4 y = __builtin_bit_cast(f32x4, gload_x4((const uint32_t *)src + 4 * j));
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[4 * j + e] = there ? y[e] : 0.0f;
+                top = max(top, __float_as_uint(x[4 * j + e]) & 0x7fffffffu);
+            }
+        }
+#pragma unroll
+        for (int o = 8; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+        const bool finite = top < 0x7f800000u;
+        // 2^e above the largest (of a subnormal one, 2^-126)
+        const int e = max((int)(top >> 23) - 126, -126);
+        uint32_t d[3][4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float v = finite ? rintf(ldexpf(x[4 * j + i], 22 - e)) : 0.0f;
+                w[i] = (uint32_t)((int)(a.scale < 0.0f ? -v : v) + 0x808080);
+            }
+            const Digits z = digits_of(w[0], w[1], w[2], w[3]);
+            d[0][j] = z.d2 ^ 0x80808080u, d[1][j] = z.d1, d[2][j] = z.d0;
+        }
+        if (u < 4 * NQ)
+#pragma unroll
+            for (int p = 0; p < 3; p++)
+                sq[((col >> 4) * 3 + p) * NQ * 64 + (u >> 2) * 64 + (u & 3) * 16 + (col & 15)] = u32x4{d[p][0], d[p][1], d[p][2], d[p][3]};
+        if (u == 0) sk[col] = finite ? ldexpf(fabsf(a.scale) * 1.44269504088896341f, e - 22) : __uint_as_float(0x7fc00000u);
+    }
+}
+
+// A wave's columns at the start of a run; `row`: the lane's column's row in the group.
+template <int NQ, int NV>
+__device__ inline void begin(Columns<NV> &x, i32x4 (&q)[3][NQ], const u32x4 *sq, const float *sk, int my_pos, int window, int row) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int p = 0; p < 3; p++)
+#pragma unroll
+        for (int c = 0; c < NQ; c++) q[p][c] = __builtin_bit_cast(i32x4, sq[(p * NQ + c) * 64 + lane]);
+#pragma unroll
+    for (int D = 0; D < NV; D++) x.o[D] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const float k = sk[lane & 15];
+    x.qs = k != k ? 0.0f : k;
+    x.m = x.R = kNone;
+    x.l = k != k ? k : 0.0f;
+    x.pos = __shfl(my_pos, row, 64);
+    x.lo = window > 0 ? max(0, x.pos + 1 - window) : 0;
+    int first = x.lo, last = x.pos;
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) {
+        first = max(first, __shfl_xor(first, o, 64));
+        last = min(last, __shfl_xor(last, o, 64));
+    }
+    x.first = __builtin_amdgcn_readfirstlane(first), x.last = __builtin_amdgcn_readfirstlane(last);
+}
+
+// What a block of 16 columns shares.
+template <int NQ, int NV>
+struct Narrow {
+    u32x4 sq[3 * NQ * 64];
+    f32x4 so[4 * NV * 64];  // O of the waves: [wave][D][lane]
+    float sk[16], sm[4][16], sl[4][16], sr[4][16];
+};
+
+typedef const __attribute__((address_space(1))) uint8_t *gbytes;
+__device__ inline __amdgpu_buffer_rsrc_t buffer_of(const void *p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, bytes, 0x00020000);
+}
+
+// 16 columns, four waves sharing the positions: rows r0 .. r0 + nr - 1 (whose
+// sequences and positions the lanes hold), heads h0 .. h0 + hn - 1; every
+// split-th run from `sub` on, of its tiles the part-th part.
+template <int NQ, int NV, bool EX>
+__device__ __attribute__((always_inline)) inline void narrow(const Args &a, Narrow<NQ, NV> &lds, int kv, int part, int r0, int nr, int h0,
+                                                             int hn, int my_seq, int my_pos, int sub, int split) {
+    const Kv8 &c = a.c;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+    const int nq = EX ? NQ : (c.qd + 63) / 64, nv = EX ? NV : c.vd / 16, qd = EX ? 64 * NQ : c.qd;
+    stage_queries<NQ, 16>(a, lds.sq, lds.sk, r0, h0, hn, 0, nr * hn);
+    __syncthreads();
+    const Runs runs = runs_of(c, my_seq, my_pos, nr);
+    unsigned long long starts = runs.starts;
+    Run run;
+    for (int n = 0; next_run(runs, starts, nr, my_seq, my_pos, a.window, run); n++) {
+        if (n % split != sub) continue;
+        const int c0 = run.first * hn, ncol = run.end * hn - c0;
+        Columns<NV> x;
+        i32x4 q[3][NQ];
+        // (columns of other runs do as this run's first or last)
+        begin<NQ, NV>(x, q, lds.sq, lds.sk, my_pos, a.window, min(max(col, c0), c0 + ncol - 1) / hn);
+        const int32_t *table = c.table + (int64_t)run.seq * c.max_pages;
+        const int t0 = run.lo >> 6, nt = (run.hi >> 6) - t0 + 1;
+        const int parts = a.ps * 4, me = part * 4 + wave;
+        int t = t0 + (int)((long long)nt * me / parts);
+        const int t1 = t0 + (int)((long long)nt * (me + 1) / parts);
+        Pages pages;
+        i32x4 k[4][NQ], v[NV];
+        f32x4 ks, vs;
+        int base[1];
+        __amdgpu_buffer_rsrc_t buf;
+        // Loads are unconditional, so that waiting for one tile's keys leaves the
+        // others' in flight; where there is no tile they read nothing (0).
+        auto load_keys = [&](int at) __attribute__((always_inline)) {
+            const int64_t tile = at < t1 ? pages.tile(c, table, kv, at) : -1;
+            base[0] = tile < 0 ? -64 : at * 64;
+            buf = buffer_of(tile < 0 ? c.codes : c.at(tile), tile < 0 ? 0 : c.tile_bytes());
+            const __amdgpu_buffer_rsrc_t sb = buffer_of(tile < 0 ? (const void *)c.scales : c.scales + tile * 8, tile < 0 ? 0 : 32);
+            ks = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sb, 0, 0, 0));
+            vs = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sb, 16, 0, 0));
+#pragma unroll
+            for (int T = 0; T < 4; T++)
+#pragma unroll
+                for (int cc = 0; cc < NQ; cc++)
+                    k[T][cc] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(buf, 16 * lane, T * 16 * qd + cc * 1024, 0));
+        };
+        auto load_values = [&] __attribute__((always_inline)) {
+#pragma unroll
+            for (int D = 0; D < NV; D++)
+                v[D] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(buf, 16 * lane, 64 * qd + D * 1024, 0));
+        };
+        if (t < t1) {
+            load_keys(t);
+            load_values();
+        }
+        for (; t < t1; t++) {
+            float kb[4] = {ks[0], ks[1], ks[2], ks[3]}, vb[4] = {vs[0], vs[1], vs[2], vs[3]};
+            if (base[0] >= 0)
+                step<NQ, NV, 1, EX>(x, q, [&](int b, int cc) { return k[b][cc]; }, [&](int D, int) { return v[D]; }, kb, vb, base, nq, nv, g);
+            load_keys(t + 1);
+            load_values();
+        }
+
+        // Merge the waves: sums as they are and their references through LDS,
+        // then every wave takes a share of the output's dims.
+        x.l += __shfl_xor(x.l, 16, 64);
+        x.l += __shfl_xor(x.l, 32, 64);
+        if (g == 0) lds.sm[wave][col] = x.m, lds.sl[wave][col] = x.l, lds.sr[wave][col] = x.R;
+#pragma unroll
+        for (int D = 0; D < NV; D++) lds.so[(wave * NV + D) * 64 + lane] = x.o[D];
+        __syncthreads();
+        float m = kNone, R = kNone, l = 0.0f, f[4];
+#pragma unroll
+        for (int w = 0; w < 4; w++) m = fmaxf(m, lds.sm[w][col]), R = fmaxf(R, lds.sr[w][col]);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            l += lds.sl[w][col] * __builtin_amdgcn_exp2f(lds.sm[w][col] - m);
+            f[w] = __builtin_amdgcn_exp2f(lds.sr[w][col] - R);
+        }
+        if (col >= c0 && col < c0 + ncol) {
+            const int64_t row = r0 + col / hn, head = h0 + col % hn;
+            float *dst = a.out + row * a.out_stride + head * c.vd;
+            float by = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(R - m) / l;
+            if (a.ps > 1) {
+                const int64_t at = (row * a.heads + head) * a.ps + part;
+                dst = a.part + at * c.vd, by = 1.0f;
+                if (g == 0 && wave == 0) a.part_ml[3 * at] = m, a.part_ml[3 * at + 1] = l, a.part_ml[3 * at + 2] = R;
+            }
+#pragma unroll
+            for (int i = 0; i < (NV + 3) / 4; i++) {
+                const int D = 4 * i + wave;
+                if (D >= nv) continue;
+                f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const f32x4 y = lds.so[(w * NV + D) * 64 + lane];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) z[e] = fmaf(y[e], f[w], z[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) z[e] *= by;
+                *(__attribute__((address_space(1))) f32x4_dw *)(dst + 16 * D + 4 * g) = __builtin_bit_cast(f32x4_dw, z);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <int NQ, int NV, bool EX>
+__global__ __launch_bounds__(256, 2) void kv8_attention_kernel(const Args a) {
+    __shared__ Narrow<NQ, NV> lds;
+    const Kv8 &c = a.c;
+    const int lane = threadIdx.x & 63;
+    // Kv heads next to each other go to the XCDs in turn, so that one head's
+    // blocks find its tiles in their L2.  Later rows of a prompt see more
+    // positions: the last groups go first.
+    int id = blockIdx.x;
+    const int kv = id % c.n_kv;
+    id /= c.n_kv;
+    const int chunk = id % a.chunks;
+    id /= a.chunks;
+    const int part = id % a.ps;
+    id /= a.ps;
+    const int sub = id / a.groups;
+    const int r0 = (a.groups - 1 - id % a.groups) * a.tt;
+    const int nr = min(a.tt, a.rows - r0);
+    const int h0 = kv * a.rep + chunk * a.rc, hn = min(a.rc, a.rep - chunk * a.rc);
+    const int my_seq = gload(a.seq + r0 + min(lane, nr - 1)), my_pos = gload(a.pos + r0 + min(lane, nr - 1));
+    narrow<NQ, NV, EX>(a, lds, kv, part, r0, nr, h0, hn, my_seq, my_pos, sub, a.split);
+}
+
+// The parts of rows whose tiles several blocks shared: a block of T threads
+// per (row, head), each group of vd / 4 of them every so many-th part; the
+// groups' sums in order.
+template <int T>
+__global__ __launch_bounds__(T) void kv8_join_kernel(const Args a) {
+    __shared__ float w[256], red;
+    __shared__ f32x4 sums[T];
+    const int vd = a.c.vd, row = blockIdx.x / a.heads, head = blockIdx.x % a.heads, i = threadIdx.x;
+    if (a.pos[row] < 0 || (unsigned)a.seq[row] >= (unsigned)a.c.n_seq) return;
+    const float *ml = a.part_ml + (int64_t)blockIdx.x * a.ps * 3, *part = a.part + (int64_t)blockIdx.x * a.ps * vd;
+    if (i < 64) {
+        float m = kNone, R = kNone, l = 0.0f, pm[4], pl[4], pr[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int p = i + 64 * k;
+            pm[k] = p < a.ps ? gload(ml + 3 * p) : kNone, pl[k] = p < a.ps ? gload(ml + 3 * p + 1) : 0.0f;
+            pr[k] = p < a.ps ? gload(ml + 3 * p + 2) : kNone;
+            m = fmaxf(m, pm[k]), R = fmaxf(R, pr[k]);
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64)), R = fmaxf(R, __shfl_xor(R, o, 64));
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (i + 64 * k < a.ps) w[i + 64 * k] = __builtin_amdgcn_exp2f(pr[k] - R);
+            l += pl[k] * __builtin_amdgcn_exp2f(pm[k] - m);
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o, 64);
+        if (i == 0) red = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(R - m) / l;
+    }
+    __syncthreads();
+    const int n = vd / 4, groups = T / n, g = i / n, at = i % n;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (g < groups)
+        for (int p = g; p < a.ps; p += groups) {
+            const f32x4 x = gload((const f32x4 *)(part + (int64_t)p * vd) + at);
+#pragma unroll
+            for (int k = 0; k < 4; k++) acc[k] = fmaf(x[k], w[p], acc[k]);
+        }
+    sums[i] = acc;
+    __syncthreads();
+    if (i >= n) return;
+    for (int k = 1; k < groups; k++) acc += sums[k * n + i];
+    float *dst = a.out + (int64_t)row * a.out_stride + (int64_t)head * vd + 4 * i;
+#pragma unroll
+    for (int k = 0; k < 4; k++) dst[k] = acc[k] * red;
+}
+
+// How a call is cut up: see Args.
+struct Plan {
+    int rc, chunks, tt, groups, split, ps;
+    uint64_t bytes;
+};
+
+Plan plan_of(const Kv8 &c, int rows, int heads, int max_pos, int window) {
+    Plan p{};
+    const int rep = heads / c.n_kv;
+    p.rc = std::min(rep, 16);
+    p.chunks = (rep + p.rc - 1) / p.rc;
+    p.tt = 16 / p.rc;
+    p.groups = (int)(((long long)rows + p.tt - 1) / p.tt);
+    const long long base = (long long)p.groups * p.chunks * c.n_kv;
+    p.split = (int)std::max<long long>(1, std::min<long long>(p.tt, 1024 / base));
+    const long long tiles = (window > 0 ? std::min((long long)window + p.tt, (long long)max_pos + 1) : max_pos + 1LL) / 64 + 1;
+    const long long units = base * p.split;
+    const long long ps = units >= 256 ? std::min((512 + units - 1) / units, tiles / 32)
+                         : tiles < 24 ? 1
+                                      : std::min<long long>({(1024 + units - 1) / units, tiles / 6, 256});
+    p.ps = (int)std::max<long long>(1, ps);
+    p.bytes = p.ps > 1 ? (uint64_t)rows * heads * p.ps * (c.vd + 3) * 4 : 0;
+    return p;
+}
+
+constexpr long long kMostThreads = 0xffffffffll;  // of a launch
+
+template <int NQ, int NV, bool EX>
+void launch(const Args &a, hipStream_t s) {
+    const long long blocks = (long long)a.groups * a.split * a.ps * a.chunks * a.c.n_kv;
+    hipLaunchKernelGGL((kv8_attention_kernel<NQ, NV, EX>), dim3((unsigned)blocks), dim3(256), 0, s, a);
 }
 
 }  // namespace
@@ -89,7 +564,7 @@ int moe_kv8_attention_workspace_size(const moe_kv8 *c, int32_t rows, int32_t hea
     if (!bytes || rows < 0 || heads <= 0 || heads % a.n_kv || max_pos < 0 || max_pos >= (int64_t)a.max_pages << a.page_shift)
         return fail(MOE_EINVAL, "moe_kv8_attention_workspace_size: bad argument (%d rows, %d heads over %d, max position %d"
                     " of %lld)", rows, heads, a.n_kv, max_pos, (long long)a.max_pages << a.page_shift);
-    *bytes = 0;
+    *bytes = rows ? plan_of(a, rows, heads, max_pos, window).bytes : 0;
     return MOE_OK;
 }
 
@@ -103,10 +578,29 @@ int moe_kv8_attention(const moe_kv8 *c, const float *q, int64_t q_stride, int32_
         return fail(MOE_EINVAL, "moe_kv8_attention: bad argument (%d rows, %d heads over %d, max position %d of %lld)", rows,
                     heads, a.c.n_kv, max_pos, (long long)a.c.max_pages << a.c.page_shift);
     if (rows == 0) return MOE_OK;
-    if (heads > 65535 || rows > (1 << 24) - 256) return fail(MOE_EUNSUP, "moe_kv8_attention: %d rows of %d heads", rows, heads);
+    const Plan p = plan_of(a.c, rows, heads, max_pos, window);
+    if (p.bytes && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < p.bytes))
+        return fail(MOE_EINVAL, "moe_kv8_attention: workspace of %llu bytes, %llu needed", (unsigned long long)workspace_bytes,
+                    (unsigned long long)p.bytes);
     a.q = q, a.seq = seq, a.pos = pos, a.out = out, a.q_stride = q_stride, a.out_stride = out_stride;
     a.rows = rows, a.heads = heads, a.rep = heads / a.c.n_kv, a.window = window, a.scale = scale;
-    hipLaunchKernelGGL(kv8_attention_kernel, dim3(rows, heads), dim3(256), 0, (hipStream_t)stream, a);
+    a.tt = p.tt, a.groups = p.groups, a.rc = p.rc, a.chunks = p.chunks, a.split = p.split, a.ps = p.ps;
+    a.part = static_cast<float *>(workspace);
+    a.part_ml = a.part + (size_t)rows * heads * p.ps * a.c.vd;
+    if ((long long)a.groups * a.split * a.ps * a.chunks * a.c.n_kv > kMostThreads / 256)
+        return fail(MOE_EUNSUP, "moe_kv8_attention: %d rows of %d heads are too many blocks", rows, heads);
+    hipStream_t s = (hipStream_t)stream;
+    const int qd = a.c.qd, vd = a.c.vd;
+    // Widths of their own: a power-of-two head and the latent cache's 192/128;
+    // the others count their operands at run time.
+    if (qd == 64 && vd == 64) launch<1, 4, true>(a, s);
+    else if (qd == 128 && vd == 128) launch<2, 8, true>(a, s);
+    else if (qd == 192 && vd == 128) launch<3, 8, true>(a, s);
+    else if (qd <= 192 && vd <= 128) launch<3, 8, false>(a, s);
+    else if (qd == 256 && vd == 256) launch<4, 16, true>(a, s);
+    else launch<4, 16, false>(a, s);
+    if (a.ps > 16) hipLaunchKernelGGL((kv8_join_kernel<256>), dim3((unsigned)rows * heads), dim3(256), 0, s, a);
+    else if (a.ps > 1) hipLaunchKernelGGL((kv8_join_kernel<64>), dim3((unsigned)rows * heads), dim3(64), 0, s, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? MOE_OK : fail(MOE_EHIP, "8-bit attention kernel: %s", hipGetErrorString(e));
 }

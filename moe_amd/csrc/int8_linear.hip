@@ -16,6 +16,7 @@
 
 #include "gmem.h"
 #include "int8.h"
+#include "lds_dma.h"
 #include "moe_internal.h"
 #include "row_value.h"
 
@@ -25,6 +26,7 @@ int fail(int code, const char *fmt, ...);
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMostK = 131072;  // 127 * 127 * K stays below 2^31
@@ -69,29 +71,64 @@ __global__ __launch_bounds__(256) void int8_pack_kernel(const uint8_t *__restric
     if (threadIdx.x == 0) scales[to] = s.scale;
 }
 
-// Rows of x, a block each; rows up to the next 16th are zeros.
+// Block b's row: the rows of a tile, 16 in turn, go to one XCD, so that the
+// bytes of a line that different rows write meet in one L2.
+__device__ inline int64_t row_of(unsigned b) { return (int64_t)((b >> 7) * 8 + (b & 7)) * 16 + (b >> 3 & 15); }
+unsigned row_blocks(int64_t rows) { return (unsigned)((rows + 127) / 128 * 128); }
+
+// Rows of x, a block each, a thread 16 values at a time (kept in registers where
+// a row has no more than kHeld of them); rows up to the next 16th are zeros.
+constexpr int kHeld = 2;
 __global__ __launch_bounds__(256) void int8_rows_kernel(const float *__restrict__ x, int64_t xs, int t, int k,
                                                         uint8_t *__restrict__ codes, float *__restrict__ scales) {
     __shared__ uint32_t red[4];
-    const int64_t to = blockIdx.x, chunks = up(k, 64) / 64;
+    const int64_t to = row_of(blockIdx.x), chunks = up(k, 64) / 64;
+    if (to >= up(t, 16)) return;
     const float *row = x + to * xs;
+    const int units = (int)chunks * 4, whole = to < t ? k / 16 : 0;
+    auto values = [&](int u, float (&v)[16]) __attribute__((always_inline)) {
+        if (u < whole) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const u32x4_dw y = gload_x4((const uint32_t *)row + 16 * u + 4 * j);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[4 * j + e] = __uint_as_float(y[e]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; e++) v[e] = to < t && 16 * u + e < k ? gload(row + 16 * u + e) : 0.0f;
+        }
+    };
+    float held[kHeld][16];
     uint32_t top = 0;
-    if (to < t)
-        for (int i = threadIdx.x; i < k; i += 256) top = max(top, magnitude(gload(row + i)));
+#pragma unroll
+    for (int j = 0; j < kHeld; j++) {
+        const int u = threadIdx.x + 256 * j;
+        if (u >= units) continue;
+        values(u, held[j]);
+#pragma unroll
+        for (int e = 0; e < 16; e++) top = max(top, magnitude(held[j][e]));
+    }
+    for (int u = threadIdx.x + 256 * kHeld; u < units; u += 256) {
+        float v[16];
+        values(u, v);
+#pragma unroll
+        for (int e = 0; e < 16; e++) top = max(top, magnitude(v[e]));
+    }
     const Int8Scale s(block_max(top, red));
-    for (int g = threadIdx.x; g < chunks * 4; g += 256) {
+    auto write = [&](int u, const float (&v)[16]) __attribute__((always_inline)) {
         uint32_t y[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            int c[4];
+        for (int j = 0; j < 4; j++) y[j] = pack4(s.code(v[4 * j]), s.code(v[4 * j + 1]), s.code(v[4 * j + 2]), s.code(v[4 * j + 3]));
+        gstore((u32x4 *)(codes + group_at(to, 16 * (int64_t)u, chunks)), u32x4{y[0], y[1], y[2], y[3]});
+    };
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int i = 16 * g + 4 * j + e;
-                c[e] = to < t && i < k ? s.code(gload(row + i)) : 0;
-            }
-            y[j] = pack4(c[0], c[1], c[2], c[3]);
-        }
-        gstore((u32x4 *)(codes + group_at(to, 16 * (int64_t)g, chunks)), u32x4{y[0], y[1], y[2], y[3]});
+    for (int j = 0; j < kHeld; j++)
+        if (threadIdx.x + 256 * j < units) write(threadIdx.x + 256 * j, held[j]);
+    for (int u = threadIdx.x + 256 * kHeld; u < units; u += 256) {
+        float v[16];
+        values(u, v);
+        write(u, v);
     }
     if (threadIdx.x == 0) scales[to] = s.scale;
 }
@@ -101,31 +138,175 @@ struct Product {
     const float *sw, *sx;
     float *y, *residual;
     int64_t ys, rs;
-    int n, t;
-    int64_t chunks;
+    int n, t, chunks;
+    int nt, tt;  // tiles of 16 channels, of 16 tokens
 };
 
-// A wave computes 16 channels of 16 tokens: lane (token, g) ends with channels
-// 4 g .. 4 g + 3.
-__global__ __launch_bounds__(256) void int8_product_kernel(const Product p) {
-    const int lane = threadIdx.x & 63;
-    const int64_t nt = blockIdx.x * 4 + (threadIdx.x >> 6), tt = blockIdx.y;
-    if (nt * 16 >= p.n) return;
-    const u32x4 *w = (const u32x4 *)(p.w + nt * p.chunks * 1024) + lane, *x = (const u32x4 *)(p.x + tt * p.chunks * 1024) + lane;
-    i32x4 acc = {0, 0, 0, 0};
-    for (int64_t c = 0; c < p.chunks; c++)
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, gload(w + 64 * c)),
-                                                    __builtin_bit_cast(i32x4, gload(x + 64 * c)), acc, 0, 0, 0);
-    const int64_t t = tt * 16 + (lane & 15), n = nt * 16 + 4 * (lane >> 4);
-    if (t >= p.t) return;
-    const float sx = gload(p.sx + t);
+// y and residual of one channel and token.
+__device__ inline void finish(const Product &p, int64_t t, int64_t n, int sum, float sx, float sw) {
+    const float v = (float)sum * (sx * sw);
+    gstore(p.y + t * p.ys + n, v);
+    if (p.residual) gstore(p.residual + t * p.rs + n, gload(p.residual + t * p.rs + n) + v);
+}
+
+// MT x NT tiles of 16 tokens by 16 channels a block, operands straight from
+// memory, the chunks of K dealt to W waves whose sums meet in LDS.
+template <int MT, int NT, int W>
+__global__ __launch_bounds__(W * 64) void int8_direct_kernel(const Product p) {
+    __shared__ i32x4 sums[W > 1 ? (W - 1) * MT * NT * 64 : 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * NT, t0 = blockIdx.y * MT;
+    const u32x4 *w[NT], *x[MT];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if (n + i >= p.n) continue;
-        const float v = (float)acc[i] * (sx * gload(p.sw + n + i));
-        gstore(p.y + t * p.ys + n + i, v);
-        if (p.residual) p.residual[t * p.rs + n + i] += v;
+    for (int j = 0; j < NT; j++) w[j] = (const u32x4 *)(p.w + (int64_t)min(n0 + j, p.nt - 1) * p.chunks * 1024) + lane;
+#pragma unroll
+    for (int i = 0; i < MT; i++) x[i] = (const u32x4 *)(p.x + (int64_t)min(t0 + i, p.tt - 1) * p.chunks * 1024) + lane;
+    i32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[i][j] = i32x4{0, 0, 0, 0};
+    // U chunks' loads at a time; past the last chunk the last one again, whose
+    // products then meet zeros.
+    constexpr int U = MT + NT <= 3 ? 8 : MT + NT <= 6 ? 4 : 2;
+    for (int c0 = wave; c0 < p.chunks; c0 += W * U) {
+        i32x4 a[U][MT], b[U][NT];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int c = min(c0 + u * W, p.chunks - 1);
+#pragma unroll
+            for (int j = 0; j < NT; j++) b[u][j] = __builtin_bit_cast(i32x4, gload(w[j] + 64 * c));
+#pragma unroll
+            for (int i = 0; i < MT; i++) a[u][i] = __builtin_bit_cast(i32x4, gload(x[i] + 64 * c));
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (c0 + u * W >= p.chunks) continue;
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int j = 0; j < NT; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u][i], b[u][j], acc[i][j], 0, 0, 0);
+        }
     }
+    if (W > 1) {
+        // Wave w ends with tiles w, w + W ...: the others' shares of them.
+        // Slot of wave v's tile: in order, its own share left out.
+        auto slot = [&](int v, int tile) { return (tile * (W - 1) + (v < tile % W ? v : v - 1)) * 64 + lane; };
+#pragma unroll
+        for (int q = 0; q < MT * NT; q++)
+            if (q % W != wave) sums[slot(wave, q)] = acc[q / NT][q % NT];
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < MT * NT; q++)
+            if (q % W == wave)
+#pragma unroll
+                for (int v = 0; v < W - 1; v++) acc[q / NT][q % NT] += sums[(q * (W - 1) + v) * 64 + lane];
+    }
+#pragma unroll
+    for (int q = 0; q < MT * NT; q++) {
+        if (W > 1 && q % W != wave) continue;
+        const int64_t n = (n0 + q % NT) * 16 + (lane & 15), t = (t0 + q / NT) * 16 + 4 * (lane >> 4);
+        if (n >= p.n) continue;
+        const float sw = gload(p.sw + n);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (t + e < p.t) finish(p, t + e, n, acc[q / NT][q % NT][e], gload(p.sx + t + e), sw);
+    }
+}
+
+// Large products: WM x WN waves of I x J 32x32 tiles each; a ring of four stages
+// of 64 values of both operands in LDS, filled by DMA three ahead.
+template <int WM, int WN, int I, int J>
+__global__ __launch_bounds__(WM *WN * 64, 2) void int8_ring_kernel(const Product p, int blocks_n, int blocks) {
+    constexpr int W = WM * WN, TM = WM * I * 2, TN = WN * J * 2, ROWS = TM + TN, EACH = ROWS / W, STAGES = 4;  // (16-row tiles)
+    static_assert(ROWS % W == 0, "whole tiles a wave");
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[STAGES * ROWS * 1024];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    // Each XCD takes tiles that follow one another, a few rows of channels at a
+    // time: its blocks in flight share both operands in its L2.
+    const int per = (blocks + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || id >= blocks) return;
+    constexpr int BAND = 4;  // channel tiles of a band
+    const int blocks_m = blocks / blocks_n, band = id / (BAND * blocks_m), in = id - band * BAND * blocks_m;
+    const int width = min(BAND, blocks_n - band * BAND);
+    const int bn = band * BAND + in % width, bm = in / width;
+    const int t0 = bm * TM, n0 = bn * TN;
+    const uint8_t *src[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        const int r = wave * EACH + e;
+        src[e] = r < TM ? p.x + (int64_t)min(t0 + r, p.tt - 1) * p.chunks * 1024
+                        : p.w + (int64_t)min(n0 + r - TM, p.nt - 1) * p.chunks * 1024;
+    }
+    const uint32_t base = lds::lds_addr(ring);
+    auto fetch = [&](int c) __attribute__((always_inline)) {
+        const uint32_t to = base + (c % STAGES) * (ROWS * 1024), from = (uint32_t)min(c, p.chunks - 1) * 1024 + lane * 16;
+#pragma unroll
+        for (int e = 0; e < EACH; e++) lds::dma16(src[e], from, to + (wave * EACH + e) * 1024);
+    };
+    i32x16 acc[I][J];
+#pragma unroll
+    for (int i = 0; i < I; i++)
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][j][e] = 0;
+    // Lane (row % 32, h) of a 32x32x32 operand: 16 values at 16 (2 half + h).
+    const int at = (lane >> 4 & 1) * 1024 + (lane >> 5) * 256 + (lane & 15) * 16;
+    fetch(0), fetch(1), fetch(2);
+    for (int c = 0; c < p.chunks; c++) {
+        lds::wait_vm_barrier<2 * EACH>();
+        fetch(c + 3);
+        const lds::lds_p stage = (lds::lds_p)(ring) + (c % STAGES) * (ROWS * 1024) + at;
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            i32x4 a[I], b[J];
+#pragma unroll
+            for (int i = 0; i < I; i++)
+                a[i] = *(const __attribute__((address_space(3))) i32x4 *)(stage + (wm * I + i) * 2048 + half * 512);
+#pragma unroll
+            for (int j = 0; j < J; j++)
+                b[j] = *(const __attribute__((address_space(3))) i32x4 *)(stage + TM * 1024 + (wn * J + j) * 2048 + half * 512);
+#pragma unroll
+            for (int i = 0; i < I; i++)
+#pragma unroll
+                for (int j = 0; j < J; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[j], acc[i][j], 0, 0, 0);
+        }
+    }
+    lds::wait_vm<0>();
+    // Lane (channel % 32, h): tokens 8 (e / 4) + 4 h + e % 4.
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+        const int64_t n = (int64_t)n0 * 16 + (wn * J + j) * 32 + (lane & 31);
+        if (n >= p.n) continue;
+        const float sw = gload(p.sw + n);
+#pragma unroll
+        for (int i = 0; i < I; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int64_t t = (int64_t)t0 * 16 + (wm * I + i) * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+                if (t < p.t) finish(p, t, n, acc[i][j][e], gload(p.sx + t), sw);
+            }
+    }
+}
+
+template <int MT, int NT, int W>
+void direct(const Product &p, hipStream_t s) {
+    hipLaunchKernelGGL((int8_direct_kernel<MT, NT, W>), dim3((p.nt + NT - 1) / NT, (p.tt + MT - 1) / MT), dim3(W * 64), 0, s, p);
+}
+template <int WM, int WN, int I, int J>
+void ring(const Product &p, hipStream_t s) {
+    const int m = (p.tt + WM * I * 2 - 1) / (WM * I * 2), n = (p.nt + WN * J * 2 - 1) / (WN * J * 2);
+    hipLaunchKernelGGL((int8_ring_kernel<WM, WN, I, J>), dim3((unsigned)((m * n + 7) / 8 * 8)), dim3(WM * WN * 64), 0, s, p, n, m * n);
+}
+
+void launch_product(const Product &p, hipStream_t s) {
+    const int64_t large = (int64_t)((p.tt + 15) / 16) * ((p.nt + 15) / 16), mid = (int64_t)((p.tt + 7) / 8) * ((p.nt + 7) / 8);
+    if (large >= 200) ring<2, 4, 4, 2>(p, s);
+    else if (mid >= 128) ring<2, 2, 2, 2>(p, s);
+    else if (p.tt == 1) direct<1, 1, 8>(p, s);
+    else direct<2, 2, 8>(p, s);
 }
 
 int sizes_ok(const char *what, int32_t n, int32_t k) {
@@ -193,10 +374,9 @@ int moe_int8_linear(const void *packed, int32_t n, int32_t k, const float *x, in
     const uint8_t *w = static_cast<const uint8_t *>(packed);
     uint8_t *xc = static_cast<uint8_t *>(workspace);
     float *sx = reinterpret_cast<float *>(xc + codes_bytes(t, k));
-    hipLaunchKernelGGL(int8_rows_kernel, dim3((unsigned)up(t, 16)), dim3(256), 0, s, x, x_stride, t, k, xc, sx);
-    const Product p{w, xc, reinterpret_cast<const float *>(w + codes_bytes(n, k)), sx, y, residual, y_stride, residual_stride, n, t,
-                    up(k, 64) / 64};
-    hipLaunchKernelGGL(int8_product_kernel, dim3((unsigned)(up(n, 64) / 64), (unsigned)(up(t, 16) / 16)), dim3(256), 0, s, p);
+    hipLaunchKernelGGL(int8_rows_kernel, dim3(row_blocks(t)), dim3(256), 0, s, x, x_stride, t, k, xc, sx);
+    launch_product(Product{w, xc, reinterpret_cast<const float *>(w + codes_bytes(n, k)), sx, y, residual, y_stride, residual_stride, n, t,
+                           (int)(up(k, 64) / 64), (n + 15) / 16, (t + 15) / 16}, s);
     return done("8-bit product kernel");
 }
 

@@ -26,7 +26,7 @@ int fail(int code, const char *fmt, ...);
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4_dw __attribute__((ext_vector_type(4), aligned(4)));  // at any float
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMostK = 131072;  // 127 * 127 * K stays below 2^31
@@ -149,6 +149,24 @@ __device__ inline void finish(const Product &p, int64_t t, int64_t n, int sum, f
     if (p.residual) gstore(p.residual + t * p.rs + n, gload(p.residual + t * p.rs + n) + v);
 }
 
+// y and residual of channels n .. n + 3 (as many as there are) of one token.
+__device__ inline void finish4(const Product &p, int64_t t, int64_t n, i32x4 sum, float sx, f32x4_dw sw) {
+    if (n + 4 > p.n) {
+        for (int e = 0; n + e < p.n; e++) finish(p, t, n + e, sum[e], sx, sw[e]);
+        return;
+    }
+    f32x4_dw v;
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = (float)sum[e] * (sx * sw[e]);
+    *(__attribute__((address_space(1))) f32x4_dw *)(p.y + t * p.ys + n) = v;
+    if (!p.residual) return;
+    __attribute__((address_space(1))) f32x4_dw *r = (__attribute__((address_space(1))) f32x4_dw *)(p.residual + t * p.rs + n);
+    f32x4_dw z = *r;
+#pragma unroll
+    for (int e = 0; e < 4; e++) z[e] += v[e];
+    *r = z;
+}
+
 // MT x NT tiles of 16 tokens by 16 channels a block, operands straight from
 // memory, the chunks of K dealt to W waves whose sums meet in LDS.
 template <int MT, int NT, int W>
@@ -214,24 +232,28 @@ __global__ __launch_bounds__(W * 64) void int8_direct_kernel(const Product p) {
     }
 }
 
-// Large products: WM x WN waves of I x J 32x32 tiles each; a ring of four stages
-// of 64 values of both operands in LDS, filled by DMA three ahead.
-template <int WM, int WN, int I, int J>
+// (The 16x16x64 instruction throughout: on random codes with every CU at work the
+// chip's power holds it to 3800 TOP/s, the 32x32x32 one to 2940, which made this
+// kernel's 256 x 256 tiles 219 us instead of 175 for 8191 x 6144 x 4096.)
+
+// Large products: WM x WN waves of I x J tiles of 16 tokens by 16 channels each;
+// a ring of STAGES stages of 64 values of both operands in LDS, filled by DMA
+// STAGES - 1 ahead.
+template <int WM, int WN, int I, int J, int STAGES>
 __global__ __launch_bounds__(WM *WN * 64, 2) void int8_ring_kernel(const Product p, int blocks_n, int blocks) {
-    constexpr int W = WM * WN, TM = WM * I * 2, TN = WN * J * 2, ROWS = TM + TN, EACH = ROWS / W, STAGES = 4;  // (16-row tiles)
-    static_assert(ROWS % W == 0, "whole tiles a wave");
+    constexpr int W = WM * WN, TM = WM * I, TN = WN * J, ROWS = TM + TN, EACH = ROWS / W;  // (16-row tiles)
+    static_assert(ROWS % W == 0 && I % 2 == 0, "whole tiles a wave");
     __shared__ __attribute__((aligned(1024))) uint8_t ring[STAGES * ROWS * 1024];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
-    // Each XCD takes tiles that follow one another, a few rows of channels at a
-    // time: its blocks in flight share both operands in its L2.
+    // Each XCD takes blocks that follow one another, a band of four channel
+    // blocks at a time: those in flight share both operands in its L2.
     const int per = (blocks + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per || id >= blocks) return;
-    constexpr int BAND = 4;  // channel tiles of a band
+    constexpr int BAND = 4;
     const int blocks_m = blocks / blocks_n, band = id / (BAND * blocks_m), in = id - band * BAND * blocks_m;
     const int width = min(BAND, blocks_n - band * BAND);
-    const int bn = band * BAND + in % width, bm = in / width;
-    const int t0 = bm * TM, n0 = bn * TN;
+    const int t0 = in / width * TM, n0 = (band * BAND + in % width) * TN;
     const uint8_t *src[EACH];
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
@@ -245,49 +267,63 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void int8_ring_kernel(const Product
 #pragma unroll
         for (int e = 0; e < EACH; e++) lds::dma16(src[e], from, to + (wave * EACH + e) * 1024);
     };
-    i32x16 acc[I][J];
+    const lds::lds_p mine = (lds::lds_p)(ring) + lane * 16;
+    auto tile = [&](int c, int t) __attribute__((always_inline)) {
+        return *(const __attribute__((address_space(3))) i32x4 *)(mine + ((c % STAGES) * ROWS + t) * 1024);
+    };
+    i32x4 acc[I][J];
 #pragma unroll
     for (int i = 0; i < I; i++)
 #pragma unroll
-        for (int j = 0; j < J; j++)
+        for (int j = 0; j < J; j++) acc[i][j] = i32x4{0, 0, 0, 0};
+    // A step's second half of tokens loads while the first is multiplied, the
+    // next step's first while the second is: that stage is whole when the step
+    // begins, so nothing waits behind the barrier.
+    i32x4 x0[I / 2], x1[I / 2], w[2][J];
+    auto first = [&](int c, i32x4 (&ww)[J]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int e = 0; e < 16; e++) acc[i][j][e] = 0;
-    // Lane (row % 32, h) of a 32x32x32 operand: 16 values at 16 (2 half + h).
-    const int at = (lane >> 4 & 1) * 1024 + (lane >> 5) * 256 + (lane & 15) * 16;
-    fetch(0), fetch(1), fetch(2);
-    for (int c = 0; c < p.chunks; c++) {
-        lds::wait_vm_barrier<2 * EACH>();
-        fetch(c + 3);
-        const lds::lds_p stage = (lds::lds_p)(ring) + (c % STAGES) * (ROWS * 1024) + at;
+        for (int j = 0; j < J; j++) ww[j] = tile(c, TM + wn * J + j);
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-            i32x4 a[I], b[J];
+        for (int i = 0; i < I / 2; i++) x0[i] = tile(c, wm * I + i);
+    };
+    auto step = [&](int c, i32x4 (&now)[J], i32x4 (&later)[J]) __attribute__((always_inline)) {
+        lds::wait_vm_barrier<(STAGES - 3) * EACH>();
+        fetch(c + STAGES - 1);
 #pragma unroll
-            for (int i = 0; i < I; i++)
-                a[i] = *(const __attribute__((address_space(3))) i32x4 *)(stage + (wm * I + i) * 2048 + half * 512);
+        for (int i = 0; i < I / 2; i++) x1[i] = tile(c, wm * I + I / 2 + i);
+#pragma unroll
+        for (int i = 0; i < I / 2; i++)
+#pragma unroll
+            for (int j = 0; j < J; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(now[j], x0[i], acc[i][j], 0, 0, 0);
+        first(c + 1, later);
+#pragma unroll
+        for (int i = 0; i < I / 2; i++)
 #pragma unroll
             for (int j = 0; j < J; j++)
-                b[j] = *(const __attribute__((address_space(3))) i32x4 *)(stage + TM * 1024 + (wn * J + j) * 2048 + half * 512);
+                acc[I / 2 + i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(now[j], x1[i], acc[I / 2 + i][j], 0, 0, 0);
+    };
 #pragma unroll
-            for (int i = 0; i < I; i++)
-#pragma unroll
-                for (int j = 0; j < J; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[j], acc[i][j], 0, 0, 0);
-        }
-    }
+    for (int c = 0; c < STAGES - 1; c++) fetch(c);
+    lds::wait_vm_barrier<(STAGES - 2) * EACH>();
+    first(0, w[0]);
+    int c = 0;
+    for (; c + 2 <= p.chunks; c += 2) step(c, w[0], w[1]), step(c + 1, w[1], w[0]);
+    if (c < p.chunks) step(c, w[0], w[1]);
     lds::wait_vm<0>();
-    // Lane (channel % 32, h): tokens 8 (e / 4) + 4 h + e % 4.
+    // Lane (token, g): channels 4 g .. 4 g + 3.
+    float sx[I];
+#pragma unroll
+    for (int i = 0; i < I; i++) sx[i] = gload(p.sx + (int64_t)min(t0 + wm * I + i, p.tt - 1) * 16 + (lane & 15));
 #pragma unroll
     for (int j = 0; j < J; j++) {
-        const int64_t n = (int64_t)n0 * 16 + (wn * J + j) * 32 + (lane & 31);
+        const int64_t n = (int64_t)(n0 + wn * J + j) * 16 + 4 * (lane >> 4);
         if (n >= p.n) continue;
-        const float sw = gload(p.sw + n);
+        const f32x4_dw sw = *(const __attribute__((address_space(1))) f32x4_dw *)(p.sw + n);
 #pragma unroll
-        for (int i = 0; i < I; i++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int64_t t = (int64_t)t0 * 16 + (wm * I + i) * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-                if (t < p.t) finish(p, t, n, acc[i][j][e], gload(p.sx + t), sw);
-            }
+        for (int i = 0; i < I; i++) {
+            const int64_t t = (int64_t)(t0 + wm * I + i) * 16 + (lane & 15);
+            if (t < p.t) finish4(p, t, n, acc[i][j], sx[i], sw);
+        }
     }
 }
 
@@ -295,18 +331,120 @@ template <int MT, int NT, int W>
 void direct(const Product &p, hipStream_t s) {
     hipLaunchKernelGGL((int8_direct_kernel<MT, NT, W>), dim3((p.nt + NT - 1) / NT, (p.tt + MT - 1) / MT), dim3(W * 64), 0, s, p);
 }
-template <int WM, int WN, int I, int J>
+template <int WM, int WN, int I, int J, int STAGES>
 void ring(const Product &p, hipStream_t s) {
-    const int m = (p.tt + WM * I * 2 - 1) / (WM * I * 2), n = (p.nt + WN * J * 2 - 1) / (WN * J * 2);
-    hipLaunchKernelGGL((int8_ring_kernel<WM, WN, I, J>), dim3((unsigned)((m * n + 7) / 8 * 8)), dim3(WM * WN * 64), 0, s, p, n, m * n);
+    const int m = (p.tt + WM * I - 1) / (WM * I), n = (p.nt + WN * J - 1) / (WN * J);
+    hipLaunchKernelGGL((int8_ring_kernel<WM, WN, I, J, STAGES>), dim3((unsigned)((m * n + 7) / 8 * 8)), dim3(WM * WN * 64), 0, s, p, n, m * n);
 }
 
+// A few rows (up to 16384 values in all): each block quantises them for itself,
+// under its first loads of weights, into LDS as [row][values]; lanes of rows past
+// the last hold zeros.  One row of 4096 x 4096 4.5 us (3.8 TB/s), against 6.6 with
+// the rows in a launch of their own; of 28672 x 4096 20 (5.8 TB/s); four rows 7.3
+// and 6.8, but a launch less to queue.
+constexpr int kFewBytes = 16384, kFewRows = 4;
+template <int W>
+__global__ __launch_bounds__(W * 64) void int8_few_kernel(const Product p, const float *x, int64_t xs, int k) {
+    __shared__ uint32_t codes[kFewBytes / 4], red[W];
+    __shared__ i32x4 sums[(W - 1) * 64];
+    __shared__ float scale[kFewRows];
+    constexpr int U = 8, T = W * 64;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int width = p.chunks * 64, row = lane & 15, g = lane >> 4;
+    const u32x4 *w = (const u32x4 *)(p.w + (int64_t)blockIdx.x * p.chunks * 1024) + lane;
+    i32x4 b[U];
+    auto load = [&](int c0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; u++) b[u] = __builtin_bit_cast(i32x4, gload(w + 64 * min(c0 + u * W, p.chunks - 1)));
+    };
+    load(wave);
+    for (int t = 0; t < p.t; t++) {
+        const float *src = x + t * xs;
+        float held[4][4];
+        uint32_t top = 0;
+        auto values = [&](int i, float (&v)[4]) __attribute__((always_inline)) {
+            if (i + 4 <= k) {
+                const u32x4_dw y = gload_x4((const uint32_t *)src + i);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = __uint_as_float(y[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = i + e < k ? gload(src + i + e) : 0.0f;
+            }
+        };
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int i = 4 * (threadIdx.x + T * j);
+            if (i < width) values(i, held[j]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) top = i < width ? max(top, magnitude(held[j][e])) : top;
+        }
+        for (int i = 4 * (threadIdx.x + T * 4); i < width; i += 4 * T) {
+            float v[4];
+            values(i, v);
+#pragma unroll
+            for (int e = 0; e < 4; e++) top = max(top, magnitude(v[e]));
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+        __syncthreads();
+        if (lane == 0) red[wave] = top;
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < W; v++) top = max(top, red[v]);
+        const Int8Scale s(top);
+        if (threadIdx.x == 0) scale[t] = s.scale;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int i = 4 * (threadIdx.x + T * j);
+            if (i < width) codes[(t * width + i) / 4] = pack4(s.code(held[j][0]), s.code(held[j][1]), s.code(held[j][2]), s.code(held[j][3]));
+        }
+        for (int i = 4 * (threadIdx.x + T * 4); i < width; i += 4 * T) {
+            float v[4];
+            values(i, v);
+            codes[(t * width + i) / 4] = pack4(s.code(v[0]), s.code(v[1]), s.code(v[2]), s.code(v[3]));
+        }
+    }
+    __syncthreads();
+    i32x4 acc = {0, 0, 0, 0};
+    for (int c0 = wave; c0 < p.chunks; c0 += W * U) {
+        if (c0 != wave) load(c0);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int c = c0 + u * W;
+            if (c >= p.chunks) continue;
+            const i32x4 y = *(const i32x4 *)&codes[(min(row, p.t - 1) * width + c * 64 + g * 16) / 4];
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[u], row < p.t ? y : i32x4{0, 0, 0, 0}, acc, 0, 0, 0);
+        }
+    }
+    if (wave) sums[(wave - 1) * 64 + lane] = acc;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int v = 0; v < W - 1; v++) acc += sums[v * 64 + lane];
+    const int64_t n = (int64_t)blockIdx.x * 16 + 4 * g;
+    if (row < p.t && n < p.n) finish4(p, row, n, acc, scale[row], *(const __attribute__((address_space(1))) f32x4_dw *)(p.sw + n));
+}
+
+// Blocks by what fills the chip (time of the product alone, us, K = 4096 or 2048
+// where n = 1024):
+//   direct, 16 x 16 (tokens x channels) for 16 rows; 32 x 32 up to 256 blocks,
+//   then 32 x 64 up to 512 (48 x 6144: 7.5 and 6.5; 256 x 1024: 4.2 and 4.7;
+//   160 x 6144: 16.4 and 10.6, ring of 64 x 128 15.9);
+//   ring, 64 x 128 below 256 blocks of 128 x 128 (512 x 6144: 22.6 and 24.3, 32 x
+//   64 27.8; 768 x 6144: 34.1 and 31.7);
+//   ring, 256 x 256 where its rounds of 256 blocks are at least 5/6 full (2048 x
+//   4096, half a round: 49.5 and 36.7 with 128 x 128; 4096 x 4096: 61 and 74; 8191
+//   x 6144, three rounds: 175 and 208).
 void launch_product(const Product &p, hipStream_t s) {
-    const int64_t large = (int64_t)((p.tt + 15) / 16) * ((p.nt + 15) / 16), mid = (int64_t)((p.tt + 7) / 8) * ((p.nt + 7) / 8);
-    if (large >= 200) ring<2, 4, 4, 2>(p, s);
-    else if (mid >= 128) ring<2, 2, 2, 2>(p, s);
-    else if (p.tt == 1) direct<1, 1, 8>(p, s);
-    else direct<2, 2, 8>(p, s);
+    auto blocks = [&](int64_t m, int64_t n) { return (p.tt + m - 1) / m * ((p.nt + n - 1) / n); };
+    const int64_t large = blocks(16, 16), rounds = (large + 255) / 256;
+    if (p.tt == 1) direct<1, 1, 8>(p, s);
+    else if (blocks(2, 2) <= 256) direct<2, 2, 8>(p, s);
+    else if (blocks(2, 4) <= 512) direct<2, 4, 8>(p, s);
+    else if (large * 6 >= rounds * 256 * 5) ring<4, 2, 4, 8, 4>(p, s);
+    else if (blocks(8, 8) >= 256) ring<2, 2, 4, 4, 5>(p, s);
+    else ring<2, 2, 2, 4, 6>(p, s);
 }
 
 int sizes_ok(const char *what, int32_t n, int32_t k) {
@@ -374,9 +512,14 @@ int moe_int8_linear(const void *packed, int32_t n, int32_t k, const float *x, in
     const uint8_t *w = static_cast<const uint8_t *>(packed);
     uint8_t *xc = static_cast<uint8_t *>(workspace);
     float *sx = reinterpret_cast<float *>(xc + codes_bytes(t, k));
+    const Product p{w, xc, reinterpret_cast<const float *>(w + codes_bytes(n, k)), sx, y, residual, y_stride, residual_stride, n, t,
+                    (int)(up(k, 64) / 64), (n + 15) / 16, (t + 15) / 16};
+    if (t <= kFewRows && t * up(k, 64) <= kFewBytes) {
+        hipLaunchKernelGGL((int8_few_kernel<8>), dim3(p.nt), dim3(512), 0, s, p, x, x_stride, k);
+        return done("8-bit product kernel");
+    }
     hipLaunchKernelGGL(int8_rows_kernel, dim3(row_blocks(t)), dim3(256), 0, s, x, x_stride, t, k, xc, sx);
-    launch_product(Product{w, xc, reinterpret_cast<const float *>(w + codes_bytes(n, k)), sx, y, residual, y_stride, residual_stride, n, t,
-                           (int)(up(k, 64) / 64), (n + 15) / 16, (t + 15) / 16}, s);
+    launch_product(p, s);
     return done("8-bit product kernel");
 }
 

@@ -553,7 +553,7 @@ int moe_kv8_sizes(const moe_kv8 *c, uint64_t *codes, uint64_t *scales, uint64_t 
  * n_seq - 1 or whose position is negative are skipped.  Where a sequence goes
  * on behind a block that `open` does not hold (its caller took it back to an
  * earlier position), that block's earlier positions are taken as they read.
- * The same step made again writes the same.  At most 2^24 - 256 rows (also
+ * The same step made again writes the same.  At most 2^24 - 512 rows (also
  * moe_kv8_load's). */
 int moe_kv8_store(const moe_kv8 *c, const float *k, int64_t k_stride, const float *v, int64_t v_stride, int32_t rows,
                   const int32_t *row_start, const int32_t *seq, const int32_t *pos, const int64_t *slots, void *stream);

@@ -512,6 +512,9 @@ int moe_int8_linear(const void *packed, int32_t n, int32_t k, const float *x, in
     const uint8_t *w = static_cast<const uint8_t *>(packed);
     uint8_t *xc = static_cast<uint8_t *>(workspace);
     float *sx = reinterpret_cast<float *>(xc + codes_bytes(t, k));
+    // (blocks of 128 x 64 at least, 512 threads at most)
+    if (up(t, 128) / 128 * (up(n, 64) / 64) * 512 > 0xffffffffll)
+        return fail(MOE_EUNSUP, "moe_int8_linear: %d tokens of %d channels are too many blocks", t, n);
     const Product p{w, xc, reinterpret_cast<const float *>(w + codes_bytes(n, k)), sx, y, residual, y_stride, residual_stride, n, t,
                     (int)(up(k, 64) / 64), (n + 15) / 16, (t + 15) / 16};
     if (t <= kFewRows && t * up(k, 64) <= kFewBytes) {

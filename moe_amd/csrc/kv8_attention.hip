@@ -446,14 +446,127 @@ __device__ __attribute__((always_inline)) inline void narrow(const Args &a, Narr
     }
 }
 
-template <int NQ, int NV, bool EX>
+// What a block of 64 columns shares: two steps of NT tiles (the queries' digits
+// before the first).
+template <int NQ, int NV, int NT>
+struct Wide {
+    static constexpr int kTile = 64 * (64 * NQ + 16 * NV);  // (or the most there may be)
+    union {
+        uint8_t tiles[2][NT * kTile];
+        u32x4 sq[4 * 3 * NQ * 64];
+    };
+    float scales[2][NT * 8], sk[64];
+};
+
+// 64 columns of one run, 16 a wave; every wave goes over all tiles, which come
+// through LDS by DMA, a step ahead.
+template <int NQ, int NV, int NT, bool EX>
+__device__ __attribute__((always_inline)) inline void wide(const Args &a, Wide<NQ, NV, NT> &lds_, int kv, int r0, int nr, int h0, int hn,
+                                                           int my_seq, int my_pos, const Runs &runs) {
+    const Kv8 &c = a.c;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+    const int nq = EX ? NQ : (c.qd + 63) / 64, nv = EX ? NV : c.vd / 16, qd = EX ? 64 * NQ : c.qd;
+    const int bytes = EX ? Wide<NQ, NV, NT>::kTile : c.tile_bytes();
+    unsigned long long starts = runs.starts;
+    Run run;
+    next_run(runs, starts, nr, my_seq, my_pos, a.window, run);
+    const int c0 = run.first * hn, ncol = (run.end - run.first) * hn;
+    stage_queries<NQ, 64>(a, lds_.sq, lds_.sk, r0, h0, hn, c0, c0 + ncol);
+    __syncthreads();
+    Columns<NV> x;
+    i32x4 q[3][NQ];
+    const int mine = wave * 16 + col, own = c0 + min(mine, ncol - 1);
+    begin<NQ, NV>(x, q, lds_.sq + wave * 3 * NQ * 64, lds_.sk + wave * 16, my_pos, a.window, own / hn);
+    // What any column of the wave sees.
+    int lo = x.lo, hi = x.pos;
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) {
+        lo = min(lo, __shfl_xor(lo, o, 64));
+        hi = max(hi, __shfl_xor(hi, o, 64));
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
+    const int32_t *table = c.table + (int64_t)run.seq * c.max_pages;
+    const int t0 = run.lo >> 6, t1 = (run.hi >> 6) + 1;
+    Pages pages;
+    const uint32_t to = lds::lds_addr(lds_.tiles[0]), to_scales = lds::lds_addr(lds_.scales[0]);
+    // Queue a step's loads; which of its tiles there are.
+    auto fetch = [&](int t, int buffer) __attribute__((always_inline)) {
+        int there = 0;
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+            const int64_t tile = t + i < t1 ? pages.tile(c, table, kv, t + i) : -1;
+            if (tile < 0) continue;
+            there |= 1 << i;
+            const uint8_t *src = c.at(tile);
+            const uint32_t dst = to + buffer * (uint32_t)sizeof(lds_.tiles[0]) + i * bytes;
+            for (int k = wave; k < bytes / 1024; k += 4) lds::dma16(src + k * 1024, lane * 16, dst + k * 1024);
+            if (wave == i % 4 && lane < 8) lds::dma4(c.scales + tile * 8, lane * 4, to_scales + buffer * (uint32_t)sizeof(lds_.scales[0]) + i * 32);
+        }
+        return there;
+    };
+    __syncthreads();  // the queries are read
+    int now = fetch(t0, 0);
+    for (int t = t0, buffer = 0; t < t1; t += NT, buffer ^= 1) {
+        lds::wait_vm_barrier<0>();
+        const int later = t + NT < t1 ? fetch(t + NT, buffer ^ 1) : 0;
+        if (t * 64 <= hi && (t + NT) * 64 > lo) {
+            float ks[4 * NT], vs[4 * NT];
+            int base[NT];
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                const bool ok = now >> i & 1;
+                base[i] = ok ? (t + i) * 64 : -64;
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    const float kk = lds_.scales[buffer][i * 8 + b], vv = lds_.scales[buffer][i * 8 + 4 + b];
+                    ks[4 * i + b] = ok ? kk : 0.0f, vs[4 * i + b] = ok ? vv : 0.0f;
+                }
+            }
+            const lds::lds_p at = (lds::lds_p)lds_.tiles[buffer] + lane * 16;
+            step<NQ, NV, NT, EX>(
+                x, q,
+                [&](int b, int cc) __attribute__((always_inline)) {
+                    return *(const __attribute__((address_space(3))) i32x4 *)(at + (b >> 2) * bytes + (b & 3) * 16 * qd + cc * 1024);
+                },
+                [&](int D, int i) __attribute__((always_inline)) {
+                    return *(const __attribute__((address_space(3))) i32x4 *)(at + i * bytes + 64 * qd + D * 1024);
+                },
+                ks, vs, base, nq, nv, g);
+        }
+        now = later;
+    }
+    x.l += __shfl_xor(x.l, 16, 64);
+    x.l += __shfl_xor(x.l, 32, 64);
+    if (mine >= ncol) return;
+    const float by = x.l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x.R - x.m) / x.l;
+    float *dst = a.out + (int64_t)(r0 + own / hn) * a.out_stride + (int64_t)(h0 + own % hn) * c.vd + 4 * g;
+#pragma unroll
+    for (int D = 0; D < NV; D++) {
+        if (!EX && D >= nv) continue;
+        f32x4_dw z;
+#pragma unroll
+        for (int e = 0; e < 4; e++) z[e] = x.o[D][e] * by;
+        *(__attribute__((address_space(1))) f32x4_dw *)(dst + 16 * D) = z;
+    }
+}
+
+// NT tiles a step for groups of 64 columns; 0: groups of 16 only.  Blocks of 64
+// columns pay where one run fills them: a group with several runs (sequences that
+// decode, ends of prompts), or with no more than 16 columns, is dealt to its blocks
+// in groups of 16 instead.
+template <int NQ, int NV, bool EX, int NT>
 __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(const Args a) {
-    __shared__ Narrow<NQ, NV> lds;
+    union Both {
+        Narrow<NQ, NV> narrow;
+        Wide<NQ, NV, NT ? NT : 1> wide;
+    };
+    __shared__ std::conditional_t<NT != 0, Both, Narrow<NQ, NV>> lds;
     const Kv8 &c = a.c;
     const int lane = threadIdx.x & 63;
     // Kv heads next to each other go to the XCDs in turn, so that one head's
     // blocks find its tiles in their L2.  Later rows of a prompt see more
-    // positions: the last groups go first.
+    // positions: the last groups go first.  A group's blocks that find no run of
+    // their own leave at once, so the first ones come together.
     int id = blockIdx.x;
     const int kv = id % c.n_kv;
     id /= c.n_kv;
@@ -466,7 +579,21 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(const Args a) {
     const int nr = min(a.tt, a.rows - r0);
     const int h0 = kv * a.rep + chunk * a.rc, hn = min(a.rc, a.rep - chunk * a.rc);
     const int my_seq = gload(a.seq + r0 + min(lane, nr - 1)), my_pos = gload(a.pos + r0 + min(lane, nr - 1));
-    narrow<NQ, NV, EX>(a, lds, kv, part, r0, nr, h0, hn, my_seq, my_pos, sub, a.split);
+    if constexpr (NT == 0) {
+        narrow<NQ, NV, EX>(a, lds, kv, part, r0, nr, h0, hn, my_seq, my_pos, sub, a.split);
+    } else {
+        const Runs runs = runs_of(c, my_seq, my_pos, nr);
+        if (__popcll(runs.starts) == 1 && __popcll(runs.valid) * hn > 16) {
+            if (sub == 0) wide<NQ, NV, NT, EX>(a, lds.wide, kv, r0, nr, h0, hn, my_seq, my_pos, runs);
+            return;
+        }
+        const int chunks = (hn + 15) / 16, rc = min(hn, 16), tt = 16 / rc;
+        const int r1 = sub / chunks * tt, h1 = sub % chunks * 16;
+        if (r1 >= nr) return;
+        const int n1 = min(tt, nr - r1), from = r1 + min(lane, n1 - 1);
+        narrow<NQ, NV, EX>(a, lds.narrow, kv, 0, r0 + r1, n1, h0 + h1, min(rc, hn - h1), __shfl(my_seq, from, 64), __shfl(my_pos, from, 64),
+                           0, 1);
+    }
 }
 
 // The parts of rows whose tiles several blocks shared: a block of T threads
@@ -519,24 +646,29 @@ __global__ __launch_bounds__(T) void kv8_join_kernel(const Args a) {
 
 // How a call is cut up: see Args.
 struct Plan {
-    int rc, chunks, tt, groups, split, ps;
+    int cols, rc, chunks, tt, groups, split, ps;  // cols: columns of a block
     uint64_t bytes;
 };
 
 Plan plan_of(const Kv8 &c, int rows, int heads, int max_pos, int window) {
     Plan p{};
     const int rep = heads / c.n_kv;
-    p.rc = std::min(rep, 16);
+    const long long wide = ((long long)rows * rep + 63) / 64 * c.n_kv;
+    p.cols = c.qd <= 192 && c.vd <= 128 && wide >= 512 ? 64 : 16;
+    p.rc = std::min(rep, p.cols);
     p.chunks = (rep + p.rc - 1) / p.rc;
-    p.tt = 16 / p.rc;
+    p.tt = p.cols / p.rc;
     p.groups = (int)(((long long)rows + p.tt - 1) / p.tt);
     const long long base = (long long)p.groups * p.chunks * c.n_kv;
-    p.split = (int)std::max<long long>(1, std::min<long long>(p.tt, 1024 / base));
+    const int narrow = std::min(p.rc, 16);  // query heads of a group of 16 columns
+    p.split = p.cols == 64 ? (p.tt + 16 / narrow - 1) / (16 / narrow) * ((p.rc + 15) / 16)
+                           : (int)std::max<long long>(1, std::min<long long>(p.tt, 1024 / base));
     const long long tiles = (window > 0 ? std::min((long long)window + p.tt, (long long)max_pos + 1) : max_pos + 1LL) / 64 + 1;
     const long long units = base * p.split;
-    const long long ps = units >= 256 ? std::min((512 + units - 1) / units, tiles / 32)
-                         : tiles < 24 ? 1
-                                      : std::min<long long>({(1024 + units - 1) / units, tiles / 6, 256});
+    const long long ps = p.cols == 64   ? 1
+                         : units >= 256 ? std::min((512 + units - 1) / units, tiles / 32)
+                         : tiles < 24   ? 1
+                                        : std::min<long long>({(1024 + units - 1) / units, tiles / 6, 256});
     p.ps = (int)std::max<long long>(1, ps);
     p.bytes = p.ps > 1 ? (uint64_t)rows * heads * p.ps * (c.vd + 3) * 4 : 0;
     return p;
@@ -544,10 +676,14 @@ Plan plan_of(const Kv8 &c, int rows, int heads, int max_pos, int window) {
 
 constexpr long long kMostThreads = 0xffffffffll;  // of a launch
 
-template <int NQ, int NV, bool EX>
+template <int NQ, int NV, bool EX, int NT>
 void launch(const Args &a, hipStream_t s) {
     const long long blocks = (long long)a.groups * a.split * a.ps * a.chunks * a.c.n_kv;
-    hipLaunchKernelGGL((kv8_attention_kernel<NQ, NV, EX>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((kv8_attention_kernel<NQ, NV, EX, NT>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+}
+template <int NQ, int NV, bool EX, int NT>
+void launch(const Args &a, bool wide, hipStream_t s) {
+    wide ? launch<NQ, NV, EX, NT>(a, s) : launch<NQ, NV, EX, 0>(a, s);
 }
 
 }  // namespace
@@ -593,12 +729,13 @@ int moe_kv8_attention(const moe_kv8 *c, const float *q, int64_t q_stride, int32_
     const int qd = a.c.qd, vd = a.c.vd;
     // Widths of their own: a power-of-two head and the latent cache's 192/128;
     // the others count their operands at run time.
-    if (qd == 64 && vd == 64) launch<1, 4, true>(a, s);
-    else if (qd == 128 && vd == 128) launch<2, 8, true>(a, s);
-    else if (qd == 192 && vd == 128) launch<3, 8, true>(a, s);
-    else if (qd <= 192 && vd <= 128) launch<3, 8, false>(a, s);
-    else if (qd == 256 && vd == 256) launch<4, 16, true>(a, s);
-    else launch<4, 16, false>(a, s);
+    const bool wide = p.cols == 64;
+    if (qd == 64 && vd == 64) launch<1, 4, true, 4>(a, wide, s);
+    else if (qd == 128 && vd == 128) launch<2, 8, true, 2>(a, wide, s);
+    else if (qd == 192 && vd == 128) launch<3, 8, true, 1>(a, wide, s);
+    else if (qd <= 192 && vd <= 128) launch<3, 8, false, 1>(a, wide, s);
+    else if (qd == 256 && vd == 256) launch<4, 16, true, 0>(a, s);
+    else launch<4, 16, false, 0>(a, s);
     if (a.ps > 16) hipLaunchKernelGGL((kv8_join_kernel<256>), dim3((unsigned)rows * heads), dim3(256), 0, s, a);
     else if (a.ps > 1) hipLaunchKernelGGL((kv8_join_kernel<64>), dim3((unsigned)rows * heads), dim3(64), 0, s, a);
     const hipError_t e = hipGetLastError();

@@ -21,7 +21,19 @@
 // 2^23 + 0x8080 in one instruction, a weight's bits are its three digits (the
 // two low ones with 128 added).  A step's sums are whole numbers too; they join
 // the f32 sums O, which have a reference of their own (R, as r; the weights' sum
-// has m).
+// has m).  Sums that stayed whole numbers over many steps would need references
+// with room above them: three bits of it cost a digit's eighth (1e-5 of the output
+// against 1e-6) and still had to move for one wave of a block in every second step.
+//
+// Decode reads the cache once and is bound by that: 64 sequences of 6000 to 12000
+// positions, 8 kv heads of 128, 235 us (5.0 TB/s of codes), one of 100001 in 128
+// parts 41 with the joining launch, 32 of up to 1500 20 (3.8 TB/s: one block a CU
+// with 12 to 24 tiles, then a merge).  Prompts are bound by the issue of vector
+// instructions: 4001 rows of 32 heads of 128 270 us (485 TFLOP/s of the attention's
+// own operations), 8000 rows 950 (550), of which the matrix pipe is busy in 29% and
+// vector instructions issue in 72% (24 to a product: joining a block's three sums 5,
+// the exponential 2, a weight's digits 3, a step's sums into O 5 for two tiles).
+// Two tiles' products a step halve that last part.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -62,6 +74,10 @@ constexpr float kLeastLog = -100.0f;     // log2 of a value scale, where it is s
 
 __device__ inline i32x4 mfma(i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
+// log2 of the product of a weight of score z and a value scale, not below it:
+// what large scores' sums round off is added.
+__device__ inline float product_log(float z, float scale) { return fmaf(fabsf(z), 0x1p-21f, z + scale); }
+
 // The largest of a column's four lanes (16 apart), in each of them.
 __device__ inline float column_max(float x) {
     const uint32_t u = __float_as_uint(x);
@@ -94,43 +110,42 @@ struct Columns {
     int first, last;    // of all columns: everything in first .. last is seen by every one
 };
 
-// One step of NT tiles: k(T, c) and v(D, t) give operands, ks and vs the blocks'
-// scales, base[t] the tiles' first positions (negative: no such tile, whose
-// scales are 0).
+// One step of NT tiles: k(b, c) and v(D, t) give operands, base[t] the tiles'
+// first positions (negative: no such tile).  Lane 8 t + b holds the scale of tile
+// t's block b of keys, lane 8 t + 4 + b that of its values (0 where there is no
+// tile): uniform values go through scalar registers.
 template <int NQ, int NV, int NT, bool EX, class K, class V>
-__device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const i32x4 (&q)[3][NQ], K k, V v, float (&ks)[4 * NT],
-                                                           float (&vs)[4 * NT], const int (&base)[NT], int nq, int nv, int g) {
+__device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const i32x4 (&q)[3][NQ], K k, V v, float scale,
+                                                           const int (&base)[NT], int nv, int g) {
     f32x4 s[4 * NT];
 #pragma unroll
     for (int b = 0; b < 4 * NT; b++) {
-        i32x4 kk[NQ], hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
-#pragma unroll
-        for (int c = 0; c < NQ; c++) kk[c] = k(b, c);
+        const i32x4 zero = {0, 0, 0, 0};
+        i32x4 d[3] = {zero, zero, zero};
 #pragma unroll
         for (int c = 0; c < NQ; c++) {
-            lo = mfma(kk[c], q[1][c], lo);
-            hi = mfma(kk[c], q[0][c], hi);
+            const i32x4 kk = k(b, c);
+#pragma unroll
+            for (int p = 0; p < 3; p++) d[p] = mfma(kk, q[p][c], d[p]);
         }
-        lo = lo << 8;
 #pragma unroll
-        for (int c = 0; c < NQ; c++) lo = mfma(kk[c], q[2][c], lo);
-#pragma unroll
-        for (int i = 0; i < 4; i++) s[b][i] = fmaf((float)hi[i], 65536.0f, (float)lo[i]);
+        for (int i = 0; i < 4; i++) s[b][i] = fmaf((float)d[0][i], 65536.0f, (float)((d[1][i] << 8) + d[2][i]));
     }
-    float all = 0.0f, sc[4 * NT];
-#pragma unroll
-    for (int b = 0; b < 4 * NT; b++) all += fabsf(ks[b]) + fabsf(vs[b]);
-    if (__builtin_expect(!(all < INFINITY), 0)) {  // a block that reads as NaN: so are the columns that see it
-#pragma unroll
+    const int lane = threadIdx.x & 63;
+    if (__builtin_expect(__any(!(fabsf(scale) < INFINITY)), 0)) {  // a block that reads as NaN: so are the columns that see it
         for (int b = 0; b < 4 * NT; b++) {
-            const int p = base[b / 4] + 16 * (b % 4);
-            if (fabsf(ks[b]) < INFINITY && fabsf(vs[b]) < INFINITY) continue;
-            if (base[b / 4] >= 0 && p <= x.pos && p + 15 >= x.lo) x.l = __uint_as_float(0x7fc00000u);
-            ks[b] = vs[b] = 0.0f;
+            const int at = b / 4 * 8 + b % 4;
+            if (fabsf(__shfl(scale, at, 64)) < INFINITY && fabsf(__shfl(scale, at + 4, 64)) < INFINITY) continue;
+            const int p = (b < 4 ? base[0] : base[NT - 1]) + 16 * (b % 4);
+            if (p <= x.pos && p + 15 >= x.lo) x.l = __uint_as_float(0x7fc00000u);
+            if (lane == at || lane == at + 4) scale = 0.0f;
         }
     }
+    const float log_ = fmaxf(__builtin_amdgcn_logf(scale), kLeastLog);
+    auto of = [&](float y, int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(y), i)); };
+    float sc[4 * NT];
 #pragma unroll
-    for (int b = 0; b < 4 * NT; b++) sc[b] = ks[b] * x.qs;
+    for (int b = 0; b < 4 * NT; b++) sc[b] = of(scale, b / 4 * 8 + b % 4) * x.qs;
     bool whole = true;
 #pragma unroll
     for (int t = 0; t < NT; t++) whole = whole && base[t] >= x.first && base[t] + 63 <= x.last;
@@ -147,9 +162,8 @@ __device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const
     float top = kNone, ref = kNone;
 #pragma unroll
     for (int b = 0; b < 4 * NT; b++) {
-        const float t = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])) * sc[b];
-        top = fmaxf(top, t);
-        ref = fmaxf(ref, t + fmaxf(__builtin_amdgcn_logf(vs[b]), kLeastLog));
+        const float z = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])) * sc[b];
+        top = fmaxf(top, z), ref = fmaxf(ref, product_log(z, of(log_, b / 4 * 8 + 4 + b % 4)));
     }
     top = column_max(top), ref = column_max(ref);
     const float f = __builtin_amdgcn_exp2f(top - ref) * kMost;
@@ -157,7 +171,7 @@ __device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const
     i32x4 w[NT][3];
 #pragma unroll
     for (int b = 0; b < 4 * NT; b++) {
-        const float scaled = fminf(vs[b] * f, 3e38f);  // (p is 0 where it would be more)
+        const float scaled = fminf(of(scale, b / 4 * 8 + 4 + b % 4) * f, 3e38f);  // (p is 0 where it would be more)
         uint32_t y[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -170,25 +184,29 @@ __device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const
     }
     const float m = fmaxf(x.m, top), R = fmaxf(x.R, ref);
     x.l = x.l * __builtin_amdgcn_exp2f(x.m - m) + sum * __builtin_amdgcn_exp2f(top - m);
-    const float keep = __builtin_amdgcn_exp2f(x.R - R), join = __builtin_amdgcn_exp2f(ref - R) * (1.0f / kMost);
+    if (__any(R > x.R)) {
+        const float keep = __builtin_amdgcn_exp2f(x.R - R);
+#pragma unroll
+        for (int D = 0; D < NV; D++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) x.o[D][i] *= keep;
+    }
+    const float in0 = __builtin_amdgcn_exp2f(ref - R) * (1.0f / kMost), in2 = in0 * 65536.0f;
     x.m = m, x.R = R;
 #pragma unroll
     for (int D = 0; D < NV; D++) {
         if (!EX && D >= nv) continue;
-        i32x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0}, vv[NT];
-#pragma unroll
-        for (int t = 0; t < NT; t++) vv[t] = v(D, t);
+        const i32x4 zero = {0, 0, 0, 0};
+        i32x4 d[3] = {zero, zero, zero};
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            lo = mfma(vv[t], w[t][1], lo);
-            hi = mfma(vv[t], w[t][0], hi);
-        }
-        lo = lo << 8;
+            const i32x4 vv = v(D, t);
 #pragma unroll
-        for (int t = 0; t < NT; t++) lo = mfma(vv[t], w[t][2], lo);
+            for (int p = 0; p < 3; p++) d[p] = mfma(vv, w[t][p], d[p]);
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            x.o[D][i] = fmaf(fmaf((float)hi[i], 65536.0f, (float)lo[i]), join, x.o[D][i] * keep);
+            x.o[D][i] = fmaf((float)d[0][i], in2, fmaf((float)((d[1][i] << 8) + d[2][i]), in0, x.o[D][i]));
     }
 }
 
@@ -346,7 +364,7 @@ __device__ __attribute__((always_inline)) inline void narrow(const Args &a, Narr
                                                              int hn, int my_seq, int my_pos, int sub, int split) {
     const Kv8 &c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    const int nq = EX ? NQ : (c.qd + 63) / 64, nv = EX ? NV : c.vd / 16, qd = EX ? 64 * NQ : c.qd;
+    const int nv = EX ? NV : c.vd / 16, qd = EX ? 64 * NQ : c.qd;
     stage_queries<NQ, 16>(a, lds.sq, lds.sk, r0, h0, hn, 0, nr * hn);
     __syncthreads();
     const Runs runs = runs_of(c, my_seq, my_pos, nr);
@@ -366,7 +384,7 @@ __device__ __attribute__((always_inline)) inline void narrow(const Args &a, Narr
         const int t1 = t0 + (int)((long long)nt * (me + 1) / parts);
         Pages pages;
         i32x4 k[4][NQ], v[NV];
-        f32x4 ks, vs;
+        float scale;
         int base[1];
         __amdgpu_buffer_rsrc_t buf;
         // Loads are unconditional, so that waiting for one tile's keys leaves the
@@ -376,8 +394,7 @@ __device__ __attribute__((always_inline)) inline void narrow(const Args &a, Narr
             base[0] = tile < 0 ? -64 : at * 64;
             buf = buffer_of(tile < 0 ? c.codes : c.at(tile), tile < 0 ? 0 : c.tile_bytes());
             const __amdgpu_buffer_rsrc_t sb = buffer_of(tile < 0 ? (const void *)c.scales : c.scales + tile * 8, tile < 0 ? 0 : 32);
-            ks = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sb, 0, 0, 0));
-            vs = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sb, 16, 0, 0));
+            scale = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sb, 4 * (lane & 7), 0, 0));
 #pragma unroll
             for (int T = 0; T < 4; T++)
 #pragma unroll
@@ -394,9 +411,8 @@ __device__ __attribute__((always_inline)) inline void narrow(const Args &a, Narr
             load_values();
         }
         for (; t < t1; t++) {
-            float kb[4] = {ks[0], ks[1], ks[2], ks[3]}, vb[4] = {vs[0], vs[1], vs[2], vs[3]};
             if (base[0] >= 0)
-                step<NQ, NV, 1, EX>(x, q, [&](int b, int cc) { return k[b][cc]; }, [&](int D, int) { return v[D]; }, kb, vb, base, nq, nv, g);
+                step<NQ, NV, 1, EX>(x, q, [&](int b, int cc) { return k[b][cc]; }, [&](int D, int) { return v[D]; }, scale, base, nv, g);
             load_keys(t + 1);
             load_values();
         }
@@ -450,7 +466,7 @@ __device__ __attribute__((always_inline)) inline void narrow(const Args &a, Narr
 // before the first).
 template <int NQ, int NV, int NT>
 struct Wide {
-    static constexpr int kTile = 64 * (64 * NQ + 16 * NV);  // (or the most there may be)
+    static constexpr int kTile = 64 * (64 * NQ + 16 * NV);
     union {
         uint8_t tiles[2][NT * kTile];
         u32x4 sq[4 * 3 * NQ * 64];
@@ -460,13 +476,12 @@ struct Wide {
 
 // 64 columns of one run, 16 a wave; every wave goes over all tiles, which come
 // through LDS by DMA, a step ahead.
-template <int NQ, int NV, int NT, bool EX>
+template <int NQ, int NV, int NT>
 __device__ __attribute__((always_inline)) inline void wide(const Args &a, Wide<NQ, NV, NT> &lds_, int kv, int r0, int nr, int h0, int hn,
                                                            int my_seq, int my_pos, const Runs &runs) {
     const Kv8 &c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-    const int nq = EX ? NQ : (c.qd + 63) / 64, nv = EX ? NV : c.vd / 16, qd = EX ? 64 * NQ : c.qd;
-    const int bytes = EX ? Wide<NQ, NV, NT>::kTile : c.tile_bytes();
+    constexpr int qd = 64 * NQ, bytes = Wide<NQ, NV, NT>::kTile;
     unsigned long long starts = runs.starts;
     Run run;
     next_run(runs, starts, nr, my_seq, my_pos, a.window, run);
@@ -510,20 +525,12 @@ __device__ __attribute__((always_inline)) inline void wide(const Args &a, Wide<N
         lds::wait_vm_barrier<0>();
         const int later = t + NT < t1 ? fetch(t + NT, buffer ^ 1) : 0;
         if (t * 64 <= hi && (t + NT) * 64 > lo) {
-            float ks[4 * NT], vs[4 * NT];
             int base[NT];
 #pragma unroll
-            for (int i = 0; i < NT; i++) {
-                const bool ok = now >> i & 1;
-                base[i] = ok ? (t + i) * 64 : -64;
-#pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    const float kk = lds_.scales[buffer][i * 8 + b], vv = lds_.scales[buffer][i * 8 + 4 + b];
-                    ks[4 * i + b] = ok ? kk : 0.0f, vs[4 * i + b] = ok ? vv : 0.0f;
-                }
-            }
+            for (int i = 0; i < NT; i++) base[i] = now >> i & 1 ? (t + i) * 64 : -64;
+            const float scale = now >> (lane >> 3 & (NT - 1)) & 1 ? lds_.scales[buffer][lane & (8 * NT - 1)] : 0.0f;
             const lds::lds_p at = (lds::lds_p)lds_.tiles[buffer] + lane * 16;
-            step<NQ, NV, NT, EX>(
+            step<NQ, NV, NT, true>(
                 x, q,
                 [&](int b, int cc) __attribute__((always_inline)) {
                     return *(const __attribute__((address_space(3))) i32x4 *)(at + (b >> 2) * bytes + (b & 3) * 16 * qd + cc * 1024);
@@ -531,7 +538,7 @@ __device__ __attribute__((always_inline)) inline void wide(const Args &a, Wide<N
                 [&](int D, int i) __attribute__((always_inline)) {
                     return *(const __attribute__((address_space(3))) i32x4 *)(at + i * bytes + 64 * qd + D * 1024);
                 },
-                ks, vs, base, nq, nv, g);
+                scale, base, NV, g);
         }
         now = later;
     }
@@ -542,7 +549,6 @@ __device__ __attribute__((always_inline)) inline void wide(const Args &a, Wide<N
     float *dst = a.out + (int64_t)(r0 + own / hn) * a.out_stride + (int64_t)(h0 + own % hn) * c.vd + 4 * g;
 #pragma unroll
     for (int D = 0; D < NV; D++) {
-        if (!EX && D >= nv) continue;
         f32x4_dw z;
 #pragma unroll
         for (int e = 0; e < 4; e++) z[e] = x.o[D][e] * by;
@@ -554,8 +560,11 @@ __device__ __attribute__((always_inline)) inline void wide(const Args &a, Wide<N
 // columns pay where one run fills them: a group with several runs (sequences that
 // decode, ends of prompts), or with no more than 16 columns, is dealt to its blocks
 // in groups of 16 instead.
+// (Heads wider than 128 take the registers of two waves: at two a SIMD 95 of them
+// were spilled, 32 sequences of 16 heads over 8 of 256 at 2000 positions 65 -> 44 us.)
 template <int NQ, int NV, bool EX, int NT>
-__global__ __launch_bounds__(256, 2) void kv8_attention_kernel(const Args a) {
+__global__ __launch_bounds__(256, NV > 8 ? 1 : 2) void kv8_attention_kernel(const Args a) {
+    static_assert(NT == 0 || EX, "widths of their own");
     union Both {
         Narrow<NQ, NV> narrow;
         Wide<NQ, NV, NT ? NT : 1> wide;
@@ -584,7 +593,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_kernel(const Args a) {
     } else {
         const Runs runs = runs_of(c, my_seq, my_pos, nr);
         if (__popcll(runs.starts) == 1 && __popcll(runs.valid) * hn > 16) {
-            if (sub == 0) wide<NQ, NV, NT, EX>(a, lds.wide, kv, r0, nr, h0, hn, my_seq, my_pos, runs);
+            if (sub == 0) wide<NQ, NV, NT>(a, lds.wide, kv, r0, nr, h0, hn, my_seq, my_pos, runs);
             return;
         }
         const int chunks = (hn + 15) / 16, rc = min(hn, 16), tt = 16 / rc;
@@ -654,7 +663,15 @@ Plan plan_of(const Kv8 &c, int rows, int heads, int max_pos, int window) {
     Plan p{};
     const int rep = heads / c.n_kv;
     const long long wide = ((long long)rows * rep + 63) / 64 * c.n_kv;
-    p.cols = c.qd <= 192 && c.vd <= 128 && wide >= 512 ? 64 : 16;
+    // Blocks of 64 columns share what they load, but are a quarter as many (us with
+    // 16 columns and with 64): 32 heads over 8 of 128, 500 rows (256 blocks of 64)
+    // 19.9 and 21.5, 700 (352) 28.6 and 28.1, 800 32.8 and 30.0, 2000 114 and 92, 8000
+    // 1182 and 949; 16 of 192/128, one tile a step, 2000 rows (512) 66 and 73, 3000
+    // (752) 143 and 121; 8 over 2 of 64, 6000 (750) 117 and 124, 8000 (1000) 225 and
+    // 217.  Widths that count their operands at run time lose (96 dims, 12000 rows of
+    // 6 heads over 2 511 and 558).
+    const int from = c.qd == 128 && c.vd == 128 ? 400 : c.qd == 192 && c.vd == 128 ? 640 : c.qd == 64 && c.vd == 64 ? 900 : 0;
+    p.cols = from && wide >= from ? 64 : 16;
     p.rc = std::min(rep, p.cols);
     p.chunks = (rep + p.rc - 1) / p.rc;
     p.tt = p.cols / p.rc;
@@ -730,10 +747,10 @@ int moe_kv8_attention(const moe_kv8 *c, const float *q, int64_t q_stride, int32_
     // Widths of their own: a power-of-two head and the latent cache's 192/128;
     // the others count their operands at run time.
     const bool wide = p.cols == 64;
-    if (qd == 64 && vd == 64) launch<1, 4, true, 4>(a, wide, s);
+    if (qd == 64 && vd == 64) launch<1, 4, true, 2>(a, wide, s);
     else if (qd == 128 && vd == 128) launch<2, 8, true, 2>(a, wide, s);
     else if (qd == 192 && vd == 128) launch<3, 8, true, 1>(a, wide, s);
-    else if (qd <= 192 && vd <= 128) launch<3, 8, false, 1>(a, wide, s);
+    else if (qd <= 192 && vd <= 128) launch<3, 8, false, 0>(a, s);
     else if (qd == 256 && vd == 256) launch<4, 16, true, 0>(a, s);
     else launch<4, 16, false, 0>(a, s);
     if (a.ps > 16) hipLaunchKernelGGL((kv8_join_kernel<256>), dim3((unsigned)rows * heads), dim3(256), 0, s, a);

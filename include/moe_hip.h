@@ -552,7 +552,9 @@ int moe_kv8_sizes(const moe_kv8 *c, uint64_t *codes, uint64_t *scales, uint64_t 
  * Rows whose slot is negative or past the pool, whose seq is outside 0 ...
  * n_seq - 1 or whose position is negative are skipped.  Where a sequence goes
  * on behind a block that `open` does not hold (its caller took it back to an
- * earlier position), that block's earlier positions are taken as they read.
+ * earlier position), that block's earlier positions are taken as they read;
+ * one that is given positions it did not write itself (another's pages, up to
+ * inside a block) first has its bytes of `open` cleared.
  * The same step made again writes the same.  At most 2^24 - 512 rows (also
  * moe_kv8_load's). */
 int moe_kv8_store(const moe_kv8 *c, const float *k, int64_t k_stride, const float *v, int64_t v_stride, int32_t rows,
@@ -589,7 +591,7 @@ int moe_kv8_attention(const moe_kv8 *c, const float *q, int64_t q_stride, int32_
  * halves a Q8_0 matrix's work on the matrix cores at the precision of 8-bit
  * activations.  Weights are packed once into memory of the caller's. */
 
-/* Bytes of n channels of k values (at most 131072), packed. */
+/* Bytes of n channels (below 2^24) of k values (at most 131072), packed. */
 int moe_int8_pack_size(int32_t n, int32_t k, uint64_t *bytes);
 /* Quantise `rows` rows of k values in format dt (F32, F16, BF16, Q8_0, Q4_0,
  * Q5_0), row_bytes apart in device memory, into channels row0 ... of a packed
@@ -599,9 +601,10 @@ int moe_int8_pack_size(int32_t n, int32_t k, uint64_t *bytes);
 int moe_int8_pack(const void *w, int32_t dt, int64_t row_bytes, int32_t rows, int32_t row0, int32_t n, int32_t k,
                   void *packed, uint64_t packed_bytes, void *stream);
 /* y [t, n] (y_stride floats apart) = x [t, k] (x_stride) W^T; residual (or
- * NULL, residual_stride) += y.  y and residual must not lie in x's memory.  At
- * most 2^20 tokens.  `workspace`: device, 256-byte aligned,
- * moe_int8_linear_workspace_size bytes; calls that share one must be ordered. */
+ * NULL, residual_stride) += y.  y and residual may each lie in x's memory, but
+ * not in each other's.  At most 2^20 tokens.  `workspace`: device, 256-byte
+ * aligned, moe_int8_linear_workspace_size bytes; calls that share one must be
+ * ordered. */
 int moe_int8_linear_workspace_size(int32_t n, int32_t k, int32_t t, uint64_t *bytes);
 int moe_int8_linear(const void *packed, int32_t n, int32_t k, const float *x, int64_t x_stride, int32_t t, float *y,
                     int64_t y_stride, float *residual, int64_t residual_stride, void *workspace, uint64_t workspace_bytes,

@@ -450,11 +450,18 @@ void launch_product(const Product &p, hipStream_t s) {
 int sizes_ok(const char *what, int32_t n, int32_t k) {
     if (n <= 0 || k <= 0) return fail(MOE_EINVAL, "%s: %d channels of %d values", what, n, k);
     if (k > kMostK) return fail(MOE_EUNSUP, "%s: %d values a channel, up to %d (sums of 32 bits)", what, k, kMostK);
-    if (n > (1 << 24)) return fail(MOE_EUNSUP, "%s: %d channels, up to %d", what, n, 1 << 24);
+    if (n >= (1 << 24)) return fail(MOE_EUNSUP, "%s: %d channels, up to %d", what, n, (1 << 24) - 1);  // (256 threads each)
     return MOE_OK;
 }
 uint64_t codes_bytes(int64_t rows, int64_t k) { return (uint64_t)(up(rows, 16) * up(k, 64)); }
 uint64_t packed_size(int64_t rows, int64_t k) { return codes_bytes(rows, k) + (uint64_t)up(rows, 16) * 4; }
+
+// Whether rows of `width` floats may lie in memory of other rows.
+bool meet(const float *a, int64_t a_stride, int64_t a_width, const float *b, int64_t b_stride, int64_t b_width, int rows) {
+    auto low = [&](const float *p, int64_t s) { return (intptr_t)p + std::min<int64_t>(0, s * (rows - 1)) * 4; };
+    auto high = [&](const float *p, int64_t s, int64_t w) { return (intptr_t)p + (std::max<int64_t>(0, s * (rows - 1)) + w) * 4; };
+    return low(a, a_stride) < high(b, b_stride, b_width) && low(b, b_stride) < high(a, a_stride, a_width);
+}
 
 int done(const char *what) {
     const hipError_t e = hipGetLastError();
@@ -517,7 +524,9 @@ int moe_int8_linear(const void *packed, int32_t n, int32_t k, const float *x, in
         return fail(MOE_EUNSUP, "moe_int8_linear: %d tokens of %d channels are too many blocks", t, n);
     const Product p{w, xc, reinterpret_cast<const float *>(w + codes_bytes(n, k)), sx, y, residual, y_stride, residual_stride, n, t,
                     (int)(up(k, 64) / 64), (n + 15) / 16, (t + 15) / 16};
-    if (t <= kFewRows && t * up(k, 64) <= kFewBytes) {
+    // (whose blocks read x for themselves, so that none may have written to it yet)
+    if (t <= kFewRows && t * up(k, 64) <= kFewBytes && !meet(x, x_stride, k, y, y_stride, n, t) &&
+        !(residual && meet(x, x_stride, k, residual, residual_stride, n, t))) {
         hipLaunchKernelGGL((int8_few_kernel<8>), dim3(p.nt), dim3(512), 0, s, p, x, x_stride, k);
         return done("8-bit product kernel");
     }

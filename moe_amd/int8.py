@@ -57,11 +57,12 @@ class Int8Linear(_OnDevice):
     def _pack(self, rows, k, device) -> None:
         n = sum(r[3] for r in rows)
         _fits(channels=n, values=k)
-        self.n, self.k, self.device = n, k, device
+        self.n, self.k = n, k
         b = C.c_uint64()
         _refused(L.lib().moe_int8_pack_size(n, k, C.byref(b)), "moe_int8_pack_size")
         _need(device.type == "cuda", f"weights on {device}: the kernels run on the GPU")
         self._index = device.index if device.index is not None else torch.cuda.current_device()
+        self.device = device = torch.device("cuda", self._index)
         with torch.cuda.device(self._index):
             self.packed = torch.empty(b.value, dtype=torch.uint8, device=device)
             at = 0
@@ -86,7 +87,8 @@ class Int8Linear(_OnDevice):
     @_on_its_device
     def __call__(self, x, y, residual=None, stream=None):
         """y [rows, channels] = x [rows, values] W^T, float32 with contiguous
-        rows; residual += y where it is given."""
+        rows; residual += y where it is given.  y and residual may each lie in
+        x's memory, but not in each other's."""
         t = x.shape[0]
         xs, ys = _rows(x, t, self.k, "x"), _rows(y, t, self.n, "y")
         rs, r = 0, None

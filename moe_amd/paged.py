@@ -363,7 +363,9 @@ class KvCache(_OnDevice):
 class KvCache8(_OnDevice):
     """One layer's keys and values in 8 bits, a scale for every block of 16
     positions of a kv head: `codes` and `open` uint8, `scales` float32 (sizes()
-    says how many of each), pages found through `table` (a PageTable's)."""
+    says how many of each), pages found through `table` (a PageTable's).  `open`
+    knows a sequence's values behind its last position: it is zeroed for one that
+    goes on behind positions which others wrote."""
 
     def __init__(self, codes, scales, open_blocks, table, *, n_kv: int, qd: int, vd: int, page: int):
         for t, dtype, name in ((codes, torch.uint8, "codes"), (scales, torch.float32, "scales"),

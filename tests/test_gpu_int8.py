@@ -76,6 +76,43 @@ def test_every_size_of_few_rows():
         close(y.cpu().numpy(), want[:t])
 
 
+@pytest.mark.parametrize("t,n", [(1, 640), (2, 640), (4, 640), (3, 5000), (9, 640), (90, 640), (700, 640)])
+@pytest.mark.parametrize("place", ["y", "residual", "both"])
+def test_results_in_the_inputs_memory(t, n, place):
+    """y = x W^T or x += x W^T over x itself, whichever kernel takes the rows:
+    what the blocks read is x as it was.  (Wider rows of y lie over x's.)"""
+    import torch
+
+    from moe_amd.int8 import Int8Linear
+
+    k = 640
+    x, w = operands(t, n, k, seed=9)
+    op = Int8Linear(cuda(w))
+    for _ in range(3):
+        wide = torch.zeros((t, n), device="cuda")
+        xd = wide[:, :k]
+        xd.copy_(cuda(x))
+        apart, before = torch.empty((t, n), device="cuda"), wide.cpu().numpy().astype(np.float64)
+        want = ref.product(x, w)
+        if place == "y":
+            op(xd, wide)
+            close(wide.cpu().numpy(), want)
+            continue
+        if place == "residual":
+            op(xd, apart, residual=wide)
+            close(apart.cpu().numpy(), want)
+        else:  # half of x's row apart from the other half
+            both = torch.zeros((t, 2 * n), device="cuda")
+            xd = both[:, n - k // 2:n + k // 2]
+            xd.copy_(cuda(x))
+            before = both[:, n:].cpu().numpy().astype(np.float64)
+            op(xd, both[:, :n], residual=both[:, n:])
+            close(both[:, :n].cpu().numpy(), want)
+            wide = both[:, n:]
+        total = before + want
+        assert (np.abs(wide.cpu().numpy() - total) <= TOL * np.abs(want) + 2.0 ** -24 * np.abs(total) * 1.0001 + 1e-44).all()
+
+
 def test_largest_sums():
     """Every product 127 x 127 or its negative, over the widest rows: the sums'
     largest sizes."""

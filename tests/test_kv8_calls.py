@@ -138,7 +138,7 @@ def pack(lib, w=P, dt=L.DT_F32, row_bytes=512, rows=64, row0=0, n=64, k=128, pac
 
 @pytest.mark.parametrize("bad", [dict(packed=None), dict(packed=P + 16), dict(x=None), dict(y=None), dict(n=0), dict(k=0),
                                  dict(t=-1), dict(t=2 ** 20 + 1), dict(ws=None), dict(ws=P + 128), dict(ws_bytes=2000),
-                                 dict(k=131073), dict(n=2 ** 24 + 1)], ids=str)
+                                 dict(k=131073), dict(n=2 ** 24), dict(n=2 ** 24 + 1)], ids=str)
 def test_product_refuses(lib, bad):
     assert product(lib, **bad) in (L.MOE_EINVAL, L.MOE_EUNSUP)
     assert lib.moe_last_error()

@@ -524,7 +524,7 @@ __device__ __attribute__((always_inline)) inline void wide(const Args &a, Wide<N
     for (int t = t0, buffer = 0; t < t1; t += NT, buffer ^= 1) {
         lds::wait_vm_barrier<0>();
         const int later = t + NT < t1 ? fetch(t + NT, buffer ^ 1) : 0;
-        if (t * 64 <= hi && (t + NT) * 64 > lo) {
+        if (t <= hi >> 6 && t + NT > lo >> 6) {
             int base[NT];
 #pragma unroll
             for (int i = 0; i < NT; i++) base[i] = now >> i & 1 ? (t + i) * 64 : -64;

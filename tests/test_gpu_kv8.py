@@ -463,6 +463,36 @@ def test_pool_past_4_gib():
         assert np.array_equal(x, y)
 
 
+@pytest.mark.parametrize("rows", [1, 3, 500])
+def test_last_positions_there_are(rows):
+    """Positions up to the last that 32 bits number, behind a window: results
+    are those of the same rows a whole number of tiles earlier."""
+    import torch
+
+    from moe_amd.paged import KvCache8
+
+    heads, n_kv, qd, vd, page, near_pages, window = 64, 8, 128, 128, 64, 27, 200
+    far_pages = 2 ** 31 // page - 1
+    k, v = (torch.randn((near_pages * page, n_kv * 128), device="cuda") for _ in range(2))
+    q = torch.randn((rows, heads * qd), device="cuda")
+    got = []
+    for pages in (near_pages, far_pages):
+        table = torch.full((1, pages), -1, dtype=torch.int32, device="cuda")
+        table[0, -near_pages:] = torch.arange(near_pages, dtype=torch.int32, device="cuda")
+        cache = KvCache8.new(near_pages, table, n_kv=n_kv, qd=qd, vd=vd, page=page)
+        first = (pages - near_pages) * page
+        at = [(0, first + p) for p in range(near_pages * page)]
+        lay = type("Lay", (), dict(table=np.arange(-(pages - near_pages), near_pages, dtype=np.int32)[None], page=page))
+        step = rows_on_gpu(lay, at, 1)
+        cache.store(k, v, step)
+        out = torch.full((rows, heads * vd), 7.0, device="cuda")
+        cache.attend(q, step.seq[-rows:].contiguous(), step.pos[-rows:].contiguous(), out, max_pos=pages * page - 1, scale=0.1,
+                     window=window)
+        got.append((cache.codes.cpu().numpy(), cache.scales.cpu().numpy(), out.cpu().numpy()))
+    for x, y in zip(*got):
+        assert np.array_equal(x, y)
+
+
 def test_captured_steps():
     """A decode step of tables, write and attention captured into a graph, with
     room for more rows than there are: every replay as the eager step."""

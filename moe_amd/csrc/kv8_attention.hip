@@ -11,10 +11,10 @@
 // meet them as whole numbers of 24 bits in three signed bytes,
 //   q scale = Q 2^(e - 22),  Q = 65536 d2 + 256 d1 + d0,  |Q| <= 2^22
 // (2^e above the head's largest), so a block's scores are
-//   s = s_k 2^(e - 22) (65536 K d2 + (256 K d1 + K d0)),
-// sums of whole numbers, exact, in one f32 rounding.  The result's layout (lane
-// = column, positions 4 g + i of each block) is the second operand of the values'
-// product.  There the weights p = 2^(s - m) meet the values' scales first:
+//   s = s_k 2^(e - 22) (256 (256 K d2 + K d1) + K d0),
+// sums of whole numbers, exact, then three roundings of 2^-24 (none below 2^24).
+// The result's layout (lane = column, positions 4 g + i of each block) is the
+// second operand of the values' product.  There the weights p = 2^(s - m) meet the values' scales first:
 //   W = p s_v C 2^(m - r),  r the largest s + log2 s_v of the step,  C = 2^23 - ..
 // so W below 2^23 keeps each block's product of weight and scale to 2^-23 of the
 // step's largest, however far apart the scales are.  Multiplied and added to
@@ -29,11 +29,12 @@
 // positions, 8 kv heads of 128, 235 us (5.0 TB/s of codes), one of 100001 in 128
 // parts 41 with the joining launch, 32 of up to 1500 20 (3.8 TB/s: one block a CU
 // with 12 to 24 tiles, then a merge).  Prompts are bound by the issue of vector
-// instructions: 4001 rows of 32 heads of 128 270 us (485 TFLOP/s of the attention's
-// own operations), 8000 rows 950 (550), of which the matrix pipe is busy in 29% and
-// vector instructions issue in 72% (24 to a product: joining a block's three sums 5,
-// the exponential 2, a weight's digits 3, a step's sums into O 5 for two tiles).
-// Two tiles' products a step halve that last part.
+// instructions beside the products: 4001 rows of 32 heads of 128 268 us (490
+// TFLOP/s of the attention's own operations), 8000 rows 945 (555), of which the
+// matrix pipe is busy in 29% and vector instructions issue in 71% (25 to a
+// score: joining three sums 4, the exponential 2, the weight and its digits 4, a
+// step's sums into O 5 for every two).  Two tiles' products a step halve that last
+// part; three and four waves a SIMD, at one tile a step, were no faster.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -87,6 +88,19 @@ __device__ inline float column_max(float x) {
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
+// A product's sums of the three digits begin at the bits of 3 x 2^22: an integer
+// below 2^22 added to those is the float 3 x 2^22 + it, so nothing is converted
+// (127 x 128 of up to 256 products stay below).
+constexpr int kZero = 0x4b400000;
+
+// 65536 d2 + 256 d1 + d0 of such sums: the constants cancel inside the two
+// multiply-adds, each of which, and the second subtraction, rounds once (2^-24;
+// not at all up to 2^24).
+__device__ inline float joined(int d2, int d1, int d0) {
+    const float u = fmaf(__int_as_float(d2) - (12582912.0f + 49152.0f), 256.0f, __int_as_float(d1));
+    return fmaf(u - 49152.0f, 256.0f, __int_as_float(d0));
+}
+
 // Four weights' digits, by digit: 2 (highest), 1, 0.
 struct Digits {
     uint32_t d2, d1, d0;
@@ -111,16 +125,17 @@ struct Columns {
 };
 
 // One step of NT tiles: k(b, c) and v(D, t) give operands, base[t] the tiles'
-// first positions (negative: no such tile).  Lane 8 t + b holds the scale of tile
-// t's block b of keys, lane 8 t + 4 + b that of its values (0 where there is no
-// tile): uniform values go through scalar registers.
-template <int NQ, int NV, int NT, bool EX, class K, class V>
-__device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const i32x4 (&q)[3][NQ], K k, V v, float scale,
+// first positions (negative: no such tile).  read() is called when the keys are
+// done with.  Lane 8 t + b holds the scale of tile t's block b of keys, lane
+// 8 t + 4 + b that of its values (0 where there is no tile): uniform values go
+// through scalar registers.
+template <int NQ, int NV, int NT, bool EX, class K, class V, class F>
+__device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const i32x4 (&q)[3][NQ], K k, V v, F read, float scale,
                                                            const int (&base)[NT], int nv, int g) {
     f32x4 s[4 * NT];
 #pragma unroll
     for (int b = 0; b < 4 * NT; b++) {
-        const i32x4 zero = {0, 0, 0, 0};
+        const i32x4 zero = {kZero, kZero, kZero, kZero};
         i32x4 d[3] = {zero, zero, zero};
 #pragma unroll
         for (int c = 0; c < NQ; c++) {
@@ -129,8 +144,9 @@ __device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const
             for (int p = 0; p < 3; p++) d[p] = mfma(kk, q[p][c], d[p]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[b][i] = fmaf((float)d[0][i], 65536.0f, (float)((d[1][i] << 8) + d[2][i]));
+        for (int i = 0; i < 4; i++) s[b][i] = joined(d[0][i], d[1][i], d[2][i]);
     }
+    read();
     const int lane = threadIdx.x & 63;
     if (__builtin_expect(__any(!(fabsf(scale) < INFINITY)), 0)) {  // a block that reads as NaN: so are the columns that see it
         for (int b = 0; b < 4 * NT; b++) {
@@ -191,12 +207,12 @@ __device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const
 #pragma unroll
             for (int i = 0; i < 4; i++) x.o[D][i] *= keep;
     }
-    const float in0 = __builtin_amdgcn_exp2f(ref - R) * (1.0f / kMost), in2 = in0 * 65536.0f;
+    const float in0 = __builtin_amdgcn_exp2f(ref - R) * (1.0f / kMost);
     x.m = m, x.R = R;
 #pragma unroll
     for (int D = 0; D < NV; D++) {
         if (!EX && D >= nv) continue;
-        const i32x4 zero = {0, 0, 0, 0};
+        const i32x4 zero = {kZero, kZero, kZero, kZero};
         i32x4 d[3] = {zero, zero, zero};
 #pragma unroll
         for (int t = 0; t < NT; t++) {
@@ -206,7 +222,7 @@ __device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const
         }
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            x.o[D][i] = fmaf((float)d[0][i], in2, fmaf((float)((d[1][i] << 8) + d[2][i]), in0, x.o[D][i]));
+            x.o[D][i] = fmaf(joined(d[0][i], d[1][i], d[2][i]), in0, x.o[D][i]);
     }
 }
 
@@ -387,8 +403,11 @@ __device__ __attribute__((always_inline)) inline void narrow(const Args &a, Narr
         float scale;
         int base[1];
         __amdgpu_buffer_rsrc_t buf;
-        // Loads are unconditional, so that waiting for one tile's keys leaves the
-        // others' in flight; where there is no tile they read nothing (0).
+        // A tile's values are asked for when its keys are done with, the next one's
+        // keys behind its values: in flight over the softmax and the other waves'
+        // work (a tile earlier took 18 to 30 more registers; 300 sequences of 9 rows
+        // at 200 positions 107 -> 103 us, 32 that decode 20.2 -> 19.9).  Where there
+        // is no tile the loads read nothing (0).
         auto load_keys = [&](int at) __attribute__((always_inline)) {
             const int64_t tile = at < t1 ? pages.tile(c, table, kv, at) : -1;
             base[0] = tile < 0 ? -64 : at * 64;
@@ -402,19 +421,19 @@ __device__ __attribute__((always_inline)) inline void narrow(const Args &a, Narr
                     k[T][cc] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(buf, 16 * lane, T * 16 * qd + cc * 1024, 0));
         };
         auto load_values = [&] __attribute__((always_inline)) {
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int D = 0; D < NV; D++)
                 v[D] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(buf, 16 * lane, 64 * qd + D * 1024, 0));
+            __builtin_amdgcn_sched_barrier(0);
         };
-        if (t < t1) {
-            load_keys(t);
-            load_values();
-        }
+        if (t < t1) load_keys(t);
         for (; t < t1; t++) {
             if (base[0] >= 0)
-                step<NQ, NV, 1, EX>(x, q, [&](int b, int cc) { return k[b][cc]; }, [&](int D, int) { return v[D]; }, scale, base, nv, g);
+                step<NQ, NV, 1, EX>(x, q, [&](int b, int cc) { return k[b][cc]; }, [&](int D, int) { return v[D]; }, load_values, scale,
+                                    base, nv, g);
+            __builtin_amdgcn_sched_barrier(0);
             load_keys(t + 1);
-            load_values();
         }
 
         // Merge the waves: sums as they are and their references through LDS,
@@ -538,7 +557,7 @@ __device__ __attribute__((always_inline)) inline void wide(const Args &a, Wide<N
                 [&](int D, int i) __attribute__((always_inline)) {
                     return *(const __attribute__((address_space(3))) i32x4 *)(at + i * bytes + 64 * qd + D * 1024);
                 },
-                scale, base, NV, g);
+                [] {}, scale, base, NV, g);
         }
         now = later;
     }
@@ -560,10 +579,12 @@ __device__ __attribute__((always_inline)) inline void wide(const Args &a, Wide<N
 // columns pay where one run fills them: a group with several runs (sequences that
 // decode, ends of prompts), or with no more than 16 columns, is dealt to its blocks
 // in groups of 16 instead.
-// (Heads wider than 128 take the registers of two waves: at two a SIMD 95 of them
-// were spilled, 32 sequences of 16 heads over 8 of 256 at 2000 positions 65 -> 44 us.)
+// Waves a SIMD: heads wider than 128 take the registers of two (at two a SIMD 95
+// were spilled, 32 sequences of 16 heads over 8 of 256 at 2000 positions 65 -> 44
+// us); heads of 64 fit three (16000 rows of 8 heads over 2 676 -> 608, 1000
+// sequences of 9 rows at 300 positions 86 -> 66).
 template <int NQ, int NV, bool EX, int NT>
-__global__ __launch_bounds__(256, NV > 8 ? 1 : 2) void kv8_attention_kernel(const Args a) {
+__global__ __launch_bounds__(256, NV > 8 ? 1 : NV > 4 ? 2 : 3) void kv8_attention_kernel(const Args a) {
     static_assert(NT == 0 || EX, "widths of their own");
     union Both {
         Narrow<NQ, NV> narrow;
@@ -664,13 +685,13 @@ Plan plan_of(const Kv8 &c, int rows, int heads, int max_pos, int window) {
     const int rep = heads / c.n_kv;
     const long long wide = ((long long)rows * rep + 63) / 64 * c.n_kv;
     // Blocks of 64 columns share what they load, but are a quarter as many (us with
-    // 16 columns and with 64): 32 heads over 8 of 128, 500 rows (256 blocks of 64)
-    // 19.9 and 21.5, 700 (352) 28.6 and 28.1, 800 32.8 and 30.0, 2000 114 and 92, 8000
-    // 1182 and 949; 16 of 192/128, one tile a step, 2000 rows (512) 66 and 73, 3000
-    // (752) 143 and 121; 8 over 2 of 64, 6000 (750) 117 and 124, 8000 (1000) 225 and
-    // 217.  Widths that count their operands at run time lose (96 dims, 12000 rows of
+    // 16 columns and with 64): 32 heads over 8 of 128, 450 rows (225 blocks of 64)
+    // 17.4 and 20.2, 600 (300) 25.3 and 24.0, 850 35.3 and 31.3, 1000 40.6 and 34.4;
+    // 16 of 192/128, one tile a step, 2100 rows (528) 69 and 75, 2600 (656) 92 and 89,
+    // 3200 126 and 119; 8 over 2 of 64, 6000 (750) 115 and 119, 8000 (1000) 190 and
+    // 182.  Widths that count their operands at run time lose (96 dims, 12000 rows of
     // 6 heads over 2 511 and 558).
-    const int from = c.qd == 128 && c.vd == 128 ? 400 : c.qd == 192 && c.vd == 128 ? 640 : c.qd == 64 && c.vd == 64 ? 900 : 0;
+    const int from = c.qd == 128 && c.vd == 128 ? 280 : c.qd == 192 && c.vd == 128 ? 640 : c.qd == 64 && c.vd == 64 ? 900 : 0;
     p.cols = from && wide >= from ? 64 : 16;
     p.rc = std::min(rep, p.cols);
     p.chunks = (rep + p.rc - 1) / p.rc;

@@ -8,7 +8,14 @@
 // 16 g .. 16 g + 15:
 //   [row / 16][k / 64][lane][16]
 // so that a wave's load of a tile is one contiguous KiB and goes into the
-// product as it is.  Rows and values past the matrix are zeros.
+// product as it is.  Values past a row's last are zeros, and so are x's rows past
+// its last (channels past the last are whatever is there: nothing reads their sums).
+//
+// Large products are bound by what the chip's power leaves of the matrix pipe:
+// 8191 x 6144 x 4096 in 175 us, 2357 TOP/s with the pipe 50% busy at 2.05 GHz, the
+// rows' codes before it 40 (168 MB, 4.2 TB/s).  Few rows are bound by the weights'
+// bytes: 32 rows of 6144 x 4096 6.3 us (4.2 TB/s) after 2.7 for the codes, one row
+// of 4096 x 4096 4.5 in all.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

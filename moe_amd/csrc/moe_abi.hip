@@ -365,6 +365,13 @@ void reap_ws(moe_layer *L) {
     }
 }
 
+// Clears device memory before the call returns: hipMemset only queues it on the null
+// stream, which a caller's non-blocking stream overtakes.
+hipError_t clear_now(void *p, size_t bytes) {
+    const hipError_t e = hipMemset(p, 0, bytes);
+    return e == hipSuccess ? hipStreamSynchronize(nullptr) : e;
+}
+
 // The workspace of `stream` for t tokens (moe_layer_forward): the layer
 // keeps one per stream, so calls on different streams never share scratch.
 // Grows without waiting for the device, geometrically (at least 1.5 times
@@ -397,7 +404,7 @@ int stream_ws(moe_layer *L, hipStream_t s, int t, int k, Workspace &out) {
     void *base = nullptr;
     hipError_t e = hipMalloc(&base, bytes);
     if (e != hipSuccess) return fail(MOE_ENOMEM, "workspace of %zu bytes for %d tokens: %s", bytes, max_t, hipGetErrorString(e));
-    if ((e = hipMemset(base, 0, kZeroBytes)) != hipSuccess) {
+    if ((e = clear_now(base, kZeroBytes)) != hipSuccess) {
         hipFree(base);
         return fail(MOE_EHIP, "workspace counters: %s", hipGetErrorString(e));
     }
@@ -937,7 +944,7 @@ int scratch_on(int device, void *&out) {
         hipError_t e = hipGetSymbolAddress(&p, HIP_SYMBOL(scratch));
         if (e != hipSuccess) return hip_fail(e, "hipGetSymbolAddress(scratch)");
         if (!p || (uintptr_t)p % 256) return fail(MOE_EHIP, "scratch array at %p is not 256-byte aligned", p);
-        if ((e = hipMemset(p, 0, kZeroBytes)) != hipSuccess) return hip_fail(e, "clearing the scratch counters");
+        if ((e = clear_now(p, kZeroBytes)) != hipSuccess) return hip_fail(e, "clearing the scratch counters");
         g_scratch_ptr[device] = p;
     }
     out = g_scratch_ptr[device];

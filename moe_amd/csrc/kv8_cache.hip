@@ -6,7 +6,7 @@
 // kv head, a wave its blocks' keys or values each: the rows of this step, and before
 // them those of earlier steps, whose values `open` keeps while their block is
 // filling.  Both kernels are streams: 16376 rows of 8 kv heads of 128 are written in
-// 48 us (168 MB, 3.5 TB/s) and read in 48 (168 MB, 3.5); 32 rows in 7.6 (three
+// 43 us (168 MB, 3.9 TB/s) and read in 48 (168 MB, 3.5); 32 rows in 6.8 (three
 // dependent loads: the row's place, its sequence's, the values) and 3.8.
 #include <hip/hip_runtime.h>
 
@@ -106,10 +106,12 @@ __device__ inline uint32_t quad_transpose(uint32_t x) {
 // tile, for one kv head, with eight waves: four blocks' keys, four blocks' values
 // (whose bytes meet in LDS).  A block of threads looks at `window` rows.  A lane
 // takes four dims of one position at a time.
-// NU: units of 16 dims there may be.
+// NU: units of 16 dims there may be.  Up to 8, three blocks a CU: 16376 rows of 8
+// heads of 128 52 -> 45 us, 256 decoding sequences 27 -> 22.
 template <int NU>
-__global__ __launch_bounds__(512) void kv8_store_kernel(const Store a, int window, int windows) {
+__global__ __launch_bounds__(512, NU <= 8 ? 6 : 4) void kv8_store_kernel(const Store a, int window, int windows) {
     __shared__ uint32_t words[NU * 64 * 4];  // [dims / 16][lane][block]
+    __shared__ f32x4_dw earlier[2][NU * 64];  // of the first block, [values, keys][dims / 16][lane]
     const Kv8 &c = a.c;
     const int kv = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int T = wave & 3;
@@ -172,14 +174,17 @@ __global__ __launch_bounds__(512) void kv8_store_kernel(const Store a, int windo
             f32x4_dw x[NU];
 #pragma unroll
             for (int u = 0; u < NU; u++) x[u] = *(const __attribute__((address_space(1))) f32x4_dw *)(src + 16 * min(u, nu - 1));
-            if (b.before && !b.held) {
-                if (!now)
-                    for (int u = 0; u < nu; u++) {
-                        f32x4_dw y;
-                        for (int e = 0; e < 4; e++) y[e] = b.scale * (float)(int8_t)gload(b.tile + b.code_byte(t, 16 * u + i + e));
+            if (b.before && !b.held) {  // (through LDS: in registers the loop took 50 more)
+                f32x4_dw *as_read = earlier[key] + lane;
+#pragma unroll 1
+                for (int u = 0; u < (now ? 0 : nu); u++) {
+                    f32x4_dw y;
 #pragma unroll
-                        for (int k = 0; k < NU; k++) x[k] = k == u ? y : x[k];
-                    }
+                    for (int e = 0; e < 4; e++) y[e] = b.scale * (float)(int8_t)gload(b.tile + b.code_byte(t, 16 * u + i + e));
+                    as_read[u * 64] = y;
+                }
+#pragma unroll
+                for (int u = 0; u < NU; u++) x[u] = now || u >= nu ? x[u] : as_read[u * 64];
             }
             uint32_t top = 0;
 #pragma unroll
@@ -304,10 +309,18 @@ int moe_kv8_store(const moe_kv8 *c, const float *k, int64_t k_stride, const floa
     if (rows == 0) return MOE_OK;
     a.k = k, a.v = v, a.ks = k_stride, a.vs = v_stride, a.rows = rows;
     a.row_start = row_start, a.seq = seq, a.pos = pos, a.slots = slots;
-    // One row a block keeps few rows' tiles side by side; 16 rows, and 64 where there
-    // are enough rows a sequence, leave fewer blocks without a tile's last row (16376
-    // rows of 8 sequences: 119 us with 16, 48 with 64, a tile a block).
-    const int window = (int64_t)rows * a.c.n_kv <= 16384 ? 1 : rows >= 32LL * a.c.n_seq ? 64 : 16;
+    // Rows that are their tile's last lie `apart` rows from each other on average: a
+    // window of about as many leaves few blocks without one and few with several.
+    // Where all rows' blocks are resident at once (three a CU) each takes one row; where
+    // there are very many, blocks of 16 rows and more start faster than they wait.  us
+    // with one row a block and as here: 1000 rows of one sequence, 8 heads of 128, 17.8
+    // and 7.0; 20 sequences of 100 34 and 10.3; 64 of 40 20.5 and 17.9; 4000 of 1 273
+    // and 237; 8 of 40, 2 heads of 64 (640 blocks) 6.0 and 7.5 without the first rule.
+    const double each = (double)rows / a.c.n_seq, apart = 1.25 * each / (1.0 + each / kTile8);
+    const int64_t blocks = (int64_t)rows * a.c.n_kv;
+    int window = blocks > 16384 ? 16 : 1;
+    if (blocks > 768)
+        while (window < 64 && 2 * window <= apart) window *= 2;
     const int windows = (rows + window - 1) / window;
     const int units = std::max(a.c.qd, a.c.vd) / 16;
     if (units <= 4) launch_store<4>(a, window, windows, (hipStream_t)stream);

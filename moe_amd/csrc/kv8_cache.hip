@@ -6,8 +6,8 @@
 // kv head, a wave its blocks' keys or values each: the rows of this step, and before
 // them those of earlier steps, whose values `open` keeps while their block is
 // filling.  Both kernels are streams: 16376 rows of 8 kv heads of 128 are written in
-// 43 us (168 MB, 3.9 TB/s) and read in 48 (168 MB, 3.5); 32 rows in 6.8 (three
-// dependent loads: the row's place, its sequence's, the values) and 3.8.
+// 43 us (168 MB, 3.9 TB/s) and read in 44 (33 where the codes are cached); 32 rows in
+// 6.8 (three dependent loads: the row's place, its sequence's, the values) and 3.9.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -237,32 +237,63 @@ __global__ __launch_bounds__(512, NU <= 8 ? 6 : 4) void kv8_store_kernel(const S
     }
 }
 
-// A row's thread takes four dims.  64 rows in turn, a tile's in a prompt, go to one
-// XCD: they read the same lines of its values.
+// A thread takes four dims of R rows.  64 rows in turn, a tile's in a prompt, go to
+// one XCD: they read the same lines of its values, four positions of a dim to a word.
+template <int R>
 __global__ __launch_bounds__(256) void kv8_load_kernel(const Kv8 c, const int64_t *__restrict__ slots, int rows,
                                                        float *__restrict__ k, int64_t ks, float *__restrict__ v, int64_t vs) {
-    const int64_t row = (int64_t)(((blockIdx.x >> 9) * 8 + (blockIdx.x & 7)) * 64 + (blockIdx.x >> 3 & 63));
-    if (row >= rows) return;
-    const int64_t slot = gload(slots + row);
+    constexpr unsigned kGroups = 64 / R;  // of rows in 64
+    const int64_t row = (int64_t)((blockIdx.x / (8 * kGroups) * 8 + (blockIdx.x & 7)) * 64 + (blockIdx.x >> 3 & (kGroups - 1)) * R);
     const int nk = k ? c.n_kv * c.qd : 0, at = (blockIdx.y * 256 + threadIdx.x) * 4;
-    if (!slot_ok(c, slot) || at >= nk + (v ? c.n_kv * c.vd : 0)) return;
+    if (row >= rows || at >= nk + (v ? c.n_kv * c.vd : 0)) return;
     const bool key = at < nk;
     const int i = key ? at : at - nk, d = key ? c.qd : c.vd, kv = i / d, dim = i - kv * d;
-    const int off = (int)(slot & ((1 << c.page_shift) - 1)), p = off & 63;
-    const int64_t tile = c.tile((int)(slot >> c.page_shift), kv, off);
-    const float scale = gload(c.scale_at(tile, key, p >> 4));
-    uint32_t w = 0;
-    if (key) {
-        w = gload((const uint32_t *)(c.at(tile) + kv8_key_byte(c.qd, p, dim)));
-    } else {
-        const uint8_t *src = c.at(tile) + c.values() + kv8_value_byte(p, dim);
+    int64_t slot[R], tile[R];
+    bool ok[R];
+    float scale[R];
+    uint32_t w[R];
 #pragma unroll
-        for (int e = 0; e < 4; e++) w |= (uint32_t)gload(src + 16 * e) << (8 * e);
+    for (int j = 0; j < R; j++) slot[j] = row + j < rows ? gload(slots + row + j) : -1;
+#pragma unroll
+    for (int j = 0; j < R; j++) {
+        ok[j] = slot_ok(c, slot[j]);
+        if (!ok[j]) slot[j] = 0;  // read, not written
+        const int off = (int)(slot[j] & ((1 << c.page_shift) - 1));
+        tile[j] = c.tile((int)(slot[j] >> c.page_shift), kv, off);
+        scale[j] = gload(c.scale_at(tile[j], key, (off & 63) >> 4));
     }
-    f32x4_dw x;
+    if (key) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) x[e] = scale * (float)(int8_t)(w >> (8 * e));
-    *(__attribute__((address_space(1))) f32x4_dw *)((key ? k + row * ks : v + row * vs) + i) = x;
+        for (int j = 0; j < R; j++) w[j] = gload((const uint32_t *)(c.at(tile[j]) + kv8_key_byte(c.qd, (int)(slot[j] & 63), dim)));
+    } else {
+        auto words = [&](int j, uint32_t (&y)[4]) {
+            const uint8_t *src = c.at(tile[j]) + c.values() + kv8_value_byte((int)(slot[j] & 60), dim);
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = gload((const uint32_t *)(src + 16 * e));
+        };
+        // Rows of a prompt find their words among the first's and the last's.
+        uint32_t first[4], last[4];
+        words(0, first);
+        if (R > 1) words(R - 1, last);
+#pragma unroll
+        for (int j = 0; j < R; j++) {
+            uint32_t y[4];
+            const bool a = slot[j] >> 2 == slot[0] >> 2;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = R == 1 || a ? first[e] : last[e];
+            if (R > 2 && !a && slot[j] >> 2 != slot[R - 1] >> 2) words(j, y);
+            const uint32_t by = (uint32_t)(slot[j] & 3);
+            const uint32_t lo = __builtin_amdgcn_perm(y[1], y[0], by | (by + 4) << 8 | 0x0c0c0000u);
+            w[j] = lo | __builtin_amdgcn_perm(y[3], y[2], by << 16 | (by + 4) << 24 | 0x0c0cu);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < R; j++) {
+        f32x4_dw x;
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = scale[j] * (float)(int8_t)(w[j] >> (8 * e));
+        if (ok[j]) *(__attribute__((address_space(1))) f32x4_dw *)((key ? k + (row + j) * ks : v + (row + j) * vs) + i) = x;
+    }
 }
 
 template <int NU>
@@ -338,8 +369,15 @@ int moe_kv8_load(const moe_kv8 *c, const int64_t *slots, int32_t rows, float *k,
     if (rows > kMostRows) return fail(MOE_EUNSUP, "moe_kv8_load: %d rows, up to %d at once", rows, kMostRows);
     if (rows == 0 || (!k && !v)) return MOE_OK;
     const int values = a.n_kv * ((k ? a.qd : 0) + (v ? a.vd : 0));
-    hipLaunchKernelGGL(kv8_load_kernel, dim3(((unsigned)rows + 511) / 512 * 512, (values + 1023) / 1024), dim3(256), 0,
-                       (hipStream_t)stream, a, slots, rows, k, k_stride, v, v_stride);
+    auto go = [&](auto load, unsigned each) {
+        hipLaunchKernelGGL(load, dim3(((unsigned)rows + 511) / 512 * (512 / each), (values + 1023) / 1024), dim3(256), 0,
+                           (hipStream_t)stream, a, slots, rows, k, k_stride, v, v_stride);
+    };
+    // us with a row and with four a thread: 16440 rows of 8 heads of 128 60 and 44, 1000
+    // 6.1 and 5.7, 300 (614400 values) 4.4 and 4.8; 300 of 16 heads of 192/128 6.6 and
+    // 6.1; 4000 of 2 heads of 64 (1.0e6) 4.5 and 4.7.
+    if ((int64_t)rows * values >= 5 << 18) go(kv8_load_kernel<4>, 4);
+    else go(kv8_load_kernel<1>, 1);
     return rc_of("8-bit cache read kernel");
 }
 

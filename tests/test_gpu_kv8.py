@@ -184,6 +184,56 @@ def test_store_and_load(shape, page, kind):
     assert (k[-2:] == 7).all() and (v[-2:] == 7).all() and (v[:, :2] == 7).all() and (v[:, 2 + n_kv * vd:] == 7).all()
 
 
+def test_store_many_sequences():
+    """Steps of few to many rows for each of 40 sequences are what the same rows
+    give sequence by sequence."""
+    import torch
+
+    from moe_amd.paged import KvCache8
+
+    n_kv, qd, vd, page, n_seq, ctx = 16, 64, 96, 64, 40, 330
+    g = np.random.default_rng(5)
+    n_pages, table = tables(g, n_seq, ctx, page)
+    lay = ref.Cache8(1, n_kv, qd, vd, page, table)
+    whole, parts = (KvCache8.new(n_pages, cuda(table), n_kv=n_kv, qd=qd, vd=vd, page=page) for _ in range(2))
+    length = [0] * n_seq
+    for most in (3, 7, 14, 33, 70, 1, 130):
+        step = g.integers(0, most + 1, n_seq)
+        at = [(s, length[s] + i) for s in range(n_seq) for i in range(step[s])]
+        k, v = (cuda(values(g, len(at), n_kv * d, "mixed")) for d in (qd, vd))
+        whole.store(k, v, rows_on_gpu(lay, at, n_seq))
+        r = 0
+        for s in range(n_seq):
+            if step[s]:
+                n = int(step[s])
+                parts.store(k[r:r + n], v[r:r + n], rows_on_gpu(lay, at[r:r + n], n_seq))
+                r += n
+        assert torch.equal(whole.codes, parts.codes) and torch.equal(whole.scales, parts.scales), most
+        length = [a + int(b) for a, b in zip(length, step)]
+
+
+@pytest.mark.parametrize("shape", [(32, 8, 128, 128), (16, 16, 192, 128)], ids=str)
+def test_load_many_rows_in_any_order(shape):
+    """As rows read a few at a time: in order, turned round, shuffled, the same
+    row twice, rows that are none between them."""
+    import torch
+
+    heads, n_kv, qd, vd = shape
+    c = filled(shape, 5, 400, 128, seed=21)
+    cache = on_gpu(c)
+    g = np.random.default_rng(3)
+    n = c.n_pages * c.page
+    order = np.arange(1, 1025) % n
+    for slots in (order, order[::-1], g.integers(0, n, 1024), np.where(g.random(1024) < 0.3, -1, order), np.repeat(order[:341], 3)[:1023]):
+        many, few = ([torch.full((len(slots), n_kv * d), 7.0, device="cuda") for d in (qd, vd)] for _ in range(2))
+        at = ints(slots, "int64")
+        cache.load(at, *many)
+        for r in range(0, len(slots), 50):
+            cache.load(at[r:r + 50], *(x[r:r + 50] for x in few))
+        for x, y in zip(many, few):
+            assert torch.equal(x, y)
+
+
 def test_store_large_steps():
     """More rows than one launch shape takes, in strides: as small steps."""
     import torch

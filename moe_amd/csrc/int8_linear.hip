@@ -437,7 +437,10 @@ __global__ __launch_bounds__(W * 64) void int8_few_kernel(const Product p, const
 // where n = 1024):
 //   direct, 16 x 16 (tokens x channels) for 16 rows; 32 x 32 up to 256 blocks,
 //   then 32 x 64 up to 512 (48 x 6144: 7.5 and 6.5; 256 x 1024: 4.2 and 4.7;
-//   160 x 6144: 16.4 and 10.6, ring of 64 x 128 15.9);
+//   160 x 6144: 16.4 and 10.6, ring of 64 x 128 15.9); 32 x 16 where half the CUs
+//   would have no block and rows are long (with the rows' codes, 32 x 1024 of 4096
+//   values 8.7 and 7.7, 24 x 4096 of 8192 13.7 and 12.3, but 48 x 2048 of 2048 7.0
+//   and 7.3);
 //   ring, 64 x 128 below 256 blocks of 128 x 128 (512 x 6144: 22.6 and 24.3, 32 x
 //   64 27.8; 768 x 6144: 34.1 and 31.7);
 //   ring, 256 x 256 where its rounds of 256 blocks are at least 5/6 full (2048 x
@@ -447,6 +450,7 @@ void launch_product(const Product &p, hipStream_t s) {
     auto blocks = [&](int64_t m, int64_t n) { return (p.tt + m - 1) / m * ((p.nt + n - 1) / n); };
     const int64_t large = blocks(16, 16), rounds = (large + 255) / 256;
     if (p.tt == 1) direct<1, 1, 8>(p, s);
+    else if (blocks(2, 2) <= 128 && p.chunks >= 64) direct<2, 1, 8>(p, s);
     else if (blocks(2, 2) <= 256) direct<2, 2, 8>(p, s);
     else if (blocks(2, 4) <= 512) direct<2, 4, 8>(p, s);
     else if (large * 6 >= rounds * 256 * 5) ring<4, 2, 4, 8, 4>(p, s);

@@ -607,7 +607,8 @@ int moe_int8_pack(const void *w, int32_t dt, int64_t row_bytes, int32_t rows, in
  * NULL, residual_stride) += y.  y and residual may each lie in x's memory, but
  * not in each other's.  At most 2^20 tokens.  `workspace`: device, 256-byte
  * aligned, moe_int8_linear_workspace_size bytes; calls that share one must be
- * ordered. */
+ * ordered.  Up to 4 tokens of up to 16384 values in all (k rounded up to 64), in
+ * memory apart from y and residual, need none (NULL, 0). */
 int moe_int8_linear_workspace_size(int32_t n, int32_t k, int32_t t, uint64_t *bytes);
 int moe_int8_linear(const void *packed, int32_t n, int32_t k, const float *x, int64_t x_stride, int32_t t, float *y,
                     int64_t y_stride, float *residual, int64_t residual_stride, void *workspace, uint64_t workspace_bytes,

@@ -523,21 +523,23 @@ int moe_int8_linear(const void *packed, int32_t n, int32_t k, const float *x, in
     if (t < 0 || t > (1 << 20)) return fail(MOE_EINVAL, "moe_int8_linear: %d tokens, up to %d", t, 1 << 20);
     if (t == 0) return MOE_OK;
     if (!packed || (uintptr_t)packed % 256 || !x || !y) return fail(MOE_EINVAL, "moe_int8_linear: bad argument");
-    if (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < packed_size(t, k))
+    // Blocks that read x for themselves need no workspace, but x as it was.
+    const bool few = t <= kFewRows && t * up(k, 64) <= kFewBytes && !meet(x, x_stride, k, y, y_stride, n, t) &&
+                     !(residual && meet(x, x_stride, k, residual, residual_stride, n, t));
+    if (few) workspace = nullptr;
+    else if (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < packed_size(t, k))
         return fail(MOE_EINVAL, "moe_int8_linear: workspace of %llu bytes (256-byte aligned), %llu needed",
                     (unsigned long long)workspace_bytes, (unsigned long long)packed_size(t, k));
     hipStream_t s = (hipStream_t)stream;
     const uint8_t *w = static_cast<const uint8_t *>(packed);
     uint8_t *xc = static_cast<uint8_t *>(workspace);
-    float *sx = reinterpret_cast<float *>(xc + codes_bytes(t, k));
+    float *sx = few ? nullptr : reinterpret_cast<float *>(xc + codes_bytes(t, k));
     // (blocks of 128 x 64 at least, 512 threads at most)
     if (up(t, 128) / 128 * (up(n, 64) / 64) * 512 > 0xffffffffll)
         return fail(MOE_EUNSUP, "moe_int8_linear: %d tokens of %d channels are too many blocks", t, n);
     const Product p{w, xc, reinterpret_cast<const float *>(w + codes_bytes(n, k)), sx, y, residual, y_stride, residual_stride, n, t,
                     (int)(up(k, 64) / 64), (n + 15) / 16, (t + 15) / 16};
-    // (whose blocks read x for themselves, so that none may have written to it yet)
-    if (t <= kFewRows && t * up(k, 64) <= kFewBytes && !meet(x, x_stride, k, y, y_stride, n, t) &&
-        !(residual && meet(x, x_stride, k, residual, residual_stride, n, t))) {
+    if (few) {
         hipLaunchKernelGGL((int8_few_kernel<8>), dim3(p.nt), dim3(512), 0, s, p, x, x_stride, k);
         return done("8-bit product kernel");
     }

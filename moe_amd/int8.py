@@ -70,7 +70,7 @@ class Int8Linear(_OnDevice):
                 _refused(L.lib().moe_int8_pack(ptr, dt, row_bytes, m, at, n, k, self.packed.data_ptr(), b.value,
                                                torch._C._cuda_getCurrentRawStream(self._index)), "moe_int8_pack")
                 at += m
-        self._where = self.packed.data_ptr()
+        self._where, self._width = self.packed.data_ptr(), -(-k // 64) * 64
         self._sizes = {}
 
     def workspace_size(self, t: int) -> int:
@@ -99,9 +99,13 @@ class Int8Linear(_OnDevice):
             self._check_device(x, y, residual)
         need = self.workspace_size(t)
         sp = self._on(stream)
-        ws = self._scratch(need, sp)
-        rc = L.lib().moe_int8_linear(self._where, self.n, self.k, x.data_ptr(), xs, t, y.data_ptr(), ys, r, rs,
-                                     ws.data_ptr(), need, sp)
+        rc = 1
+        if t * self._width <= 16384 and t <= 4:  # no workspace, unless results lie in x's memory
+            rc = L.lib().moe_int8_linear(self._where, self.n, self.k, x.data_ptr(), xs, t, y.data_ptr(), ys, r, rs, None, 0, sp)
+        if rc:
+            ws = self._scratch(need, sp)
+            rc = L.lib().moe_int8_linear(self._where, self.n, self.k, x.data_ptr(), xs, t, y.data_ptr(), ys, r, rs,
+                                         ws.data_ptr(), need, sp)
         if rc:
             _refused(rc, "moe_int8_linear")
         return y

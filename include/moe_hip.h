@@ -524,10 +524,12 @@ int moe_kv4_select(const moe_kv4 *c, const float *q, int64_t q_stride, int32_t r
  *           keys [block][qd / 16][position][16 dims], then its values
  *           [vd / 16][g 4][16 dims][block][i 4] of position 16 block + 4 g + i
  *   scales  f32 [page][kv head][page / 64 tiles][keys, values][block]
- *   open    per sequence and kv head, the f32 values of blocks that are not
- *           full yet (two of them, 128 (qd + vd) bytes) and which ones they are
- *           (32 bytes); zeros: none.  A block's codes are therefore those of its
- *           positions' values, however the steps that wrote them were cut.
+ *   open    per sequence and kv head, f32 values of two blocks (128 (qd + vd)
+ *           bytes): of the one that is not full yet, and of the one that the last
+ *           step went on in those before the step; then which blocks they are and
+ *           how many values (32 bytes); zeros: none.  A block's codes are therefore
+ *           those of its positions' values, however the steps that wrote them were
+ *           cut.
  * No counterpart in the reference, which keeps f32 (src/model.rs:93-114). */
 typedef struct moe_kv8 {
     void *codes;           /* device, 16-byte aligned, as scales and open */
@@ -551,11 +553,12 @@ int moe_kv8_sizes(const moe_kv8 *c, uint64_t *codes, uint64_t *scales, uint64_t 
  * rows are row_start[i] to row_start[i + 1] - 1, its next positions in order.
  * Rows whose slot is negative or past the pool, whose seq is outside 0 ...
  * n_seq - 1 or whose position is negative are skipped.  Where a sequence goes
- * on behind a block that `open` does not hold (its caller took it back to an
- * earlier position), that block's earlier positions are taken as they read;
+ * on inside a block of which `open` does not hold all earlier positions (its caller
+ * took it back to an earlier position), those are taken as they read;
  * one that is given positions it did not write itself (another's pages, up to
  * inside a block) first has its bytes of `open` cleared.
- * The same step made again writes the same.  At most 2^24 - 512 rows (also
+ * The same step made again writes the same, and another one from the same position
+ * what it would have written without this one.  At most 2^24 - 512 rows (also
  * moe_kv8_load's). */
 int moe_kv8_store(const moe_kv8 *c, const float *k, int64_t k_stride, const float *v, int64_t v_stride, int32_t rows,
                   const int32_t *row_start, const int32_t *seq, const int32_t *pos, const int64_t *slots, void *stream);

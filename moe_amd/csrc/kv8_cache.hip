@@ -69,7 +69,8 @@ __device__ inline bool slot_ok(const Kv8 &c, int64_t slot) {
 }
 
 // What `open` says of a sequence's kv head: for keys (values: [2], [3]) in each
-// of two halves the block whose values it holds, plus 1, and how many of them.
+// of two halves the block whose values it holds, plus 1, and how many of them, the
+// block's first, are the sequence's.
 struct Half {
     int block1, count;
 };
@@ -162,6 +163,7 @@ __global__ __launch_bounds__(512, NU <= 8 ? 6 : 4) void kv8_store_kernel(const S
                     if (__builtin_amdgcn_readlane((int)my_tags[2 * h], at) == was + 1 &&
                         __builtin_amdgcn_readlane((int)my_tags[2 * h + 1], at) >= had)
                         half = h;
+            const int near = half < 0 ? 0 : half;  // that block's, from now on
             b.held = half < 0 ? nullptr : halves + half * kBlock8 * b.d;
             b.scale = half < 0 && b.before ? gload(scale) : 0.0f;
 
@@ -194,23 +196,25 @@ __global__ __launch_bounds__(512, NU <= 8 ? 6 : 4) void kv8_store_kernel(const S
                     x[u][e] = there && u < nu ? x[u][e] : 0.0f;
                     top = max(top, magnitude(x[u][e]));
                 }
-            // The step's last block of the sequence: what it holds so far is kept
-            // where the block before is not (another wave may be reading that one,
-            // and a step that is made again finds it).
-            if (keeps) {
-                const bool same = (p >> 4) == was, full = in == 15;
-                const int to = half < 0 ? 0 : same ? half : 1 - half;
+            // Kept: of the block that the step goes on in the values before it (which
+            // may be what its codes read as), so that the step made again, or another
+            // from there, finds them whatever this one makes of the codes; of the last
+            // block, while it is filling, all of them, in the other half if it is
+            // another block (that one's wave may be reading).  A half's count is how
+            // many of its values are still the sequence's, so the first's goes back to
+            // `had`, and nothing stays of earlier steps and sequences.
+            const bool full = in == 15, on = had && (p >> 6) * 4 + T == was, same = (p >> 4) == was && had;
+            if (on || keeps) {
+                const bool all = keeps && !full;
+                const int to = on || !had ? near : 1 - near, lo = on && half >= 0 ? b.before : 0, hi = all ? in + 1 : on ? had : 0;
                 float *dst = halves + to * kBlock8 * b.d;
-                if (!full && t <= in && !(half >= 0 && same && t < b.before))  // (those before lie there)
+                if (t >= lo && t < hi)
 #pragma unroll
                     for (int u = 0; u < NU; u++)
                         if (u < nu) *(__attribute__((address_space(1))) f32x4_dw *)(dst + t * b.d + 16 * u + i) = x[u];
                 if (lane == 0) {
-                    if (!full) tags[to] = Half{(p >> 4) + 1, in + 1};
-                    // Nothing that an earlier block or sequence left stays, but the
-                    // half that this step has read.
-                    for (int h = 0; h < 2; h++)
-                        if (h != half && (full || h != to)) tags[h] = Half{0, 0};
+                    tags[to] = all ? Half{(p >> 4) + 1, in + 1} : on ? Half{was + 1, had} : Half{0, 0};
+                    if (keeps && (same || !had)) tags[1 - to] = Half{0, 0};
                 }
             }
             const Int8Scale q(wave_max(top));

@@ -551,8 +551,11 @@ int moe_kv8_sizes(const moe_kv8 *c, uint64_t *codes, uint64_t *scales, uint64_t 
  * [rows, n_kv * qd] and v [rows, n_kv * vd] f32, k_stride and v_stride floats
  * apart.  row_start, seq, pos and slots are moe_pages_advance's: sequence i's
  * rows are row_start[i] to row_start[i + 1] - 1, its next positions in order.
- * Rows whose slot is negative or past the pool, whose seq is outside 0 ...
- * n_seq - 1 or whose position is negative are skipped.  Where a sequence goes
+ * Rows whose slot is negative or past the pool, whose seq is not that sequence
+ * (or outside 0 ... n_seq - 1) or whose position is negative are skipped: the step
+ * begins at a sequence's first row that is not, and ends with its last.  Of those
+ * between, a block of 16 positions that no row is written to stays as it was;
+ * in others their positions hold zeros.  Where a sequence goes
  * on inside a block of which `open` does not hold all earlier positions (its caller
  * took it back to an earlier position), those are taken as they read;
  * one that is given positions it did not write itself (another's pages, up to

@@ -125,23 +125,59 @@ __global__ __launch_bounds__(512, NU <= 8 ? 6 : 4) void kv8_store_kernel(const S
     const int mine = which * window + min(lane, window - 1), from = min(mine, a.rows - 1);
     const int64_t my_slot = gload(a.slots + from);
     const int my_seq = gload(a.seq + from), my_pos = gload(a.pos + from);
+    // Rows that are to be skipped may lie anywhere among a sequence's, so whose row
+    // each is, or -1: of the window, the one behind it and the 64 before it (a tile's
+    // last row and all others of the tile).
+    auto row_of = [&](int j) {
+        const int64_t slot = gload(a.slots + j);
+        const int s = gload(a.seq + j), p = gload(a.pos + j);
+        return slot_ok(c, slot) && p >= 0 ? s : -1;
+    };
+    const int start = which * window, next_of = row_of(min(mine + 1, a.rows - 1)), past = start - 64 + lane;
+    const int past_of = past >= 0 ? row_of(past) : -1;
     const bool good = lane < window && mine < a.rows && slot_ok(c, my_slot) && (unsigned)my_seq < (unsigned)c.n_seq && my_pos >= 0;
     const int my_r0 = good ? max(0, min(mine, gload(a.row_start + my_seq))) : 0;
     const int my_r1 = good ? max(mine + 1, min(a.rows, gload(a.row_start + my_seq + 1))) : 0;
     const u32x4 my_tags = good ? gload((const u32x4 *)(c.open_at(my_seq, kv) + 2 * kBlock8 * 4 * (c.qd + c.vd) + (key ? 0 : 16)))
                                : u32x4{0, 0, 0, 0};
-    unsigned long long last = __ballot(good && ((my_pos & 63) == 63 || mine + 1 == my_r1));
+    const bool followed = good && mine + 1 < my_r1 && next_of == my_seq;
+    bool ends = good && ((my_pos & 63) == 63 || !followed);
+    if (ends && !followed)
+        for (int j = mine + 2, of_tile = min(my_r1, mine + 64 - (my_pos & 63)); ends && j < of_tile; j++) ends = row_of(j) != my_seq;
+    const unsigned long long follow = __ballot(followed);
+    unsigned long long last = __ballot(ends);
     for (; last; last &= last - 1) {
         const int at = __builtin_ctzll(last), r = which * window + at;
         const int64_t slot = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(my_slot >> 32), at) << 32 |
                                        (uint32_t)__builtin_amdgcn_readlane((int)my_slot, at));
         const int s = __builtin_amdgcn_readlane(my_seq, at), p = __builtin_amdgcn_readlane(my_pos, at);
         const int r0 = __builtin_amdgcn_readlane(my_r0, at), r1 = __builtin_amdgcn_readlane(my_r1, at);
-        const int p0 = max(0, p - (r - r0));  // the sequence's first row's
-        const int first = max(p0, p & ~63) >> 4 & 3, final = p >> 4 & 3;  // the blocks that the step has rows of
+        // Rows r - 63 .. r that are the sequence's and written; those of the tile, by
+        // its positions; whether any lies before the tile.
+        const int t0 = r - (p & 63);
+        const unsigned long long late = __ballot(good && my_seq == s && mine >= r0), early = __ballot(past_of == s && past >= r0);
+        const unsigned long long rows = late << (63 - at) | (at < 63 ? early >> (at + 1) : 0), there = rows >> (63 - (p & 63));
+        // The sequence's first row from j on, before row `end` (or -1).
+        auto first_row = [&](int j, int end) {
+            for (; j < end; j += 64) {
+                const unsigned long long some = __ballot(j + lane < end && row_of(min(j + lane, end - 1)) == s);
+                if (some) return j + __builtin_ctzll(some);
+            }
+            return -1;
+        };
+        bool behind = t0 > r0;
+        if (behind) {
+            const int j = t0 - 1 - start;  // (-64 at least)
+            behind = (j >= 0 ? late >> j : early >> (j + 64)) & 1 || first_row(r0, t0) >= 0;
+        }
+        const bool ends_here = !(follow >> at & 1) && first_row(r + 2, r1) < 0;
+        // The position of the first row in the tile.
+        const int p0 = behind ? p & ~63 : (p & ~63) + __builtin_ctzll(there);
+        auto of_block = [&](int k) { return (uint32_t)(there >> (16 * k)) & 0xffffu; };
+        const int final = p >> 4 & 3;
         const int64_t tile = c.tile((int)(slot >> c.page_shift), kv, (int)(slot & ((1 << c.page_shift) - 1)));
         uint8_t *codes = c.at(tile) + (key ? 0 : c.values());
-        if (T >= first && T <= final) {
+        if (of_block(T)) {
             const int start = (p & ~63) + 16 * T, end = min(p, start + 15), in = end & 15;
             Block b;
             b.key = key, b.T = T, b.d = key ? c.qd : c.vd;
@@ -154,16 +190,18 @@ __global__ __launch_bounds__(512, NU <= 8 ? 6 : 4) void kv8_store_kernel(const S
             uint8_t *open = c.open_at(s, kv);
             Half *tags = (Half *)(open + 2 * kBlock8 * 4 * (c.qd + c.vd)) + (key ? 0 : 2);
             float *halves = (float *)open + (key ? 0 : 2 * kBlock8 * c.qd);
-            const int was = p0 >> 4, had = p0 & 15;
-            const bool keeps = T == final && r + 1 == r1;
-            int half = -1;
-            if (had)
+            const bool keeps = T == final && ends_here;
+            int was = 0, had = 0, half = -1;
+            auto went_on = [&](int first) {  // from position `first` on
+                was = first >> 4, had = first & 15;
+                if (had)
 #pragma unroll
-                for (int h = 0; h < 2; h++)
-                    if (__builtin_amdgcn_readlane((int)my_tags[2 * h], at) == was + 1 &&
-                        __builtin_amdgcn_readlane((int)my_tags[2 * h + 1], at) >= had)
-                        half = h;
-            const int near = half < 0 ? 0 : half;  // that block's, from now on
+                    for (int h = 0; h < 2; h++)
+                        if (__builtin_amdgcn_readlane((int)my_tags[2 * h], at) == was + 1 &&
+                            __builtin_amdgcn_readlane((int)my_tags[2 * h + 1], at) >= had)
+                            half = h;
+            };
+            if (!behind) went_on(p0);
             b.held = half < 0 ? nullptr : halves + half * kBlock8 * b.d;
             b.scale = half < 0 && b.before ? gload(scale) : 0.0f;
 
@@ -171,8 +209,8 @@ __global__ __launch_bounds__(512, NU <= 8 ? 6 : 4) void kv8_store_kernel(const S
             const int t = key ? lane >> 2 : (lane >> 4) * 4 + (lane & 3), i = key ? 4 * (lane & 3) : lane & 12;
             // Loads are unconditional (units past the last read it again), so that
             // they are in flight together.
-            const bool now = t >= b.before, there = t < b.before + b.n;
-            const float *src = (!now && b.held ? b.held + t * b.d : b.row + (int64_t)(now && there ? t - b.before : 0) * b.stride) + i;
+            const bool now = t >= b.before, some = !now || (of_block(T) >> t & 1);
+            const float *src = (!now && b.held ? b.held + t * b.d : b.row + (int64_t)(now && some ? t - b.before : 0) * b.stride) + i;
             f32x4_dw x[NU];
 #pragma unroll
             for (int u = 0; u < NU; u++) x[u] = *(const __attribute__((address_space(1))) f32x4_dw *)(src + 16 * min(u, nu - 1));
@@ -193,7 +231,7 @@ __global__ __launch_bounds__(512, NU <= 8 ? 6 : 4) void kv8_store_kernel(const S
             for (int u = 0; u < NU; u++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    x[u][e] = there && u < nu ? x[u][e] : 0.0f;
+                    x[u][e] = some && u < nu ? x[u][e] : 0.0f;
                     top = max(top, magnitude(x[u][e]));
                 }
             // Kept: of the block that the step goes on in the values before it (which
@@ -203,8 +241,10 @@ __global__ __launch_bounds__(512, NU <= 8 ? 6 : 4) void kv8_store_kernel(const S
             // another block (that one's wave may be reading).  A half's count is how
             // many of its values are still the sequence's, so the first's goes back to
             // `had`, and nothing stays of earlier steps and sequences.
-            const bool full = in == 15, on = had && (p >> 6) * 4 + T == was, same = (p >> 4) == was && had;
+            const bool full = in == 15, on = !behind && had && (p >> 6) * 4 + T == was;
             if (on || keeps) {
+                if (behind) went_on(max(0, p - (r - first_row(r0, t0))));
+                const int near = half < 0 ? 0 : half;  // the first block's, from now on
                 const bool all = keeps && !full;
                 const int to = on || !had ? near : 1 - near, lo = on && half >= 0 ? b.before : 0, hi = all ? in + 1 : on ? had : 0;
                 float *dst = halves + to * kBlock8 * b.d;
@@ -214,7 +254,7 @@ __global__ __launch_bounds__(512, NU <= 8 ? 6 : 4) void kv8_store_kernel(const S
                         if (u < nu) *(__attribute__((address_space(1))) f32x4_dw *)(dst + t * b.d + 16 * u + i) = x[u];
                 if (lane == 0) {
                     tags[to] = all ? Half{(p >> 4) + 1, in + 1} : on ? Half{was + 1, had} : Half{0, 0};
-                    if (keeps && (same || !had)) tags[1 - to] = Half{0, 0};
+                    if (keeps && (on || !had)) tags[1 - to] = Half{0, 0};
                 }
             }
             const Int8Scale q(wave_max(top));
@@ -231,11 +271,12 @@ __global__ __launch_bounds__(512, NU <= 8 ? 6 : 4) void kv8_store_kernel(const S
         // The values' words: position by position inside, block by block.
         uint8_t *values = c.at(tile) + c.values();
         for (int w = threadIdx.x; w < c.vd * 4; w += 512) {
-            if (first == 0 && final == 3) {
+            if (of_block(0) && of_block(1) && of_block(2) && of_block(3)) {
                 gstore((u32x4 *)(values + w * 16), *(const u32x4 *)&words[w * 4]);
                 continue;
             }
-            for (int k = first; k <= final; k++) gstore((uint32_t *)(values + w * 16 + k * 4), words[w * 4 + k]);
+            for (int k = 0; k < 4; k++)
+                if (of_block(k)) gstore((uint32_t *)(values + w * 16 + k * 4), words[w * 4 + k]);
         }
         __syncthreads();
     }

@@ -416,8 +416,10 @@ class KvCache8(_OnDevice):
     def store(self, k, v, rows: Rows, stream=None) -> None:
         """Write a step's rows k [rows, kv heads * key width], v [rows, kv
         heads * value width] (float32): `rows` as PageTable.advance fills it
-        (moe_kv8_store).  Rows of negative slots are skipped; the same step made
-        again writes the same."""
+        (moe_kv8_store).  Rows of negative slots, of no sequence or no position
+        are skipped wherever they lie: the step begins at a sequence's first row
+        that is not and ends with its last.  The same step made again writes the
+        same."""
         n, start, seq, pos, slot, _ = rows._args
         ks, vs = _rows(k, n, self.n_kv * self.qd, "k"), _rows(v, n, self.n_kv * self.vd, "v")
         _need(rows.n_seq == self.table.shape[0], f"rows of {rows.n_seq} sequences, the table has {self.table.shape[0]}")

@@ -15,13 +15,16 @@
 // sums of whole numbers, exact, then three roundings of 2^-24 (none below 2^24).
 // The result's layout (lane = column, positions 4 g + i of each block) is the
 // second operand of the values' product.  There the weights p = 2^(s - m) meet the values' scales first:
-//   W = p s_v C 2^(m - r),  r the largest s + log2 s_v of the step,  C = 2^23 - ..
+//   W = p s_v C 2^-r,  r the largest s - m + log2 s_v of the step,  C = 2^23 - ..
 // so W below 2^23 keeps each block's product of weight and scale to 2^-23 of the
 // step's largest, however far apart the scales are.  Multiplied and added to
 // 2^23 + 0x8080 in one instruction, a weight's bits are its three digits (the
 // two low ones with 128 added).  A step's sums are whole numbers too; they join
-// the f32 sums O, which have a reference of their own (R, as r; the weights' sum
-// has m).  Sums that stayed whole numbers over many steps would need references
+// the f32 sums O, which are multiples of 2^(m + e) (the weights' sum's of 2^m).
+// Everything is in differences from m, and m and e are whole numbers, so that no
+// step's scores, however large, round what earlier steps left: one position whose
+// score is 1e20 above the others gives its value to 2^-23.
+// Sums that stayed whole numbers over many steps would need references
 // with room above them: three bits of it cost a digit's eighth (1e-5 of the output
 // against 1e-6) and still had to move for one wave of a block in every second step.
 //
@@ -59,7 +62,7 @@ struct Args {
     Kv8 c;
     const float *q;
     const int32_t *seq, *pos;
-    float *out, *part, *part_ml;  // part [row][head][ps][vd], part_ml [row][head][ps][m, l, R]
+    float *out, *part, *part_ml;  // part [row][head][ps][vd], part_ml [row][head][ps][m, l, e]
     int64_t q_stride, out_stride;
     int rows, heads, rep, window;
     float scale;
@@ -69,15 +72,11 @@ struct Args {
     int ps;          // blocks that share a run's tiles
 };
 
-constexpr float kNone = -1e30f;          // below every score: where nothing has been seen
+constexpr float kNone = -3e38f;          // below every score: where nothing has been seen
 constexpr float kMost = 8355000.0f;      // largest weight (C): its digits' room is 8355711, what exp2 errs by taken off
 constexpr float kLeastLog = -100.0f;     // log2 of a value scale, where it is smaller or 0
 
 __device__ inline i32x4 mfma(i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
-
-// log2 of the product of a weight of score z and a value scale, not below it:
-// what large scores' sums round off is added.
-__device__ inline float product_log(float z, float scale) { return fmaf(fabsf(z), 0x1p-21f, z + scale); }
 
 // The largest of a column's four lanes (16 apart), in each of them.
 __device__ inline float column_max(float x) {
@@ -118,7 +117,7 @@ __device__ inline Digits digits_of(uint32_t w0, uint32_t w1, uint32_t w2, uint32
 template <int NV>
 struct Columns {
     f32x4 o[NV];
-    float m, R, l;      // (l: this lane's positions only)
+    float m, e, l;      // whole numbers, see above; this lane's positions' weights
     float qs;           // 2^(e - 22) |scale| log2(e)
     int pos, lo;        // what a column sees: positions lo .. pos
     int first, last;    // of all columns: everything in first .. last is seen by every one
@@ -175,14 +174,29 @@ __device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const
             sc[b] = 1.0f;
         }
     }
-    float top = kNone, ref = kNone;
+    float most[4 * NT], top = kNone;
 #pragma unroll
     for (int b = 0; b < 4 * NT; b++) {
-        const float z = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])) * sc[b];
-        top = fmaxf(top, z), ref = fmaxf(ref, product_log(z, of(log_, b / 4 * 8 + 4 + b % 4)));
+        most[b] = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3]));
+        top = fmaxf(top, most[b] * sc[b]);
     }
-    top = column_max(top), ref = column_max(ref);
-    const float f = __builtin_amdgcn_exp2f(top - ref) * kMost;
+    top = column_max(top);
+    // Scores whose rounding is more than the weights' range bears: all are rounded,
+    // as the largest is (where not all positions are seen they have been).
+    if (__builtin_expect(whole && __any(fabsf(top) > 4194304.0f), 0)) {
+#pragma unroll
+        for (int b = 0; b < 4 * NT; b++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[b][i] *= sc[b];
+            most[b] *= sc[b], sc[b] = 1.0f;
+        }
+    }
+    top = __builtin_ceilf(top);
+    float ref = kLeastLog - 2.0f;  // (where nothing is seen)
+#pragma unroll
+    for (int b = 0; b < 4 * NT; b++) ref = fmaxf(ref, fmaf(most[b], sc[b], -top) + of(log_, b / 4 * 8 + 4 + b % 4));
+    ref = column_max(ref);
+    const float f = __builtin_amdgcn_exp2f(-ref) * kMost;
     float sum = 0.0f;
     i32x4 w[NT][3];
 #pragma unroll
@@ -198,17 +212,17 @@ __device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const
         const Digits d = digits_of(y[0], y[1], y[2], y[3]);
         w[b / 4][0][b % 4] = (int)d.d2, w[b / 4][1][b % 4] = (int)d.d1, w[b / 4][2][b % 4] = (int)d.d0;
     }
-    const float m = fmaxf(x.m, top), R = fmaxf(x.R, ref);
+    const float m = fmaxf(x.m, top), was = x.e + (x.m - m), now = ref + (top - m), e = fmaxf(was, __builtin_ceilf(now));
     x.l = x.l * __builtin_amdgcn_exp2f(x.m - m) + sum * __builtin_amdgcn_exp2f(top - m);
-    if (__any(R > x.R)) {
-        const float keep = __builtin_amdgcn_exp2f(x.R - R);
+    if (__any(e > was)) {
+        const float keep = __builtin_amdgcn_exp2f(was - e);
 #pragma unroll
         for (int D = 0; D < NV; D++)
 #pragma unroll
             for (int i = 0; i < 4; i++) x.o[D][i] *= keep;
     }
-    const float in0 = __builtin_amdgcn_exp2f(ref - R) * (1.0f / kMost);
-    x.m = m, x.R = R;
+    const float in0 = __builtin_amdgcn_exp2f(now - e) * (1.0f / kMost);
+    x.m = m, x.e = e;
 #pragma unroll
     for (int D = 0; D < NV; D++) {
         if (!EX && D >= nv) continue;
@@ -346,7 +360,7 @@ __device__ inline void begin(Columns<NV> &x, i32x4 (&q)[3][NQ], const u32x4 *sq,
     for (int D = 0; D < NV; D++) x.o[D] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const float k = sk[lane & 15];
     x.qs = k != k ? 0.0f : k;
-    x.m = x.R = kNone;
+    x.m = kNone, x.e = 0.0f;
     x.l = k != k ? k : 0.0f;
     x.pos = __shfl(my_pos, row, 64);
     x.lo = window > 0 ? max(0, x.pos + 1 - window) : 0;
@@ -364,7 +378,7 @@ template <int NQ, int NV>
 struct Narrow {
     u32x4 sq[3 * NQ * 64];
     f32x4 so[4 * NV * 64];  // O of the waves: [wave][D][lane]
-    float sk[16], sm[4][16], sl[4][16], sr[4][16];
+    float sk[16], sm[4][16], sl[4][16], se[4][16];
 };
 
 typedef const __attribute__((address_space(1))) uint8_t *gbytes;
@@ -440,26 +454,28 @@ __device__ __attribute__((always_inline)) inline void narrow(const Args &a, Narr
         // then every wave takes a share of the output's dims.
         x.l += __shfl_xor(x.l, 16, 64);
         x.l += __shfl_xor(x.l, 32, 64);
-        if (g == 0) lds.sm[wave][col] = x.m, lds.sl[wave][col] = x.l, lds.sr[wave][col] = x.R;
+        if (g == 0) lds.sm[wave][col] = x.m, lds.sl[wave][col] = x.l, lds.se[wave][col] = x.e;
 #pragma unroll
         for (int D = 0; D < NV; D++) lds.so[(wave * NV + D) * 64 + lane] = x.o[D];
         __syncthreads();
-        float m = kNone, R = kNone, l = 0.0f, f[4];
+        float m = kNone, e = -INFINITY, l = 0.0f, f[4];
 #pragma unroll
-        for (int w = 0; w < 4; w++) m = fmaxf(m, lds.sm[w][col]), R = fmaxf(R, lds.sr[w][col]);
+        for (int w = 0; w < 4; w++) m = fmaxf(m, lds.sm[w][col]);
 #pragma unroll
         for (int w = 0; w < 4; w++) {
+            f[w] = lds.se[w][col] + (lds.sm[w][col] - m), e = fmaxf(e, f[w]);
             l += lds.sl[w][col] * __builtin_amdgcn_exp2f(lds.sm[w][col] - m);
-            f[w] = __builtin_amdgcn_exp2f(lds.sr[w][col] - R);
         }
+#pragma unroll
+        for (int w = 0; w < 4; w++) f[w] = __builtin_amdgcn_exp2f(f[w] - e);
         if (col >= c0 && col < c0 + ncol) {
             const int64_t row = r0 + col / hn, head = h0 + col % hn;
             float *dst = a.out + row * a.out_stride + head * c.vd;
-            float by = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(R - m) / l;
+            float by = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(e) / l;
             if (a.ps > 1) {
                 const int64_t at = (row * a.heads + head) * a.ps + part;
                 dst = a.part + at * c.vd, by = 1.0f;
-                if (g == 0 && wave == 0) a.part_ml[3 * at] = m, a.part_ml[3 * at + 1] = l, a.part_ml[3 * at + 2] = R;
+                if (g == 0 && wave == 0) a.part_ml[3 * at] = m, a.part_ml[3 * at + 1] = l, a.part_ml[3 * at + 2] = e;
             }
 #pragma unroll
             for (int i = 0; i < (NV + 3) / 4; i++) {
@@ -470,10 +486,10 @@ __device__ __attribute__((always_inline)) inline void narrow(const Args &a, Narr
                 for (int w = 0; w < 4; w++) {
                     const f32x4 y = lds.so[(w * NV + D) * 64 + lane];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) z[e] = fmaf(y[e], f[w], z[e]);
+                    for (int k = 0; k < 4; k++) z[k] = fmaf(y[k], f[w], z[k]);
                 }
 #pragma unroll
-                for (int e = 0; e < 4; e++) z[e] *= by;
+                for (int k = 0; k < 4; k++) z[k] *= by;
                 *(__attribute__((address_space(1))) f32x4_dw *)(dst + 16 * D + 4 * g) = __builtin_bit_cast(f32x4_dw, z);
             }
         }
@@ -564,7 +580,7 @@ __device__ __attribute__((always_inline)) inline void wide(const Args &a, Wide<N
     x.l += __shfl_xor(x.l, 16, 64);
     x.l += __shfl_xor(x.l, 32, 64);
     if (mine >= ncol) return;
-    const float by = x.l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x.R - x.m) / x.l;
+    const float by = x.l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x.e) / x.l;
     float *dst = a.out + (int64_t)(r0 + own / hn) * a.out_stride + (int64_t)(h0 + own % hn) * c.vd + 4 * g;
 #pragma unroll
     for (int D = 0; D < NV; D++) {
@@ -637,24 +653,27 @@ __global__ __launch_bounds__(T) void kv8_join_kernel(const Args a) {
     if (a.pos[row] < 0 || (unsigned)a.seq[row] >= (unsigned)a.c.n_seq) return;
     const float *ml = a.part_ml + (int64_t)blockIdx.x * a.ps * 3, *part = a.part + (int64_t)blockIdx.x * a.ps * vd;
     if (i < 64) {
-        float m = kNone, R = kNone, l = 0.0f, pm[4], pl[4], pr[4];
+        float m = kNone, e = -INFINITY, l = 0.0f, pm[4], pl[4], pe[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const int p = i + 64 * k;
             pm[k] = p < a.ps ? gload(ml + 3 * p) : kNone, pl[k] = p < a.ps ? gload(ml + 3 * p + 1) : 0.0f;
-            pr[k] = p < a.ps ? gload(ml + 3 * p + 2) : kNone;
-            m = fmaxf(m, pm[k]), R = fmaxf(R, pr[k]);
+            pe[k] = p < a.ps ? gload(ml + 3 * p + 2) : 0.0f;
+            m = fmaxf(m, pm[k]);
         }
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64)), R = fmaxf(R, __shfl_xor(R, o, 64));
+        for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            if (i + 64 * k < a.ps) w[i + 64 * k] = __builtin_amdgcn_exp2f(pr[k] - R);
+            pe[k] += pm[k] - m, e = fmaxf(e, pe[k]);
             l += pl[k] * __builtin_amdgcn_exp2f(pm[k] - m);
         }
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o, 64);
-        if (i == 0) red = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(R - m) / l;
+        for (int o = 32; o >= 1; o >>= 1) e = fmaxf(e, __shfl_xor(e, o, 64)), l += __shfl_xor(l, o, 64);
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (i + 64 * k < a.ps) w[i + 64 * k] = __builtin_amdgcn_exp2f(pe[k] - e);
+        if (i == 0) red = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(e) / l;
     }
     __syncthreads();
     const int n = vd / 4, groups = T / n, g = i / n, at = i % n;

@@ -17,7 +17,9 @@
  *   - Device pointers are HIP device addresses on the context's device.
  *     `stream` is a hipStream_t passed as void* (NULL = the null stream).
  *   - A forward call is asynchronous on `stream` and never waits for the
- *     device.  Calls are reentrant per stream, as the reference's
+ *     device (but a device's first moe_layer_forward_noalloc, which prepares its
+ *     scratch, and a first call on a stream that is being captured).  Calls are
+ *     reentrant per stream, as the reference's
  *     Model::feed_forward(&self, ..., st: &mut State, ...) is per sequence
  *     (src/model.rs:836): moe_layer_forward keeps one workspace per stream it
  *     is called on, and moe_layer_forward_ws runs on a workspace the caller

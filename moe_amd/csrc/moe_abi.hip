@@ -365,11 +365,28 @@ void reap_ws(moe_layer *L) {
     }
 }
 
+__global__ __launch_bounds__(256) void clear_kernel(uint32_t *p, uint32_t words) {
+    for (uint32_t i = threadIdx.x; i < words; i += 256) p[i] = 0;
+}
+
 // Clears device memory before the call returns: hipMemset only queues it on the null
-// stream, which a caller's non-blocking stream overtakes.
+// stream, which a caller's non-blocking stream overtakes.  (Waits for whatever other
+// streams the null stream waits for.)
 hipError_t clear_now(void *p, size_t bytes) {
     const hipError_t e = hipMemset(p, 0, bytes);
     return e == hipSuccess ? hipStreamSynchronize(nullptr) : e;
+}
+
+// Clears a new workspace of stream s in s's order, without a wait.  While s is
+// captured a kernel would be the graph's, so the clear is made at once.
+hipError_t clear_on(void *p, size_t bytes, hipStream_t s) {
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    if (s && (hipStreamIsCapturing(s, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone)) {
+        (void)hipGetLastError();
+        return clear_now(p, bytes);
+    }
+    hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(256), 0, s, static_cast<uint32_t *>(p), (uint32_t)(bytes / 4));
+    return hipGetLastError();
 }
 
 // The workspace of `stream` for t tokens (moe_layer_forward): the layer
@@ -378,8 +395,10 @@ hipError_t clear_now(void *p, size_t bytes) {
 // the old size, in 64-token steps) so that rising token counts allocate
 // O(final size) in total; the outgrown workspace is retired and freed at a
 // later growth once the work queued on it has finished.  A reserved layer
-// does not grow: a larger call fails.
-int stream_ws(moe_layer *L, hipStream_t s, int t, int k, Workspace &out) {
+// does not grow: a larger call fails.  `now`: what is new is ready for any
+// stream's work on return (a reservation's: a graph captured on s may be
+// replayed on another stream).
+int stream_ws(moe_layer *L, hipStream_t s, int t, int k, Workspace &out, bool now = false) {
     std::lock_guard<std::mutex> g(L->mu);
     StreamWs *cur = nullptr;
     for (StreamWs &e : L->ws)
@@ -404,7 +423,7 @@ int stream_ws(moe_layer *L, hipStream_t s, int t, int k, Workspace &out) {
     void *base = nullptr;
     hipError_t e = hipMalloc(&base, bytes);
     if (e != hipSuccess) return fail(MOE_ENOMEM, "workspace of %zu bytes for %d tokens: %s", bytes, max_t, hipGetErrorString(e));
-    if ((e = clear_now(base, kZeroBytes)) != hipSuccess) {
+    if ((e = now ? clear_now(base, kZeroBytes) : clear_on(base, kZeroBytes, s)) != hipSuccess) {
         hipFree(base);
         return fail(MOE_EHIP, "workspace counters: %s", hipGetErrorString(e));
     }
@@ -1360,7 +1379,7 @@ int moe_layer_reserve_stream(moe_layer *L, int32_t max_t, void *stream) {
         L->reserved_k = std::max(L->reserved_k, k);
     }
     Workspace w;
-    return stream_ws(L, (hipStream_t)stream, max_t, k, w);
+    return stream_ws(L, (hipStream_t)stream, max_t, k, w, true);
 }
 
 int moe_layer_reserve(moe_layer *L, int32_t max_t) { return moe_layer_reserve_stream(L, max_t, nullptr); }

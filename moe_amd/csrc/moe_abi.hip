@@ -74,12 +74,14 @@ struct StreamWs {
     hipStream_t stream;
     Workspace w;
     int k;
+    size_t size;  // of its memory (w may take less)
 };
-// An outgrown or released workspace: free once `done` (recorded on its
+// An outgrown or released workspace: any stream's once `done` (recorded on its
 // stream when it was retired, after the last work that used it) has
-// completed; without an event, at moe_layer_destroy.
+// completed; without an event, freed at moe_layer_destroy.
 struct Retired {
     void *base;
+    size_t size;
     hipEvent_t done;
 };
 
@@ -340,17 +342,36 @@ size_t ws_layout(const moe_layer *L, int max_t, int k, Workspace *w, char *base)
     return off;
 }
 
-// Retire a stream's workspace: queued work may still use it, so it is
-// freed only once an event recorded on the stream now has completed.
-void retire_ws(moe_layer *L, void *base, hipStream_t s) {
+// Retire a stream's workspace: queued work may still use it, so its memory
+// is another's only once an event recorded on the stream now has completed.
+void retire_ws(moe_layer *L, void *base, size_t size, hipStream_t s) {
     hipEvent_t ev = nullptr;
     if (hipEventCreateWithFlags(&ev, hipEventDisableTiming) == hipSuccess && hipEventRecord(ev, s) != hipSuccess) {
         hipEventDestroy(ev);
         ev = nullptr;
     }
-    L->retired.push_back({base, ev});
+    L->retired.push_back({base, size, ev});
 }
-// Free the retired workspaces whose event has completed (a query, no wait).
+// The smallest retired workspace of `bytes` or more whose event has completed (a
+// query, no wait), or null; its size.
+void *take_retired(moe_layer *L, size_t bytes, size_t &size) {
+    int best = -1;
+    for (size_t i = 0; i < L->retired.size(); i++) {
+        const Retired &r = L->retired[i];
+        if (r.size >= bytes && (best < 0 || r.size < L->retired[best].size) && r.done && hipEventQuery(r.done) == hipSuccess)
+            best = (int)i;
+    }
+    (void)hipGetLastError();  // (one that has not completed)
+    if (best < 0) return nullptr;
+    const Retired r = L->retired[best];
+    hipEventDestroy(r.done);
+    L->retired[best] = L->retired.back();
+    L->retired.pop_back();
+    size = r.size;
+    return r.base;
+}
+// Free the retired workspaces whose event has completed.  hipFree waits for the
+// whole device, so no forward call does this but one that finds no memory.
 void reap_ws(moe_layer *L) {
     for (size_t i = 0; i < L->retired.size();) {
         Retired &r = L->retired[i];
@@ -393,8 +414,8 @@ hipError_t clear_on(void *p, size_t bytes, hipStream_t s) {
 // keeps one per stream, so calls on different streams never share scratch.
 // Grows without waiting for the device, geometrically (at least 1.5 times
 // the old size, in 64-token steps) so that rising token counts allocate
-// O(final size) in total; the outgrown workspace is retired and freed at a
-// later growth once the work queued on it has finished.  A reserved layer
+// O(final size) in total; the outgrown workspace is retired, and taken for
+// another stream once the work queued on it has finished.  A reserved layer
 // does not grow: a larger call fails.  `now`: what is new is ready for any
 // stream's work on return (a reservation's: a graph captured on s may be
 // replayed on another stream).
@@ -418,10 +439,15 @@ int stream_ws(moe_layer *L, hipStream_t s, int t, int k, Workspace &out, bool no
         }
         max_t = std::max(max_t, cur->w.max_t), kk = std::max(kk, cur->k);
     }
-    reap_ws(L);
     const size_t bytes = ws_layout(L, max_t, kk, nullptr, nullptr);
-    void *base = nullptr;
-    hipError_t e = hipMalloc(&base, bytes);
+    size_t size = bytes;
+    void *base = take_retired(L, bytes, size);
+    hipError_t e = base ? hipSuccess : hipMalloc(&base, bytes);
+    if (e != hipSuccess && !L->retired.empty()) {
+        (void)hipGetLastError();
+        reap_ws(L);
+        e = hipMalloc(&base, bytes);
+    }
     if (e != hipSuccess) return fail(MOE_ENOMEM, "workspace of %zu bytes for %d tokens: %s", bytes, max_t, hipGetErrorString(e));
     if ((e = now ? clear_now(base, kZeroBytes) : clear_on(base, kZeroBytes, s)) != hipSuccess) {
         hipFree(base);
@@ -430,11 +456,12 @@ int stream_ws(moe_layer *L, hipStream_t s, int t, int k, Workspace &out, bool no
     Workspace w;
     ws_layout(L, max_t, kk, &w, static_cast<char *>(base));
     if (cur) {
-        retire_ws(L, cur->w.base, s);
+        retire_ws(L, cur->w.base, cur->size, s);
         cur->w = w;
         cur->k = kk;
+        cur->size = size;
     } else {
-        L->ws.push_back({s, w, kk});
+        L->ws.push_back({s, w, kk, size});
     }
     out = w;
     return MOE_OK;
@@ -1390,7 +1417,7 @@ int moe_layer_release_stream(moe_layer *L, void *stream) {
     std::lock_guard<std::mutex> lk(L->mu);
     for (size_t i = 0; i < L->ws.size(); i++) {
         if (L->ws[i].stream != (hipStream_t)stream) continue;
-        retire_ws(L, L->ws[i].w.base, L->ws[i].stream);
+        retire_ws(L, L->ws[i].w.base, L->ws[i].size, L->ws[i].stream);
         L->ws.erase(L->ws.begin() + i);
         break;
     }

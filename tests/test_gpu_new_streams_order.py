@@ -54,6 +54,52 @@ def test_calls_do_not_wait_for_the_null_stream(name):
         assert np.isfinite(g).all() and rel_err(g, w) <= TOL
 
 
+def test_growth_does_not_wait_for_other_streams():
+    """Token counts that rise on several streams, streams dropped and others begun,
+    with a long kernel on the null stream: calls return, and memory that changed
+    hands gives what fresh memory does."""
+    import torch
+
+    from moe_amd import synth
+    from moe_amd.layer import Context
+
+    host = synth.build_host_layer(synth.SHAPES["tiny_mixtral"], 3)
+    ctx = Context(0)
+    quiet, gl = synth.make_layer(ctx, host), synth.make_layer(ctx, host)
+    xs = [torch.from_numpy(synth.activations(11 + t, t, host.shape.hidden)).cuda() for t in (1, 24, 40, 100, 3, 200)]
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    outs = [[torch.full_like(x, float("nan")) for x in xs] for _ in streams]
+    want = [torch.empty_like(x) for x in xs]
+    for x, out in zip(xs, want):
+        quiet.feed_forward(x, out)
+    for x in xs[:3]:  # memory to change hands
+        gl.feed_forward(x, torch.empty_like(x), stream=streams[0])
+    torch.cuda.synchronize()
+    a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    done = torch.cuda.Event()
+    torch.cuda._sleep(1_000_000)
+    a.record()
+    torch.cuda._sleep(10_000_000)
+    b.record()
+    b.synchronize()
+    torch.cuda._sleep(int(10_000_000 * 1000 / a.elapsed_time(b)))  # a second
+    done.record()
+    for s, some in zip(streams, outs):
+        for x, out in zip(xs, some):
+            gl.feed_forward(x, out, stream=s)
+    assert not done.query()  # (the null stream's kernel still runs)
+    torch.cuda.synchronize()
+    for some in outs:
+        for w, g in zip(want, some):
+            assert rel_err(g.cpu().numpy(), w.cpu().numpy()) <= TOL
+    for s, some in zip(streams, outs):
+        gl.release_stream(s)
+        for x, w, out in zip(xs, want, some):
+            out.fill_(float("nan"))
+            gl.feed_forward(x, out)
+            assert rel_err(out.cpu().numpy(), w.cpu().numpy()) <= TOL
+
+
 def test_a_reservation_is_ready_when_it_returns():
     """A reserved stream's workspace is cleared by then, whatever the null stream
     does later: the first call may be a captured one that another stream replays."""

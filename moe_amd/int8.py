@@ -25,7 +25,8 @@ class Int8Linear(_OnDevice):
     """y = x W^T in 8 bits.  `weights`: tensors [channels, values] (float32,
     float16 or bfloat16, contiguous rows) or one of them; several over the same
     input become one product, their channels one behind the other.  They are
-    quantised once, on torch's current stream of their device, and not kept."""
+    quantised once, on torch's current stream of their device, and not kept; that
+    is done when the object is made, so its calls may go to any stream."""
 
     def __init__(self, weights):
         ws = list(weights) if isinstance(weights, (list, tuple)) else [weights]
@@ -70,6 +71,7 @@ class Int8Linear(_OnDevice):
                 _refused(L.lib().moe_int8_pack(ptr, dt, row_bytes, m, at, n, k, self.packed.data_ptr(), b.value,
                                                torch._C._cuda_getCurrentRawStream(self._index)), "moe_int8_pack")
                 at += m
+            torch.cuda.current_stream().synchronize()
         self._where, self._width = self.packed.data_ptr(), -(-k // 64) * 64
         self._sizes = {}
 

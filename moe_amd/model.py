@@ -613,6 +613,8 @@ class Model:
         self.attn_scale = float(np.float32(s.rope.attn_scale()) / np.sqrt(np.float32(qd), dtype=np.float32))
         self._ws = self._mws = None
         self._ws_t = 0
+        if self.device.type == "cuda":  # the vectors' copies: calls may go to any stream
+            torch.cuda.current_stream(self.device).synchronize()
 
     # -- helpers ---------------------------------------------------------
     def _vec(self, name: str, optional: bool = False):
@@ -646,7 +648,8 @@ class Model:
                   sparse: Optional[Sparse] = None):
         """State for n_seq sequences of up to ctx positions; with cache="q4" or
         "int8" (4 or 8 bits a value) a PagedState (head widths that are multiples
-        of 32, up to 256), whose contexts may be of any length."""
+        of 32, up to 256), whose contexts may be of any length.  Made on torch's
+        current stream, behind which the first step is ordered by the caller."""
         if cache in ("q4", "int8"):
             return PagedState(self, n_seq, ctx, page, pages, sparse, cache)
         if cache != "f32" or pages is not None or sparse is not None:

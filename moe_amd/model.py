@@ -781,6 +781,8 @@ class Model:
         h = lay.get("heads")
         if h is None:
             s, bias = self.spec, lay["bias"]
+            if bias[2] is not None and bias[2].numel() != s.kv_heads * s.head_dim:  # (the others: HeadRope's checks)
+                raise ValueError(f"a bias of {bias[2].numel()} values for {s.kv_heads} value heads of {s.head_dim}")
             h = lay["heads"] = HeadRope(s.heads, s.kv_heads, s.head_dim, self.inv_freq, dim=s.head_dim // 2 * 2, eps=s.eps,
                                         q_norm=lay["q_norm"], k_norm=lay["k_norm"], q_bias=bias[0], k_bias=bias[1],
                                         v_bias=bias[2])

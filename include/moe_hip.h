@@ -583,8 +583,9 @@ int moe_kv8_load(const moe_kv8 *c, const int64_t *slots, int32_t rows, float *k,
  * position of a block whose keys or values read as NaN, or whose query is not
  * finite, is NaN; what positions hold that no row sees does not matter.
  * Codes are exact; a query counts to 2^-22 of its head's largest value, a weight
- * times its block's value scale to 2^-23 of the largest such product within 64
- * or 128 positions (to up to 2^-16 where all those value scales are below 2^-100).
+ * times its block's value scale to 2^-23 of the largest such product among blocks
+ * within 64 or 128 positions whose value scales are within 2^5 of each other (to up
+ * to 2^-16 where they are below 2^-100).
  * Scores may be of any size; one that times log2(e) leaves f32's range is infinite.
  * `workspace`: device, 16-byte aligned, moe_kv8_attention_workspace_size bytes
  * (its arguments as the call's; it may be 0 bytes).  Calls that share one must

@@ -17,9 +17,12 @@
 // second operand of the values' product.  There the weights p = 2^(s - m) meet the values' scales first:
 //   W = p s_v C 2^-r,  r the largest s - m + log2 s_v of the step,  C = 2^23 - ..
 // so W below 2^23 keeps each block's product of weight and scale to 2^-23 of the
-// step's largest, however far apart the scales are.  Multiplied and added to
-// 2^23 + 0x8080 in one instruction, a weight's bits are its three digits (the
-// two low ones with 128 added).  A step's sums are whole numbers too; they join
+// step's largest.  A step takes blocks whose value scales lie within 2^5 of each
+// other and goes over its tiles once more for others, so that what is small in some
+// of a head's dims keeps its precision beside what is large in others (in the same
+// pass a block 2^-16 of its neighbours kept 7 bits).  Multiplied and added to 2^23 +
+// 0x8080 in one instruction, a weight's bits are its three digits (the two low ones
+// with 128 added).  A step's sums are whole numbers too; they join
 // the f32 sums O, which are multiples of 2^(m + e) (the weights' sum's of 2^m).
 // Everything is in differences from m, and m and e are whole numbers, so that no
 // step's scores, however large, round what earlier steps left: one position whose
@@ -123,14 +126,15 @@ struct Columns {
     int first, last;    // of all columns: everything in first .. last is seen by every one
 };
 
-// One step of NT tiles: k(b, c) and v(D, t) give operands, base[t] the tiles'
-// first positions (negative: no such tile).  read() is called when the keys are
-// done with.  Lane 8 t + b holds the scale of tile t's block b of keys, lane
-// 8 t + 4 + b that of its values (0 where there is no tile): uniform values go
-// through scalar registers.
+// One step of NT tiles over their blocks `todo` (a bit each), or those of them whose
+// value scales are near the largest; returns which are left.  k(b, c) and v(D, t)
+// give operands, base[t] the tiles' first positions (negative: no such tile).  read()
+// is called when the keys are done with.  Lane 8 t + b holds the scale of tile t's
+// block b of keys, lane 8 t + 4 + b that of its values (0 where there is no tile):
+// uniform values go through scalar registers.
 template <int NQ, int NV, int NT, bool EX, class K, class V, class F>
-__device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const i32x4 (&q)[3][NQ], K k, V v, F read, float scale,
-                                                           const int (&base)[NT], int nv, int g) {
+__device__ __attribute__((always_inline)) inline int step(Columns<NV> &x, const i32x4 (&q)[3][NQ], K k, V v, F read, float scale,
+                                                          const int (&base)[NT], int nv, int g, int todo) {
     f32x4 s[4 * NT];
 #pragma unroll
     for (int b = 0; b < 4 * NT; b++) {
@@ -147,14 +151,28 @@ __device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const
     }
     read();
     const int lane = threadIdx.x & 63;
-    if (__builtin_expect(__any(!(fabsf(scale) < INFINITY)), 0)) {  // a block that reads as NaN: so are the columns that see it
-        for (int b = 0; b < 4 * NT; b++) {
+    auto exponent = [&](float y) { return (int)(__float_as_uint(y) >> 23); };
+    // Value scales' exponents within 2 of the first's are within 2^5 of each other
+    // (0: zeros, anyone's).
+    int now = todo, first = x.first;
+    const int about = __builtin_amdgcn_readlane(exponent(scale), 4) - 2;
+    if (__builtin_expect(__ballot(!(fabsf(scale) < INFINITY)) |
+                             (__ballot(scale != 0.0f && (unsigned)(exponent(scale) - about) > 4) & (NT > 1 ? 0xf0f0 : 0xf0)), 0)) {
+        for (int b = 0; b < 4 * NT; b++) {  // a block that reads as NaN: so are the columns that see it
             const int at = b / 4 * 8 + b % 4;
             if (fabsf(__shfl(scale, at, 64)) < INFINITY && fabsf(__shfl(scale, at + 4, 64)) < INFINITY) continue;
             const int p = (b < 4 ? base[0] : base[NT - 1]) + 16 * (b % 4);
             if (p <= x.pos && p + 15 >= x.lo) x.l = __uint_as_float(0x7fc00000u);
             if (lane == at || lane == at + 4) scale = 0.0f;
         }
+        // Blocks of the largest scales, 2^5 down at most; `first`: a step that is not whole.
+        const int mine = lane & 4 && todo >> ((lane >> 1 & 4) + (lane & 3)) & 1 ? exponent(scale) : -1;
+        int largest = max(mine, __shfl_xor(mine, 1, 64));
+        largest = max(largest, __shfl_xor(largest, 2, 64));
+        largest = max(largest, __shfl_xor(largest, 8, 64));
+        const uint32_t near = (uint32_t)__ballot(mine == 0 || mine >= largest - 4);
+        now = todo & ((near >> 4 & 15) | (near >> 12 & 15) << 4);
+        if (now != (1 << 4 * NT) - 1) first = 0x7fffffff;
     }
     const float log_ = fmaxf(__builtin_amdgcn_logf(scale), kLeastLog);
     auto of = [&](float y, int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(y), i)); };
@@ -163,14 +181,14 @@ __device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const
     for (int b = 0; b < 4 * NT; b++) sc[b] = of(scale, b / 4 * 8 + b % 4) * x.qs;
     bool whole = true;
 #pragma unroll
-    for (int t = 0; t < NT; t++) whole = whole && base[t] >= x.first && base[t] + 63 <= x.last;
+    for (int t = 0; t < NT; t++) whole = whole && base[t] >= first && base[t] + 63 <= x.last;
     if (!whole) {
 #pragma unroll
         for (int b = 0; b < 4 * NT; b++) {
             const int p = base[b / 4] + 16 * (b % 4) + 4 * g;
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                s[b][i] = base[b / 4] >= 0 && p + i >= x.lo && p + i <= x.pos ? s[b][i] * sc[b] : -INFINITY;
+                s[b][i] = (now >> b & 1) && base[b / 4] >= 0 && p + i >= x.lo && p + i <= x.pos ? s[b][i] * sc[b] : -INFINITY;
             sc[b] = 1.0f;
         }
     }
@@ -212,7 +230,7 @@ __device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const
         const Digits d = digits_of(y[0], y[1], y[2], y[3]);
         w[b / 4][0][b % 4] = (int)d.d2, w[b / 4][1][b % 4] = (int)d.d1, w[b / 4][2][b % 4] = (int)d.d0;
     }
-    const float m = fmaxf(x.m, top), was = x.e + (x.m - m), now = ref + (top - m), e = fmaxf(was, __builtin_ceilf(now));
+    const float m = fmaxf(x.m, top), was = x.e + (x.m - m), here = ref + (top - m), e = fmaxf(was, __builtin_ceilf(here));
     x.l = x.l * __builtin_amdgcn_exp2f(x.m - m) + sum * __builtin_amdgcn_exp2f(top - m);
     if (__any(e > was)) {
         const float keep = __builtin_amdgcn_exp2f(was - e);
@@ -221,7 +239,7 @@ __device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const
 #pragma unroll
             for (int i = 0; i < 4; i++) x.o[D][i] *= keep;
     }
-    const float in0 = __builtin_amdgcn_exp2f(now - e) * (1.0f / kMost);
+    const float in0 = __builtin_amdgcn_exp2f(here - e) * (1.0f / kMost);
     x.m = m, x.e = e;
 #pragma unroll
     for (int D = 0; D < NV; D++) {
@@ -238,6 +256,7 @@ __device__ __attribute__((always_inline)) inline void step(Columns<NV> &x, const
         for (int i = 0; i < 4; i++)
             x.o[D][i] = fmaf(joined(d[0][i], d[1][i], d[2][i]), in0, x.o[D][i]);
     }
+    return todo & ~now;
 }
 
 // Lanes of my_seq and my_pos that begin a run of one sequence's rows or are
@@ -442,12 +461,14 @@ __device__ __attribute__((always_inline)) inline void narrow(const Args &a, Narr
             __builtin_amdgcn_sched_barrier(0);
         };
         if (t < t1) load_keys(t);
-        for (; t < t1; t++) {
+        for (int todo = 15; t < t1;) {
             if (base[0] >= 0)
-                step<NQ, NV, 1, EX>(x, q, [&](int b, int cc) { return k[b][cc]; }, [&](int D, int) { return v[D]; }, load_values, scale,
-                                    base, nv, g);
+                todo = step<NQ, NV, 1, EX>(x, q, [&](int b, int cc) { return k[b][cc]; }, [&](int D, int) { return v[D]; }, load_values,
+                                           scale, base, nv, g, todo);
+            else todo = 0;
             __builtin_amdgcn_sched_barrier(0);
-            load_keys(t + 1);
+            if (todo == 0) t++, todo = 15;  // (else the same tile's once more)
+            load_keys(t);
         }
 
         // Merge the waves: sums as they are and their references through LDS,
@@ -560,20 +581,30 @@ __device__ __attribute__((always_inline)) inline void wide(const Args &a, Wide<N
         lds::wait_vm_barrier<0>();
         const int later = t + NT < t1 ? fetch(t + NT, buffer ^ 1) : 0;
         if (t <= hi >> 6 && t + NT > lo >> 6) {
-            int base[NT];
+            auto go = [&](int tt, lds::lds_p at, float scale, int todo) __attribute__((always_inline)) {
+                int base[NT];
 #pragma unroll
-            for (int i = 0; i < NT; i++) base[i] = now >> i & 1 ? (t + i) * 64 : -64;
-            const float scale = now >> (lane >> 3 & (NT - 1)) & 1 ? lds_.scales[buffer][lane & (8 * NT - 1)] : 0.0f;
-            const lds::lds_p at = (lds::lds_p)lds_.tiles[buffer] + lane * 16;
-            step<NQ, NV, NT, true>(
-                x, q,
-                [&](int b, int cc) __attribute__((always_inline)) {
-                    return *(const __attribute__((address_space(3))) i32x4 *)(at + (b >> 2) * bytes + (b & 3) * 16 * qd + cc * 1024);
-                },
-                [&](int D, int i) __attribute__((always_inline)) {
-                    return *(const __attribute__((address_space(3))) i32x4 *)(at + i * bytes + 64 * qd + D * 1024);
-                },
-                [] {}, scale, base, NV, g);
+                for (int i = 0; i < NT; i++) base[i] = now >> i & 1 ? (tt + i) * 64 : -64;
+                return step<NQ, NV, NT, true>(
+                    x, q,
+                    [&](int b, int cc) __attribute__((always_inline)) {
+                        return *(const __attribute__((address_space(3))) i32x4 *)(at + (b >> 2) * bytes + (b & 3) * 16 * qd + cc * 1024);
+                    },
+                    [&](int D, int i) __attribute__((always_inline)) {
+                        return *(const __attribute__((address_space(3))) i32x4 *)(at + i * bytes + 64 * qd + D * 1024);
+                    },
+                    [] {}, scale, base, NV, g, todo);
+            };
+            auto scale_of = [&] { return now >> (lane >> 3 & (NT - 1)) & 1 ? lds_.scales[buffer][lane & (8 * NT - 1)] : 0.0f; };
+            // (A loop around one copy of the step took 8 us more for a prompt's 267; above,
+            // for 16 columns, two copies took 0 to 4% more.)
+            int todo = go(t, (lds::lds_p)lds_.tiles[buffer] + lane * 16, scale_of(), (1 << 4 * NT) - 1);
+            while (__builtin_expect(todo, 0)) {
+                int tt = t;
+                lds::lds_p at = (lds::lds_p)lds_.tiles[buffer] + lane * 16;
+                asm volatile("" : "+s"(tt), "+v"(at)::"memory");  // (operands are read again, not kept)
+                todo = go(tt, at, scale_of(), todo);
+            }
         }
         now = later;
     }

@@ -134,7 +134,7 @@ __global__ __launch_bounds__(512, NU <= 8 ? 6 : 4) void kv8_store_kernel(const S
         return slot_ok(c, slot) && p >= 0 ? s : -1;
     };
     const int start = which * window, next_of = row_of(min(mine + 1, a.rows - 1)), past = start - 64 + lane;
-    const int past_of = past >= 0 ? row_of(past) : -1;
+    const int past_row = row_of(max(past, 0)), past_of = past >= 0 ? past_row : -1;
     const bool good = lane < window && mine < a.rows && slot_ok(c, my_slot) && (unsigned)my_seq < (unsigned)c.n_seq && my_pos >= 0;
     const int my_r0 = good ? max(0, min(mine, gload(a.row_start + my_seq))) : 0;
     const int my_r1 = good ? max(mine + 1, min(a.rows, gload(a.row_start + my_seq + 1))) : 0;
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(512, NU <= 8 ? 6 : 4) void kv8_store_kernel(const S
                                : u32x4{0, 0, 0, 0};
     const bool followed = good && mine + 1 < my_r1 && next_of == my_seq;
     bool ends = good && ((my_pos & 63) == 63 || !followed);
-    if (ends && !followed)
+    if (__builtin_expect(ends && !followed && mine + 2 < my_r1 && (my_pos & 63) < 62, 0))
         for (int j = mine + 2, of_tile = min(my_r1, mine + 64 - (my_pos & 63)); ends && j < of_tile; j++) ends = row_of(j) != my_seq;
     const unsigned long long follow = __ballot(followed);
     unsigned long long last = __ballot(ends);
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(512, NU <= 8 ? 6 : 4) void kv8_store_kernel(const S
             const int j = t0 - 1 - start;  // (-64 at least)
             behind = (j >= 0 ? late >> j : early >> (j + 64)) & 1 || first_row(r0, t0) >= 0;
         }
-        const bool ends_here = !(follow >> at & 1) && first_row(r + 2, r1) < 0;
+        const bool ends_here = !(follow >> at & 1) && (r + 2 >= r1 || first_row(r + 2, r1) < 0);
         // The position of the first row in the tile.
         const int p0 = behind ? p & ~63 : (p & ~63) + __builtin_ctzll(there);
         auto of_block = [&](int k) { return (uint32_t)(there >> (16 * k)) & 0xffffu; };

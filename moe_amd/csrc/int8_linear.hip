@@ -11,11 +11,13 @@
 // product as it is.  Values past a row's last are zeros, and so are x's rows past
 // its last (channels past the last are whatever is there: nothing reads their sums).
 //
-// Large products are bound by what the chip's power leaves of the matrix pipe:
-// 8191 x 6144 x 4096 in 175 us, 2357 TOP/s with the pipe 50% busy at 2.05 GHz, the
-// rows' codes before it 40 (168 MB, 4.2 TB/s).  Few rows are bound by the weights'
-// bytes: 32 rows of 6144 x 4096 6.3 us (4.2 TB/s) after 2.7 for the codes, one row
-// of 4096 x 4096 4.5 in all.
+// Large products: 8191 x 6144 x 4096 in 175 us, 2357 TOP/s (the library's own takes
+// 183), the rows' codes before it 40 (168 MB, 4.2 TB/s).  A step of the 256 x 256
+// kernel takes the matrix pipe 1024 of its 2067 cycles, and the LDS port, with 12
+// operand tiles a wave for 32 products and the DMA's writes, about as many; the two
+// overlap little (pipe 50% busy at 2.05 GHz, waves waiting 44% of their time).  Few
+// rows are bound by the weights' bytes: 32 rows of 6144 x 4096 6.8 us (3.8 TB/s) after
+// 3.0 for the codes, one row of 4096 x 4096 5.0 in all (3.4 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -192,7 +194,7 @@ __global__ __launch_bounds__(W * 64) void int8_direct_kernel(const Product p) {
 #pragma unroll
         for (int j = 0; j < NT; j++) acc[i][j] = i32x4{0, 0, 0, 0};
     // U chunks' loads at a time; past the last chunk the last one again, whose
-    // products then meet zeros.
+    // products are left out.
     constexpr int U = MT + NT <= 3 ? 8 : MT + NT <= 6 ? 4 : 2;
     for (int c0 = wave; c0 < p.chunks; c0 += W * U) {
         i32x4 a[U][MT], b[U][NT];
@@ -346,7 +348,7 @@ void ring(const Product &p, hipStream_t s) {
 
 // A few rows (up to 16384 values in all): each block quantises them for itself,
 // under its first loads of weights, into LDS as [row][values]; lanes of rows past
-// the last hold zeros.  One row of 4096 x 4096 4.5 us (3.8 TB/s), against 6.6 with
+// the last hold zeros.  One row of 4096 x 4096 5.0 us (3.4 TB/s), against 6.6 with
 // the rows in a launch of their own; of 28672 x 4096 20 (5.8 TB/s); four rows 7.3
 // and 6.8, but a launch less to queue.
 constexpr int kFewBytes = 16384, kFewRows = 4;

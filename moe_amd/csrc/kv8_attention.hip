@@ -33,10 +33,10 @@
 //
 // Decode reads the cache once and is bound by that: 64 sequences of 6000 to 12000
 // positions, 8 kv heads of 128, 235 us (5.0 TB/s of codes), one of 100001 in 128
-// parts 41 with the joining launch, 32 of up to 1500 20 (3.8 TB/s: one block a CU
+// parts 40 with the joining launch, 32 of up to 1500 19 (4.0 TB/s: one block a CU
 // with 12 to 24 tiles, then a merge).  Prompts are bound by the issue of vector
-// instructions beside the products: 4001 rows of 32 heads of 128 268 us (490
-// TFLOP/s of the attention's own operations), 8000 rows 945 (555), of which the
+// instructions beside the products: 4001 rows of 32 heads of 128 271 us (484
+// TFLOP/s of the attention's own operations), 8000 rows 955 (549), of which the
 // matrix pipe is busy in 29% and vector instructions issue in 71% (25 to a
 // score: joining three sums 4, the exponential 2, the weight and its digits 4, a
 // step's sums into O 5 for every two).  Two tiles' products a step halve that last

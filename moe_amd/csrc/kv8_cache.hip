@@ -6,8 +6,9 @@
 // kv head, a wave its blocks' keys or values each: the rows of this step, and before
 // them those of earlier steps, whose values `open` keeps while their block is
 // filling.  Both kernels are streams: 16376 rows of 8 kv heads of 128 are written in
-// 43 us (168 MB, 3.9 TB/s) and read in 44 (33 where the codes are cached); 32 rows in
-// 6.8 (three dependent loads: the row's place, its sequence's, the values) and 3.9.
+// 44 us (168 MB, 3.9 TB/s; 46 to 50 where nothing is cached) and read in 43 (33 where
+// the codes are cached); 32 rows in 7.6 (three dependent loads: the row's place, its
+// sequence's, the values) and 3.9.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

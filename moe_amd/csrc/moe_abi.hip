@@ -386,10 +386,6 @@ void reap_ws(moe_layer *L) {
     }
 }
 
-__global__ __launch_bounds__(256) void clear_kernel(uint32_t *p, uint32_t words) {
-    for (uint32_t i = threadIdx.x; i < words; i += 256) p[i] = 0;
-}
-
 // Clears device memory before the call returns: hipMemset only queues it on the null
 // stream, which a caller's non-blocking stream overtakes.  (Waits for whatever other
 // streams the null stream waits for.)
@@ -406,8 +402,7 @@ hipError_t clear_on(void *p, size_t bytes, hipStream_t s) {
         (void)hipGetLastError();
         return clear_now(p, bytes);
     }
-    hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(256), 0, s, static_cast<uint32_t *>(p), (uint32_t)(bytes / 4));
-    return hipGetLastError();
+    return launch_clear(p, bytes, s);
 }
 
 // The workspace of `stream` for t tokens (moe_layer_forward): the layer

@@ -183,6 +183,10 @@ bool route_one_ok(int H, int E);
 hipError_t launch_route_one(const float *W, const float *x, int n_rows, int E, int H, float temp, float *logits,
                             const GateParams &p, const DispatchArgs &d, unsigned *counter, hipStream_t s);
 
+// Zeros `bytes` (a few, a multiple of 4) at p.  (Here and not where it is called: a
+// kernel beside the 64 MiB scratch array would load that with it.)
+hipError_t launch_clear(void *p, size_t bytes, hipStream_t s);
+
 // y = the gates' exp (glibc expf port) over n values; diagnostics.
 hipError_t launch_expf(const float *x, float *y, size_t n, hipStream_t s);
 

@@ -1330,6 +1330,10 @@ __global__ __launch_bounds__(kDispatchThreads) __attribute__((amdgpu_waves_per_e
     if (threadIdx.x == 0) *counter = 0u;
 }
 
+__global__ __launch_bounds__(256) void clear_kernel(uint32_t *p, uint32_t words) {
+    for (uint32_t i = threadIdx.x; i < words; i += 256) p[i] = 0;
+}
+
 __global__ void expf_kernel(const float *__restrict__ x, float *__restrict__ y, size_t n) {
     size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
     size_t stride = (size_t)gridDim.x * blockDim.x;
@@ -1480,6 +1484,11 @@ hipError_t launch_dispatch(const DispatchArgs &a, int32_t *chunk_scratch, size_t
         hipLaunchKernelGGL(dispatch_place_kernel<kDispatchThreads>, dim3(nc), dim3(kDispatchThreads), 0, s, a,
                            chunk_scratch);
     }
+    return hipGetLastError();
+}
+
+hipError_t launch_clear(void *p, size_t bytes, hipStream_t s) {
+    hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(256), 0, s, static_cast<uint32_t *>(p), (uint32_t)(bytes / 4));
     return hipGetLastError();
 }
 

@@ -57,7 +57,8 @@ class HeadRope(_OnDevice):
     def __call__(self, q, k, pos, v=None, *, q_out=None, k_out=None, v_out=None, stream=None):
         """Rows q [rows, heads * width] and k [rows, n_kv * width] (float32,
         contiguous rows) at positions pos (int32 [rows]), in place or into
-        q_out and k_out; v [rows, values] gets v_bias, where there is one."""
+        q_out and k_out, which otherwise share no memory with them; v [rows,
+        values] gets v_bias, where there is one."""
         n = q.shape[0]
         _fits(rows=n)
         q_out, k_out = q if q_out is None else q_out, k if k_out is None else k_out
